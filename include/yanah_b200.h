@@ -409,6 +409,120 @@ int yn_scale_rows(const void* y, const float* scale, int64_t rows, int32_t cols,
  * (T, shared_inter) bf16 and its gates sigmoid(g) (T) fp32 in `ws`. */
 int yn_rows_route_shared(const yn_dims* dims, int32_t T, void* ws, void** act_sh, float** sgate);
 
+/* ------------------------------------------------------- scored routing */
+
+/* Element types of the entry points below. */
+#define YN_F32 0
+#define YN_BF16 1
+#define YN_F16 2
+
+#define YN_SCORE_SOFTMAX 0
+#define YN_SCORE_SIGMOID 1
+
+/* How rows of router logits choose their experts. */
+typedef struct yn_route_rule {
+  int32_t n_experts;   /* E <= 1024 */
+  int32_t top_k;       /* k <= 31 */
+  int32_t score;       /* YN_SCORE_SOFTMAX or YN_SCORE_SIGMOID */
+  int32_t n_groups;    /* experts in equal, consecutive groups (1: no groups), <= 32 */
+  int32_t top_groups;  /* groups that a row may use */
+  int32_t group_top;   /* a group's score: the sum of its 1 or 2 largest choice values */
+  int32_t norm_topk;   /* 1: the weights are divided by their sum */
+  float scale;         /* factor of the weights */
+} yn_route_rule;
+
+/* Routing by a rule (yn_route is the softmax top-k form of the reference's
+ * models, mlx_backend.py:308-316; this one has no counterpart there). logits:
+ * (rows, E) of `dtype`, rows `row_stride` elements apart. s = softmax or
+ * sigmoid of the logits; the choice value of an expert is s + bias (bias:
+ * (E) fp32 or NULL); the top_groups groups with the best scores are kept, and
+ * of their experts the k with the largest choice values are chosen, in
+ * descending order, ties to the lower id (groups alike). The order is that of
+ * exact arithmetic; without a bias it is the order of the logits. weights: s
+ * of the chosen (without the bias), renormalised if asked, times `scale`, in
+ * fp32. An expert does not take part (it has no share of a softmax either)
+ * where `available` ((E) bytes, NULL: all) is 0, its logit is -inf or NaN; one
+ * whose bias is -inf or NaN is not chosen. A row with fewer than k experts
+ * left ends in ids of -1 with weight 0. Logits of +inf share the softmax's
+ * mass. ids (rows, k) int32, weights (rows, k). Launches one kernel. */
+int yn_route_scored(const yn_route_rule* rule, const void* logits, int32_t dtype, int64_t row_stride, int64_t rows,
+                    const float* bias, const uint8_t* available, int32_t* ids, float* weights, void* stream);
+/* Where yn_rows_route of T rows left the router logits (T, E) fp32 in `ws`. */
+int yn_rows_route_logits(const yn_dims* dims, int32_t T, void* ws, float** logits);
+
+/* -------------------------------------------- products in 8-bit integers */
+
+/* `n_mats` matrices of (rows, cols) signed 8-bit codes with one fp32 scale per
+ * row (output channel): value = code * scale. Rows `row_stride` and matrices
+ * `mat_stride` bytes apart, both and the base multiples of 16; scales of a
+ * matrix contiguous, those of matrices `scale_stride` elements apart. */
+typedef struct yn_i8_mat {
+  const void* codes;
+  const float* scales;
+  int64_t row_stride, mat_stride, scale_stride;
+  int32_t n_mats, rows, cols;   /* cols <= 131072: a sum stays inside 32 bits */
+} yn_i8_mat;
+
+/* Rows of x (rows, cols) of `dtype` as 8-bit codes with one scale each: scale =
+ * max|x| / 127, code = the whole number nearest to 127 x / max|x|, ties to even
+ * (the same for a weight's channels). A row with an infinity or a NaN gets a NaN
+ * scale (its products are NaN, no other row's), a row of zeros scale 0. Strides
+ * in elements. */
+int yn_i8_quant_rows(const void* x, int32_t dtype, int64_t row_stride, int64_t rows, int32_t cols, void* codes,
+                     int64_t code_stride, float* scales, void* stream);
+
+/* y (rows, w->rows) = x (rows, w->cols) times the transpose of w, the rows of x
+ * as above, sums exact in 32 bits, then * row scale * channel scale in fp32 and
+ * one rounding to y_dtype (QuantizedLinear's counterpart, mlx_backend.py:305-306,
+ * for matrices with channel scales). At most 8 rows run on dp4a in one kernel
+ * that makes the codes itself; more on the tensor cores (tcgen05, kind::i8). ws:
+ * yn_i8_linear_ws_bytes bytes, 256-byte aligned, need not be cleared. */
+size_t yn_i8_linear_ws_bytes(int64_t rows, int32_t cols);
+int yn_i8_linear(const yn_i8_mat* w, const void* x, int32_t dtype, int64_t x_stride, int64_t rows, void* y,
+                 int32_t y_dtype, int64_t y_stride, void* ws, size_t ws_bytes, void* stream);
+
+/* The routed experts of an MoE layer in that form (the counterpart of yn_moe_up +
+ * yn_moe_down and of yn_tc_experts, mlx_backend.py:411-459): for every row and its
+ * experts ids (rows, top_k), g = gate_e x, u = up_e x, a = silu(g) u as an 8-bit row
+ * with its own scale, out[t] = residual[t] + sum_j weights[t][j] down_e a, summed in
+ * fp32 in column order and rounded once to `dtype` (that of x, residual and out).
+ * gate, up: (E, I, H); down: (E, H, I); E <= 1024, top_k <= 32, rows * top_k <= 2^22.
+ * An id of -1 has no expert (yn_route_scored ends rows so); another id outside [0, E)
+ * is left out and reported by yn_i8_error. residual may be NULL, out may be it. ws:
+ * yn_i8_experts_ws_bytes bytes, 256-byte aligned, need not be cleared. */
+size_t yn_i8_experts_ws_bytes(int64_t rows, int32_t top_k, int32_t n_experts, int32_t hidden, int32_t inter,
+                              int32_t dtype);
+int yn_i8_experts(const yn_i8_mat* gate, const yn_i8_mat* up, const yn_i8_mat* down, const void* x, int32_t dtype,
+                  int64_t x_stride, int64_t rows, const int32_t* ids, const float* weights, int32_t top_k,
+                  const void* residual, int64_t res_stride, void* out, int64_t out_stride, void* ws, size_t ws_bytes,
+                  void* stream);
+/* Read and clear the current device's error word of these entry points
+ * (synchronises the stream). */
+int yn_i8_error(void* stream, int32_t* code_out);
+
+/* --------------------------------------------- token log probabilities */
+
+/* What rows of logits say of given tokens (the verify rows of a draft,
+ * speculative.py:121-193, and any caller that scores text). logits: (rows,
+ * vocab) of `dtype`, rows `row_stride` elements apart, aligned to their
+ * element only. Per row, with m the largest logit and S = sum exp(z - m):
+ *   logprob = z[token] - m - log S;  entropy = log S - sum exp(z - m) (z - m) / S;
+ *   rank = how many tokens come before it (a larger logit, or the same at a lower id);
+ *   top_ids / top_logprobs (rows, n_top): the n_top <= 64 largest, in that order.
+ * Sums in fp32 relative to the row's maximum, without their largest term (so
+ * that log S is exact when one token has nearly all the mass). Logits of -inf
+ * have no mass and are never listed (id -1, log probability -inf); a row of
+ * them alone has log probabilities of -inf and entropy 0. Logits of +inf share
+ * the mass. A NaN makes the row's log probabilities and entropy NaN, its rank
+ * and ids -1. A token outside [0, vocab) gives NaN and rank -1. tokens, with
+ * logprob and rank, may be NULL; so may entropy; top_* with n_top = 0. ws:
+ * yn_logprobs_ws_bytes bytes, need not be cleared. Launches one kernel, or two
+ * where few rows are split over the device. */
+size_t yn_logprobs_ws_bytes(int64_t rows, int64_t vocab, int32_t dtype, int32_t n_top);
+int yn_token_logprobs(const void* logits, int32_t dtype, int64_t row_stride, int64_t rows, int64_t vocab,
+                      const int32_t* tokens, int32_t n_top, float* logprob, float* entropy, int32_t* rank,
+                      int32_t* top_ids, float* top_logprobs, void* ws, size_t ws_bytes, void* stream);
+
 /* ---------------------------------------------------------- slot copies */
 
 /* Copy `n` expert records host -> slot arena (io_lanes.py:121-126

@@ -65,6 +65,16 @@ class EpSymPtrs(C.Structure):
     _fields_ = [(n, C.c_void_p) for n in ("x_all", "ids_all", "y", "flags", "counter")]
 
 
+class RouteRuleStruct(C.Structure):
+    _fields_ = [("n_experts", C.c_int32), ("top_k", C.c_int32), ("score", C.c_int32), ("n_groups", C.c_int32),
+                ("top_groups", C.c_int32), ("group_top", C.c_int32), ("norm_topk", C.c_int32), ("scale", C.c_float)]
+
+
+class I8Mat(C.Structure):
+    _fields_ = [("codes", C.c_void_p), ("scales", C.c_void_p), ("row_stride", C.c_int64), ("mat_stride", C.c_int64),
+                ("scale_stride", C.c_int64), ("n_mats", C.c_int32), ("rows", C.c_int32), ("cols", C.c_int32)]
+
+
 YN_IPC_HANDLE_BYTES = 64
 
 _P = C.c_void_p
@@ -132,6 +142,18 @@ _SIGS = {
     "yn_pairs_combine": (C.c_int, [C.POINTER(Dims), _P, _P, _P, _P, _P, _I, _P, _P]),
     "yn_gather_kperm": (C.c_int, [_P, _P, C.c_int64, _I, _I, _I, _P, _P]),
     "yn_scale_rows": (C.c_int, [_P, _P, C.c_int64, _I, _P, _P]),
+    "yn_route_scored": (C.c_int, [C.POINTER(RouteRuleStruct), _P, _I, C.c_int64, C.c_int64, _P, _P, _P, _P, _P]),
+    "yn_rows_route_logits": (C.c_int, [C.POINTER(Dims), _I, _P, C.POINTER(C.c_void_p)]),
+    "yn_i8_quant_rows": (C.c_int, [_P, _I, C.c_int64, C.c_int64, _I, _P, C.c_int64, _P, _P]),
+    "yn_i8_linear_ws_bytes": (C.c_size_t, [C.c_int64, _I]),
+    "yn_i8_linear": (C.c_int, [C.POINTER(I8Mat), _P, _I, C.c_int64, C.c_int64, _P, _I, C.c_int64, _P, C.c_size_t, _P]),
+    "yn_i8_experts_ws_bytes": (C.c_size_t, [C.c_int64, _I, _I, _I, _I, _I]),
+    "yn_i8_experts": (C.c_int, [C.POINTER(I8Mat), C.POINTER(I8Mat), C.POINTER(I8Mat), _P, _I, C.c_int64, C.c_int64, _P,
+                                _P, _I, _P, C.c_int64, _P, C.c_int64, _P, C.c_size_t, _P]),
+    "yn_i8_error": (C.c_int, [_P, C.POINTER(C.c_int32)]),
+    "yn_logprobs_ws_bytes": (C.c_size_t, [C.c_int64, C.c_int64, _I, _I]),
+    "yn_token_logprobs": (C.c_int, [_P, _I, C.c_int64, C.c_int64, C.c_int64, _P, _I, _P, _P, _P, _P, _P, _P,
+                                    C.c_size_t, _P]),
     "yn_rows_route_shared": (C.c_int, [C.POINTER(Dims), _I, _P, C.POINTER(C.c_void_p), C.POINTER(C.c_void_p)]),
 }
 

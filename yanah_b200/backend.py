@@ -32,6 +32,10 @@ Differences from the MLX backend, all outside the MoE path:
   activations and gates come from the row routing) runs as one more grouped
   GEMM over every row in `moe_finalize`.
 
+With `rule` the layers are routed by a `routing.RouteRule` (scores, a bias on the
+choice, groups) on the same logits; the lookahead probabilities stay softmax
+probabilities, whose order is that of the logits.
+
 Every call is asynchronous on the backend's stream; `fence()` blocks until the
 work that reads pool slots has finished.
 """
@@ -46,6 +50,7 @@ import torch
 from . import _lib
 from .device import DeviceLayer, ExpertArena, Workspace, dims_struct, record_struct, stream_ptr
 from .formats import ExpertLayout, ModelGeometry, RecordSpec
+from .routing import RouteRule, route_scored
 from .synthetic import StackConfig, dense_layer
 
 
@@ -93,8 +98,14 @@ class CudaExpertMemory:
 class CudaMoEBackend:
     supports_lazy_moe = True
 
-    def __init__(self, cfg: StackConfig, device="cuda", lookahead: int = 2, stream: Optional[torch.cuda.Stream] = None):
+    def __init__(self, cfg: StackConfig, device="cuda", lookahead: int = 2, stream: Optional[torch.cuda.Stream] = None,
+                 rule: Optional[RouteRule] = None, choice_bias: Optional[torch.Tensor] = None):
+        if rule is not None and rule.top_k != cfg.top_k:
+            raise ValueError(f"the rule chooses {rule.top_k} experts, the configuration {cfg.top_k}")
+        if choice_bias is not None and rule is None:
+            raise ValueError("choice_bias needs a rule")
         self.cfg = cfg
+        self.rule, self.choice_bias = rule, choice_bias      # choice_bias: (layers, E) fp32
         self.device = torch.device(device)
         self.stream = stream or torch.cuda.current_stream(self.device)
         self.geometry = ModelGeometry(n_layers=cfg.n_layers, n_mtp_layers=0, n_experts=cfg.n_experts,
@@ -199,8 +210,18 @@ class CudaMoEBackend:
                                                 h1.data_ptr(), T, tg, len(targets), self.ws.ptr, self._st()))
         x = self.ws.tensor("x", (T, self.cfg.hidden), torch.bfloat16)
         logits = self.ws.tensor("logits", (T, self.cfg.n_experts), torch.float32)
+        if self.rule is not None:
+            K = self.cfg.top_k
+            self._route_by_rule(layer, logits, (self.ws.tensor("ids", (T, K), torch.int32),
+                                                self.ws.tensor("weights", (T, K), torch.float32)))
         self._pre = {"layer": layer, "T": T, "targets": targets}
         return h1, x, logits
+
+    def _route_by_rule(self, layer: int, logits: torch.Tensor, out) -> None:
+        """Ids and weights of the rule over those of the softmax top-k."""
+        bias = None if self.choice_bias is None else self.choice_bias[layer]
+        with torch.cuda.device(self.device), torch.cuda.stream(self.stream):
+            route_scored(logits, self.rule, bias, out=out)
 
     def _grouped_supported(self, layer: int) -> Optional[str]:
         spec = self.cfg.record_spec(layer)
@@ -232,6 +253,9 @@ class CudaMoEBackend:
         _lib.check(lib.yn_rows_route(C.byref(self.dims), C.byref(self._structs[layer]), h1.data_ptr(), T,
                                      x.data_ptr(), ids.data_ptr(), w.data_ptr(), self._route_ws.data_ptr(),
                                      self._route_ws.numel(), self._st()))
+        if self.rule is not None:
+            from .prefill import route_logits
+            self._route_by_rule(layer, route_logits(self._route_ws, self.dims, T), (ids, w))
         self._pre = {"layer": layer, "T": T, "targets": [], "rows": (ids, w)}
         return h1, x, None
 

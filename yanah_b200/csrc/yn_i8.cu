@@ -1,0 +1,725 @@
+// Rows in 8-bit integers, the products of few rows (dp4a), the grouping and the
+// joining of the experts' products, and the C ABI of all of it. The tensor-core
+// product of many rows is in yn_i8.cuh.
+#include <cuda.h>
+#include <cuda_runtime.h>
+
+#include <algorithm>
+#include <string>
+
+#include "yanah_b200.h"
+#include "yn_common.cuh"
+#include "yn_i8.cuh"
+#include "yn_internal.h"
+
+namespace ynb {
+
+// Element type at run time, where a load is not what a kernel waits for.
+YN_DEV float i8_load(int dt, const void* p, size_t i) {
+  return dt == YN_F32 ? I8In<float>::load(p, i) : dt == YN_BF16 ? I8In<__nv_bfloat16>::load(p, i) : I8In<__half>::load(p, i);
+}
+YN_DEV void i8_store(int dt, void* p, size_t i, float v) {
+  if (dt == YN_F32) reinterpret_cast<float*>(p)[i] = v;
+  else if (dt == YN_BF16) reinterpret_cast<__nv_bfloat16*>(p)[i] = __float2bfloat16_rn(v);
+  else reinterpret_cast<__half*>(p)[i] = __float2half_rn(v);
+}
+
+// ------------------------------------------------------------- row codes
+constexpr int I8_QT = 128;     // threads of a row
+constexpr int I8_QHOLD = 4;    // 8-element pieces a thread keeps in registers between the two steps
+
+// One block per row: the largest magnitude, then the codes. Rows of up to
+// I8_QT * 8 * I8_QHOLD = 4096 elements are read once, longer ones a second time from
+// L2. The codes go to row `to[j]` for each of the `copies` entries of the row's list
+// (or to the row itself): a row's codes are made once for all of its experts.
+template <typename T, bool VEC>
+__global__ void __launch_bounds__(I8_QT) k_i8_quant(const void* x, long long ldx, int K, const int32_t* to, int copies,
+                                                    int8_t* codes, long long ldc, float* scales) {
+  __shared__ uint32_t buf[I8_QT / 32];
+  const size_t row = blockIdx.x, base = row * (size_t)ldx;
+  const int tid = threadIdx.x, n8 = VEC ? K / 8 : 0;
+  float f[I8_QHOLD][8];
+  uint32_t m = 0;
+#pragma unroll
+  for (int i = 0; i < I8_QHOLD; ++i) {
+    const int at = tid + i * I8_QT;
+    if (at < n8) {
+      i8_load8<T>(x, base + 8 * (size_t)at, f[i]);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) m = max(m, i8_abs_bits(f[i][j]));
+    }
+  }
+  for (int at = tid + I8_QHOLD * I8_QT; at < n8; at += I8_QT) {
+    float g[8];
+    i8_load8<T>(x, base + 8 * (size_t)at, g);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) m = max(m, i8_abs_bits(g[j]));
+  }
+  for (int k = 8 * n8 + tid; k < K; k += I8_QT) m = max(m, i8_abs_bits(I8In<T>::load(x, base + k)));
+  const I8Row q(block_max_u32(m, buf));
+  const float scale = q.scale();
+  const int n_to = to ? copies : 1;
+  auto out = [&](int j) -> long long { return to ? to[row * copies + j] : (long long)row; };
+  if (tid < n_to && out(tid) >= 0) scales[out(tid)] = scale;
+  auto put8 = [&](int at, const float (&g)[8]) {
+    const uint2 c = make_uint2(i8_pack4(q.code(g[0]), q.code(g[1]), q.code(g[2]), q.code(g[3])),
+                               i8_pack4(q.code(g[4]), q.code(g[5]), q.code(g[6]), q.code(g[7])));
+    for (int j = 0; j < n_to; ++j) {
+      const long long r = out(j);
+      if (r >= 0) *reinterpret_cast<uint2*>(codes + r * ldc + 8 * at) = c;
+    }
+  };
+#pragma unroll
+  for (int i = 0; i < I8_QHOLD; ++i)
+    if (tid + i * I8_QT < n8) put8(tid + i * I8_QT, f[i]);
+  for (int at = tid + I8_QHOLD * I8_QT; at < n8; at += I8_QT) {
+    float g[8];
+    i8_load8<T>(x, base + 8 * (size_t)at, g);
+    put8(at, g);
+  }
+  for (int k = 8 * n8 + tid; k < K; k += I8_QT) {
+    const int8_t c = (int8_t)q.code(I8In<T>::load(x, base + k));
+    for (int j = 0; j < n_to; ++j)
+      if (out(j) >= 0) codes[out(j) * ldc + k] = c;
+  }
+}
+
+int launch_quant(int dt, const void* x, long long ldx, long long rows, int K, const int32_t* to, int copies,
+                 int8_t* codes, long long ldc, float* scales, cudaStream_t st) {
+  const size_t size = dt == YN_F32 ? 4 : 2;
+  const bool vec = reinterpret_cast<uintptr_t>(x) % 16 == 0 && (ldx * size) % 16 == 0 &&
+                   reinterpret_cast<uintptr_t>(codes) % 8 == 0 && ldc % 8 == 0;
+  const dim3 g((unsigned)rows), b(I8_QT);
+#define YN_Q(T)                                                                                            \
+  if (vec) k_i8_quant<T, true><<<g, b, 0, st>>>(x, ldx, K, to, copies, codes, ldc, scales);               \
+  else k_i8_quant<T, false><<<g, b, 0, st>>>(x, ldx, K, to, copies, codes, ldc, scales)
+  if (dt == YN_F32) { YN_Q(float); }
+  else if (dt == YN_BF16) { YN_Q(__nv_bfloat16); }
+  else { YN_Q(__half); }
+#undef YN_Q
+  const cudaError_t e = cudaGetLastError();
+  return e == cudaSuccess ? YN_OK : host_fail(YN_E_CUDA, std::string("row codes: ") + cudaGetErrorString(e));
+}
+
+// ------------------------------------------------- few rows: dp4a products
+constexpr int I8_GT = 256;           // threads
+constexpr int I8_GW = I8_GT / 32;
+constexpr int I8_GK = 512;           // codes of K that a warp takes in one step, 16 per lane
+
+YN_DEV int dot16(const uint4& a, const uint4& b, int acc) {
+  acc = __dp4a((int)a.x, (int)b.x, acc);
+  acc = __dp4a((int)a.y, (int)b.y, acc);
+  acc = __dp4a((int)a.z, (int)b.z, acc);
+  return __dp4a((int)a.w, (int)b.w, acc);
+}
+
+// 16 codes from column `off` of a row of K (off < K), zero past its end.
+YN_DEV uint4 i8_codes16(const int8_t* row, int off, int K) {
+  if (off + 16 <= K) return ldg_nc_v4(row + off);
+  uint32_t w[4] = {0, 0, 0, 0};
+  for (int i = 0; off + i < K; ++i) w[i >> 2] |= (uint32_t)(uint8_t)row[off + i] << (8 * (i & 3));
+  return make_uint4(w[0], w[1], w[2], w[3]);
+}
+
+// Codes and scale of one row of K elements into shared memory by `n` threads (the
+// whole block, or one warp), zero up to KP.
+template <bool BLOCK>
+YN_DEV void i8_row_smem(int dt, const void* x, size_t base, int K, int KP, int8_t* codes, float* scale, uint32_t* buf) {
+  const int at = BLOCK ? threadIdx.x : threadIdx.x & 31, n = BLOCK ? (int)blockDim.x : 32;
+  uint32_t m = 0;
+  for (int k = at; k < K; k += n) m = max(m, i8_abs_bits(i8_load(dt, x, base + k)));
+  if (BLOCK) m = block_max_u32(m, buf);
+  else m = __reduce_max_sync(0xffffffffu, m);
+  const I8Row q(m);
+  if (at == 0) *scale = q.scale();
+  for (int k = 4 * at; k < KP; k += 4 * n) {
+    int c[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) c[i] = k + i < K ? q.code(i8_load(dt, x, base + k + i)) : 0;
+    *reinterpret_cast<uint32_t*>(codes + k) = i8_pack4(c[0], c[1], c[2], c[3]);
+  }
+}
+
+struct I8Mat {
+  const int8_t* codes;
+  const float* scales;
+  long long row_stride, mat_stride, scale_stride;
+};
+
+// R rows of codes (row pointers) times T rows in shared memory: per-lane sums, then the
+// whole dot product on every lane.
+template <int R, int T, int U>
+YN_DEV void i8_dots(const int8_t* const (&w)[R], const int8_t* xs, int KP, int K, int lane, int (&acc)[R][T]) {
+#pragma unroll
+  for (int r = 0; r < R; ++r)
+#pragma unroll
+    for (int t = 0; t < T; ++t) acc[r][t] = 0;
+  for (int k0 = 0; k0 < K; k0 += U * I8_GK) {
+    uint4 a[U][R];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int off = k0 + u * I8_GK + 16 * lane;
+#pragma unroll
+      for (int r = 0; r < R; ++r) a[u][r] = off < K ? i8_codes16(w[r], off, K) : make_uint4(0, 0, 0, 0);
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int off = k0 + u * I8_GK + 16 * lane;
+      if (off < K) {
+#pragma unroll
+        for (int t = 0; t < T; ++t) {
+          const uint4 x = *reinterpret_cast<const uint4*>(xs + t * KP + off);
+#pragma unroll
+          for (int r = 0; r < R; ++r) acc[r][t] = dot16(a[u][r], x, acc[r][t]);
+        }
+      }
+    }
+  }
+#pragma unroll
+  for (int r = 0; r < R; ++r)
+#pragma unroll
+    for (int t = 0; t < T; ++t) acc[r][t] = __reduce_add_sync(0xffffffffu, acc[r][t]);
+}
+
+// y (T, N) of T <= 8 rows: every block makes the rows' codes itself (they are a few KB),
+// then its warps take 4 output channels at a time through the matrix, which is read once:
+// bound by that read.
+template <int T>
+__global__ void __launch_bounds__(I8_GT) k_i8_few(int dt, const void* x, long long ldx, int K, int KP, const I8Mat w,
+                                                  int N, int odt, void* y, long long ldy) {
+  extern __shared__ __align__(16) int8_t xs[];
+  __shared__ float sx[T];
+  __shared__ uint32_t buf[I8_GW];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  if (T == 1) i8_row_smem<true>(dt, x, 0, K, KP, xs, sx, buf);
+  else if (warp < T) i8_row_smem<false>(dt, x, (size_t)warp * ldx, K, KP, xs + warp * KP, sx + warp, buf);
+  __syncthreads();
+  constexpr int R = 4;
+  for (long long n0 = ((long long)blockIdx.x * I8_GW + warp) * R; n0 < N; n0 += (long long)gridDim.x * I8_GW * R) {
+    const int8_t* rows[R];
+#pragma unroll
+    for (int r = 0; r < R; ++r) rows[r] = w.codes + (n0 + r < N ? n0 + r : (long long)N - 1) * w.row_stride;
+    int acc[R][T];
+    i8_dots<R, T, 2>(rows, xs, KP, K, lane, acc);
+#pragma unroll
+    for (int r = 0; r < R; ++r)
+#pragma unroll
+      for (int t = 0; t < T; ++t)
+        if (lane == r * T + t && n0 + r < N)
+          i8_store(odt, y, (size_t)t * ldy + n0 + r, (float)acc[r][t] * sx[t] * w.scales[n0 + r]);
+  }
+}
+
+// Few (row, expert) pairs: gate and up of 2 units per warp, the pair's row codes made by
+// every block, SwiGLU in fp32 to act (pairs, I).
+__global__ void __launch_bounds__(I8_GT) k_i8_up_few(int dt, const void* x, long long ldx, int H, int HP, const int32_t* ids,
+                                                     int k, int E, const I8Mat gate, const I8Mat up, int I, float* act) {
+  extern __shared__ __align__(16) int8_t xs[];
+  __shared__ float sx;
+  __shared__ uint32_t buf[I8_GW];
+  const int p = blockIdx.y, e = ids[p], warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  if (e < 0 || e >= E) {
+    if (e != -1 && threadIdx.x == 0 && blockIdx.x == 0) raise_error(&g_i8_err, YN_ERR_BAD_EXPERT);
+    return;
+  }
+  i8_row_smem<true>(dt, x, (size_t)(p / k) * ldx, H, HP, xs, &sx, buf);
+  __syncthreads();
+  const int u0 = 2 * (blockIdx.x * I8_GW + warp);
+  if (u0 >= I) return;
+  const int u1 = u0 + 1 < I ? u0 + 1 : u0;
+  const int8_t* g = gate.codes + e * gate.mat_stride;
+  const int8_t* v = up.codes + e * up.mat_stride;
+  const int8_t* rows[4] = {g + u0 * gate.row_stride, v + u0 * up.row_stride, g + u1 * gate.row_stride,
+                           v + u1 * up.row_stride};
+  int acc[4][1];
+  i8_dots<4, 1, 2>(rows, xs, HP, H, lane, acc);
+  if (lane < 2 && u0 + lane < I) {
+    const int u = u0 + lane;
+    const float gv = (float)(lane ? acc[2][0] : acc[0][0]) * sx * gate.scales[e * gate.scale_stride + u];
+    const float uv = (float)(lane ? acc[3][0] : acc[1][0]) * sx * up.scales[e * up.scale_stride + u];
+    act[(size_t)p * I + u] = i8_swiglu(gv, uv);
+  }
+}
+
+// The down products of a row's experts and their weighted sum: a block makes the codes of
+// the row's k activations, its warps take 2 outputs each through all k experts.
+__global__ void __launch_bounds__(I8_GT) k_i8_down_few(const float* act, int I, int IP, const int32_t* ids, const float* wts,
+                                                       int k, int E, const I8Mat down, int H, int odt, const void* res,
+                                                       long long ldr, void* out, long long ldo) {
+  extern __shared__ __align__(16) int8_t as[];
+  __shared__ float sa[32];
+  const int t = blockIdx.y, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  for (int j = warp; j < k; j += I8_GW) {
+    const int e = ids[(size_t)t * k + j];
+    if (e >= 0 && e < E)
+      i8_row_smem<false>(YN_F32, act, ((size_t)t * k + j) * I, I, IP, as + j * IP, sa + j, nullptr);
+  }
+  __syncthreads();
+  const int h0 = 2 * (blockIdx.x * I8_GW + warp);
+  if (h0 >= H) return;
+  const int h1 = h0 + 1 < H ? h0 + 1 : h0;
+  float sum = 0.0f;   // of output h0 + (lane & 1)
+  for (int j = 0; j < k; ++j) {
+    const int e = ids[(size_t)t * k + j];
+    if (e < 0 || e >= E) continue;
+    const int8_t* d = down.codes + e * down.mat_stride;
+    const int8_t* rows[2] = {d + h0 * down.row_stride, d + h1 * down.row_stride};
+    int acc[2][1];
+    i8_dots<2, 1, 1>(rows, as + j * IP, IP, I, lane, acc);
+    const int h = lane & 1 ? h1 : h0;
+    sum = fmaf(wts[(size_t)t * k + j],
+               (float)(lane & 1 ? acc[1][0] : acc[0][0]) * sa[j] * down.scales[e * down.scale_stride + h], sum);
+  }
+  if (lane < 2 && h0 + lane < H) {
+    const size_t h = h0 + lane;
+    i8_store(odt, out, (size_t)t * ldo + h, (res ? i8_load(odt, res, (size_t)t * ldr + h) : 0.0f) + sum);
+  }
+}
+
+// --------------------------------------------- many rows: grouping, joining
+constexpr int I8_PLAN_T = 1024;
+constexpr int I8_MAX_E = 1024;
+
+// Pairs of one expert made contiguous and cut into chunks of at most NB rows. Which place
+// a pair takes inside its expert does not change its product. pair_of: (row, column) ->
+// pair, -1 where there is no expert. n_out[0] = chunks, [1] = pairs.
+__global__ void __launch_bounds__(I8_PLAN_T) k_i8_plan(const int32_t* ids, int P, int E, int NB, int32_t* pair_of,
+                                                       I8Chunk* chunks, int* n_out) {
+  __shared__ int cnt[I8_MAX_E], first[I8_MAX_E];
+  __shared__ int2 ws[I8_PLAN_T / 32];
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  for (int e = tid; e < I8_MAX_E; e += I8_PLAN_T) cnt[e] = 0;
+  __syncthreads();
+  for (int i = tid; i < P; i += I8_PLAN_T) {
+    const int e = ids[i];
+    if (e >= 0 && e < E) pair_of[i] = atomicAdd(&cnt[e], 1);
+    else {
+      pair_of[i] = -1;
+      if (e != -1) raise_error(&g_i8_err, YN_ERR_BAD_EXPERT);
+    }
+  }
+  __syncthreads();
+  const int c = tid < E ? cnt[tid] : 0, nc = (c + NB - 1) / NB;
+  int2 inc = make_int2(c, nc);
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int a = __shfl_up_sync(0xffffffffu, inc.x, o), b = __shfl_up_sync(0xffffffffu, inc.y, o);
+    if (lane >= o) { inc.x += a; inc.y += b; }
+  }
+  if (lane == 31) ws[warp] = inc;
+  __syncthreads();
+  int2 base = make_int2(0, 0), all = make_int2(0, 0);
+  for (int w = 0; w < I8_PLAN_T / 32; ++w) {
+    const int2 q = ws[w];
+    if (w < warp) { base.x += q.x; base.y += q.y; }
+    all.x += q.x;
+    all.y += q.y;
+  }
+  const int start = base.x + inc.x - c, at = base.y + inc.y - nc;
+  if (tid < E) {
+    first[tid] = start;
+    for (int i = 0; i < nc; ++i) chunks[at + i] = I8Chunk{tid, start + i * NB, min(NB, c - i * NB)};
+  }
+  if (tid == 0) {
+    n_out[0] = all.y;
+    n_out[1] = all.x;
+  }
+  __syncthreads();
+  for (int i = tid; i < P; i += I8_PLAN_T)
+    if (pair_of[i] >= 0) pair_of[i] += first[ids[i]];
+}
+
+// The activations' 8-bit codes: one warp per pair, from 16-bit values relative to the
+// largest of each 32 units (the pair's largest is the largest of those).
+__global__ void __launch_bounds__(256) k_i8_act_codes(const int16_t* act, long long lda, const float* bscale, int nb, int I,
+                                                      const int* n_pairs, int8_t* codes, long long ldc, float* scales) {
+  const int lane = threadIdx.x & 31;
+  const long long p = (long long)blockIdx.x * 8 + (threadIdx.x >> 5);
+  if (p >= *n_pairs) return;
+  const float* bs = bscale + p * nb;
+  uint32_t m = 0;
+  for (int b = lane; b < nb; b += 32) m = max(m, __float_as_uint(bs[b]));
+  const I8Row q(__reduce_max_sync(0xffffffffu, m));
+  if (lane == 0) scales[p] = q.scale();
+  const int16_t* a = act + p * lda;
+  for (int u = 8 * lane; u < I; u += 256) {   // lda and ldc are whole 16-byte pieces of 8 values
+    const uint4 v = *reinterpret_cast<const uint4*>(a + u);
+    const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+    const float s = bs[u >> 5] * (1.0f / 32767.0f);
+    int c[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) c[i] = q.code((float)(int16_t)(w[i >> 1] >> (16 * (i & 1))) * s);
+    *reinterpret_cast<uint2*>(codes + p * ldc + u) = make_uint2(i8_pack4(c[0], c[1], c[2], c[3]), i8_pack4(c[4], c[5], c[6], c[7]));
+  }
+}
+
+// out[t] = residual[t] + sum_j w_j y[pair_of[t][j]] in fp32, columns in order, rounded once.
+template <typename O, typename Y>
+__global__ void k_i8_combine(const Y* y, long long ldy, const int32_t* pair_of, const float* w, int k, int H,
+                             const void* res, long long ldr, void* out, long long ldo) {
+  const size_t t = blockIdx.y;
+  const int h = 4 * (blockIdx.x * blockDim.x + threadIdx.x);
+  if (h >= H) return;
+  float acc[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+  for (int j = 0; j < k; ++j) {
+    const int p = pair_of[t * k + j];
+    if (p < 0) continue;
+    const float wj = w[t * k + j];
+    const Y* row = y + (size_t)p * ldy + h;   // rows of y are padded to whole vectors
+    float v[4];
+    if constexpr (sizeof(Y) == 4) {
+      const float4 q = *reinterpret_cast<const float4*>(row);
+      v[0] = q.x; v[1] = q.y; v[2] = q.z; v[3] = q.w;
+    } else {
+      const uint2 q = *reinterpret_cast<const uint2*>(row);
+      v[0] = bf16_to_f32((uint16_t)(q.x & 0xFFFFu)); v[1] = bf16_to_f32((uint16_t)(q.x >> 16));
+      v[2] = bf16_to_f32((uint16_t)(q.y & 0xFFFFu)); v[3] = bf16_to_f32((uint16_t)(q.y >> 16));
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) acc[i] = fmaf(wj, v[i], acc[i]);
+  }
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+    if (h + i < H) {
+      const float r = res ? I8In<O>::load(res, t * ldr + h + i) : 0.0f;
+      reinterpret_cast<O*>(out)[t * ldo + h + i] = i8_out<O>(r + acc[i]);
+    }
+}
+
+// ---------------------------------------------------------------- host side
+size_t up_to(size_t v, size_t m) { return (v + m - 1) / m * m; }
+
+int tmap_2d(CUtensorMap* m, const void* base, long long cols, long long rows, long long stride, int box_rows) {
+  TmapEncode fn;
+  int rc = host_tmap_encode(&fn);
+  if (rc) return rc;
+  const cuuint64_t dims[2] = {(cuuint64_t)cols, (cuuint64_t)rows}, strides[1] = {(cuuint64_t)stride};
+  const cuuint32_t box[2] = {128u, (cuuint32_t)box_rows}, one[2] = {1u, 1u};
+  const CUresult r = fn(m, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void*>(base), dims, strides, box, one,
+                        CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                        CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  return r == CUDA_SUCCESS ? YN_OK : host_fail(YN_E_CUDA, "cuTensorMapEncodeTiled failed: " + std::to_string((int)r));
+}
+int tmap_mats(CUtensorMap* m, const yn_i8_mat& w) {
+  TmapEncode fn;
+  int rc = host_tmap_encode(&fn);
+  if (rc) return rc;
+  const cuuint64_t dims[3] = {(cuuint64_t)w.cols, (cuuint64_t)w.rows, (cuuint64_t)w.n_mats};
+  const cuuint64_t strides[2] = {(cuuint64_t)w.row_stride,
+                                 (cuuint64_t)(w.n_mats > 1 ? w.mat_stride : w.row_stride * (int64_t)w.rows)};
+  const cuuint32_t box[3] = {128u, 128u, 1u}, one[3] = {1u, 1u, 1u};
+  const CUresult r = fn(m, CU_TENSOR_MAP_DATA_TYPE_UINT8, 3, const_cast<void*>(w.codes), dims, strides, box, one,
+                        CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                        CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  return r == CUDA_SUCCESS ? YN_OK : host_fail(YN_E_CUDA, "cuTensorMapEncodeTiled failed: " + std::to_string((int)r));
+}
+
+int sm_count(int* out) {
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e == cudaSuccess) e = cudaDeviceGetAttribute(out, cudaDevAttrMultiProcessorCount, dev);
+  return e == cudaSuccess ? YN_OK : host_fail(YN_E_CUDA, std::string("device attributes: ") + cudaGetErrorString(e));
+}
+
+template <typename O, bool UP, int NB>
+int launch_gemm(const I8Gemm& a, const I8Maps& maps, long long max_tiles, cudaStream_t st) {
+  const void* kern = reinterpret_cast<const void*>(k_i8_gemm<O, UP, NB>);
+  int rc = host_set_smem(kern, I8Cfg<UP, NB>::SMEM), sms = 0;
+  if (rc || (rc = sm_count(&sms))) return rc;
+  const unsigned grid = (unsigned)std::max<long long>(1, std::min<long long>(max_tiles, sms));
+  k_i8_gemm<O, UP, NB><<<grid, I8_THREADS, I8Cfg<UP, NB>::SMEM, st>>>(a, maps);
+  const cudaError_t e = cudaGetLastError();
+  return e == cudaSuccess ? YN_OK : host_fail(YN_E_CUDA, std::string("8-bit product: ") + cudaGetErrorString(e));
+}
+template <typename O>
+int launch_gemm_nb(int nb, const I8Gemm& a, const I8Maps& maps, long long max_tiles, cudaStream_t st) {
+  if (nb <= 32) return launch_gemm<O, false, 32>(a, maps, max_tiles, st);
+  if (nb <= 64) return launch_gemm<O, false, 64>(a, maps, max_tiles, st);
+  if (nb <= 128) return launch_gemm<O, false, 128>(a, maps, max_tiles, st);
+  return launch_gemm<O, false, 256>(a, maps, max_tiles, st);
+}
+int launch_gemm_out(int odt, int nb, const I8Gemm& a, const I8Maps& maps, long long max_tiles, cudaStream_t st) {
+  if (odt == YN_F32) return launch_gemm_nb<float>(nb, a, maps, max_tiles, st);
+  if (odt == YN_BF16) return launch_gemm_nb<__nv_bfloat16>(nb, a, maps, max_tiles, st);
+  return launch_gemm_nb<__half>(nb, a, maps, max_tiles, st);
+}
+int box_rows(int nb) { return nb <= 32 ? 32 : nb <= 64 ? 64 : nb <= 128 ? 128 : 256; }
+
+bool dtype_ok(int dt) { return dt == YN_F32 || dt == YN_BF16 || dt == YN_F16; }
+int dtype_size(int dt) { return dt == YN_F32 ? 4 : 2; }
+I8Mat mat_of(const yn_i8_mat& w) {
+  return I8Mat{reinterpret_cast<const int8_t*>(w.codes), w.scales, w.row_stride, w.mat_stride, w.scale_stride};
+}
+
+constexpr int I8_MAX_K = 131072;   // 127^2 * 131072 < 2^31
+constexpr int I8_FEW = 8;          // rows of a product on dp4a
+
+int check_mat(const yn_i8_mat& w, const char* what) {
+  const std::string n(what);
+  if (!w.codes || !w.scales) return host_fail(YN_E_INVALID, n + ": null pointer");
+  if (w.n_mats < 1 || w.rows < 1 || w.cols < 1) return host_fail(YN_E_INVALID, n + ": empty matrix");
+  if (w.cols > I8_MAX_K) return host_fail(YN_E_UNSUPPORTED, n + ": at most 131072 columns (32-bit sums)");
+  if (reinterpret_cast<uintptr_t>(w.codes) % 16 || w.row_stride % 16 || (w.n_mats > 1 && w.mat_stride % 16))
+    return host_fail(YN_E_INVALID, n + ": rows of codes must start at multiples of 16 bytes");
+  if (w.row_stride < w.cols || (w.n_mats > 1 && (w.mat_stride < 1 || w.scale_stride < w.rows)))
+    return host_fail(YN_E_INVALID, n + ": rows or matrices overlap");
+  if (w.row_stride >= (1ll << 40) || w.mat_stride >= (1ll << 40)) return host_fail(YN_E_UNSUPPORTED, n + ": stride above 2^40");
+  return YN_OK;
+}
+
+bool linear_few(long long rows, long long k) { return rows <= I8_FEW && rows * (long long)up_to(k, I8_GK) <= 96 * 1024; }
+
+template <int T>
+int launch_few(int dt, const void* x, long long ldx, int K, const I8Mat& w, int N, int odt, void* y, long long ldy, int sms,
+               cudaStream_t st) {
+  const int KP = (int)up_to(K, I8_GK);
+  const size_t smem = (size_t)T * KP;
+  int rc = host_set_smem(reinterpret_cast<const void*>(k_i8_few<T>), 96 * 1024);
+  if (rc) return rc;
+  const int grid = std::min((N + 4 * I8_GW - 1) / (4 * I8_GW), 3 * sms);
+  k_i8_few<T><<<grid, I8_GT, smem, st>>>(dt, x, ldx, K, KP, w, N, odt, y, ldy);
+  const cudaError_t e = cudaGetLastError();
+  return e == cudaSuccess ? YN_OK : host_fail(YN_E_CUDA, std::string("8-bit product: ") + cudaGetErrorString(e));
+}
+
+// Workspace of the experts' products.
+struct ExpertsWs {
+  size_t n_out, pair_of, chunks, codes, sx, act, bscale, acodes, sa, y, total;
+  long long ldc, lda, ldac, ldy;
+  int nb;
+};
+// Rows per chunk: enough for the mean expert. Small tiles read an expert's weights once per
+// tile (from L2 after the first) but multiply fewer absent rows.
+int chunk_rows(long long pairs, int E) {
+  const long long mean = pairs / std::max(1, E);
+  return mean <= 16 ? 32 : mean <= 48 ? 64 : 128;
+}
+bool experts_few(long long pairs, int k, int H, int I) {
+  return pairs <= 40 && up_to(H, I8_GK) <= 96 * 1024 && k * up_to(I, I8_GK) <= 96 * 1024;
+}
+
+ExpertsWs experts_ws(long long rows, int k, int E, int H, int I, int odt) {
+  ExpertsWs L{};
+  size_t o = 0;
+  auto take = [&](size_t b) { const size_t at = o; o = up_to(o + b, 256); return at; };
+  const size_t P = (size_t)rows * k;
+  if (experts_few((long long)P, k, H, I)) {
+    L.act = take(P * I * 4);
+    L.total = o;
+    return L;
+  }
+  L.nb = chunk_rows((long long)P, E);
+  L.ldc = (long long)up_to(H, 16);
+  L.lda = (long long)up_to(I, 16);
+  L.ldac = (long long)up_to(I, 16);
+  L.ldy = (long long)up_to(H, 16);
+  L.n_out = take(8);
+  L.pair_of = take(P * 4);
+  L.chunks = take((E + P / L.nb + 1) * sizeof(I8Chunk));
+  L.codes = take(P * L.ldc);
+  L.sx = take(P * 4);
+  L.act = take(P * L.lda * 2);
+  L.bscale = take(P * (up_to(I, 32) / 32) * 4);
+  L.acodes = take(P * L.ldac);
+  L.sa = take(P * 4);
+  L.y = take(P * L.ldy * (odt == YN_BF16 ? 2 : 4));
+  L.total = o;
+  return L;
+}
+
+}  // namespace ynb
+
+using namespace ynb;
+
+extern "C" int yn_i8_quant_rows(const void* x, int32_t dtype, int64_t row_stride, int64_t rows, int32_t cols, void* codes,
+                                int64_t code_stride, float* scales, void* stream) {
+  if (!dtype_ok(dtype)) return host_fail(YN_E_INVALID, "unknown dtype");
+  if (rows < 0 || rows > 0x7fffffffLL || cols < 1 || row_stride < cols || code_stride < cols)
+    return host_fail(YN_E_INVALID, "rows must be in [0, 2^31), strides at least cols, cols at least 1");
+  if (rows == 0) return YN_OK;
+  if (!x || !codes || !scales) return host_fail(YN_E_INVALID, "null argument");
+  if (reinterpret_cast<uintptr_t>(x) % dtype_size(dtype)) return host_fail(YN_E_INVALID, "x must be aligned to its element");
+  return launch_quant(dtype, x, row_stride, rows, cols, nullptr, 1, reinterpret_cast<int8_t*>(codes), code_stride, scales,
+                      reinterpret_cast<cudaStream_t>(stream));
+}
+
+extern "C" size_t yn_i8_linear_ws_bytes(int64_t rows, int32_t cols) {
+  if (rows < 1 || cols < 1 || linear_few(rows, cols)) return 0;
+  return up_to((size_t)rows * up_to(cols, 16), 256) + (size_t)rows * 4;
+}
+
+extern "C" int yn_i8_linear(const yn_i8_mat* w, const void* x, int32_t dtype, int64_t x_stride, int64_t rows, void* y,
+                            int32_t y_dtype, int64_t y_stride, void* ws, size_t ws_bytes, void* stream) {
+  if (!w) return host_fail(YN_E_INVALID, "null argument");
+  int rc = check_mat(*w, "matrix");
+  if (rc) return rc;
+  if (w->n_mats != 1) return host_fail(YN_E_INVALID, "one matrix");
+  if (!dtype_ok(dtype) || !dtype_ok(y_dtype)) return host_fail(YN_E_INVALID, "unknown dtype");
+  if (rows < 0 || rows > 0x7fffff00LL || x_stride < w->cols || y_stride < w->rows)
+    return host_fail(YN_E_INVALID, "rows must be in [0, 2^31 - 256), strides at least the row lengths");
+  if (rows == 0) return YN_OK;
+  if (!x || !y) return host_fail(YN_E_INVALID, "null argument");
+  if (reinterpret_cast<uintptr_t>(x) % dtype_size(dtype) || reinterpret_cast<uintptr_t>(y) % dtype_size(y_dtype))
+    return host_fail(YN_E_INVALID, "x and y must be aligned to their elements");
+  cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
+  if (linear_few(rows, w->cols)) {
+    const I8Mat m = mat_of(*w);
+    int sms = 0;
+    if ((rc = sm_count(&sms))) return rc;
+#define YN_FEW(T) \
+  case T: return launch_few<T>(dtype, x, x_stride, w->cols, m, w->rows, y_dtype, y, y_stride, sms, st)
+    switch ((int)rows) {
+      YN_FEW(1);
+      YN_FEW(2);
+      YN_FEW(3);
+      YN_FEW(4);
+      YN_FEW(5);
+      YN_FEW(6);
+      YN_FEW(7);
+      YN_FEW(8);
+    }
+#undef YN_FEW
+  }
+  if (!ws || reinterpret_cast<uintptr_t>(ws) % 256 || ws_bytes < yn_i8_linear_ws_bytes(rows, w->cols))
+    return host_fail(YN_E_INVALID, "workspace too small or not 256-byte aligned");
+  int8_t* codes = reinterpret_cast<int8_t*>(ws);
+  const long long ldc = (long long)up_to(w->cols, 16);
+  float* sx = reinterpret_cast<float*>(codes + up_to((size_t)rows * ldc, 256));
+  if ((rc = launch_quant(dtype, x, x_stride, rows, w->cols, nullptr, 1, codes, ldc, sx, st))) return rc;
+  I8Gemm a{};
+  a.rows = (int)rows;
+  a.channels = w->rows;
+  a.K = w->cols;
+  a.sx = sx;
+  a.sw = w->scales;
+  a.y = y;
+  a.y_stride = y_stride;
+  const int nb = box_rows((int)std::min<int64_t>(rows, 256));
+  I8Maps maps{};
+  if ((rc = tmap_mats(&maps.a, *w)) || (rc = tmap_2d(&maps.b, codes, w->cols, rows, ldc, nb))) return rc;
+  const long long tiles = (long long)((rows + nb - 1) / nb) * ((w->rows + 127) / 128);
+  return launch_gemm_out(y_dtype, nb, a, maps, tiles, st);
+}
+
+extern "C" size_t yn_i8_experts_ws_bytes(int64_t rows, int32_t top_k, int32_t n_experts, int32_t hidden, int32_t inter,
+                                         int32_t dtype) {
+  if (rows < 1 || top_k < 1 || n_experts < 1 || hidden < 1 || inter < 1 || !dtype_ok(dtype)) return 0;
+  return experts_ws(rows, top_k, n_experts, hidden, inter, dtype).total;
+}
+
+extern "C" int yn_i8_experts(const yn_i8_mat* gate, const yn_i8_mat* up, const yn_i8_mat* down, const void* x, int32_t dtype,
+                             int64_t x_stride, int64_t rows, const int32_t* ids, const float* weights, int32_t top_k,
+                             const void* residual, int64_t res_stride, void* out, int64_t out_stride, void* ws,
+                             size_t ws_bytes, void* stream) {
+  if (!gate || !up || !down) return host_fail(YN_E_INVALID, "null argument");
+  int rc = check_mat(*gate, "gate");
+  if (rc || (rc = check_mat(*up, "up")) || (rc = check_mat(*down, "down"))) return rc;
+  const int E = gate->n_mats, H = gate->cols, I = gate->rows;
+  if (up->n_mats != E || up->rows != I || up->cols != H || down->n_mats != E || down->rows != H || down->cols != I)
+    return host_fail(YN_E_INVALID, "gate and up are (E, I, H), down is (E, H, I)");
+  if (E > I8_MAX_E || top_k < 1 || top_k > 32) return host_fail(YN_E_UNSUPPORTED, "at most 1024 experts, top_k in [1, 32]");
+  if (!dtype_ok(dtype)) return host_fail(YN_E_INVALID, "unknown dtype");
+  if (rows < 0 || rows * top_k > (1 << 22) || x_stride < H || out_stride < H || (residual && res_stride < H))
+    return host_fail(YN_E_INVALID, "rows * top_k must be in [0, 2^22], strides at least hidden");
+  if (rows == 0) return YN_OK;
+  if (!x || !ids || !weights || !out || !ws) return host_fail(YN_E_INVALID, "null argument");
+  const int size = dtype_size(dtype);
+  if (reinterpret_cast<uintptr_t>(x) % size || reinterpret_cast<uintptr_t>(out) % size ||
+      (residual && reinterpret_cast<uintptr_t>(residual) % size))
+    return host_fail(YN_E_INVALID, "rows must be aligned to their element");
+  const ExpertsWs L = experts_ws(rows, top_k, E, H, I, dtype);
+  if (ws_bytes < L.total || reinterpret_cast<uintptr_t>(ws) % 256)
+    return host_fail(YN_E_INVALID, "workspace too small or not 256-byte aligned");
+  uint8_t* b = reinterpret_cast<uint8_t*>(ws);
+  cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
+  const int P = (int)(rows * top_k);
+  const I8Mat mg = mat_of(*gate), mu = mat_of(*up), md = mat_of(*down);
+  if (experts_few(P, top_k, H, I)) {
+    float* act = reinterpret_cast<float*>(b + L.act);
+    const int HP = (int)up_to(H, I8_GK), IP = (int)up_to(I, I8_GK);
+    if ((rc = host_set_smem(reinterpret_cast<const void*>(k_i8_up_few), 96 * 1024)) ||
+        (rc = host_set_smem(reinterpret_cast<const void*>(k_i8_down_few), 96 * 1024)))
+      return rc;
+    k_i8_up_few<<<dim3((I + 2 * I8_GW - 1) / (2 * I8_GW), P), I8_GT, HP, st>>>(dtype, x, x_stride, H, HP, ids, top_k, E, mg, mu,
+                                                                             I, act);
+    k_i8_down_few<<<dim3((H + 2 * I8_GW - 1) / (2 * I8_GW), (unsigned)rows), I8_GT, (size_t)top_k * IP, st>>>(
+        act, I, IP, ids, weights, top_k, E, md, H, dtype, residual, res_stride, out, out_stride);
+    const cudaError_t e = cudaGetLastError();
+    return e == cudaSuccess ? YN_OK : host_fail(YN_E_CUDA, std::string("experts: ") + cudaGetErrorString(e));
+  }
+  int* n_out = reinterpret_cast<int*>(b + L.n_out);
+  int32_t* pair_of = reinterpret_cast<int32_t*>(b + L.pair_of);
+  I8Chunk* chunks = reinterpret_cast<I8Chunk*>(b + L.chunks);
+  int8_t* codes = reinterpret_cast<int8_t*>(b + L.codes);
+  float* sx = reinterpret_cast<float*>(b + L.sx);
+  int16_t* act = reinterpret_cast<int16_t*>(b + L.act);
+  float* bscale = reinterpret_cast<float*>(b + L.bscale);
+  int8_t* acodes = reinterpret_cast<int8_t*>(b + L.acodes);
+  float* sa = reinterpret_cast<float*>(b + L.sa);
+  void* y = b + L.y;
+  k_i8_plan<<<1, I8_PLAN_T, 0, st>>>(ids, P, E, L.nb, pair_of, chunks, n_out);
+  if ((rc = launch_quant(dtype, x, x_stride, rows, H, pair_of, top_k, codes, L.ldc, sx, st))) return rc;
+  const long long max_chunks = E + P / L.nb + 1;
+  I8Maps maps{};
+  if ((rc = tmap_mats(&maps.a, *gate)) || (rc = tmap_mats(&maps.a_up, *up)) || (rc = tmap_2d(&maps.b, codes, H, P, L.ldc, L.nb)))
+    return rc;
+  I8Gemm g{};
+  g.chunks = chunks;
+  g.n_chunks = n_out;
+  g.rows = P;
+  g.channels = I;
+  g.K = H;
+  g.sx = sx;
+  g.sw = gate->scales;
+  g.sw_up = up->scales;
+  g.sw_stride = gate->scale_stride;
+  g.sw_up_stride = up->scale_stride;
+  g.y = act;
+  g.y_stride = L.lda;
+  g.bscale = bscale;
+  const long long tu = max_chunks * ((I + 127) / 128), td = max_chunks * ((H + 127) / 128);
+  rc = L.nb == 32   ? launch_gemm<float, true, 32>(g, maps, tu, st)
+       : L.nb == 64 ? launch_gemm<float, true, 64>(g, maps, tu, st)
+                    : launch_gemm<float, true, 128>(g, maps, tu, st);
+  if (rc) return rc;
+  const int nbk = (int)up_to(I, 32) / 32;
+  k_i8_act_codes<<<(P + 7) / 8, 256, 0, st>>>(act, L.lda, bscale, nbk, I, n_out + 1, acodes, L.ldac, sa);
+  I8Maps md2{};
+  if ((rc = tmap_mats(&md2.a, *down)) || (rc = tmap_2d(&md2.b, acodes, I, P, L.ldac, L.nb))) return rc;
+  I8Gemm d{};
+  d.chunks = chunks;
+  d.n_chunks = n_out;
+  d.rows = P;
+  d.channels = H;
+  d.K = I;
+  d.sx = sa;
+  d.sw = down->scales;
+  d.sw_stride = down->scale_stride;
+  d.y = y;
+  d.y_stride = L.ldy;
+  const bool yb = dtype == YN_BF16;
+  if ((rc = launch_gemm_out(yb ? YN_BF16 : YN_F32, L.nb, d, md2, td, st))) return rc;
+  const dim3 cg((H + 4 * 128 - 1) / (4 * 128), (unsigned)rows);
+  if (yb)
+    k_i8_combine<__nv_bfloat16, uint16_t><<<cg, 128, 0, st>>>(reinterpret_cast<const uint16_t*>(y), L.ldy, pair_of, weights,
+                                                              top_k, H, residual, res_stride, out, out_stride);
+  else if (dtype == YN_F16)
+    k_i8_combine<__half, float><<<cg, 128, 0, st>>>(reinterpret_cast<const float*>(y), L.ldy, pair_of, weights, top_k, H,
+                                                    residual, res_stride, out, out_stride);
+  else
+    k_i8_combine<float, float><<<cg, 128, 0, st>>>(reinterpret_cast<const float*>(y), L.ldy, pair_of, weights, top_k, H,
+                                                   residual, res_stride, out, out_stride);
+  const cudaError_t e = cudaGetLastError();
+  return e == cudaSuccess ? YN_OK : host_fail(YN_E_CUDA, std::string("experts: ") + cudaGetErrorString(e));
+}
+
+extern "C" int yn_i8_error(void* stream, int32_t* code_out) {
+  if (!code_out) return host_fail(YN_E_INVALID, "null argument");
+  cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
+  void* p = nullptr;
+  cudaError_t e = cudaGetSymbolAddress(&p, g_i8_err);
+  if (e == cudaSuccess) e = cudaMemcpyAsync(code_out, p, 4, cudaMemcpyDeviceToHost, st);
+  if (e == cudaSuccess) e = cudaMemsetAsync(p, 0, 4, st);
+  if (e == cudaSuccess) e = cudaStreamSynchronize(st);
+  return e == cudaSuccess ? YN_OK : host_fail(YN_E_CUDA, std::string("yn_i8_error: ") + cudaGetErrorString(e));
+}

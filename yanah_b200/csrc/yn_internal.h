@@ -1,5 +1,6 @@
 // Host-side helpers shared by the C-ABI translation units.
 #pragma once
+#include <cuda.h>
 #include <cuda_runtime.h>
 #include <stdint.h>
 
@@ -17,6 +18,12 @@ int host_check_qmat(const yn_qmat& m, int rows, int cols, int bits, const char* 
 
 // Raise a kernel's dynamic shared-memory limit (once per device).
 int host_set_smem(const void* kernel, size_t bytes);
+
+// The driver's cuTensorMapEncodeTiled.
+using TmapEncode = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*,
+                                const cuuint64_t*, const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave,
+                                CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+int host_tmap_encode(TmapEncode* out);
 
 // Output arrays of the post-attention kernel (rows 0..T-1 of each).
 struct PostAttnOut {

@@ -1,0 +1,560 @@
+// Log probabilities of given tokens, their ranks, the rows' entropies and the
+// likeliest alternatives, and their C ABI. No counterpart in the reference, which
+// compares greedy choices of the verify pass (speculative.py:121-193).
+//
+// Per row of logits z with maximum m at token *:  R = sum over the others of
+// exp(z - m), log S = log1p(R), logprob = (z[t] - m) - log S, entropy = log S -
+// sum exp(z - m)(z - m) / S. The sum leaves the largest term out so that log S
+// keeps its relative accuracy when that term has nearly all the mass.
+//
+// Bound by reading the logits once. A block holds a chunk of the row in
+// registers (VPT 16-byte loads per thread, all in flight at once), takes the
+// chunk's maximum first and only then the exponentials, one ex2 per element
+// against a maximum that does not move; chunks (and blocks, where a row is split
+// over several because there are few) are joined by rescaling two sums.
+// The alternatives cost little beside that: every thread knows its own maximum
+// from the first step, so the n-th largest of the 256 thread maxima bounds the
+// n-th largest element from below, and only the about n threads that reach it
+// have their elements looked at again (from L2).
+#include <cuda_runtime.h>
+
+#include <algorithm>
+#include <string>
+
+#include "yanah_b200.h"
+#include "yn_common.cuh"
+#include "yn_internal.h"
+
+namespace ynb {
+
+constexpr int LP_THREADS = 256;
+constexpr int LP_WARPS = LP_THREADS / 32;
+constexpr int LP_MAX_TOP = 64;
+constexpr int LP_CAND = 1024;        // candidates of one chunk that are ranked by counting
+constexpr int LP_MAX_SPLITS = 256;   // blocks of one row: one thread each in the join
+constexpr float LP_LOG2E = 1.44269504088896341f;
+constexpr float LP_LN2 = 0.69314718055994531f;
+
+// Sums of a part of a row: maximum m (-inf: nothing in it), R = sum exp(z - m)
+// without one largest term, D = sum exp(z - m) (z - m).
+struct LpSums {
+  float m, R, D;
+  int rank;   // elements of the part that come before the given token
+};
+struct __align__(16) LpPart {
+  LpSums s;
+  int nan;
+  int pad[3];
+};
+
+struct LpArgs {
+  const uint8_t* z;
+  long long ld, rows;
+  int V, n_top, splits, split_vecs;
+  const int32_t* tokens;
+  float* logprob;
+  float* entropy;
+  int32_t* rank;
+  int32_t* top_ids;
+  float* top_lp;
+  LpPart* parts;                 // (rows, splits)
+  unsigned long long* lists;     // (rows, splits, n_top) keys, descending, 0: none
+};
+
+template <typename T>
+struct LpType;
+template <>
+struct LpType<float> {
+  static constexpr int PER = 4;
+  static constexpr uint32_t NEG = 0xFF800000u;
+  YN_DEV static void unpack(uint32_t w, float* f) { f[0] = __uint_as_float(w); }
+  YN_DEV static uint32_t max_nan(uint32_t a, uint32_t b) {
+    float d;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(d) : "f"(__uint_as_float(a)), "f"(__uint_as_float(b)));
+    return __float_as_uint(d);
+  }
+  YN_DEV static float load(const void* p) { return __ldg(reinterpret_cast<const float*>(p)); }
+};
+template <>
+struct LpType<__nv_bfloat16> {
+  static constexpr int PER = 8;
+  static constexpr uint32_t NEG = 0xFF80FF80u;
+  YN_DEV static void unpack(uint32_t w, float* f) {
+    f[0] = __uint_as_float(w << 16);
+    f[1] = __uint_as_float(w & 0xFFFF0000u);
+  }
+  YN_DEV static uint32_t max_nan(uint32_t a, uint32_t b) {
+    uint32_t d;
+    asm("max.NaN.bf16x2 %0, %1, %2;" : "=r"(d) : "r"(a), "r"(b));
+    return d;
+  }
+  YN_DEV static float load(const void* p) { return bf16_to_f32(__ldg(reinterpret_cast<const uint16_t*>(p))); }
+};
+template <>
+struct LpType<__half> {
+  static constexpr int PER = 8;
+  static constexpr uint32_t NEG = 0xFC00FC00u;
+  YN_DEV static void unpack(uint32_t w, float* f) {
+    f[0] = f16_to_f32((uint16_t)(w & 0xFFFFu));
+    f[1] = f16_to_f32((uint16_t)(w >> 16));
+  }
+  YN_DEV static uint32_t max_nan(uint32_t a, uint32_t b) {
+    uint32_t d;
+    asm("max.NaN.f16x2 %0, %1, %2;" : "=r"(d) : "r"(a), "r"(b));
+    return d;
+  }
+  YN_DEV static float load(const void* p) { return f16_to_f32(__ldg(reinterpret_cast<const uint16_t*>(p))); }
+};
+
+// The elements of a 16-byte vector, in order.
+template <typename T>
+YN_DEV void lp_unpack(const uint4& v, float (&f)[LpType<T>::PER]) {
+  constexpr int W = LpType<T>::PER / 4;
+  LpType<T>::unpack(v.x, f);
+  LpType<T>::unpack(v.y, f + W);
+  LpType<T>::unpack(v.z, f + 2 * W);
+  LpType<T>::unpack(v.w, f + 3 * W);
+}
+
+YN_DEV float lp_ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+// Joins part b to part a.
+YN_DEV void lp_join(LpSums& a, const LpSums& b) {
+  a.rank += b.rank;
+  if (b.m == -__int_as_float(0x7f800000)) return;
+  const bool up = b.m > a.m;
+  const LpSums hi = up ? b : a, lo = up ? a : b;
+  if (lo.m != -__int_as_float(0x7f800000)) {
+    const float d = hi.m == lo.m ? 0.0f : lo.m - hi.m;   // equal also where both are +inf
+    const float f = d == 0.0f ? 1.0f : expf(d);
+    a.R = hi.R + f * (1.0f + lo.R);
+    a.D = hi.D + (f > 0.0f ? f * (lo.D + d * (1.0f + lo.R)) : 0.0f);
+  } else {
+    a.R = hi.R;
+    a.D = hi.D;
+  }
+  a.m = hi.m;
+}
+
+// A row's answer from its sums, by one thread. z_tok: the token's logit.
+YN_DEV void lp_write(const LpArgs& a, long long row, const LpSums& s, bool nan, int tok, float z_tok, float* log_s) {
+  const float inf = __int_as_float(0x7f800000), none = __int_as_float(0x7fc00000);
+  const float ls = log1pf(s.R);
+  *log_s = nan ? none : ls;
+  if (a.entropy) a.entropy[row] = nan ? none : s.m == -inf ? 0.0f : ls - s.D / (1.0f + s.R);
+  if (!a.tokens) return;
+  const bool ok = !nan && tok >= 0 && tok < a.V;
+  a.rank[row] = ok ? s.rank : -1;
+  a.logprob[row] = !ok ? none : z_tok == -inf ? -inf : z_tok == s.m ? -ls : (z_tok - s.m) - ls;
+}
+YN_DEV void lp_write_top(const LpArgs& a, long long row, int j, unsigned long long key, float m, float log_s, bool nan) {
+  const float z = f32_from_ukey((uint32_t)(key >> 32));
+  a.top_ids[row * a.n_top + j] = key && !nan ? (int32_t)(0xFFFFFFFFu - (uint32_t)key) : -1;
+  a.top_lp[row * a.n_top + j] = nan ? log_s : !key ? -__int_as_float(0x7f800000) : z == m ? -log_s : (z - m) - log_s;
+}
+
+// Largest 64-bit key over the block, on every thread. buf: LP_WARPS words that no
+// other call since the last barrier but one uses.
+YN_DEV unsigned long long lp_block_max(unsigned long long k, unsigned long long* buf) {
+  const uint32_t hi = __reduce_max_sync(0xffffffffu, (uint32_t)(k >> 32));
+  const uint32_t lo = __reduce_max_sync(0xffffffffu, (uint32_t)(k >> 32) == hi ? (uint32_t)k : 0u);
+  if ((threadIdx.x & 31) == 0) buf[threadIdx.x >> 5] = ((unsigned long long)hi << 32) | lo;
+  __syncthreads();
+  unsigned long long best = buf[0];
+  for (int w = 1; w < (int)(blockDim.x >> 5); ++w) best = best < buf[w] ? buf[w] : best;
+  return best;
+}
+
+template <typename T, int VPT>
+__global__ void __launch_bounds__(LP_THREADS) k_logprobs(const LpArgs a) {
+  using L = LpType<T>;
+  constexpr int PER = L::PER;
+  constexpr uint32_t KEY_NEG = 0x007FFFFFu;   // f32_ukey(-inf)
+  __shared__ uint32_t tkey[LP_THREADS];
+  __shared__ float wmax[LP_WARPS], wr[LP_WARPS], wd[LP_WARPS];
+  __shared__ int wcnt[LP_WARPS], wrank[LP_WARPS];
+  __shared__ uint32_t thr_s;
+  __shared__ int n_cand;
+  __shared__ unsigned long long cand[LP_CAND], list[LP_MAX_TOP], buf[2][LP_WARPS];
+  __shared__ float log_s_s, m_s;
+
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const long long row = blockIdx.x / a.splits;
+  const int split = (int)(blockIdx.x % a.splits);
+  const float inf = __int_as_float(0x7f800000);
+  const uint8_t* p = a.z + (size_t)row * a.ld * sizeof(T);
+  // Vectors are aligned: the row's first element is element `lead` of vector 0, and
+  // what a vector holds beside the row lies inside the same 16 bytes as an element of it.
+  const int lead = (int)((reinterpret_cast<uintptr_t>(p) & 15u) / sizeof(T));
+  const uint8_t* base = p - lead * sizeof(T);
+  const int n_vecs = (int)(((long long)lead + a.V + PER - 1) / PER);
+  const int v0 = split * a.split_vecs, v1 = min(n_vecs, v0 + a.split_vecs);
+  const int tok = a.tokens ? a.tokens[row] : -1;
+  const bool ranked = tok >= 0 && tok < a.V;
+  const float z_tok = ranked ? L::load(p + (size_t)tok * sizeof(T)) : inf;
+
+  LpSums sums = {-inf, 0.0f, 0.0f, 0};   // kept by thread 0
+  int have = 0;                           // entries of `list`
+  bool nan = false;
+  for (int c0 = v0; c0 < v1 && !nan; c0 += LP_THREADS * VPT) {
+    uint4 v[VPT];
+#pragma unroll
+    for (int i = 0; i < VPT; ++i) {
+      const int at = c0 + i * LP_THREADS + tid;
+      v[i] = at < v1 ? ldg_nc_v4(base + (size_t)at * 16) : make_uint4(L::NEG, L::NEG, L::NEG, L::NEG);
+    }
+    if ((c0 == 0 && lead) || c0 + LP_THREADS * VPT >= n_vecs) {  // what lies outside the row reads as -inf
+#pragma unroll
+      for (int i = 0; i < VPT; ++i) {
+        const int at = c0 + i * LP_THREADS + tid;
+        const long long e0 = (long long)at * PER - lead;
+        if (at < v1 && (e0 < 0 || e0 + PER > a.V)) {
+          uint32_t w[4] = {v[i].x, v[i].y, v[i].z, v[i].w};
+#pragma unroll
+          for (int j = 0; j < PER; ++j)
+            if (e0 + j < 0 || e0 + j >= a.V) {
+              if (PER == 4) w[j] = L::NEG;
+              else w[j / 2] = (j & 1) ? (w[j / 2] & 0xFFFFu) | (L::NEG & 0xFFFF0000u)
+                                      : (w[j / 2] & 0xFFFF0000u) | (L::NEG & 0xFFFFu);
+            }
+          v[i] = make_uint4(w[0], w[1], w[2], w[3]);
+        }
+      }
+    }
+    uint32_t mx = L::NEG;
+#pragma unroll
+    for (int i = 0; i < VPT; ++i)
+      mx = L::max_nan(mx, L::max_nan(L::max_nan(v[i].x, v[i].y), L::max_nan(v[i].z, v[i].w)));
+    float tm;
+    {
+      float f[2];
+      L::unpack(mx, f);
+      tm = PER == 4 ? f[0] : (f[0] > f[1] || f[0] != f[0] ? f[0] : f[1]);
+    }
+    const uint32_t tk = f32_ukey(tm);
+    tkey[tid] = tk;
+    const uint32_t wk = __reduce_max_sync(0xffffffffu, tk);
+    if (lane == 0) wmax[warp] = f32_from_ukey(wk);
+    if (tid == 0) n_cand = 0;
+    nan = __syncthreads_or(tm != tm) != 0;
+    if (nan) break;
+    float m = wmax[0];
+#pragma unroll
+    for (int w = 1; w < LP_WARPS; ++w) m = fmaxf(m, wmax[w]);
+    const uint32_t floor_key = have == a.n_top && a.n_top ? (uint32_t)(list[a.n_top - 1] >> 32) : KEY_NEG;
+    const bool search = a.n_top > 0 && m > -inf && f32_ukey(m) > floor_key;
+    if (search && warp == 0) {
+      // the n-th largest thread maximum, its low 16 bits left out (a few more candidates)
+      uint32_t k[LP_WARPS], t = 0;
+#pragma unroll
+      for (int w = 0; w < LP_WARPS; ++w) k[w] = tkey[lane + 32 * w];
+      for (int b = 31; b >= 16; --b) {
+        const uint32_t x = t | (1u << b);
+        int c = 0;
+#pragma unroll
+        for (int w = 0; w < LP_WARPS; ++w) c += k[w] >= x;
+        if (__reduce_add_sync(0xffffffffu, c) >= a.n_top) t = x;
+      }
+      if (lane == 0) thr_s = max(t, floor_key + 1);   // equal to the floor: a higher id, comes after it
+    }
+    // sums relative to the chunk's maximum; cnt: elements equal to it
+    float r = 0.0f, d = 0.0f;
+    int cnt = 0, before = 0;
+    // y = z log2(e) - ml is (z - m) log2(e) + del, del the rounding of ml = m log2(e), which is taken out of the
+    // sums at the end; for maxima so large that del is not small the subtraction comes first and del is 0
+    const bool large = !(fabsf(m) < 4096.0f);
+    const float ml = m * LP_LOG2E, del = large ? 0.0f : fmaf(m, LP_LOG2E, -ml);
+    if (m > -inf && m < inf) {
+      if (tm < m && !large) {
+#pragma unroll
+        for (int i = 0; i < VPT; ++i) {
+          float f[PER];
+          lp_unpack<T>(v[i], f);
+#pragma unroll
+          for (int j = 0; j < PER; ++j) {
+            const float y = fmaxf(fmaf(f[j], LP_LOG2E, -ml), -200.0f), e = lp_ex2(y);
+            r += e;
+            d = fmaf(e, y, d);
+          }
+        }
+      } else {
+#pragma unroll
+        for (int i = 0; i < VPT; ++i) {
+          float f[PER];
+          lp_unpack<T>(v[i], f);
+#pragma unroll
+          for (int j = 0; j < PER; ++j) {
+            const float y = fmaxf(fmaf(f[j] - m, LP_LOG2E, del), -200.0f), e = lp_ex2(y);
+            cnt += f[j] == m;
+            r += f[j] == m ? 0.0f : e;
+            d = f[j] == m ? d : fmaf(e, y, d);
+          }
+        }
+      }
+    } else if (tm == inf) {
+#pragma unroll
+      for (int i = 0; i < VPT; ++i) {
+        float f[PER];
+        lp_unpack<T>(v[i], f);
+#pragma unroll
+        for (int j = 0; j < PER; ++j) cnt += f[j] == inf;
+      }
+    }
+    if (ranked && tm >= z_tok) {
+#pragma unroll
+      for (int i = 0; i < VPT; ++i) {
+        float f[PER];
+        lp_unpack<T>(v[i], f);
+        const int at = c0 + i * LP_THREADS + tid;
+        const long long e0 = (long long)at * PER - lead;
+        if (at >= v1) break;
+#pragma unroll
+        for (int j = 0; j < PER; ++j) before += f[j] > z_tok || (f[j] == z_tok && e0 + j >= 0 && e0 + j < tok);
+      }
+    }
+    r = warp_sum_f32(r);
+    d = warp_sum_f32(d);
+    cnt = __reduce_add_sync(0xffffffffu, cnt);
+    before = __reduce_add_sync(0xffffffffu, before);
+    if (lane == 0) {
+      wr[warp] = r;
+      wd[warp] = d;
+      wcnt[warp] = cnt;
+      wrank[warp] = before;
+    }
+    __syncthreads();
+    if (tid == 0) {
+      LpSums c = {m, 0.0f, 0.0f, 0};
+      int n_max = 0;
+      for (int w = 0; w < LP_WARPS; ++w) {
+        c.R += wr[w];
+        c.D += wd[w];
+        n_max += wcnt[w];
+        c.rank += wrank[w];
+      }
+      if (m > -inf && m < inf) {
+        const float f = exp2f(-del);
+        c.D = f * (c.D - del * c.R) * LP_LN2;
+        c.R *= f;
+      }
+      c.R += (float)(n_max - 1);
+      lp_join(sums, c);
+    }
+    if (search) {
+      const uint32_t thr = thr_s;
+      // the elements of every thread of this warp that reaches the threshold, one thread's
+      // vectors at a time, one lane per vector
+      unsigned who = __ballot_sync(0xffffffffu, tk >= thr);
+      while (who) {
+        const int o = __ffs(who) - 1;
+        who &= who - 1;
+        const int at = c0 + lane * LP_THREADS + 32 * warp + o;
+        if (lane < VPT && at < v1) {
+          float f[PER];
+          lp_unpack<T>(ldg_nc_v4(base + (size_t)at * 16), f);
+          const long long e0 = (long long)at * PER - lead;
+#pragma unroll
+          for (int j = 0; j < PER; ++j) {
+            const uint32_t k = f32_ukey(f[j]);
+            if (k >= thr && e0 + j >= 0 && e0 + j < a.V) {
+              const int q = atomicAdd(&n_cand, 1);
+              if (q < LP_CAND) cand[q] = ((unsigned long long)k << 32) | (0xFFFFFFFFu - (uint32_t)(e0 + j));
+            }
+          }
+        }
+        __syncwarp();
+      }
+      __syncthreads();
+      int n = n_cand;
+      if (n + have > LP_CAND) {
+        // many equal or near logits: the n largest one after another, over the whole chunk
+        unsigned long long prev = ~0ull;
+        int got = 0;
+        for (int q = 0; q < a.n_top; ++q) {
+          unsigned long long best = 0;
+          for (int at = c0 + tid; at < min(v1, c0 + LP_THREADS * VPT); at += LP_THREADS) {
+            float f[PER];
+            lp_unpack<T>(ldg_nc_v4(base + (size_t)at * 16), f);
+            const long long e0 = (long long)at * PER - lead;
+#pragma unroll
+            for (int j = 0; j < PER; ++j) {
+              const unsigned long long k =
+                  ((unsigned long long)f32_ukey(f[j]) << 32) | (0xFFFFFFFFu - (uint32_t)(e0 + j));
+              if (e0 + j >= 0 && e0 + j < a.V && f[j] > -inf && k < prev && k > best) best = k;
+            }
+          }
+          prev = lp_block_max(best, buf[q & 1]);
+          if (!prev) break;
+          if (tid == 0) cand[q] = prev;
+          ++got;
+        }
+        __syncthreads();
+        n = got;
+      }
+      // candidates and the list so far, each placed by how many are larger (keys are distinct)
+      if (tid < have) cand[n + tid] = list[tid];
+      __syncthreads();
+      const int total = n + have;
+      for (int i = tid; i < total; i += LP_THREADS) {
+        const unsigned long long k = cand[i];
+        int place = 0;
+        for (int q = 0; q < total; ++q) place += cand[q] > k;
+        if (place < a.n_top) list[place] = k;
+      }
+      have = min(total, a.n_top);
+    }
+    __syncthreads();
+  }
+  if (a.splits > 1) {
+    const long long at = row * a.splits + split;
+    if (tid == 0) {
+      LpPart q = {sums, nan ? 1 : 0, {0, 0, 0}};
+      a.parts[at] = q;
+    }
+    if (tid < a.n_top) a.lists[at * a.n_top + tid] = tid < have ? list[tid] : 0ull;
+    return;
+  }
+  if (tid == 0) {
+    lp_write(a, row, sums, nan, tok, z_tok, &log_s_s);
+    m_s = sums.m;
+  }
+  if (a.n_top) {
+    __syncthreads();
+    if (tid < a.n_top) lp_write_top(a, row, tid, tid < have ? list[tid] : 0ull, m_s, log_s_s, nan);
+  }
+}
+
+// The join of a row's parts, one block per row, one thread per part: sums over the
+// block, then the alternatives as an n_top-step merge of the parts' sorted lists.
+template <typename T>
+__global__ void __launch_bounds__(LP_MAX_SPLITS) k_logprobs_join(const LpArgs a) {
+  using L = LpType<T>;
+  __shared__ unsigned long long buf[2][LP_WARPS];
+  __shared__ LpSums ws[LP_WARPS];
+  __shared__ float log_s_s, m_s;
+  const int tid = threadIdx.x;
+  const long long row = blockIdx.x;
+  const bool on = tid < a.splits;
+  const long long at = row * a.splits + tid;
+  LpSums s = {-__int_as_float(0x7f800000), 0.0f, 0.0f, 0};
+  int bad = 0;
+  if (on) {
+    const LpPart q = a.parts[at];
+    s = q.s;
+    bad = q.nan;
+  }
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) {
+    LpSums b;
+    b.m = __shfl_xor_sync(0xffffffffu, s.m, o);
+    b.R = __shfl_xor_sync(0xffffffffu, s.R, o);
+    b.D = __shfl_xor_sync(0xffffffffu, s.D, o);
+    b.rank = __shfl_xor_sync(0xffffffffu, s.rank, o);
+    lp_join(s, b);
+  }
+  if ((tid & 31) == 0) ws[tid >> 5] = s;
+  const bool nan = __syncthreads_or(bad) != 0;
+  if (tid == 0) {
+    for (int w = 1; w < (int)(blockDim.x >> 5); ++w) lp_join(s, ws[w]);
+    const int tok = a.tokens ? a.tokens[row] : -1;
+    const float z_tok = tok >= 0 && tok < a.V ? L::load(a.z + ((size_t)row * a.ld + tok) * sizeof(T)) : 0.0f;
+    lp_write(a, row, s, nan, tok, z_tok, &log_s_s);
+    m_s = s.m;
+  }
+  if (!a.n_top) return;
+  const unsigned long long* mine = a.lists + at * a.n_top;
+  int next = 0;
+  unsigned long long head = on ? mine[0] : 0ull, win = 0;
+  for (int j = 0; j < a.n_top; ++j) {
+    const unsigned long long best = lp_block_max(head, buf[j & 1]);
+    if (tid == j) win = best;
+    if (best && head == best) head = ++next < a.n_top ? mine[next] : 0ull;
+  }
+  __syncthreads();
+  if (tid < a.n_top) lp_write_top(a, row, tid, win, m_s, log_s_s, nan);
+}
+
+// How a row is split: enough blocks for two waves when the rows alone are fewer,
+// each with at least one 16-byte load per thread.
+int lp_splits(long long rows, long long vocab, int size) {
+  const long long vecs = (vocab * size + 15) / 16 + 1;
+  if (rows >= 2 * 148) return 1;
+  const long long want = (2 * 148 + rows - 1) / rows, most = (vecs + LP_THREADS - 1) / LP_THREADS;
+  return (int)std::max<long long>(1, std::min<long long>(LP_MAX_SPLITS, std::min(want, most)));
+}
+
+template <typename T>
+void launch_logprobs(const LpArgs& a, cudaStream_t st) {
+  const unsigned grid = (unsigned)(a.rows * a.splits);
+  if (a.split_vecs <= LP_THREADS) k_logprobs<T, 1><<<grid, LP_THREADS, 0, st>>>(a);
+  else if (a.split_vecs <= 2 * LP_THREADS) k_logprobs<T, 2><<<grid, LP_THREADS, 0, st>>>(a);
+  else if (a.split_vecs <= 4 * LP_THREADS) k_logprobs<T, 4><<<grid, LP_THREADS, 0, st>>>(a);
+  else k_logprobs<T, 8><<<grid, LP_THREADS, 0, st>>>(a);
+  if (a.splits > 1) {
+    const int threads = std::max((a.splits + 31) / 32 * 32, a.n_top > 32 ? 64 : 32);
+    k_logprobs_join<T><<<(unsigned)a.rows, threads, 0, st>>>(a);
+  }
+}
+
+}  // namespace ynb
+
+using namespace ynb;
+
+namespace {
+int lp_size(int dtype) { return dtype == YN_F32 ? 4 : dtype == YN_BF16 || dtype == YN_F16 ? 2 : 0; }
+}  // namespace
+
+extern "C" size_t yn_logprobs_ws_bytes(int64_t rows, int64_t vocab, int32_t dtype, int32_t n_top) {
+  const int size = lp_size(dtype);
+  if (rows < 1 || vocab < 1 || vocab > 0x7fffff00LL || !size || n_top < 0 || n_top > LP_MAX_TOP) return 0;
+  const long long s = lp_splits(rows, vocab, size);
+  return s == 1 ? 0 : (size_t)(rows * s) * (sizeof(LpPart) + 8 * (size_t)n_top);
+}
+
+extern "C" int yn_token_logprobs(const void* logits, int32_t dtype, int64_t row_stride, int64_t rows, int64_t vocab,
+                                 const int32_t* tokens, int32_t n_top, float* logprob, float* entropy, int32_t* rank,
+                                 int32_t* top_ids, float* top_logprobs, void* ws, size_t ws_bytes, void* stream) {
+  const int size = lp_size(dtype);
+  if (!size) return host_fail(YN_E_INVALID, "unknown dtype");
+  if (vocab < 1 || rows < 0 || row_stride < vocab) return host_fail(YN_E_INVALID, "row_stride must be at least vocab, vocab at least 1");
+  if (vocab > 0x7fffff00LL || rows > 0x7fffffffLL / LP_MAX_SPLITS)
+    return host_fail(YN_E_UNSUPPORTED, "vocab below 2^31 - 255, at most 8388607 rows");
+  if (n_top < 0 || n_top > LP_MAX_TOP || n_top > vocab) return host_fail(YN_E_INVALID, "n_top must be in [0, min(64, vocab)]");
+  if (rows == 0) return YN_OK;
+  if (!logits || (tokens && (!logprob || !rank)) || (n_top && (!top_ids || !top_logprobs)))
+    return host_fail(YN_E_INVALID, "null argument");
+  if (reinterpret_cast<uintptr_t>(logits) % size) return host_fail(YN_E_INVALID, "logits must be aligned to their element");
+  LpArgs a{};
+  a.z = reinterpret_cast<const uint8_t*>(logits);
+  a.ld = row_stride;
+  a.rows = rows;
+  a.V = (int)vocab;
+  a.n_top = n_top;
+  a.splits = lp_splits(rows, vocab, size);
+  const long long vecs = (vocab * size + 15) / 16 + 1;   // one more: a row may start inside a vector
+  a.split_vecs = (int)((vecs + a.splits - 1) / a.splits);
+  a.tokens = tokens;
+  a.logprob = logprob;
+  a.entropy = entropy;
+  a.rank = rank;
+  a.top_ids = top_ids;
+  a.top_lp = top_logprobs;
+  if (a.splits > 1) {
+    const size_t need = yn_logprobs_ws_bytes(rows, vocab, dtype, n_top);
+    if (!ws || ws_bytes < need || reinterpret_cast<uintptr_t>(ws) % 16)
+      return host_fail(YN_E_INVALID, "workspace too small or not 16-byte aligned");
+    a.parts = reinterpret_cast<LpPart*>(ws);
+    a.lists = reinterpret_cast<unsigned long long*>(a.parts + rows * a.splits);
+  }
+  cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
+  if (dtype == YN_F32) launch_logprobs<float>(a, st);
+  else if (dtype == YN_BF16) launch_logprobs<__nv_bfloat16>(a, st);
+  else launch_logprobs<__half>(a, st);
+  const cudaError_t e = cudaGetLastError();
+  if (e != cudaSuccess) return host_fail(YN_E_CUDA, std::string("yn_token_logprobs: ") + cudaGetErrorString(e));
+  return YN_OK;
+}

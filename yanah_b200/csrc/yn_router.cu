@@ -1,0 +1,378 @@
+// Routing of rows of router logits by a rule (softmax or sigmoid scores, a
+// balance bias, groups of experts, top k, renormalised weights), and its C ABI.
+// No counterpart in the reference, whose routers are softmax top-k without a
+// bias (mlx_backend.py:308-316; that form is yn_route).
+//
+// Mathematics, per row of logits z: s_e = exp(z_e - m) / sum or 1 / (1 +
+// exp(-z_e)); c_e = s_e + b_e orders the experts; a group's score is the sum of
+// its `group_top` largest c; the k largest c inside the `top_groups` best groups
+// are chosen (ties: lower id first) and weighted by s, not c.
+//
+// The order is that of exact arithmetic. Without a bias and groups c is a
+// monotone function of z, so the logits themselves are compared. Otherwise the
+// row is ordered in fp32, whose error on c is bounded (below); only where two
+// neighbours of the chosen order, or the last group in and the first one out,
+// are nearer than that bound is the row ordered again in fp64 by the same warp.
+//
+// One warp per row, keys in registers: L = 32 / (groups rounded up to a power of
+// two) lanes hold one group, element i of a lane being expert
+// (lane / L) * per_group + lane % L + i * L. A row is at most 4 KB, so the kernel
+// is bound by the latency of the warp's k rounds of argmax (two redux each), not
+// by memory.
+#include <cuda_runtime.h>
+
+#include <string>
+
+#include "yanah_b200.h"
+#include "yn_common.cuh"
+#include "yn_internal.h"
+
+namespace ynb {
+
+constexpr int RT_WARPS = 4;          // rows per block
+constexpr int RT_MAX_E = 1024;
+constexpr int RT_MAX_K = 31;         // lane k holds the first expert not chosen
+
+struct RouterArgs {
+  const void* z;
+  long long ld;
+  long long rows;
+  const float* bias;
+  const uint8_t* avail;
+  int32_t* ids;
+  float* w;
+  int E, K, G, per, L, kept, group_top;
+  bool softmax, norm;
+  float scale;
+};
+
+template <typename T>
+YN_DEV float rt_load(const void* z, long long i);
+template <>
+YN_DEV float rt_load<float>(const void* z, long long i) { return __ldg(reinterpret_cast<const float*>(z) + i); }
+template <>
+YN_DEV float rt_load<__nv_bfloat16>(const void* z, long long i) {
+  return bf16_to_f32(__ldg(reinterpret_cast<const uint16_t*>(z) + i));
+}
+template <>
+YN_DEV float rt_load<__half>(const void* z, long long i) {
+  return f16_to_f32(__ldg(reinterpret_cast<const uint16_t*>(z) + i));
+}
+
+YN_DEV double warp_max_f64(double v) {
+#pragma unroll
+  for (int m = 16; m > 0; m >>= 1) v = fmax(v, __shfl_xor_sync(0xffffffffu, v, m));
+  return v;
+}
+YN_DEV double warp_sum_f64(double v) {
+#pragma unroll
+  for (int m = 16; m > 0; m >>= 1) v += __shfl_xor_sync(0xffffffffu, v, m);
+  return v;
+}
+// Where lane `lane` finds its element i, or -1.
+YN_DEV int rt_expert(const RouterArgs& a, int lane, int i) {
+  const int g = lane / a.L, at = lane % a.L + i * a.L;
+  return g < a.G && at < a.per ? g * a.per + at : -1;
+}
+
+// The two largest of a lane's values merged over the L lanes of its group, then
+// whether the group is among the `kept` best (its rank by score, ties to the
+// lower group). far: smallest distance between a group that is in and one that
+// is out, for the caller's check.
+template <typename F>
+YN_DEV bool rt_group_kept(const RouterArgs& a, int lane, F hi, F lo, F none, F* far) {
+  for (int m = 1; m < a.L; m <<= 1) {
+    const F h2 = __shfl_xor_sync(0xffffffffu, hi, m), l2 = __shfl_xor_sync(0xffffffffu, lo, m);
+    const F mn = hi < h2 ? hi : h2, mx = hi < h2 ? h2 : hi, l = lo < l2 ? l2 : lo;
+    hi = mx;
+    lo = mn < l ? l : mn;
+  }
+  F score = hi;
+  if (a.group_top > 1 && lo != none) score = hi + lo;
+  const int g = lane / a.L;
+  int rank = 0;
+  for (int o = 0; o < a.G; ++o) {
+    const F s = __shfl_sync(0xffffffffu, score, o * a.L);
+    rank += s > score || (s == score && o < g);
+  }
+  const bool in = g < a.G && rank < a.kept;
+  F lowest_in = in && score != none ? score : -none, best_out = !in && g < a.G ? score : none;
+#pragma unroll
+  for (int m = 16; m > 0; m >>= 1) {
+    const F x = __shfl_xor_sync(0xffffffffu, lowest_in, m), y = __shfl_xor_sync(0xffffffffu, best_out, m);
+    lowest_in = x < lowest_in ? x : lowest_in;
+    best_out = y > best_out ? y : best_out;
+  }
+  *far = best_out == none ? -none : lowest_in - best_out;
+  return in;
+}
+
+// The row's choice in fp64 (values in this warp's shared memory): lane j < K
+// returns the id at place j.
+template <typename T>
+__device__ __noinline__ int rt_choose_f64(const RouterArgs& a, long long row, int lane, double* val) {
+  const double none = -__longlong_as_double(0x7ff0000000000000LL);
+  const int nv = (a.per + a.L - 1) / a.L;
+  double m = none;
+  for (int i = 0; i < nv; ++i) {
+    const int e = rt_expert(a, lane, i);
+    if (e < 0) continue;
+    const float z = rt_load<T>(a.z, row * a.ld + e);
+    const bool ok = z > -__int_as_float(0x7f800000) && (!a.avail || a.avail[e]);  // false for NaN
+    val[e] = ok ? (double)z : none;
+    m = fmax(m, val[e]);
+  }
+  m = warp_max_f64(m);
+  double sum = 0.0;
+  for (int i = 0; i < nv; ++i) {
+    const int e = rt_expert(a, lane, i);
+    if (e < 0 || val[e] == none) continue;
+    double s;
+    if (a.softmax) sum += s = val[e] == m ? 1.0 : exp(val[e] - m);
+    else s = 1.0 / (1.0 + exp(-val[e]));
+    val[e] = s;
+  }
+  if (a.softmax) sum = warp_sum_f64(sum);
+  double hi = none, lo = none;
+  for (int i = 0; i < nv; ++i) {
+    const int e = rt_expert(a, lane, i);
+    if (e < 0 || val[e] == none) continue;
+    if (a.softmax) val[e] /= sum;
+    if (a.bias) {
+      const double c = val[e] + (double)a.bias[e];
+      val[e] = c > none ? c : none;
+    }
+    if (val[e] > hi) { lo = hi; hi = val[e]; }
+    else if (val[e] > lo) lo = val[e];
+  }
+  if (a.G > 1) {
+    double far;
+    const bool in = rt_group_kept(a, lane, hi, lo, none, &far);
+    for (int i = 0; i < nv; ++i) {
+      const int e = rt_expert(a, lane, i);
+      if (e < 0) continue;
+      if (!in) val[e] = none;
+      else if (!a.bias && val[e] > none) val[e] = (double)rt_load<T>(a.z, row * a.ld + e);  // the logits' order
+    }
+  }
+  int mine = -1;
+  for (int j = 0; j < a.K; ++j) {
+    double best = none;
+    int at = RT_MAX_E;
+    for (int i = 0; i < nv; ++i) {
+      const int e = rt_expert(a, lane, i);
+      if (e >= 0 && val[e] > best) { best = val[e]; at = e; }
+    }
+    const double top = warp_max_f64(best);
+    const int id = (int)__reduce_min_sync(0xffffffffu, best == top ? (unsigned)at : (unsigned)RT_MAX_E);
+    if (top == none) break;
+    if (at == id) val[id] = none;
+    if (lane == j) mine = id;
+  }
+  return mine;
+}
+
+// NV: elements per lane. BY_SCORE: the order needs the scores (a bias or groups);
+// otherwise the logits order the experts.
+template <typename T, int NV, bool BY_SCORE>
+__global__ void __launch_bounds__(32 * RT_WARPS) k_router(const RouterArgs a) {
+  extern __shared__ double rt_smem[];   // BY_SCORE: E doubles per warp
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const long long row = (long long)blockIdx.x * RT_WARPS + warp;
+  if (row >= a.rows) return;
+  const float inf = __int_as_float(0x7f800000);
+  float v[NV];
+  float m = -inf;
+#pragma unroll
+  for (int i = 0; i < NV; ++i) {
+    const int e = rt_expert(a, lane, i);
+    const float z = e >= 0 ? rt_load<T>(a.z, row * a.ld + e) : -inf;
+    v[i] = z > -inf && (!a.avail || a.avail[e]) ? z : -inf;
+    m = fmaxf(m, v[i]);
+  }
+  m = f32_from_ukey(__reduce_max_sync(0xffffffffu, f32_ukey(m)));
+  float sum = 0.0f;
+  if (a.softmax && (BY_SCORE || !a.norm)) {
+#pragma unroll
+    for (int i = 0; i < NV; ++i)
+      sum += v[i] == -inf ? 0.0f : v[i] == m ? 1.0f : __expf(v[i] - m);   // all +inf logits share the mass
+    sum = warp_sum_f32(sum);
+  }
+  uint32_t key[NV];
+  bool near = false;
+  float tol = 0.0f;
+  if (BY_SCORE) {
+    // |c - exact| <= tol + 2^-24 |c|, tol relative to the row's largest score: __expf
+    // is off by 2 + 1.2 |x| ulp and |x| e^x <= 0.4 for x <= 0, so the exponentials
+    // stay within 2^-21 of the largest; the softmax sum of at most 64 terms a lane and
+    // 5 shuffled adds within 69 * 2^-24 < 5e-6 of itself. Scores below e^-80 are not
+    // told apart (1e-30).
+    const float inv = a.softmax ? 1.0f / sum : 1.0f;
+    float hi = -inf, lo = -inf;
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      const int e = rt_expert(a, lane, i);
+      if (v[i] == -inf) {
+        key[i] = 0;
+        continue;
+      }
+      const float s = a.softmax ? (v[i] == m ? inv : __expf(v[i] - m) * inv)
+                                : __fdividef(1.0f, 1.0f + __expf(fminf(-v[i], 80.0f)));
+      const float c = a.bias ? s + __ldg(a.bias + e) : s;
+      if (!(c > -inf)) {   // a bias of -inf or NaN takes the expert out
+        key[i] = 0;
+        continue;
+      }
+      key[i] = f32_ukey(a.bias ? c : v[i]);   // without a bias the logits have the scores' order, exactly
+      if (c > hi) { lo = hi; hi = c; }
+      else if (c > lo) lo = c;
+    }
+    const float smax = a.softmax ? inv : __fdividef(1.0f, 1.0f + __expf(fminf(-m, 80.0f)));
+    tol = (a.softmax ? 1.6e-5f : 2.0e-6f) * smax + 1e-30f;
+    if (a.G > 1) {
+      float far;
+      const bool in = rt_group_kept(a, lane, hi, lo, -inf, &far);
+      const float mag = f32_from_ukey(__reduce_max_sync(0xffffffffu, f32_ukey(hi == -inf ? 0.0f : fabsf(hi))));
+      near = far <= 2.0f * tol + 5.0e-7f * mag;
+      if (!in) {
+#pragma unroll
+        for (int i = 0; i < NV; ++i) key[i] = 0;
+      }
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < NV; ++i) key[i] = v[i] == -inf ? 0u : f32_ukey(v[i]);
+  }
+  // K rounds (one more where neighbours are compared): the largest key, the lowest id that has it
+  const bool compared = BY_SCORE && a.bias;
+  const int rounds = compared ? a.K + 1 : a.K;
+  int mine = -1;
+  uint32_t my_key = 0;
+  for (int j = 0; j < rounds; ++j) {
+    uint32_t best = 0;
+    int bi = 0;
+#pragma unroll
+    for (int i = 0; i < NV; ++i)
+      if (key[i] > best) { best = key[i]; bi = i; }
+    const uint32_t top = __reduce_max_sync(0xffffffffu, best);
+    if (top == 0) break;
+    const int at = best == top ? rt_expert(a, lane, bi) : RT_MAX_E;
+    const int id = (int)__reduce_min_sync(0xffffffffu, (unsigned)at);
+    if (at == id) {
+#pragma unroll
+      for (int i = 0; i < NV; ++i)
+        if (i == bi) key[i] = 0;
+    }
+    if (lane == j) { mine = id; my_key = top; }
+  }
+  float z = mine >= 0 ? rt_load<T>(a.z, row * a.ld + mine) : -inf;
+  if (BY_SCORE) {
+    if (compared) {
+      const float b = mine >= 0 ? a.bias[mine] : 0.0f;
+      const int nid = __shfl_down_sync(0xffffffffu, mine, 1);
+      const float nz = __shfl_down_sync(0xffffffffu, z, 1), nb = __shfl_down_sync(0xffffffffu, b, 1);
+      const uint32_t nk = __shfl_down_sync(0xffffffffu, my_key, 1);
+      // equal logits with equal biases are equal in exact arithmetic too, except at the last place: what is
+      // near the first one left out is not looked at
+      if (lane < a.K && mine >= 0 && nid >= 0 && !(z == nz && b == nb && lane < a.K - 1)) {
+        const float c = f32_from_ukey(my_key), nc = f32_from_ukey(nk);
+        near |= c - nc <= 2.0f * tol + 2.5e-7f * fmaxf(fabsf(c), fabsf(nc));
+      }
+    }
+    if (__any_sync(0xffffffffu, near)) {
+      mine = rt_choose_f64<T>(a, row, lane, rt_smem + (size_t)warp * a.E);
+      z = mine >= 0 ? rt_load<T>(a.z, row * a.ld + mine) : -inf;
+    }
+  }
+  if (lane >= a.K) { mine = -1; z = -inf; }
+  // Weights from the chosen logits alone, relative to the largest of them (M) where
+  // they are renormalised, so that scores far below the row's largest keep their ratio.
+  float w;
+  if (a.norm) {
+    const float M = f32_from_ukey(__reduce_max_sync(0xffffffffu, f32_ukey(z)));
+    if (a.softmax) w = z == -inf ? 0.0f : z == M ? 1.0f : expf(z - M);
+    else if (M < 0.0f) w = z == -inf ? 0.0f : expf(z - M) / (1.0f + expf(z));
+    else w = z == -inf ? 0.0f : 1.0f / (1.0f + expf(-z));
+    const float t = warp_sum_f32(w);
+    w = t > 0.0f ? w / t * a.scale : 0.0f;
+  } else {
+    if (a.softmax) w = z == -inf ? 0.0f : (z == m ? 1.0f : expf(z - m)) / sum * a.scale;
+    else w = z == -inf ? 0.0f : 1.0f / (1.0f + expf(-z)) * a.scale;
+  }
+  if (lane < a.K) {
+    a.ids[row * a.K + lane] = mine;
+    a.w[row * a.K + lane] = w;
+  }
+}
+
+template <typename T, bool BY_SCORE>
+void launch_router(const RouterArgs& a, int nv, cudaStream_t st) {
+  const unsigned grid = (unsigned)((a.rows + RT_WARPS - 1) / RT_WARPS);
+  const size_t smem = BY_SCORE ? (size_t)RT_WARPS * a.E * sizeof(double) : 0;
+  const dim3 b(32 * RT_WARPS);
+  if (nv <= 2) k_router<T, 2, BY_SCORE><<<grid, b, smem, st>>>(a);
+  else if (nv <= 4) k_router<T, 4, BY_SCORE><<<grid, b, smem, st>>>(a);
+  else if (nv <= 8) k_router<T, 8, BY_SCORE><<<grid, b, smem, st>>>(a);
+  else if (nv <= 16) k_router<T, 16, BY_SCORE><<<grid, b, smem, st>>>(a);
+  else if (nv <= 32) k_router<T, 32, BY_SCORE><<<grid, b, smem, st>>>(a);
+  else k_router<T, 64, BY_SCORE><<<grid, b, smem, st>>>(a);
+}
+
+}  // namespace ynb
+
+using namespace ynb;
+
+extern "C" int yn_route_scored(const yn_route_rule* rule, const void* logits, int32_t dtype, int64_t row_stride,
+                               int64_t rows, const float* bias, const uint8_t* available, int32_t* ids,
+                               float* weights, void* stream) {
+  if (!rule) return host_fail(YN_E_INVALID, "null argument");
+  const yn_route_rule& r = *rule;
+  if (r.n_experts < 1 || r.top_k < 1 || r.top_k > r.n_experts)
+    return host_fail(YN_E_INVALID, "top_k must be in [1, n_experts]");
+  if (r.n_experts > RT_MAX_E || r.top_k > RT_MAX_K)
+    return host_fail(YN_E_UNSUPPORTED, "at most 1024 experts and top_k 31");
+  if (r.score != YN_SCORE_SOFTMAX && r.score != YN_SCORE_SIGMOID)
+    return host_fail(YN_E_INVALID, "score must be YN_SCORE_SOFTMAX or YN_SCORE_SIGMOID");
+  if (r.n_groups < 1 || r.n_experts % r.n_groups || r.top_groups < 1 || r.top_groups > r.n_groups)
+    return host_fail(YN_E_INVALID, "n_groups must divide n_experts, top_groups must be in [1, n_groups]");
+  if (r.n_groups > 32) return host_fail(YN_E_UNSUPPORTED, "at most 32 groups");
+  if (r.group_top != 1 && r.group_top != 2) return host_fail(YN_E_INVALID, "group_top must be 1 or 2");
+  if (r.top_k > r.top_groups * (r.n_experts / r.n_groups))
+    return host_fail(YN_E_INVALID, "top_k is larger than the kept groups");
+  if (dtype != YN_F32 && dtype != YN_BF16 && dtype != YN_F16) return host_fail(YN_E_INVALID, "unknown dtype");
+  if (rows < 0 || rows > 0x7fffffffLL || row_stride < r.n_experts)
+    return host_fail(YN_E_INVALID, "rows must be in [0, 2^31), row_stride at least n_experts");
+  if (rows == 0) return YN_OK;
+  if (!logits || !ids || !weights) return host_fail(YN_E_INVALID, "null argument");
+  RouterArgs a{};
+  a.z = logits;
+  a.ld = row_stride;
+  a.rows = rows;
+  a.bias = bias;
+  a.avail = available;
+  a.ids = ids;
+  a.w = weights;
+  a.E = r.n_experts;
+  a.K = r.top_k;
+  // keeping every group is the same as having none
+  a.G = r.top_groups == r.n_groups ? 1 : r.n_groups;
+  a.per = a.E / a.G;
+  int p2 = 1;
+  while (p2 < a.G) p2 *= 2;
+  a.L = 32 / p2;
+  a.kept = r.top_groups;
+  a.group_top = r.group_top;
+  a.softmax = r.score == YN_SCORE_SOFTMAX;
+  a.norm = r.norm_topk != 0;
+  a.scale = r.scale;
+  const bool by_score = bias || a.G > 1;
+  const int nv = (a.per + a.L - 1) / a.L;
+  cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
+  if (dtype == YN_F32) by_score ? launch_router<float, true>(a, nv, st) : launch_router<float, false>(a, nv, st);
+  else if (dtype == YN_BF16)
+    by_score ? launch_router<__nv_bfloat16, true>(a, nv, st) : launch_router<__nv_bfloat16, false>(a, nv, st);
+  else by_score ? launch_router<__half, true>(a, nv, st) : launch_router<__half, false>(a, nv, st);
+  const cudaError_t e = cudaGetLastError();
+  if (e != cudaSuccess) return host_fail(YN_E_CUDA, std::string("yn_route_scored: ") + cudaGetErrorString(e));
+  return YN_OK;
+}

@@ -47,33 +47,11 @@ RouteWs route_ws(const yn_dims& d, int rows) {
   return L;
 }
 
-using EncodeTiled = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*,
-                                 const cuuint64_t*, const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave,
-                                 CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
-
-// cuTensorMapEncodeTiled through the runtime's driver entry point (no link
-// against the driver library).
-int encode_fn(EncodeTiled* out) {
-  static std::mutex mu;
-  static EncodeTiled fn = nullptr;
-  std::lock_guard<std::mutex> lock(mu);
-  if (!fn) {
-    void* p = nullptr;
-    cudaDriverEntryPointQueryResult q;
-    YN_CUDA_T(cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &q));
-    if (!p || q != cudaDriverEntryPointSuccess)
-      return host_fail(YN_E_CUDA, "cuTensorMapEncodeTiled is not available from the driver");
-    fn = reinterpret_cast<EncodeTiled>(p);
-  }
-  *out = fn;
-  return YN_OK;
-}
-
 // Row maps over `rows` rows of `cols` 16-bit elements: boxes of 64 elements x
 // 16 << i rows, 128-byte swizzle (the UMMA K-major layout), zero fill.
 int make_row_maps(const void* base, long long rows, int cols, bool bf16, TcMaps* maps) {
-  EncodeTiled fn;
-  int rc = encode_fn(&fn);
+  TmapEncode fn;
+  int rc = host_tmap_encode(&fn);
   if (rc) return rc;
   if (reinterpret_cast<uintptr_t>(base) % 16 || (cols * 2) % 16)
     return host_fail(YN_E_INVALID, "tensor-map rows must be 16-byte aligned");
@@ -98,6 +76,26 @@ size_t tc_smem(int Kd, int bits) {
   return 1024 + (size_t)TC_S * (TC_A_BYTES + TC_B_BYTES) + ring + (2 * TC_S + 4) * 8 + 16;
 }
 }  // namespace
+
+namespace ynb {
+// cuTensorMapEncodeTiled through the runtime's driver entry point (no link
+// against the driver library).
+int host_tmap_encode(TmapEncode* out) {
+  static std::mutex mu;
+  static TmapEncode fn = nullptr;
+  std::lock_guard<std::mutex> lock(mu);
+  if (!fn) {
+    void* p = nullptr;
+    cudaDriverEntryPointQueryResult q;
+    YN_CUDA_T(cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &q));
+    if (!p || q != cudaDriverEntryPointSuccess)
+      return host_fail(YN_E_CUDA, "cuTensorMapEncodeTiled is not available from the driver");
+    fn = reinterpret_cast<TmapEncode>(p);
+  }
+  *out = fn;
+  return YN_OK;
+}
+}  // namespace ynb
 
 extern "C" size_t yn_rows_route_bytes(const yn_dims* dims, int32_t max_rows) {
   if (!dims || max_rows < 1 || max_rows > ROUTE_MAX_ROWS) return 0;
@@ -186,6 +184,13 @@ extern "C" int yn_rows_route_shared(const yn_dims* dims, int32_t T, void* ws, vo
   const RouteWs L = route_ws(*dims, T);
   *act_sh = reinterpret_cast<uint8_t*>(ws) + L.act_sh;
   *sgate = reinterpret_cast<float*>(reinterpret_cast<uint8_t*>(ws) + L.sgate);
+  return YN_OK;
+}
+
+extern "C" int yn_rows_route_logits(const yn_dims* dims, int32_t T, void* ws, float** logits) {
+  if (!dims || !ws || !logits) return host_fail(YN_E_INVALID, "null argument");
+  if (T < 1 || T > ROUTE_MAX_ROWS) return host_fail(YN_E_UNSUPPORTED, "rows must be in [1, 4096]");
+  *logits = reinterpret_cast<float*>(reinterpret_cast<uint8_t*>(ws) + route_ws(*dims, T).logits);
   return YN_OK;
 }
 

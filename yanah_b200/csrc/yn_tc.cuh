@@ -36,6 +36,7 @@
 #include "yn_common.cuh"
 #include "yn_moe.cuh"
 #include "yn_mma.cuh"
+#include "yn_tcgen05.cuh"
 
 namespace ynb {
 
@@ -100,19 +101,6 @@ YN_DEV int kperm_fmt(int k) {
   return (k & ~15) | (2 * p + (j == MmaFmt<BITS>::hi(p) ? 1 : 0));
 }
 
-YN_DEV uint64_t tc_desc(uint32_t smem_addr) {
-  // K-major, 128-byte swizzle: start address (>>4), leading offset 1 (unused
-  // for swizzled K-major), stride offset 1024 bytes between 8-row atoms,
-  // version 1, layout type 2 (SWIZZLE_128B)
-  uint64_t d = 0;
-  d |= (uint64_t)((smem_addr >> 4) & 0x3FFFu);
-  d |= (uint64_t)1u << 16;
-  d |= (uint64_t)(1024u >> 4) << 32;
-  d |= (uint64_t)1u << 46;
-  d |= (uint64_t)2u << 61;
-  return d;
-}
-
 YN_DEV uint32_t tc_idesc(int n, bool bf16) {
   // f32 accumulate (bits 4-5 = 1), A and B fp16 (format 0) or bf16 (format 1),
   // both K-major, N >> 3 at bits 17-22, M >> 4 at bits 24-28
@@ -127,14 +115,6 @@ YN_DEV void tc_mma(uint32_t tmem_d, uint64_t adesc, uint64_t bdesc, uint32_t ide
       "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}"
       ::"r"(tmem_d), "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate));
 }
-
-YN_DEV void tc_commit(uint64_t* bar) {
-  asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_u32(bar))
-               : "memory");
-}
-
-YN_DEV void tc_fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
-YN_DEV void tc_fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
 
 // 32 consecutive fp32 columns of this thread's TMEM lane.
 YN_DEV void tc_ld32(uint32_t taddr, float (&v)[32]) {
@@ -278,17 +258,6 @@ YN_DEV void tc_dequant_gen(const uint8_t* codes, uint16_t sc_bits, uint16_t bi_b
 YN_DEV float swiglu_bf16_fast(float g, float u) {
   const float sg = bf16r(__fdividef(1.0f, 1.0f + __expf(-g)));
   return bf16r(__fmul_rn(bf16r(__fmul_rn(g, sg)), u));
-}
-
-YN_DEV void tc_tma_rows(void* dst, const CUtensorMap* map, int x, int y, uint64_t* bar) {
-  asm volatile(
-      "cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];" ::
-          "r"(smem_u32(dst)), "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(smem_u32(bar))
-      : "memory");
-}
-
-YN_DEV void mbar_arrive1(uint64_t* bar) {
-  asm volatile("mbarrier.arrive.release.cta.shared::cta.b64 _, [%0];" ::"r"(smem_u32(bar)) : "memory");
 }
 
 // Warp-specialised persistent form. 32 * (TC_PW + TC_EPW + 2) threads: warps

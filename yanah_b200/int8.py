@@ -1,0 +1,152 @@
+"""Matrix products in 8-bit integers with one scale per row (token) and one per output
+channel, and the routed experts of an MoE layer in that form.
+
+Beside the group-affine products of the records (``yn_qlinear``, ``yn_tc_experts``):
+those keep the checkpoint's 2 / 4 / 8-bit codes, these trade memory (one byte per
+weight) for the tensor cores' integer rate. ``PrefillStack(experts="int8")`` runs its
+prompt passes on them, ``speculation.verify_rows`` its LM head.
+
+    w = quantize_rows(weight)                  # (N, K) -> codes, channel scales; once
+    y = int8_linear(x, w)                      # (T, K) -> (T, N)
+    out = int8_experts(x, ids, weights, gate, up, down, residual=h)
+
+Every call quantises the rows it is given (code = the whole number nearest to
+127 x / max|x|). Sums are exact in 32 bits.
+"""
+from __future__ import annotations
+
+import ctypes as C
+from typing import NamedTuple, Optional
+
+import torch
+
+from . import _lib
+from .launch import DTYPES, check_floats, check_like, elsewhere, row_stride, rows_of, run_there
+
+
+class Int8Matrix(NamedTuple):
+    """``codes`` (N, K) int8, or (E, N, K) for a matrix per expert, and ``scales`` (N) or
+    (E, N) fp32 of the output channels. Rows of codes start at multiples of 16 bytes, as
+    ``quantize_rows`` lays them out."""
+    codes: torch.Tensor
+    scales: torch.Tensor
+
+
+def quantize_rows(x: torch.Tensor, stream: Optional[torch.cuda.Stream] = None) -> Int8Matrix:
+    """Rows (..., K) as 8-bit codes with one scale each: activations per token, weights
+    per output channel. A row with an infinity or a NaN gets a NaN scale."""
+    check_floats(x, "x")
+    if elsewhere(x.device, stream):
+        return run_there(lambda: quantize_rows(x), x.device, stream, (x,))
+    if x.dim() < 1 or x.shape[-1] < 1:
+        raise ValueError("x must have at least one column")
+    k = x.shape[-1]
+    flat = rows_of(x.reshape(-1, k), "x")
+    rows = flat.shape[0]
+    codes = torch.empty((rows, (k + 15) // 16 * 16), dtype=torch.int8, device=x.device)
+    scales = torch.empty((rows,), dtype=torch.float32, device=x.device)
+    _lib.check(_lib.lib().yn_i8_quant_rows(flat.data_ptr(), DTYPES[x.dtype], row_stride(flat), rows, k, codes.data_ptr(),
+                                           codes.stride(0), scales.data_ptr(),
+                                           torch.cuda.current_stream(x.device).cuda_stream))
+    lead = x.shape[:-1]
+    return Int8Matrix(codes.view(*lead, codes.shape[-1])[..., :k], scales.view(lead))
+
+
+def _mat(w: Int8Matrix, like: torch.Tensor, what: str) -> _lib.I8Mat:
+    codes, scales = w
+    if codes.dtype != torch.int8 or scales.dtype != torch.float32:
+        raise TypeError(f"{what} must have int8 codes and float32 scales")
+    if codes.dim() not in (2, 3) or scales.shape != codes.shape[:-1]:
+        raise ValueError(f"{what}: codes (N, K) or (E, N, K) with scales (N) or (E, N)")
+    if codes.device != like.device or scales.device != like.device:
+        raise ValueError(f"{what} is not on {like.device}")
+    n, k = codes.shape[-2:]
+    e = codes.shape[0] if codes.dim() == 3 else 1
+    if (k > 1 and codes.stride(-1) != 1) or (n > 1 and scales.stride(-1) != 1):
+        raise ValueError(f"{what}: a row's codes and a matrix's scales must be adjacent")
+    rs = codes.stride(-2) if n > 1 else (k + 15) // 16 * 16
+    many = codes.dim() == 3 and e > 1
+    return _lib.I8Mat(codes.data_ptr(), scales.data_ptr(), rs, codes.stride(0) if many else rs * n,
+                      scales.stride(0) if many else n, e, n, k)
+
+
+def int8_linear(x: torch.Tensor, w: Int8Matrix, out_dtype: Optional[torch.dtype] = None,
+                stream: Optional[torch.cuda.Stream] = None) -> torch.Tensor:
+    """x (T, K) in fp32, bf16 or fp16 times the transpose of w (N, K): (T, N) in
+    ``out_dtype`` (default: that of x), rounded once from fp32. Any number of rows."""
+    check_floats(x, "x")
+    if elsewhere(x.device, stream):
+        return run_there(lambda: int8_linear(x, w, out_dtype), x.device, stream, (x, *w))
+    x = rows_of(x, "x")
+    if w.codes.dim() != 2:
+        raise ValueError("w must be one matrix (N, K)")
+    m = _mat(w, x, "w")
+    if x.shape[1] != m.cols:
+        raise ValueError(f"x has {x.shape[1]} columns, w {m.cols}")
+    out_dtype = out_dtype or x.dtype
+    if out_dtype not in DTYPES:
+        raise TypeError(f"out_dtype must be float32, bfloat16 or float16, not {out_dtype}")
+    rows = x.shape[0]
+    y = torch.empty((rows, m.rows), dtype=out_dtype, device=x.device)
+    lib = _lib.lib()
+    nb = int(lib.yn_i8_linear_ws_bytes(rows, m.cols))
+    ws = torch.empty(nb, dtype=torch.uint8, device=x.device) if nb else None
+    _lib.check(lib.yn_i8_linear(C.byref(m), x.data_ptr(), DTYPES[x.dtype], row_stride(x), rows, y.data_ptr(),
+                                DTYPES[out_dtype], m.rows, None if ws is None else ws.data_ptr(), nb,
+                                torch.cuda.current_stream(x.device).cuda_stream))
+    return y
+
+
+def int8_experts(x: torch.Tensor, ids: torch.Tensor, weights: torch.Tensor, gate: Int8Matrix, up: Int8Matrix,
+                 down: Int8Matrix, residual: Optional[torch.Tensor] = None,
+                 stream: Optional[torch.cuda.Stream] = None, out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """residual + sum over a row's experts of weight * down(silu(gate x) * up x).
+
+    x (T, H); ids (T, k) int32 and weights (T, k) fp32 as ``routing.route_scored``
+    returns them: an id of -1 has no expert (any other id outside [0, E) is left out and
+    reported by ``check_error``). gate, up: (E, I, H); down: (E, H, I). The activations
+    are quantised per (row, expert), the sum is fp32 and rounded once to the type of x.
+    ``out``: (T, H) to write, rows of adjacent elements; it may be the residual."""
+    check_floats(x, "x")
+    if elsewhere(x.device, stream):
+        return run_there(lambda: int8_experts(x, ids, weights, gate, up, down, residual, out=out), x.device, stream,
+                         (x, ids, weights, residual, out, *gate, *up, *down))
+    x = rows_of(x, "x")
+    rows, h = x.shape
+    if ids.dim() != 2:
+        raise ValueError("ids must be (T, k)")
+    k = ids.shape[1]
+    check_like(ids, x, (rows, k), (torch.int32,), "ids")
+    check_like(weights, x, (rows, k), (torch.float32,), "weights")
+    g, u, d = _mat(gate, x, "gate"), _mat(up, x, "up"), _mat(down, x, "down")
+    if g.cols != h:
+        raise ValueError(f"x has {h} columns, gate {g.cols}")
+    ids, weights = ids.contiguous(), weights.contiguous()
+    if residual is not None:
+        check_like(residual, x, (rows, h), (x.dtype,), "residual")
+        residual = rows_of(residual, "residual")
+    if out is None:
+        out = torch.empty((rows, h), dtype=x.dtype, device=x.device)
+    else:
+        check_like(out, x, (rows, h), (x.dtype,), "out")
+        if rows_of(out, "out") is not out:
+            raise ValueError("out must have rows of adjacent elements that do not overlap")
+    lib, dt = _lib.lib(), DTYPES[x.dtype]
+    nb = int(lib.yn_i8_experts_ws_bytes(rows, k, g.n_mats, h, g.rows, dt))
+    ws = torch.empty(nb, dtype=torch.uint8, device=x.device)
+    _lib.check(lib.yn_i8_experts(C.byref(g), C.byref(u), C.byref(d), x.data_ptr(), dt, row_stride(x), rows,
+                                 ids.data_ptr(), weights.data_ptr(), k,
+                                 None if residual is None else residual.data_ptr(),
+                                 0 if residual is None else row_stride(residual), out.data_ptr(), row_stride(out),
+                                 ws.data_ptr(), nb,
+                                 torch.cuda.current_stream(x.device).cuda_stream))
+    return out
+
+
+def check_error(device=None) -> int:
+    """Read and clear the error word of the 8-bit products on a device (synchronises its
+    current stream): 0, or a code as ``CudaMoEBackend.check_error`` returns."""
+    code = C.c_int32(0)
+    with torch.cuda.device(device):
+        _lib.check(_lib.lib().yn_i8_error(torch.cuda.current_stream().cuda_stream, C.byref(code)))
+    return code.value

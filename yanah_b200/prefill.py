@@ -8,6 +8,11 @@ the reference's prefill sweep plans its staging groups (sweep.py:80-138); the gr
 (`yn_tc_experts`, 128 weight rows x up to 256 rows per tile); the combine in
 column order plus the residual (`yn_pairs_combine`). The grouping runs on the
 device (`yn_prefill_plan`); `plan_prefill` is its host restatement.
+
+Two things can be chosen: `rule` routes by a `routing.RouteRule` instead of the
+softmax top-k (the logits of `yn_rows_route` through `yn_route_scored`), and
+`experts="int8"` holds the routed experts as 8-bit matrices with channel scales
+(made once from the records) and runs a layer's experts as `int8.int8_experts`.
 """
 from __future__ import annotations
 
@@ -19,11 +24,23 @@ import torch
 
 from . import _lib
 from .device import DeviceLayer, ExpertArena, dims_struct, fill_synthetic_experts, stream_ptr
+from .formats import RecordSpec
+from .int8 import Int8Matrix, int8_experts, quantize_rows
+from .int8 import check_error as int8_error
+from .routing import RouteRule, route_scored
 from .synthetic import StackConfig, dense_layer
 
 TILE_ROWS = 256      # token rows per tile
 UP_UNITS = 64        # gate/up units per tile (128 weight rows)
 DOWN_ROWS = 128      # down output rows per tile
+
+
+def route_logits(ws: torch.Tensor, dims: _lib.Dims, rows: int) -> torch.Tensor:
+    """The router logits (rows, E) fp32 that `yn_rows_route` of that many rows left in its workspace."""
+    p = C.c_void_p()
+    _lib.check(_lib.lib().yn_rows_route_logits(C.byref(dims), rows, ws.data_ptr(), C.byref(p)))
+    off, n = p.value - ws.data_ptr(), rows * dims.n_experts * 4
+    return ws[off:off + n].view(torch.float32).view(rows, dims.n_experts)
 
 
 class TcTile(C.Structure):
@@ -52,15 +69,49 @@ def plan_prefill(ids: np.ndarray, n_experts: int, inter: int, hidden: int):
             np.array(down, np.int32).reshape(-1, 4))
 
 
+def int8_matrices(arena: ExpertArena, spec: RecordSpec, n_experts: int, hidden: int, inter: int,
+                  first_slot: int = 0) -> Tuple[Int8Matrix, Int8Matrix, Int8Matrix]:
+    """The gate, up and down matrices (E, I, H), (E, I, H), (E, H, I) of the records in
+    slots first_slot.. of an arena, dequantised and quantised again with one scale per
+    output channel. Once, at load time."""
+    lib, out = _lib.lib(), []
+    dev = arena.buf.device
+    with torch.cuda.device(dev):
+        for part, (rows, cols) in enumerate(((inter, hidden), (inter, hidden), (hidden, inter))):
+            codes = torch.zeros((n_experts, rows, (cols + 15) // 16 * 16), dtype=torch.int8, device=dev)
+            scales = torch.empty((n_experts, rows), dtype=torch.float32, device=dev)
+            full = torch.empty((rows, cols), dtype=torch.float32, device=dev)
+            for e in range(n_experts):
+                rec = arena.base + (first_slot + e) * arena.slot_bytes
+                m = _lib.QMat(*(rec + spec.offsets[3 * part + i] for i in range(3)), rows, cols, spec.bits,
+                              spec.group_size)
+                _lib.check(lib.yn_dequantize(C.byref(m), full.data_ptr(), stream_ptr()))
+                q = quantize_rows(full)
+                codes[e, :, :cols] = q.codes
+                scales[e] = q.scales
+            out.append(Int8Matrix(codes[..., :cols], scales))
+    return tuple(out)
+
+
 class PrefillStack:
     """Resident experts and dense weights of `layers` of `cfg`, and the
     buffers for prompts of up to `max_rows` rows in total. A layer runs
     entirely on the device (routing, grouping, GEMMs, combine): no host
-    synchronisation."""
+    synchronisation. rule / choice_bias: route by a rule, with a bias (layers, E)
+    fp32 on its choice. experts: "records" (4-bit codes as they are) or "int8"."""
 
     def __init__(self, cfg: StackConfig, max_rows: int, device: str = "cuda",
-                 layers: Optional[Sequence[int]] = None):
+                 layers: Optional[Sequence[int]] = None, rule: Optional[RouteRule] = None,
+                 choice_bias: Optional[torch.Tensor] = None, experts: str = "records"):
+        if experts not in ("records", "int8"):
+            raise ValueError(f"experts must be 'records' or 'int8', not {experts!r}")
+        if rule is not None and rule.top_k != cfg.top_k:
+            raise ValueError(f"the rule chooses {rule.top_k} experts, the configuration {cfg.top_k}")
+        if choice_bias is not None and rule is None:
+            raise ValueError("choice_bias needs a rule")
         self.cfg = cfg
+        self.rule, self.choice_bias = rule, choice_bias
+        self.int8: Optional[List[Tuple[Int8Matrix, Int8Matrix, Int8Matrix]]] = [] if experts == "int8" else None
         self.device = torch.device(device)
         self.layer_ids = list(range(cfg.n_layers)) if layers is None else list(layers)
         self.dims = dims_struct(cfg)
@@ -70,6 +121,9 @@ class PrefillStack:
             spec = cfg.record_spec(l)
             arena = ExpertArena(cfg.n_experts, spec.slot_bytes, self.device)
             fill_synthetic_experts(arena, cfg, l)
+            if self.int8 is not None:
+                self.int8.append(int8_matrices(arena, spec, cfg.n_experts, cfg.hidden, cfg.moe_inter))
+                arena = ExpertArena(1, 16, self.device)      # the records are not kept
             self.arenas.append(arena)
             self.layers.append(DeviceLayer(cfg, l, dense_layer(cfg, l), arena, 0, None, self.device))
         self.structs = [L.struct() for L in self.layers]
@@ -111,6 +165,13 @@ class PrefillStack:
         D, L = C.byref(self.dims), C.byref(self.structs[i])
         _lib.check(lib.yn_rows_route(D, L, h.data_ptr(), T, self.x.data_ptr(), self.ids.data_ptr(), self.w.data_ptr(),
                                      self.route_ws.data_ptr(), self.route_ws.numel(), st))
+        if self.rule is not None:
+            route_scored(route_logits(self.route_ws, self.dims, T), self.rule,
+                         None if self.choice_bias is None else self.choice_bias[i], stream=stream,
+                         out=(self.ids[:T], self.w[:T]))
+        if self.int8 is not None:
+            int8_experts(self.x[:T], self.ids[:T], self.w[:T], *self.int8[i], residual=h, stream=stream, out=out)
+            return
         _lib.check(lib.yn_prefill_plan(D, self.ids.data_ptr(), T, self.pair_row.data_ptr(), self.pair_of.data_ptr(),
                                        self.tiles_up.data_ptr(), self.max_up, self.tiles_dn.data_ptr(), self.max_dn,
                                        self.n_tiles.data_ptr(), self.err.data_ptr(), st))
@@ -131,7 +192,9 @@ class PrefillStack:
                                         h.data_ptr(), T, out.data_ptr(), st))
 
     def plan(self, T: int):
-        """Host copies of the last layer's ids, pair -> row and (row, column) -> pair."""
+        """Host copies of the last layer's ids, pair -> row and (row, column) -> pair (record experts)."""
+        if self.int8 is not None:
+            raise ValueError("the 8-bit experts keep their grouping to themselves")
         K = self.cfg.top_k
         return (self.ids[:T].cpu().numpy(), self.pair_row[:T * K].cpu().numpy(),
                 self.pair_of[:T * K].cpu().numpy().reshape(T, K))
@@ -151,7 +214,7 @@ class PrefillStack:
         _lib.check(_lib.lib().yn_route_error(self.route_ws.data_ptr(), C.byref(self.dims), stream_ptr(),
                                              C.byref(rc)))
         self.err.zero_()
-        return code or rc.value
+        return code or rc.value or (int8_error(self.device) if self.int8 is not None else 0)
 
 
 def kperm_inverse(a: np.ndarray) -> np.ndarray:

@@ -1,0 +1,95 @@
+"""Routing of rows of router logits by a rule: softmax or sigmoid scores, a bias for
+balance that moves the choice but not the weights, groups of experts, the top k and
+their (renormalised) weights.
+
+Beside ``yn_route``, which is the softmax top-k of the reference's models
+(mlx_backend.py:308-316). ``PrefillStack(rule=...)`` and ``CudaMoEBackend(rule=...)``
+route their layers by such a rule; the ids and weights are those that
+``int8.int8_experts`` and the record-based expert kernels take.
+
+    rule = RouteRule(top_k=8, score="sigmoid", n_groups=8, top_groups=4, scale=2.5)
+    ids, weights = route_scored(logits, rule, bias=balance)
+"""
+from __future__ import annotations
+
+import ctypes as C
+from dataclasses import dataclass
+from typing import Optional, Tuple
+
+import torch
+
+from . import _lib
+from .launch import DTYPES, check_floats, check_like, elsewhere, row_stride, rows_of, run_there
+
+SCORES = {"softmax": 0, "sigmoid": 1}
+
+
+@dataclass(frozen=True)
+class RouteRule:
+    """How a row chooses its experts.
+
+    top_k: experts per row (<= 31). score: "softmax" or "sigmoid". n_groups: the
+    experts in that many equal, consecutive groups, of which a row uses the
+    ``top_groups`` best; a group's score is the sum of its ``group_top`` (1 or 2)
+    largest choice values. norm_topk: divide the weights by their sum. scale:
+    factor of the weights."""
+    top_k: int
+    score: str = "softmax"
+    n_groups: int = 1
+    top_groups: int = 1
+    group_top: int = 2
+    norm_topk: bool = True
+    scale: float = 1.0
+
+    def __post_init__(self):
+        if self.score not in SCORES:
+            raise ValueError(f"score must be 'softmax' or 'sigmoid', not {self.score!r}")
+        object.__setattr__(self, "_structs", {})
+
+    def struct(self, n_experts: int) -> _lib.RouteRuleStruct:
+        s = self._structs.get(n_experts)
+        if s is None:
+            s = self._structs[n_experts] = _lib.RouteRuleStruct(
+                n_experts, self.top_k, SCORES[self.score], self.n_groups, self.top_groups, self.group_top,
+                int(self.norm_topk), self.scale)
+        return s
+
+
+def route_scored(logits: torch.Tensor, rule: RouteRule, bias: Optional[torch.Tensor] = None,
+                 available: Optional[torch.Tensor] = None, stream: Optional[torch.cuda.Stream] = None,
+                 out: Optional[Tuple[torch.Tensor, torch.Tensor]] = None) -> Tuple[torch.Tensor, torch.Tensor]:
+    """Ids (T, k) int32 and weights (T, k) fp32 of rows of router logits (T, E) in
+    fp32, bf16 or fp16.
+
+    The choice value of an expert is its score plus ``bias`` (E) fp32; ids are in
+    descending order of it, equal ones by id; the order is that of exact arithmetic.
+    The weights are the scores of the chosen. An expert does not take part where
+    ``available`` (E) (bool or uint8) is false or its logit is -inf or NaN; rows with
+    fewer than k experts left end in ids of -1 with weight 0. Any number of rows.
+    ``out``: contiguous ids and weights to write."""
+    check_floats(logits, "logits")
+    if elsewhere(logits.device, stream):
+        return run_there(lambda: route_scored(logits, rule, bias, available, out=out), logits.device, stream,
+                         (logits, bias, available, *(out or ())))
+    logits = rows_of(logits, "logits")
+    rows, e = logits.shape
+    if bias is not None:
+        check_like(bias, logits, (e,), (torch.float32,), "bias")
+        bias = bias.contiguous()
+    if available is not None:
+        check_like(available, logits, (e,), (torch.bool, torch.uint8), "available")
+        available = available.contiguous()
+    if out is None:
+        ids = torch.empty((rows, rule.top_k), dtype=torch.int32, device=logits.device)
+        weights = torch.empty((rows, rule.top_k), dtype=torch.float32, device=logits.device)
+    else:
+        ids, weights = out
+        check_like(ids, logits, (rows, rule.top_k), (torch.int32,), "out ids")
+        check_like(weights, logits, (rows, rule.top_k), (torch.float32,), "out weights")
+        if not (ids.is_contiguous() and weights.is_contiguous()):
+            raise ValueError("out must be contiguous")
+    _lib.check(_lib.lib().yn_route_scored(
+        C.byref(rule.struct(e)), logits.data_ptr(), DTYPES[logits.dtype], row_stride(logits), rows,
+        None if bias is None else bias.data_ptr(), None if available is None else available.data_ptr(),
+        ids.data_ptr(), weights.data_ptr(), torch.cuda.current_stream(logits.device).cuda_stream))
+    return ids, weights

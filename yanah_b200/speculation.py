@@ -16,10 +16,14 @@ this library runs on the batch path (`ExpertParallelStack` with
   context growth since the last plain step.
 
 Depth starts at the requested maximum, clamped to [1, 16].
+
+`verify_rows` is the end of such a round: the verify rows' logits by an 8-bit LM head,
+what they say of the drafted tokens, and how many of those are accepted
+(speculative.py:121-193 compares greedy choices).
 """
 from __future__ import annotations
 
-from typing import List, Union
+from typing import List, NamedTuple, Union
 
 CALIBRATE = "calibrate"
 PLAIN = "plain"
@@ -66,3 +70,33 @@ class AdaptiveSpeculationPolicy:
             else:
                 self.depth = max(1, self.depth // 2)
                 self.draft = []
+
+
+class VerifyAnswer(NamedTuple):
+    """Of a draft of d tokens, on the device: `accepted` () int64, how many are accepted;
+    `next_token` () int32, the greedy choice after the last accepted one; `answers`
+    (logprobs.TokenLogprobs), per row what it says of its drafted token (the last row has
+    none) and its likeliest tokens."""
+    accepted: "torch.Tensor"
+    next_token: "torch.Tensor"
+    answers: "logprobs.TokenLogprobs"
+
+
+def verify_rows(rows, head, draft, n_top: int = 1) -> VerifyAnswer:
+    """The answer of a verify pass. rows: (1 + d, H), the final normalised hidden rows of the
+    last token and the d drafted ones; head: the LM head as an `int8.Int8Matrix` (V, H);
+    draft: (d,) int32. Row i answers for draft[i]: a drafted token is accepted while every
+    one up to it is its row's greedy choice (the largest logit, equal ones by the lower
+    id). Nothing is copied to the host."""
+    import torch
+
+    from .int8 import int8_linear
+    from .logprobs import token_logprobs
+    if draft.dim() != 1 or rows.dim() != 2 or rows.shape[0] != draft.shape[0] + 1:
+        raise ValueError("rows must be (1 + d, H) for a draft of d tokens")
+    if n_top < 1:
+        raise ValueError("n_top must be at least 1: the next token is the first of them")
+    tokens = torch.cat((draft, draft.new_full((1,), -1)))
+    answers = token_logprobs(int8_linear(rows, head, out_dtype=torch.float32), tokens, n_top=n_top)
+    accepted = torch.cumprod(answers.rank[:-1] == 0, 0).sum()
+    return VerifyAnswer(accepted, answers.top_ids[:, 0].gather(0, accepted.view(1))[0], answers)
