@@ -62,8 +62,9 @@ __global__ void __launch_bounds__(I8_QT) k_i8_quant(const void* x, long long ldx
   auto out = [&](int j) -> long long { return to ? to[row * copies + j] : (long long)row; };
   if (tid < n_to && out(tid) >= 0) scales[out(tid)] = scale;
   auto put8 = [&](int at, const float (&g)[8]) {
-    const uint2 c = make_uint2(i8_pack4(q.code(g[0]), q.code(g[1]), q.code(g[2]), q.code(g[3])),
-                               i8_pack4(q.code(g[4]), q.code(g[5]), q.code(g[6]), q.code(g[7])));
+    uint32_t w[2];
+    q.codes(g, w);
+    const uint2 c = make_uint2(w[0], w[1]);
     for (int j = 0; j < n_to; ++j) {
       const long long r = out(j);
       if (r >= 0) *reinterpret_cast<uint2*>(codes + r * ldc + 8 * at) = c;
@@ -78,7 +79,10 @@ __global__ void __launch_bounds__(I8_QT) k_i8_quant(const void* x, long long ldx
     put8(at, g);
   }
   for (int k = 8 * n8 + tid; k < K; k += I8_QT) {
-    const int8_t c = (int8_t)q.code(I8In<T>::load(x, base + k));
+    const float g[4] = {I8In<T>::load(x, base + k), 0.0f, 0.0f, 0.0f};
+    uint32_t w[1];
+    q.codes(g, w);
+    const int8_t c = (int8_t)w[0];
     for (int j = 0; j < n_to; ++j)
       if (out(j) >= 0) codes[out(j) * ldc + k] = c;
   }
@@ -133,10 +137,12 @@ YN_DEV void i8_row_smem(int dt, const void* x, size_t base, int K, int KP, int8_
   const I8Row q(m);
   if (at == 0) *scale = q.scale();
   for (int k = 4 * at; k < KP; k += 4 * n) {
-    int c[4];
+    float f[4];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) c[i] = k + i < K ? q.code(i8_load(dt, x, base + k + i)) : 0;
-    *reinterpret_cast<uint32_t*>(codes + k) = i8_pack4(c[0], c[1], c[2], c[3]);
+    for (int i = 0; i < 4; ++i) f[i] = k + i < K ? i8_load(dt, x, base + k + i) : 0.0f;
+    uint32_t w[1];
+    q.codes(f, w);
+    *reinterpret_cast<uint32_t*>(codes + k) = w[0];
   }
 }
 
@@ -346,10 +352,12 @@ __global__ void __launch_bounds__(256) k_i8_act_codes(const int16_t* act, long l
     const uint4 v = *reinterpret_cast<const uint4*>(a + u);
     const uint32_t w[4] = {v.x, v.y, v.z, v.w};
     const float s = bs[u >> 5] * (1.0f / 32767.0f);
-    int c[8];
+    float f[8];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) c[i] = q.code((float)(int16_t)(w[i >> 1] >> (16 * (i & 1))) * s);
-    *reinterpret_cast<uint2*>(codes + p * ldc + u) = make_uint2(i8_pack4(c[0], c[1], c[2], c[3]), i8_pack4(c[4], c[5], c[6], c[7]));
+    for (int i = 0; i < 8; ++i) f[i] = (float)(int16_t)(w[i >> 1] >> (16 * (i & 1))) * s;
+    uint32_t c[2];
+    q.codes(f, c);
+    *reinterpret_cast<uint2*>(codes + p * ldc + u) = make_uint2(c[0], c[1]);
   }
 }
 
@@ -594,6 +602,8 @@ extern "C" int yn_i8_linear(const yn_i8_mat* w, const void* x, int32_t dtype, in
   a.sw = w->scales;
   a.y = y;
   a.y_stride = y_stride;
+  a.store_cols = w->rows;
+  a.pairs = reinterpret_cast<uintptr_t>(y) % 4 == 0 && y_stride % 2 == 0;
   const int nb = box_rows((int)std::min<int64_t>(rows, 256));
   I8Maps maps{};
   if ((rc = tmap_mats(&maps.a, *w)) || (rc = tmap_2d(&maps.b, codes, w->cols, rows, ldc, nb))) return rc;
@@ -697,6 +707,8 @@ extern "C" int yn_i8_experts(const yn_i8_mat* gate, const yn_i8_mat* up, const y
   d.sw_stride = down->scale_stride;
   d.y = y;
   d.y_stride = L.ldy;
+  d.store_cols = (int)L.ldy;
+  d.pairs = true;
   const bool yb = dtype == YN_BF16;
   if ((rc = launch_gemm_out(yb ? YN_BF16 : YN_F32, L.nb, d, md2, td, st))) return rc;
   const dim3 cg((H + 4 * 128 - 1) / (4 * 128), (unsigned)rows);

@@ -41,6 +41,17 @@ YN_DEV __nv_bfloat16 i8_out<__nv_bfloat16>(float v) { return __float2bfloat16_rn
 template <>
 YN_DEV __half i8_out<__half>(float v) { return __float2half_rn(v); }
 
+template <typename O>
+YN_DEV uint32_t i8_pack2(float lo, float hi) {
+  if constexpr (std::is_same_v<O, __half>) {
+    __half2 h = __floats2half2_rn(lo, hi);
+    return *reinterpret_cast<uint32_t*>(&h);
+  } else {
+    __nv_bfloat162 h = __floats2bfloat162_rn(lo, hi);
+    return *reinterpret_cast<uint32_t*>(&h);
+  }
+}
+
 // Element by element; 8 at a time where rows are 16-byte aligned.
 template <typename T>
 YN_DEV void i8_load8(const void* p, size_t i, float (&f)[8]) {
@@ -75,18 +86,36 @@ struct I8Row {
   YN_DEV float scale() const {
     return __float_as_uint(amax) >= 0x7F800000u ? __int_as_float(0x7fc00000) : __fdiv_rn(amax, 127.0f);
   }
-  YN_DEV int code(float x) const {
-    float y = __fmul_rn(x, inv), q = rintf(y);
-    if (exact || fabsf(fabsf(y - q) - 0.5f) < 6.2e-5f)
-      q = amax > 0.0f ? (float)rint(127.0 * (double)x / (double)amax) : 0.0f;
-    return __float_as_uint(amax) >= 0x7F800000u ? 0 : (int)q;   // NaN * 0 stays out of the codes
+  // The codes of N values (N a multiple of 4), four to a word. Adding 1.5 * 2^23 rounds y to
+  // the nearest whole number, ties to even, and leaves it in the low bits.
+  template <int N>
+  YN_DEV void codes(const float (&x)[N], uint32_t (&out)[N / 4]) const {
+    float t[N];
+    bool near = exact;
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      const float y = __fmul_rn(x[i], inv);
+      t[i] = __fadd_rn(y, 12582912.0f);
+      near |= fabsf(__fsub_rn(y, __fsub_rn(t[i], 12582912.0f))) > 0.5f - 6.2e-5f;
+    }
+    if (near) {
+#pragma unroll
+      for (int i = 0; i < N; ++i) {
+        const float y = __fmul_rn(x[i], inv);
+        if (exact || fabsf(__fsub_rn(y, __fsub_rn(t[i], 12582912.0f))) > 0.5f - 6.2e-5f)
+          t[i] = amax > 0.0f ? __fadd_rn((float)rint(127.0 * (double)x[i] / (double)amax), 12582912.0f) : 12582912.0f;
+      }
+    }
+    const bool none = __float_as_uint(amax) >= 0x7F800000u;   // infinities and NaN stay out of the codes
+#pragma unroll
+    for (int i = 0; i < N / 4; ++i) {
+      const uint32_t lo = __byte_perm(__float_as_uint(t[4 * i]), __float_as_uint(t[4 * i + 1]), 0x0040);
+      const uint32_t hi = __byte_perm(__float_as_uint(t[4 * i + 2]), __float_as_uint(t[4 * i + 3]), 0x0040);
+      out[i] = none ? 0u : __byte_perm(lo, hi, 0x5410);
+    }
   }
 };
 YN_DEV uint32_t i8_abs_bits(float x) { return __float_as_uint(x) & 0x7FFFFFFFu; }
-
-YN_DEV uint32_t i8_pack4(int a, int b, int c, int d) {
-  return (uint32_t)(a & 255) | ((uint32_t)(b & 255) << 8) | ((uint32_t)(c & 255) << 16) | ((uint32_t)d << 24);
-}
 
 YN_DEV uint32_t block_max_u32(uint32_t v, uint32_t* buf) {
   v = __reduce_max_sync(0xffffffffu, v);
@@ -117,6 +146,8 @@ struct I8Gemm {
   long long sw_stride, sw_up_stride;
   void* y;                 // (rows, y_stride): output, or UP: int16 activations
   long long y_stride;
+  int store_cols;          // columns of a row that may be written: channels, or more where rows are padded
+  bool pairs;              // 16-bit outputs may be written two channels at a time (4-byte aligned rows)
   float* bscale;           // UP: (rows, ceil(channels / 32)) scales of the activations' blocks
 };
 struct I8Maps {
@@ -244,30 +275,63 @@ __global__ void __launch_bounds__(I8_THREADS, 1) k_i8_gemm(const I8Gemm a, const
       if (!ok) break;
       tc_fence_after();
       const uint32_t base = tmem + (uint32_t)(b * F::COLS) + ((uint32_t)(32 * (warp & 3)) << 16);
+      // A lane holds one channel of 16 rows: two lanes exchange so that each writes two adjacent
+      // channels of every second row (even lanes the even rows).
+      const bool odd = lane & 1, two = (r | 1) < a.store_cols;
+      const uint32_t sel = odd ? 0x3276u : 0x5410u;
       for (int c0 = 16 * half; c0 < c.n; c0 += 32) {
         int v[16], w[16];
         i8_ld16(base + (uint32_t)c0, v);
         if (UP) i8_ld16(base + (uint32_t)(NB + c0), w);
-        const float sx = lane < 16 && c0 + lane < c.n ? a.sx[c.p0 + c0 + lane] : 0.0f;
+        const int left = c.n - c0;
+        const float sx = lane < min(16, left) ? a.sx[c.p0 + c0 + lane] : 0.0f;
         i8_ld_wait(v);
         if (UP) i8_ld_wait(w);
+        const long long row = c.p0 + c0;
+        if (UP) {
+          // 16 bits relative to the largest of these 32 units: off by at most 2^-16 of it, 1/516 of
+          // a step of the 8-bit code that follows
+          uint32_t* out = reinterpret_cast<uint32_t*>(reinterpret_cast<int16_t*>(a.y) + (row + odd) * a.y_stride + (r & ~1));
+          float bm = 0.0f;
 #pragma unroll
-        for (int k = 0; k < 16; ++k) {
-          const float s = __shfl_sync(0xffffffffu, sx, k);
-          if (c0 + k >= c.n) break;
-          const float g = (float)v[k] * s * sw;
-          const long long row = c.p0 + c0 + k;
-          if (UP) {
-            const float act = in ? i8_swiglu(g, (float)w[k] * s * su) : 0.0f;
-            // 16 bits relative to the largest of these 32 units: off by at most 2^-16 of it,
-            // 1/516 of a step of the 8-bit code that follows
-            const uint32_t mb = __reduce_max_sync(0xffffffffu, i8_abs_bits(act));
-            const float bm = __uint_as_float(mb);
-            const float q = bm > 0.0f ? rintf(act * __fdividef(32767.0f, bm)) : 0.0f;
-            if (in) reinterpret_cast<int16_t*>(a.y)[row * a.y_stride + r] = (int16_t)max(-32767, min(32767, (int)q));
-            if (lane == 0 && in) a.bscale[row * ((a.channels + 31) / 32) + (r >> 5)] = bm;
-          } else if (in) {
-            reinterpret_cast<O*>(a.y)[row * a.y_stride + r] = i8_out<O>(g);
+          for (int k = 0; k < 16; k += 2) {
+            float t[2];
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+              const float s = __shfl_sync(0xffffffffu, sx, k + i);
+              const float act = i8_swiglu((float)v[k + i] * s * sw, (float)w[k + i] * s * su);
+              const uint32_t mb = __reduce_max_sync(0xffffffffu, i8_abs_bits(act));
+              const float m = __uint_as_float(mb);
+              if (lane == k + i) bm = m;
+              t[i] = fmaf(act, m > 0.0f ? __fdividef(32767.0f, m) : 0.0f, 12582912.0f);   // the code in the low bits
+            }
+            const uint32_t own = __byte_perm(__float_as_uint(t[0]), __float_as_uint(t[1]), 0x5410);
+            const uint32_t other = __shfl_xor_sync(0xffffffffu, own, 1);
+            if (k + odd < left && (r & ~1) < a.channels) out[(size_t)k * a.y_stride / 2] = __byte_perm(own, other, sel);
+          }
+          if (lane < min(16, left) && u0 + 32 * (warp & 3) < a.channels)
+            a.bscale[(row + lane) * ((a.channels + 31) / 32) + (u0 >> 5) + (warp & 3)] = bm;
+        } else if (sizeof(O) == 2 && a.pairs) {
+          uint32_t* out = reinterpret_cast<uint32_t*>(reinterpret_cast<O*>(a.y) + (row + odd) * a.y_stride + (r & ~1));
+#pragma unroll
+          for (int k = 0; k < 16; k += 2) {
+            const float f0 = (float)v[k] * __shfl_sync(0xffffffffu, sx, k) * sw;
+            const float f1 = (float)v[k + 1] * __shfl_sync(0xffffffffu, sx, k + 1) * sw;
+            const uint32_t own = i8_pack2<O>(f0, f1);
+            const uint32_t other = __shfl_xor_sync(0xffffffffu, own, 1);
+            const uint32_t pk = __byte_perm(own, other, sel);
+            if (k + odd < left) {
+              if (two) out[(size_t)k * a.y_stride / 2] = pk;
+              else if ((r & ~1) < a.channels)
+                reinterpret_cast<uint16_t*>(out)[(size_t)k * a.y_stride] = (uint16_t)pk;
+            }
+          }
+        } else {
+          O* out = reinterpret_cast<O*>(a.y) + row * a.y_stride + r;
+#pragma unroll
+          for (int k = 0; k < 16; ++k) {
+            const float f = (float)v[k] * __shfl_sync(0xffffffffu, sx, k) * sw;
+            if (k < left && in) out[(size_t)k * a.y_stride] = i8_out<O>(f);
           }
         }
       }

@@ -15,11 +15,13 @@
 // The alternatives cost little beside that: every thread knows its own maximum
 // from the first step, so the n-th largest of the 256 thread maxima bounds the
 // n-th largest element from below, and only the about n threads that reach it
-// have their elements looked at again (from L2).
+// have their elements looked at again (from L2). Two fp32 values go through one
+// instruction where they can (fma.rn.f32x2).
 #include <cuda_runtime.h>
 
 #include <algorithm>
 #include <string>
+#include <type_traits>
 
 #include "yanah_b200.h"
 #include "yn_common.cuh"
@@ -73,7 +75,13 @@ struct LpType<float> {
     asm("max.NaN.f32 %0, %1, %2;" : "=f"(d) : "f"(__uint_as_float(a)), "f"(__uint_as_float(b)));
     return __float_as_uint(d);
   }
+  // -inf as a finite value whose exponential is 0 against any maximum above -4096
+  YN_DEV static uint32_t floor(uint32_t a) { return __float_as_uint(fmaxf(__uint_as_float(a), -1e30f)); }
   YN_DEV static float load(const void* p) { return __ldg(reinterpret_cast<const float*>(p)); }
+  // how many values of `a` are above `t` (a value in both halves, for 16-bit types), added to `c`
+  YN_DEV static uint32_t splat(float t) { return __float_as_uint(t); }
+  YN_DEV static void count(uint32_t a, uint32_t t, uint32_t& c) { c += __uint_as_float(a) > __uint_as_float(t); }
+  YN_DEV static int counted(uint32_t c) { return (int)c; }
 };
 template <>
 struct LpType<__nv_bfloat16> {
@@ -88,7 +96,21 @@ struct LpType<__nv_bfloat16> {
     asm("max.NaN.bf16x2 %0, %1, %2;" : "=r"(d) : "r"(a), "r"(b));
     return d;
   }
+  YN_DEV static uint32_t floor(uint32_t a) {
+    uint32_t d;
+    asm("max.bf16x2 %0, %1, %2;" : "=r"(d) : "r"(a), "r"(0xF149F149u));   // -1e30
+    return d;
+  }
   YN_DEV static float load(const void* p) { return bf16_to_f32(__ldg(reinterpret_cast<const uint16_t*>(p))); }
+  YN_DEV static uint32_t splat(float t) { return (__float_as_uint(t) >> 16) * 0x10001u; }
+  YN_DEV static void count(uint32_t a, uint32_t t, uint32_t& c) {   // counts of at most 256 are exact in bf16
+    __nv_bfloat162 x = *reinterpret_cast<__nv_bfloat162*>(&a), y = *reinterpret_cast<__nv_bfloat162*>(&t);
+    __nv_bfloat162 s = __hadd2(*reinterpret_cast<__nv_bfloat162*>(&c), __hgt2(x, y));
+    c = *reinterpret_cast<uint32_t*>(&s);
+  }
+  YN_DEV static int counted(uint32_t c) {
+    return (int)(__uint_as_float(c << 16) + __uint_as_float(c & 0xFFFF0000u));
+  }
 };
 template <>
 struct LpType<__half> {
@@ -103,8 +125,34 @@ struct LpType<__half> {
     asm("max.NaN.f16x2 %0, %1, %2;" : "=r"(d) : "r"(a), "r"(b));
     return d;
   }
+  YN_DEV static uint32_t floor(uint32_t a) {
+    uint32_t d;
+    asm("max.f16x2 %0, %1, %2;" : "=r"(d) : "r"(a), "r"(0xFBFFFBFFu));   // -65504
+    return d;
+  }
   YN_DEV static float load(const void* p) { return f16_to_f32(__ldg(reinterpret_cast<const uint16_t*>(p))); }
+  YN_DEV static uint32_t splat(float t) { return __half_as_ushort(__float2half_rn(t)) * 0x10001u; }
+  YN_DEV static void count(uint32_t a, uint32_t t, uint32_t& c) {
+    __half2 s = __hadd2(*reinterpret_cast<__half2*>(&c), __hgt2(*reinterpret_cast<__half2*>(&a), *reinterpret_cast<__half2*>(&t)));
+    c = *reinterpret_cast<uint32_t*>(&s);
+  }
+  YN_DEV static int counted(uint32_t c) {
+    return (int)(f16_to_f32((uint16_t)(c & 0xFFFFu)) + f16_to_f32((uint16_t)(c >> 16)));
+  }
 };
+
+// The largest value of the type below a finite t, as fp32.
+template <typename T>
+YN_DEV float lp_below(float t) {
+  constexpr uint32_t step = sizeof(T) == 4 ? 1u : std::is_same_v<T, __half> ? 0u : 0x10000u;
+  if constexpr (step == 0) {
+    const uint16_t h = __half_as_ushort(__float2half_rn(__fadd_rn(t, 0.0f)));
+    return f16_to_f32(h == 0 ? (uint16_t)0x8001u : (uint16_t)(h & 0x8000u ? h + 1 : h - 1));
+  } else {
+    const uint32_t b = __float_as_uint(__fadd_rn(t, 0.0f));
+    return __uint_as_float(b == 0 ? 0x80000000u + step : b & 0x80000000u ? b + step : b - step);
+  }
+}
 
 // The elements of a 16-byte vector, in order.
 template <typename T>
@@ -114,6 +162,24 @@ YN_DEV void lp_unpack(const uint4& v, float (&f)[LpType<T>::PER]) {
   LpType<T>::unpack(v.y, f + W);
   LpType<T>::unpack(v.z, f + 2 * W);
   LpType<T>::unpack(v.w, f + 3 * W);
+}
+
+// Two fp32 values per instruction.
+YN_DEV uint64_t lp_pair(float lo, float hi) {
+  uint64_t d;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(d) : "f"(lo), "f"(hi));
+  return d;
+}
+YN_DEV void lp_unpair(uint64_t d, float& lo, float& hi) { asm("mov.b64 {%0, %1}, %2;" : "=f"(lo), "=f"(hi) : "l"(d)); }
+YN_DEV uint64_t lp_fma2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t d;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
+  return d;
+}
+YN_DEV uint64_t lp_add2(uint64_t a, uint64_t b) {
+  uint64_t d;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+  return d;
 }
 
 YN_DEV float lp_ex2(float x) {
@@ -170,7 +236,7 @@ YN_DEV unsigned long long lp_block_max(unsigned long long k, unsigned long long*
 }
 
 template <typename T, int VPT>
-__global__ void __launch_bounds__(LP_THREADS) k_logprobs(const LpArgs a) {
+__global__ void __launch_bounds__(LP_THREADS, 4) k_logprobs(const LpArgs a) {
   using L = LpType<T>;
   constexpr int PER = L::PER;
   constexpr uint32_t KEY_NEG = 0x007FFFFFu;   // f32_ukey(-inf)
@@ -186,6 +252,7 @@ __global__ void __launch_bounds__(LP_THREADS) k_logprobs(const LpArgs a) {
   const long long row = blockIdx.x / a.splits;
   const int split = (int)(blockIdx.x % a.splits);
   const float inf = __int_as_float(0x7f800000);
+  const float z_big = sizeof(T) == 4 ? 3.402823466e38f : std::is_same_v<T, __half> ? 65504.0f : 3.38953139e38f;
   const uint8_t* p = a.z + (size_t)row * a.ld * sizeof(T);
   // Vectors are aligned: the row's first element is element `lead` of vector 0, and
   // what a vector holds beside the row lies inside the same 16 bytes as an element of it.
@@ -247,19 +314,29 @@ __global__ void __launch_bounds__(LP_THREADS) k_logprobs(const LpArgs a) {
     for (int w = 1; w < LP_WARPS; ++w) m = fmaxf(m, wmax[w]);
     const uint32_t floor_key = have == a.n_top && a.n_top ? (uint32_t)(list[a.n_top - 1] >> 32) : KEY_NEG;
     const bool search = a.n_top > 0 && m > -inf && f32_ukey(m) > floor_key;
-    if (search && warp == 0) {
-      // the n-th largest thread maximum, its low 16 bits left out (a few more candidates)
-      uint32_t k[LP_WARPS], t = 0;
+    // A bound of the n-th largest from below: the list's last entry once it is full; else the
+    // smallest warp maximum (n <= 8 warps), or the n-th largest thread maximum.
+    uint32_t thr = floor_key + 1;   // equal to the list's last: a higher id, comes after it
+    bool bisect = false;
+    if (search && floor_key == KEY_NEG) {
+      float lo = wmax[0];
 #pragma unroll
-      for (int w = 0; w < LP_WARPS; ++w) k[w] = tkey[lane + 32 * w];
-      for (int b = 31; b >= 16; --b) {
-        const uint32_t x = t | (1u << b);
-        int c = 0;
+      for (int w = 1; w < LP_WARPS; ++w) lo = fminf(lo, wmax[w]);
+      bisect = a.n_top > LP_WARPS || lo == -inf;
+      if (!bisect) thr = f32_ukey(lo);
+      else if (warp == 0) {
+        uint32_t k[LP_WARPS], t = 0;
 #pragma unroll
-        for (int w = 0; w < LP_WARPS; ++w) c += k[w] >= x;
-        if (__reduce_add_sync(0xffffffffu, c) >= a.n_top) t = x;
+        for (int w = 0; w < LP_WARPS; ++w) k[w] = tkey[lane + 32 * w];
+        for (int b = 31; b >= 16; --b) {   // the low 16 bits left out: a few more candidates
+          const uint32_t x = t | (1u << b);
+          int c = 0;
+#pragma unroll
+          for (int w = 0; w < LP_WARPS; ++w) c += k[w] >= x;
+          if (__reduce_add_sync(0xffffffffu, c) >= a.n_top) t = x;
+        }
+        if (lane == 0) thr_s = max(t, KEY_NEG + 1);
       }
-      if (lane == 0) thr_s = max(t, floor_key + 1);   // equal to the floor: a higher id, comes after it
     }
     // sums relative to the chunk's maximum; cnt: elements equal to it
     float r = 0.0f, d = 0.0f;
@@ -270,17 +347,28 @@ __global__ void __launch_bounds__(LP_THREADS) k_logprobs(const LpArgs a) {
     const float ml = m * LP_LOG2E, del = large ? 0.0f : fmaf(m, LP_LOG2E, -ml);
     if (m > -inf && m < inf) {
       if (tm < m && !large) {
+        const uint64_t l2 = lp_pair(LP_LOG2E, LP_LOG2E), ml2 = lp_pair(-ml, -ml);
+        uint64_t r2 = 0, d2 = 0;
 #pragma unroll
         for (int i = 0; i < VPT; ++i) {
+          const uint4 q = make_uint4(L::floor(v[i].x), L::floor(v[i].y), L::floor(v[i].z), L::floor(v[i].w));
           float f[PER];
-          lp_unpack<T>(v[i], f);
+          lp_unpack<T>(q, f);
 #pragma unroll
-          for (int j = 0; j < PER; ++j) {
-            const float y = fmaxf(fmaf(f[j], LP_LOG2E, -ml), -200.0f), e = lp_ex2(y);
-            r += e;
-            d = fmaf(e, y, d);
+          for (int j = 0; j < PER; j += 2) {
+            const uint64_t y = lp_fma2(lp_pair(f[j], f[j + 1]), l2, ml2);
+            float y0, y1;
+            lp_unpair(y, y0, y1);
+            const uint64_t e = lp_pair(lp_ex2(y0), lp_ex2(y1));
+            r2 = lp_add2(r2, e);
+            d2 = lp_fma2(e, y, d2);
           }
         }
+        float r1, d1;
+        lp_unpair(r2, r, r1);
+        lp_unpair(d2, d, d1);
+        r += r1;
+        d += d1;
       } else {
 #pragma unroll
         for (int i = 0; i < VPT; ++i) {
@@ -305,15 +393,41 @@ __global__ void __launch_bounds__(LP_THREADS) k_logprobs(const LpArgs a) {
       }
     }
     if (ranked && tm >= z_tok) {
+      // before the token's own vector equal logits count too: above the value just below
+      const int tv = (int)(((long long)lead + tok) / PER);
+      if (z_tok > -inf) {
+        const uint32_t above = L::splat(z_tok), from = L::splat(z_tok < inf ? lp_below<T>(z_tok) : z_big);
+        uint32_t c = 0;
 #pragma unroll
-      for (int i = 0; i < VPT; ++i) {
-        float f[PER];
-        lp_unpack<T>(v[i], f);
-        const int at = c0 + i * LP_THREADS + tid;
-        const long long e0 = (long long)at * PER - lead;
-        if (at >= v1) break;
+        for (int i = 0; i < VPT; ++i) {
+          const int at = c0 + i * LP_THREADS + tid;
+          const uint32_t t = at < tv ? from : above;
+          L::count(v[i].x, t, c);
+          L::count(v[i].y, t, c);
+          L::count(v[i].z, t, c);
+          L::count(v[i].w, t, c);
+        }
+        before = L::counted(c);
+      } else if (tv > c0 + tid) {
+        // a barred token: every logit above -inf, and the barred ones of a lower id
+        for (int at = c0 + tid; at < min(min(v1, tv), c0 + LP_THREADS * VPT); at += LP_THREADS) before += at == 0 ? PER - lead : PER;
+      }
+      if (z_tok == -inf) {
 #pragma unroll
-        for (int j = 0; j < PER; ++j) before += f[j] > z_tok || (f[j] == z_tok && e0 + j >= 0 && e0 + j < tok);
+        for (int i = 0; i < VPT; ++i) {
+          const int at = c0 + i * LP_THREADS + tid;
+          float f[PER];
+          lp_unpack<T>(v[i], f);
+#pragma unroll
+          for (int j = 0; j < PER; ++j) before += at >= tv && f[j] > -inf;
+        }
+      }
+      if (tv >= c0 && tv < min(v1, c0 + LP_THREADS * VPT) && (tv - c0) % LP_THREADS == tid) {
+        // inside it, those of a lower id
+        for (int j = 0; j < PER; ++j) {
+          const long long e = (long long)tv * PER + j - lead;
+          if (e >= 0 && e < tok) before += L::load(p + e * sizeof(T)) == z_tok;
+        }
       }
     }
     r = warp_sum_f32(r);
@@ -345,7 +459,7 @@ __global__ void __launch_bounds__(LP_THREADS) k_logprobs(const LpArgs a) {
       lp_join(sums, c);
     }
     if (search) {
-      const uint32_t thr = thr_s;
+      if (bisect) thr = thr_s;
       // the elements of every thread of this warp that reaches the threshold, one thread's
       // vectors at a time, one lane per vector
       unsigned who = __ballot_sync(0xffffffffu, tk >= thr);
@@ -407,8 +521,8 @@ __global__ void __launch_bounds__(LP_THREADS) k_logprobs(const LpArgs a) {
       }
       have = min(total, a.n_top);
     }
-    __syncthreads();
   }
+  __syncthreads();
   if (a.splits > 1) {
     const long long at = row * a.splits + split;
     if (tid == 0) {

@@ -17,8 +17,10 @@
 // One warp per row, keys in registers: L = 32 / (groups rounded up to a power of
 // two) lanes hold one group, element i of a lane being expert
 // (lane / L) * per_group + lane % L + i * L. A row is at most 4 KB, so the kernel
-// is bound by the latency of the warp's k rounds of argmax (two redux each), not
-// by memory.
+// is bound by issuing instructions, not by memory. The choice takes few of them: the
+// k-th largest of the 32 lane maxima (k redux) bounds the k-th largest key from
+// below; the keys that reach it, little more than k, are gathered one per lane and
+// placed by counting the larger ones.
 #include <cuda_runtime.h>
 
 #include <string>
@@ -41,7 +43,7 @@ struct RouterArgs {
   const uint8_t* avail;
   int32_t* ids;
   float* w;
-  int E, K, G, per, L, kept, group_top;
+  int E, K, G, per, L, log_l, kept, group_top;
   bool softmax, norm;
   float scale;
 };
@@ -69,18 +71,25 @@ YN_DEV double warp_sum_f64(double v) {
   for (int m = 16; m > 0; m >>= 1) v += __shfl_xor_sync(0xffffffffu, v, m);
   return v;
 }
+// 1 / (1 + e^-z) by two approximations of 1 and 2 ulp (z above -80).
+YN_DEV float rt_sigmoid(float z) {
+  float r;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(1.0f + __expf(fminf(-z, 80.0f))));
+  return r;
+}
+
 // Where lane `lane` finds its element i, or -1.
 YN_DEV int rt_expert(const RouterArgs& a, int lane, int i) {
-  const int g = lane / a.L, at = lane % a.L + i * a.L;
+  const int g = lane >> a.log_l, at = (lane & (a.L - 1)) + (i << a.log_l);
   return g < a.G && at < a.per ? g * a.per + at : -1;
 }
 
 // The two largest of a lane's values merged over the L lanes of its group, then
 // whether the group is among the `kept` best (its rank by score, ties to the
-// lower group). far: smallest distance between a group that is in and one that
-// is out, for the caller's check.
+// lower group). far, or null: the smallest distance between a group that is in and
+// one that is out, for the caller's check in fp32.
 template <typename F>
-YN_DEV bool rt_group_kept(const RouterArgs& a, int lane, F hi, F lo, F none, F* far) {
+YN_DEV bool rt_group_kept(const RouterArgs& a, int lane, F hi, F lo, F none, float* far) {
   for (int m = 1; m < a.L; m <<= 1) {
     const F h2 = __shfl_xor_sync(0xffffffffu, hi, m), l2 = __shfl_xor_sync(0xffffffffu, lo, m);
     const F mn = hi < h2 ? hi : h2, mx = hi < h2 ? h2 : hi, l = lo < l2 ? l2 : lo;
@@ -89,21 +98,18 @@ YN_DEV bool rt_group_kept(const RouterArgs& a, int lane, F hi, F lo, F none, F* 
   }
   F score = hi;
   if (a.group_top > 1 && lo != none) score = hi + lo;
-  const int g = lane / a.L;
+  const int g = lane >> a.log_l;
   int rank = 0;
   for (int o = 0; o < a.G; ++o) {
-    const F s = __shfl_sync(0xffffffffu, score, o * a.L);
+    const F s = __shfl_sync(0xffffffffu, score, o << a.log_l);
     rank += s > score || (s == score && o < g);
   }
   const bool in = g < a.G && rank < a.kept;
-  F lowest_in = in && score != none ? score : -none, best_out = !in && g < a.G ? score : none;
-#pragma unroll
-  for (int m = 16; m > 0; m >>= 1) {
-    const F x = __shfl_xor_sync(0xffffffffu, lowest_in, m), y = __shfl_xor_sync(0xffffffffu, best_out, m);
-    lowest_in = x < lowest_in ? x : lowest_in;
-    best_out = y > best_out ? y : best_out;
+  if (far) {
+    const float lowest_in = f32_from_ukey(__reduce_min_sync(0xffffffffu, in && score != none ? f32_ukey((float)score) : ~0u));
+    const float best_out = f32_from_ukey(__reduce_max_sync(0xffffffffu, f32_ukey(!in && g < a.G ? (float)score : (float)none)));
+    *far = best_out == (float)none ? -(float)none : lowest_in - best_out;
   }
-  *far = best_out == none ? -none : lowest_in - best_out;
   return in;
 }
 
@@ -146,8 +152,7 @@ __device__ __noinline__ int rt_choose_f64(const RouterArgs& a, long long row, in
     else if (val[e] > lo) lo = val[e];
   }
   if (a.G > 1) {
-    double far;
-    const bool in = rt_group_kept(a, lane, hi, lo, none, &far);
+    const bool in = rt_group_kept(a, lane, hi, lo, none, (float*)nullptr);
     for (int i = 0; i < nv; ++i) {
       const int e = rt_expert(a, lane, i);
       if (e < 0) continue;
@@ -177,6 +182,7 @@ __device__ __noinline__ int rt_choose_f64(const RouterArgs& a, long long row, in
 template <typename T, int NV, bool BY_SCORE>
 __global__ void __launch_bounds__(32 * RT_WARPS) k_router(const RouterArgs a) {
   extern __shared__ double rt_smem[];   // BY_SCORE: E doubles per warp
+  __shared__ unsigned long long cand[RT_WARPS][32];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const long long row = (long long)blockIdx.x * RT_WARPS + warp;
   if (row >= a.rows) return;
@@ -187,10 +193,20 @@ __global__ void __launch_bounds__(32 * RT_WARPS) k_router(const RouterArgs a) {
   for (int i = 0; i < NV; ++i) {
     const int e = rt_expert(a, lane, i);
     const float z = e >= 0 ? rt_load<T>(a.z, row * a.ld + e) : -inf;
-    v[i] = z > -inf && (!a.avail || a.avail[e]) ? z : -inf;
-    m = fmaxf(m, v[i]);
+    v[i] = z > -inf ? z : -inf;   // NaN too
   }
-  m = f32_from_ukey(__reduce_max_sync(0xffffffffu, f32_ukey(m)));
+  if (a.avail) {
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      const int e = rt_expert(a, lane, i);
+      if (e >= 0 && !a.avail[e]) v[i] = -inf;
+    }
+  }
+  if (BY_SCORE || (a.softmax && !a.norm)) {
+#pragma unroll
+    for (int i = 0; i < NV; ++i) m = fmaxf(m, v[i]);
+    m = f32_from_ukey(__reduce_max_sync(0xffffffffu, f32_ukey(m)));
+  }
   float sum = 0.0f;
   if (a.softmax && (BY_SCORE || !a.norm)) {
 #pragma unroll
@@ -217,7 +233,7 @@ __global__ void __launch_bounds__(32 * RT_WARPS) k_router(const RouterArgs a) {
         continue;
       }
       const float s = a.softmax ? (v[i] == m ? inv : __expf(v[i] - m) * inv)
-                                : __fdividef(1.0f, 1.0f + __expf(fminf(-v[i], 80.0f)));
+                                : rt_sigmoid(v[i]);
       const float c = a.bias ? s + __ldg(a.bias + e) : s;
       if (!(c > -inf)) {   // a bias of -inf or NaN takes the expert out
         key[i] = 0;
@@ -227,7 +243,7 @@ __global__ void __launch_bounds__(32 * RT_WARPS) k_router(const RouterArgs a) {
       if (c > hi) { lo = hi; hi = c; }
       else if (c > lo) lo = c;
     }
-    const float smax = a.softmax ? inv : __fdividef(1.0f, 1.0f + __expf(fminf(-m, 80.0f)));
+    const float smax = a.softmax ? inv : rt_sigmoid(m);
     tol = (a.softmax ? 1.6e-5f : 2.0e-6f) * smax + 1e-30f;
     if (a.G > 1) {
       float far;
@@ -243,27 +259,62 @@ __global__ void __launch_bounds__(32 * RT_WARPS) k_router(const RouterArgs a) {
 #pragma unroll
     for (int i = 0; i < NV; ++i) key[i] = v[i] == -inf ? 0u : f32_ukey(v[i]);
   }
-  // K rounds (one more where neighbours are compared): the largest key, the lowest id that has it
+  // The first K (one more where neighbours are compared), descending, ties to the lower id.
   const bool compared = BY_SCORE && a.bias;
-  const int rounds = compared ? a.K + 1 : a.K;
+  const int places = compared ? a.K + 1 : a.K;
   int mine = -1;
   uint32_t my_key = 0;
-  for (int j = 0; j < rounds; ++j) {
-    uint32_t best = 0;
-    int bi = 0;
+  uint32_t cur = 0, bound = 0;
 #pragma unroll
-    for (int i = 0; i < NV; ++i)
-      if (key[i] > best) { best = key[i]; bi = i; }
-    const uint32_t top = __reduce_max_sync(0xffffffffu, best);
-    if (top == 0) break;
-    const int at = best == top ? rt_expert(a, lane, bi) : RT_MAX_E;
-    const int id = (int)__reduce_min_sync(0xffffffffu, (unsigned)at);
-    if (at == id) {
+  for (int i = 0; i < NV; ++i) cur = max(cur, key[i]);
+  for (int j = 0; j < places; ++j) {
+    bound = __reduce_max_sync(0xffffffffu, cur);
+    if (cur == bound) cur = 0;   // equal lane maxima go together: the bound is lower then, and still one
+  }
+  bound = max(bound, 1u);
+  int n = 0;
+#pragma unroll
+  for (int i = 0; i < NV; ++i) {
+    const unsigned who = __ballot_sync(0xffffffffu, key[i] >= bound);
+    if (who) {
+      const int at = n + __popc(who & ((1u << lane) - 1u));
+      if (key[i] >= bound && at < 32)
+        cand[warp][at] = ((unsigned long long)key[i] << 32) | (0xFFFFFFFFu - (uint32_t)rt_expert(a, lane, i));
+      n += __popc(who);
+    }
+  }
+  if (n <= 32) {
+    __syncwarp();
+    const unsigned long long own = lane < n ? cand[warp][lane] : 0;
+    int place = 0;
+    for (int q = 0; q < n; ++q) place += cand[warp][q] > own;
+    __syncwarp();
+    if (lane < n) cand[warp][place] = own;
+    __syncwarp();
+    if (lane < min(n, places)) {
+      const unsigned long long c = cand[warp][lane];
+      mine = (int)(0xFFFFFFFFu - (uint32_t)c);
+      my_key = (uint32_t)(c >> 32);
+    }
+  } else {
+    // many equal keys, or k near 32: one after another, two redux each
+    for (int j = 0; j < places; ++j) {
+      uint32_t best = 0;
+      int bi = 0;
 #pragma unroll
       for (int i = 0; i < NV; ++i)
-        if (i == bi) key[i] = 0;
+        if (key[i] > best) { best = key[i]; bi = i; }
+      const uint32_t top = __reduce_max_sync(0xffffffffu, best);
+      if (top == 0) break;
+      const int at = best == top ? rt_expert(a, lane, bi) : RT_MAX_E;
+      const int id = (int)__reduce_min_sync(0xffffffffu, (unsigned)at);
+      if (at == id) {
+#pragma unroll
+        for (int i = 0; i < NV; ++i)
+          if (i == bi) key[i] = 0;
+      }
+      if (lane == j) { mine = id; my_key = top; }
     }
-    if (lane == j) { mine = id; my_key = top; }
   }
   float z = mine >= 0 ? rt_load<T>(a.z, row * a.ld + mine) : -inf;
   if (BY_SCORE) {
@@ -360,6 +411,7 @@ extern "C" int yn_route_scored(const yn_route_rule* rule, const void* logits, in
   int p2 = 1;
   while (p2 < a.G) p2 *= 2;
   a.L = 32 / p2;
+  while ((1 << a.log_l) < a.L) ++a.log_l;
   a.kept = r.top_groups;
   a.group_top = r.group_top;
   a.softmax = r.score == YN_SCORE_SOFTMAX;
