@@ -7,16 +7,17 @@
 // sum exp(z - m)(z - m) / S. The sum leaves the largest term out so that log S
 // keeps its relative accuracy when that term has nearly all the mass.
 //
-// Bound by reading the logits once. A block holds a chunk of the row in
-// registers (VPT 16-byte loads per thread, all in flight at once), takes the
-// chunk's maximum first and only then the exponentials, one ex2 per element
-// against a maximum that does not move; chunks (and blocks, where a row is split
-// over several because there are few) are joined by rescaling two sums.
-// The alternatives cost little beside that: every thread knows its own maximum
-// from the first step, so the n-th largest of the 256 thread maxima bounds the
-// n-th largest element from below, and only the about n threads that reach it
-// have their elements looked at again (from L2). Two fp32 values go through one
-// instruction where they can (fma.rn.f32x2).
+// Bound by reading the logits once. A thread holds VPT 16-byte pieces of the row in
+// registers (all loads in flight at once), takes their maximum and sums their
+// exponentials relative to it, one ex2 per element and two fp32 values per
+// instruction elsewhere (fma.rn.f32x2); pieces and threads are joined by rescaling two
+// sums. Only a thread that may hold the row's maximum sums without that element; the
+// others' sums are off by 2^-24 of themselves, of a smaller part of S.
+// The alternatives cost little beside that: in its first pieces a block takes a bound
+// of the n-th largest from below (of its 8 warps' or 256 threads' maxima), and from
+// then on only the threads whose maximum reaches it, a few times n in all, have their
+// elements looked at again (from L2).
+// Rows are split over blocks where there are few; a second kernel joins the parts.
 #include <cuda_runtime.h>
 
 #include <algorithm>
@@ -188,22 +189,30 @@ YN_DEV float lp_ex2(float x) {
   return y;
 }
 
-// Joins part b to part a.
+// Joins part b to part a (the ranks apart).
 YN_DEV void lp_join(LpSums& a, const LpSums& b) {
-  a.rank += b.rank;
-  if (b.m == -__int_as_float(0x7f800000)) return;
+  const float inf = __int_as_float(0x7f800000);
   const bool up = b.m > a.m;
-  const LpSums hi = up ? b : a, lo = up ? a : b;
-  if (lo.m != -__int_as_float(0x7f800000)) {
-    const float d = hi.m == lo.m ? 0.0f : lo.m - hi.m;   // equal also where both are +inf
-    const float f = d == 0.0f ? 1.0f : expf(d);
-    a.R = hi.R + f * (1.0f + lo.R);
-    a.D = hi.D + (f > 0.0f ? f * (lo.D + d * (1.0f + lo.R)) : 0.0f);
-  } else {
-    a.R = hi.R;
-    a.D = hi.D;
-  }
-  a.m = hi.m;
+  const float hm = up ? b.m : a.m, hR = up ? b.R : a.R, hD = up ? b.D : a.D;
+  const float lm = up ? a.m : b.m, lR = up ? a.R : b.R, lD = up ? a.D : b.D;
+  const float d = hm == lm ? 0.0f : lm - hm, f = lm == -inf ? 0.0f : expf(d);   // both +inf: d = 0
+  a.m = hm;
+  a.R = fmaf(f, 1.0f + lR, hR);
+  a.D = f > 0.0f ? fmaf(f, fmaf(d, 1.0f + lR, lD), hD) : hD;
+}
+
+// The join of the 32 lanes' parts, on every lane.
+YN_DEV LpSums lp_warp_join(const LpSums& s) {
+  const float inf = __int_as_float(0x7f800000);
+  LpSums o;
+  o.m = f32_from_ukey(__reduce_max_sync(0xffffffffu, f32_ukey(s.m)));
+  const bool top = s.m == o.m;
+  const int first = __ffs(__ballot_sync(0xffffffffu, top)) - 1;
+  const float d = top ? 0.0f : s.m - o.m, f = s.m == -inf ? 0.0f : top ? 1.0f : expf(d);
+  o.R = warp_sum_f32((int)(threadIdx.x & 31) == first && s.m > -inf ? s.R : f * (1.0f + s.R));
+  o.D = warp_sum_f32(f > 0.0f ? f * fmaf(d, 1.0f + s.R, s.D) : 0.0f);
+  o.rank = __reduce_add_sync(0xffffffffu, s.rank);
+  return o;
 }
 
 // A row's answer from its sums, by one thread. z_tok: the token's logit.
@@ -240,9 +249,8 @@ __global__ void __launch_bounds__(LP_THREADS, 4) k_logprobs(const LpArgs a) {
   using L = LpType<T>;
   constexpr int PER = L::PER;
   constexpr uint32_t KEY_NEG = 0x007FFFFFu;   // f32_ukey(-inf)
-  __shared__ uint32_t tkey[LP_THREADS];
-  __shared__ float wmax[LP_WARPS], wr[LP_WARPS], wd[LP_WARPS];
-  __shared__ int wcnt[LP_WARPS], wrank[LP_WARPS];
+  __shared__ uint32_t tkey[LP_THREADS], wkey[LP_WARPS];
+  __shared__ LpSums wsum[LP_WARPS];
   __shared__ uint32_t thr_s;
   __shared__ int n_cand;
   __shared__ unsigned long long cand[LP_CAND], list[LP_MAX_TOP], buf[2][LP_WARPS];
@@ -263,11 +271,15 @@ __global__ void __launch_bounds__(LP_THREADS, 4) k_logprobs(const LpArgs a) {
   const int tok = a.tokens ? a.tokens[row] : -1;
   const bool ranked = tok >= 0 && tok < a.V;
   const float z_tok = ranked ? L::load(p + (size_t)tok * sizeof(T)) : inf;
+  const int tv = ranked ? (int)(((long long)lead + tok) / PER) : 0;
 
-  LpSums sums = {-inf, 0.0f, 0.0f, 0};   // kept by thread 0
-  int have = 0;                           // entries of `list`
-  bool nan = false;
-  for (int c0 = v0; c0 < v1 && !nan; c0 += LP_THREADS * VPT) {
+  LpSums sums = {-inf, 0.0f, 0.0f, 0};
+  bool bad = false;        // a NaN
+  bool known = false;      // the block has a bound of its n-th largest
+  uint32_t thr = KEY_NEG + 1;
+  float ref = inf;         // threads whose maximum reaches it leave it out of their sums
+  if (tid == 0) n_cand = 0;
+  for (int c0 = v0; c0 < v1; c0 += LP_THREADS * VPT) {
     uint4 v[VPT];
 #pragma unroll
     for (int i = 0; i < VPT; ++i) {
@@ -278,18 +290,17 @@ __global__ void __launch_bounds__(LP_THREADS, 4) k_logprobs(const LpArgs a) {
 #pragma unroll
       for (int i = 0; i < VPT; ++i) {
         const int at = c0 + i * LP_THREADS + tid;
+        if (at != 0 && at != n_vecs - 1) continue;
         const long long e0 = (long long)at * PER - lead;
-        if (at < v1 && (e0 < 0 || e0 + PER > a.V)) {
-          uint32_t w[4] = {v[i].x, v[i].y, v[i].z, v[i].w};
+        uint32_t w[4] = {v[i].x, v[i].y, v[i].z, v[i].w};
 #pragma unroll
-          for (int j = 0; j < PER; ++j)
-            if (e0 + j < 0 || e0 + j >= a.V) {
-              if (PER == 4) w[j] = L::NEG;
-              else w[j / 2] = (j & 1) ? (w[j / 2] & 0xFFFFu) | (L::NEG & 0xFFFF0000u)
-                                      : (w[j / 2] & 0xFFFF0000u) | (L::NEG & 0xFFFFu);
-            }
-          v[i] = make_uint4(w[0], w[1], w[2], w[3]);
-        }
+        for (int j = 0; j < PER; ++j)
+          if (e0 + j < 0 || e0 + j >= a.V) {
+            if (PER == 4) w[j] = L::NEG;
+            else w[j / 2] = (j & 1) ? (w[j / 2] & 0xFFFFu) | (L::NEG & 0xFFFF0000u)
+                                    : (w[j / 2] & 0xFFFF0000u) | (L::NEG & 0xFFFFu);
+          }
+        v[i] = make_uint4(w[0], w[1], w[2], w[3]);
       }
     }
     uint32_t mx = L::NEG;
@@ -302,51 +313,50 @@ __global__ void __launch_bounds__(LP_THREADS, 4) k_logprobs(const LpArgs a) {
       L::unpack(mx, f);
       tm = PER == 4 ? f[0] : (f[0] > f[1] || f[0] != f[0] ? f[0] : f[1]);
     }
+    bad |= tm != tm;
     const uint32_t tk = f32_ukey(tm);
-    tkey[tid] = tk;
-    const uint32_t wk = __reduce_max_sync(0xffffffffu, tk);
-    if (lane == 0) wmax[warp] = f32_from_ukey(wk);
-    if (tid == 0) n_cand = 0;
-    nan = __syncthreads_or(tm != tm) != 0;
-    if (nan) break;
-    float m = wmax[0];
+    if (!known) {
+      __syncthreads();
+      tkey[tid] = tk;
+      const uint32_t wk = __reduce_max_sync(0xffffffffu, tk);
+      if (lane == 0) wkey[warp] = wk;
+      __syncthreads();
+      uint32_t hi = wkey[0], lo = wkey[0];
 #pragma unroll
-    for (int w = 1; w < LP_WARPS; ++w) m = fmaxf(m, wmax[w]);
-    const uint32_t floor_key = have == a.n_top && a.n_top ? (uint32_t)(list[a.n_top - 1] >> 32) : KEY_NEG;
-    const bool search = a.n_top > 0 && m > -inf && f32_ukey(m) > floor_key;
-    // A bound of the n-th largest from below: the list's last entry once it is full; else the
-    // smallest warp maximum (n <= 8 warps), or the n-th largest thread maximum.
-    uint32_t thr = floor_key + 1;   // equal to the list's last: a higher id, comes after it
-    bool bisect = false;
-    if (search && floor_key == KEY_NEG) {
-      float lo = wmax[0];
+      for (int w = 1; w < LP_WARPS; ++w) {
+        hi = max(hi, wkey[w]);
+        lo = min(lo, wkey[w]);
+      }
+      ref = f32_from_ukey(hi);
+      known = hi > KEY_NEG;
+      if (a.n_top && known) {
+        if (a.n_top <= LP_WARPS && lo > KEY_NEG) {
+          thr = lo;
+        } else {
+          if (warp == 0) {   // the n-th largest thread maximum, its low 16 bits left out (a few more candidates)
+            uint32_t k[LP_WARPS], t = 0;
 #pragma unroll
-      for (int w = 1; w < LP_WARPS; ++w) lo = fminf(lo, wmax[w]);
-      bisect = a.n_top > LP_WARPS || lo == -inf;
-      if (!bisect) thr = f32_ukey(lo);
-      else if (warp == 0) {
-        uint32_t k[LP_WARPS], t = 0;
+            for (int w = 0; w < LP_WARPS; ++w) k[w] = tkey[lane + 32 * w];
+            for (int b = 31; b >= 16; --b) {
+              const uint32_t x = t | (1u << b);
+              int c = 0;
 #pragma unroll
-        for (int w = 0; w < LP_WARPS; ++w) k[w] = tkey[lane + 32 * w];
-        for (int b = 31; b >= 16; --b) {   // the low 16 bits left out: a few more candidates
-          const uint32_t x = t | (1u << b);
-          int c = 0;
-#pragma unroll
-          for (int w = 0; w < LP_WARPS; ++w) c += k[w] >= x;
-          if (__reduce_add_sync(0xffffffffu, c) >= a.n_top) t = x;
+              for (int w = 0; w < LP_WARPS; ++w) c += k[w] >= x;
+              if (__reduce_add_sync(0xffffffffu, c) >= a.n_top) t = x;
+            }
+            if (lane == 0) thr_s = t;
+          }
+          __syncthreads();
+          thr = max(thr_s, KEY_NEG + 1);
+          known = thr > KEY_NEG + 1;   // fewer than n threads with a finite logit: look again in the next pieces
         }
-        if (lane == 0) thr_s = max(t, KEY_NEG + 1);
       }
     }
-    // sums relative to the chunk's maximum; cnt: elements equal to it
-    float r = 0.0f, d = 0.0f;
-    int cnt = 0, before = 0;
-    // y = z log2(e) - ml is (z - m) log2(e) + del, del the rounding of ml = m log2(e), which is taken out of the
-    // sums at the end; for maxima so large that del is not small the subtraction comes first and del is 0
-    const bool large = !(fabsf(m) < 4096.0f);
-    const float ml = m * LP_LOG2E, del = large ? 0.0f : fmaf(m, LP_LOG2E, -ml);
-    if (m > -inf && m < inf) {
-      if (tm < m && !large) {
+    if (tm > -inf) {
+      // y is (z - tm) log2(e) + del, del the rounding of tm log2(e), which is taken out of the sums
+      LpSums c = {tm, 0.0f, 0.0f, 0};
+      if (tm < ref && fabsf(tm) < 4096.0f) {
+        const float ml = tm * LP_LOG2E, del = fmaf(tm, LP_LOG2E, -ml);
         const uint64_t l2 = lp_pair(LP_LOG2E, LP_LOG2E), ml2 = lp_pair(-ml, -ml);
         uint64_t r2 = 0, d2 = 0;
 #pragma unroll
@@ -364,38 +374,36 @@ __global__ void __launch_bounds__(LP_THREADS, 4) k_logprobs(const LpArgs a) {
             d2 = lp_fma2(e, y, d2);
           }
         }
-        float r1, d1;
-        lp_unpair(r2, r, r1);
-        lp_unpair(d2, d, d1);
-        r += r1;
-        d += d1;
+        float r0, r1, d0, d1;
+        lp_unpair(r2, r0, r1);
+        lp_unpair(d2, d0, d1);
+        const float s = r0 + r1, f = lp_ex2(-del);
+        c.R = fmaf(f, s, -1.0f);
+        c.D = f * fmaf(-del, s, d0 + d1) * LP_LN2;
       } else {
+        int cnt = 0;
+        float d = 0.0f;
 #pragma unroll
         for (int i = 0; i < VPT; ++i) {
           float f[PER];
           lp_unpack<T>(v[i], f);
 #pragma unroll
           for (int j = 0; j < PER; ++j) {
-            const float y = fmaxf(fmaf(f[j] - m, LP_LOG2E, del), -200.0f), e = lp_ex2(y);
-            cnt += f[j] == m;
-            r += f[j] == m ? 0.0f : e;
-            d = f[j] == m ? d : fmaf(e, y, d);
+            const bool top = f[j] == tm;
+            const float y = fmaxf((f[j] - tm) * LP_LOG2E, -200.0f), e = top ? 0.0f : lp_ex2(y);
+            cnt += top;
+            c.R += e;
+            d = top ? d : fmaf(e, y, d);
           }
         }
+        c.R += (float)(cnt - 1);
+        c.D = d * LP_LN2;
       }
-    } else if (tm == inf) {
-#pragma unroll
-      for (int i = 0; i < VPT; ++i) {
-        float f[PER];
-        lp_unpack<T>(v[i], f);
-#pragma unroll
-        for (int j = 0; j < PER; ++j) cnt += f[j] == inf;
-      }
+      lp_join(sums, c);
     }
     if (ranked && tm >= z_tok) {
-      // before the token's own vector equal logits count too: above the value just below
-      const int tv = (int)(((long long)lead + tok) / PER);
       if (z_tok > -inf) {
+        // before the token's own vector equal logits count too: above the value just below
         const uint32_t above = L::splat(z_tok), from = L::splat(z_tok < inf ? lp_below<T>(z_tok) : z_big);
         uint32_t c = 0;
 #pragma unroll
@@ -407,61 +415,29 @@ __global__ void __launch_bounds__(LP_THREADS, 4) k_logprobs(const LpArgs a) {
           L::count(v[i].z, t, c);
           L::count(v[i].w, t, c);
         }
-        before = L::counted(c);
-      } else if (tv > c0 + tid) {
+        sums.rank += L::counted(c);
+      } else {
         // a barred token: every logit above -inf, and the barred ones of a lower id
-        for (int at = c0 + tid; at < min(min(v1, tv), c0 + LP_THREADS * VPT); at += LP_THREADS) before += at == 0 ? PER - lead : PER;
-      }
-      if (z_tok == -inf) {
 #pragma unroll
         for (int i = 0; i < VPT; ++i) {
           const int at = c0 + i * LP_THREADS + tid;
           float f[PER];
           lp_unpack<T>(v[i], f);
 #pragma unroll
-          for (int j = 0; j < PER; ++j) before += at >= tv && f[j] > -inf;
+          for (int j = 0; j < PER; ++j) sums.rank += at < v1 && (at < tv ? (at > 0 || j >= lead) : f[j] > -inf);
         }
       }
       if (tv >= c0 && tv < min(v1, c0 + LP_THREADS * VPT) && (tv - c0) % LP_THREADS == tid) {
         // inside it, those of a lower id
         for (int j = 0; j < PER; ++j) {
           const long long e = (long long)tv * PER + j - lead;
-          if (e >= 0 && e < tok) before += L::load(p + e * sizeof(T)) == z_tok;
+          if (e >= 0 && e < tok) sums.rank += L::load(p + e * sizeof(T)) == z_tok;
         }
       }
     }
-    r = warp_sum_f32(r);
-    d = warp_sum_f32(d);
-    cnt = __reduce_add_sync(0xffffffffu, cnt);
-    before = __reduce_add_sync(0xffffffffu, before);
-    if (lane == 0) {
-      wr[warp] = r;
-      wd[warp] = d;
-      wcnt[warp] = cnt;
-      wrank[warp] = before;
-    }
-    __syncthreads();
-    if (tid == 0) {
-      LpSums c = {m, 0.0f, 0.0f, 0};
-      int n_max = 0;
-      for (int w = 0; w < LP_WARPS; ++w) {
-        c.R += wr[w];
-        c.D += wd[w];
-        n_max += wcnt[w];
-        c.rank += wrank[w];
-      }
-      if (m > -inf && m < inf) {
-        const float f = exp2f(-del);
-        c.D = f * (c.D - del * c.R) * LP_LN2;
-        c.R *= f;
-      }
-      c.R += (float)(n_max - 1);
-      lp_join(sums, c);
-    }
-    if (search) {
-      if (bisect) thr = thr_s;
-      // the elements of every thread of this warp that reaches the threshold, one thread's
-      // vectors at a time, one lane per vector
+    if (a.n_top) {
+      // the elements of every thread of this warp that reaches the bound, one thread's vectors at a
+      // time, one lane per vector
       unsigned who = __ballot_sync(0xffffffffu, tk >= thr);
       while (who) {
         const int o = __ffs(who) - 1;
@@ -480,49 +456,53 @@ __global__ void __launch_bounds__(LP_THREADS, 4) k_logprobs(const LpArgs a) {
             }
           }
         }
-        __syncwarp();
       }
-      __syncthreads();
-      int n = n_cand;
-      if (n + have > LP_CAND) {
-        // many equal or near logits: the n largest one after another, over the whole chunk
-        unsigned long long prev = ~0ull;
-        int got = 0;
-        for (int q = 0; q < a.n_top; ++q) {
-          unsigned long long best = 0;
-          for (int at = c0 + tid; at < min(v1, c0 + LP_THREADS * VPT); at += LP_THREADS) {
-            float f[PER];
-            lp_unpack<T>(ldg_nc_v4(base + (size_t)at * 16), f);
-            const long long e0 = (long long)at * PER - lead;
-#pragma unroll
-            for (int j = 0; j < PER; ++j) {
-              const unsigned long long k =
-                  ((unsigned long long)f32_ukey(f[j]) << 32) | (0xFFFFFFFFu - (uint32_t)(e0 + j));
-              if (e0 + j >= 0 && e0 + j < a.V && f[j] > -inf && k < prev && k > best) best = k;
-            }
-          }
-          prev = lp_block_max(best, buf[q & 1]);
-          if (!prev) break;
-          if (tid == 0) cand[q] = prev;
-          ++got;
-        }
-        __syncthreads();
-        n = got;
-      }
-      // candidates and the list so far, each placed by how many are larger (keys are distinct)
-      if (tid < have) cand[n + tid] = list[tid];
-      __syncthreads();
-      const int total = n + have;
-      for (int i = tid; i < total; i += LP_THREADS) {
-        const unsigned long long k = cand[i];
-        int place = 0;
-        for (int q = 0; q < total; ++q) place += cand[q] > k;
-        if (place < a.n_top) list[place] = k;
-      }
-      have = min(total, a.n_top);
     }
   }
-  __syncthreads();
+  sums = lp_warp_join(sums);
+  if (lane == 0) wsum[warp] = sums;
+  const bool nan = __syncthreads_or(bad) != 0;
+  if (warp == 0) {
+    const LpSums none = {-inf, 0.0f, 0.0f, 0};
+    sums = lp_warp_join(lane < LP_WARPS ? wsum[lane] : none);
+  }
+  int have = 0;
+  if (a.n_top) {
+    int n = n_cand;
+    if (n > LP_CAND) {
+      // many equal or ascending logits: the n largest one after another, over the whole part
+      unsigned long long prev = ~0ull;
+      __syncthreads();   // n_cand and cand have been read by all
+      n = 0;
+      for (int q = 0; q < a.n_top; ++q) {
+        unsigned long long best = 0;
+        for (int at = v0 + tid; at < v1; at += LP_THREADS) {
+          float f[PER];
+          lp_unpack<T>(ldg_nc_v4(base + (size_t)at * 16), f);
+          const long long e0 = (long long)at * PER - lead;
+#pragma unroll
+          for (int j = 0; j < PER; ++j) {
+            const unsigned long long k = ((unsigned long long)f32_ukey(f[j]) << 32) | (0xFFFFFFFFu - (uint32_t)(e0 + j));
+            if (e0 + j >= 0 && e0 + j < a.V && f[j] > -inf && k < prev && k > best) best = k;
+          }
+        }
+        prev = lp_block_max(best, buf[q & 1]);
+        if (!prev) break;
+        if (tid == 0) list[q] = prev;
+        ++n;
+      }
+    } else {
+      // each candidate placed by how many are larger (keys are distinct)
+      for (int i = tid; i < n; i += LP_THREADS) {
+        const unsigned long long k = cand[i];
+        int place = 0;
+        for (int q = 0; q < n; ++q) place += cand[q] > k;
+        if (place < a.n_top) list[place] = k;
+      }
+    }
+    have = min(n, a.n_top);
+    __syncthreads();
+  }
   if (a.splits > 1) {
     const long long at = row * a.splits + split;
     if (tid == 0) {
@@ -561,19 +541,14 @@ __global__ void __launch_bounds__(LP_MAX_SPLITS) k_logprobs_join(const LpArgs a)
     s = q.s;
     bad = q.nan;
   }
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) {
-    LpSums b;
-    b.m = __shfl_xor_sync(0xffffffffu, s.m, o);
-    b.R = __shfl_xor_sync(0xffffffffu, s.R, o);
-    b.D = __shfl_xor_sync(0xffffffffu, s.D, o);
-    b.rank = __shfl_xor_sync(0xffffffffu, s.rank, o);
-    lp_join(s, b);
-  }
+  s = lp_warp_join(s);
   if ((tid & 31) == 0) ws[tid >> 5] = s;
   const bool nan = __syncthreads_or(bad) != 0;
+  if (tid < 32) {
+    const LpSums none = {-__int_as_float(0x7f800000), 0.0f, 0.0f, 0};
+    s = lp_warp_join(tid < (int)(blockDim.x >> 5) ? ws[tid] : none);
+  }
   if (tid == 0) {
-    for (int w = 1; w < (int)(blockDim.x >> 5); ++w) lp_join(s, ws[w]);
     const int tok = a.tokens ? a.tokens[row] : -1;
     const float z_tok = tok >= 0 && tok < a.V ? L::load(a.z + ((size_t)row * a.ld + tok) * sizeof(T)) : 0.0f;
     lp_write(a, row, s, nan, tok, z_tok, &log_s_s);

@@ -12,7 +12,7 @@
 // monotone function of z, so the logits themselves are compared. Otherwise the
 // row is ordered in fp32, whose error on c is bounded (below); only where two
 // neighbours of the chosen order, or the last group in and the first one out,
-// are nearer than that bound is the row ordered again in fp64 by the same warp.
+// are nearer than that bound are the candidates, or the groups, ordered in fp64.
 //
 // One warp per row, keys in registers: L = 32 / (groups rounded up to a power of
 // two) lanes hold one group, element i of a lane being expert
@@ -78,16 +78,20 @@ YN_DEV float rt_sigmoid(float z) {
   return r;
 }
 
-// Where lane `lane` finds its element i, or -1.
-YN_DEV int rt_expert(const RouterArgs& a, int lane, int i) {
-  const int g = lane >> a.log_l, at = (lane & (a.L - 1)) + (i << a.log_l);
-  return g < a.G && at < a.per ? g * a.per + at : -1;
-}
+// A lane's part of a row: its elements are experts first + (i << log_l), i < count.
+struct RtLane {
+  int first, count;
+  YN_DEV RtLane(const RouterArgs& a, int lane) {
+    const int g = lane >> a.log_l, at = lane & (a.L - 1);
+    first = g * a.per + at;
+    count = g < a.G && at < a.per ? (a.per - at + a.L - 1) >> a.log_l : 0;
+  }
+};
 
-// The two largest of a lane's values merged over the L lanes of its group, then
-// whether the group is among the `kept` best (its rank by score, ties to the
-// lower group). far, or null: the smallest distance between a group that is in and
-// one that is out, for the caller's check in fp32.
+// Whether the lane's group is among the `kept` best: hi, lo are the two largest values of
+// the lane, merged over the L lanes of its group; the group's rank is by score, ties to
+// the lower group. far, or null: the smallest distance between a group that is in and one
+// that is out, for the caller's check in fp32.
 template <typename F>
 YN_DEV bool rt_group_kept(const RouterArgs& a, int lane, F hi, F lo, F none, float* far) {
   for (int m = 1; m < a.L; m <<= 1) {
@@ -96,8 +100,7 @@ YN_DEV bool rt_group_kept(const RouterArgs& a, int lane, F hi, F lo, F none, flo
     hi = mx;
     lo = mn < l ? l : mn;
   }
-  F score = hi;
-  if (a.group_top > 1 && lo != none) score = hi + lo;
+  const F score = a.group_top > 1 && lo != none ? hi + lo : hi;
   const int g = lane >> a.log_l;
   int rank = 0;
   for (int o = 0; o < a.G; ++o) {
@@ -113,60 +116,80 @@ YN_DEV bool rt_group_kept(const RouterArgs& a, int lane, F hi, F lo, F none, flo
   return in;
 }
 
-// The row's choice in fp64 (values in this warp's shared memory): lane j < K
-// returns the id at place j.
+// A row's scores in fp64: 1 / sum exp(z - m) of a softmax (1 for sigmoids).
 template <typename T>
-__device__ __noinline__ int rt_choose_f64(const RouterArgs& a, long long row, int lane, double* val) {
-  const double none = -__longlong_as_double(0x7ff0000000000000LL);
-  const int nv = (a.per + a.L - 1) / a.L;
-  double m = none;
-  for (int i = 0; i < nv; ++i) {
-    const int e = rt_expert(a, lane, i);
-    if (e < 0) continue;
-    const float z = rt_load<T>(a.z, row * a.ld + e);
-    const bool ok = z > -__int_as_float(0x7f800000) && (!a.avail || a.avail[e]);  // false for NaN
-    val[e] = ok ? (double)z : none;
-    m = fmax(m, val[e]);
-  }
-  m = warp_max_f64(m);
+YN_DEV double rt_inv_sum_f64(const RouterArgs& a, const RtLane& own, long long row, double m) {
   double sum = 0.0;
-  for (int i = 0; i < nv; ++i) {
-    const int e = rt_expert(a, lane, i);
-    if (e < 0 || val[e] == none) continue;
-    double s;
-    if (a.softmax) sum += s = val[e] == m ? 1.0 : exp(val[e] - m);
-    else s = 1.0 / (1.0 + exp(-val[e]));
-    val[e] = s;
+  for (int i = 0; i < own.count; ++i) {
+    const int e = own.first + (i << a.log_l);
+    const double z = rt_load<T>(a.z, row * a.ld + e);
+    if (z > -__longlong_as_double(0x7ff0000000000000LL) && (!a.avail || a.avail[e])) sum += z == m ? 1.0 : exp(z - m);
   }
-  if (a.softmax) sum = warp_sum_f64(sum);
+  return 1.0 / warp_sum_f64(sum);
+}
+// Choice value of expert e, which takes part; -inf where its bias takes it out.
+template <typename T>
+YN_DEV double rt_choice_f64(const RouterArgs& a, long long row, int e, double m, double inv) {
+  const double z = rt_load<T>(a.z, row * a.ld + e);
+  const double s = !a.softmax ? 1.0 / (1.0 + exp(-z)) : z == m ? inv : exp(z - m) * inv;
+  if (!a.bias) return s;
+  const double none = -__longlong_as_double(0x7ff0000000000000LL), c = s + (double)a.bias[e];
+  return c > none ? c : none;
+}
+
+// The groups kept, decided in fp64.
+template <typename T>
+__device__ __noinline__ bool rt_groups_f64(const RouterArgs& a, long long row, int lane, double m) {
+  const double none = -__longlong_as_double(0x7ff0000000000000LL);
+  const RtLane own(a, lane);
+  const double inv = a.softmax ? rt_inv_sum_f64<T>(a, own, row, m) : 1.0;
   double hi = none, lo = none;
-  for (int i = 0; i < nv; ++i) {
-    const int e = rt_expert(a, lane, i);
-    if (e < 0 || val[e] == none) continue;
-    if (a.softmax) val[e] /= sum;
-    if (a.bias) {
-      const double c = val[e] + (double)a.bias[e];
-      val[e] = c > none ? c : none;
-    }
-    if (val[e] > hi) { lo = hi; hi = val[e]; }
-    else if (val[e] > lo) lo = val[e];
+  for (int i = 0; i < own.count; ++i) {
+    const int e = own.first + (i << a.log_l);
+    const float z = rt_load<T>(a.z, row * a.ld + e);
+    if (!(z > -__int_as_float(0x7f800000)) || (a.avail && !a.avail[e])) continue;
+    const double c = rt_choice_f64<T>(a, row, e, m, inv);
+    if (c > hi) { lo = hi; hi = c; }
+    else if (c > lo) lo = c;
   }
-  if (a.G > 1) {
-    const bool in = rt_group_kept(a, lane, hi, lo, none, (float*)nullptr);
-    for (int i = 0; i < nv; ++i) {
-      const int e = rt_expert(a, lane, i);
-      if (e < 0) continue;
-      if (!in) val[e] = none;
-      else if (!a.bias && val[e] > none) val[e] = (double)rt_load<T>(a.z, row * a.ld + e);  // the logits' order
-    }
+  return rt_group_kept(a, lane, hi, lo, none, (float*)nullptr);
+}
+
+// The place of this lane's candidate (id, or -1) among the n <= 32 candidates, by fp64.
+template <typename T>
+__device__ __noinline__ int rt_place_f64(const RouterArgs& a, long long row, int lane, int id, int n, double m) {
+  const double none = -__longlong_as_double(0x7ff0000000000000LL);
+  const double inv = a.softmax ? rt_inv_sum_f64<T>(a, RtLane(a, lane), row, m) : 1.0;
+  const double c = id >= 0 ? rt_choice_f64<T>(a, row, id, m, inv) : none;
+  int place = 0;
+  for (int q = 0; q < n; ++q) {
+    const double o = __shfl_sync(0xffffffffu, c, q);
+    const int oid = __shfl_sync(0xffffffffu, id, q);
+    place += o > c || (o == c && oid < id);
+  }
+  return place;
+}
+
+// The row's choice from the values of the kept groups in fp64, one after another; lane
+// j < K returns the id at place j. For rows with more near candidates than lanes.
+template <typename T>
+__device__ __noinline__ int rt_choose_f64(const RouterArgs& a, long long row, int lane, bool in, double m, double* val) {
+  const double none = -__longlong_as_double(0x7ff0000000000000LL);
+  const RtLane own(a, lane);
+  const double inv = a.softmax ? rt_inv_sum_f64<T>(a, own, row, m) : 1.0;
+  for (int i = 0; i < own.count; ++i) {
+    const int e = own.first + (i << a.log_l);
+    const float z = rt_load<T>(a.z, row * a.ld + e);
+    const bool on = in && z > -__int_as_float(0x7f800000) && (!a.avail || a.avail[e]);
+    val[e] = on ? rt_choice_f64<T>(a, row, e, m, inv) : none;
   }
   int mine = -1;
   for (int j = 0; j < a.K; ++j) {
     double best = none;
     int at = RT_MAX_E;
-    for (int i = 0; i < nv; ++i) {
-      const int e = rt_expert(a, lane, i);
-      if (e >= 0 && val[e] > best) { best = val[e]; at = e; }
+    for (int i = 0; i < own.count; ++i) {
+      const int e = own.first + (i << a.log_l);
+      if (val[e] > best) { best = val[e]; at = e; }
     }
     const double top = warp_max_f64(best);
     const int id = (int)__reduce_min_sync(0xffffffffu, best == top ? (unsigned)at : (unsigned)RT_MAX_E);
@@ -187,36 +210,32 @@ __global__ void __launch_bounds__(32 * RT_WARPS) k_router(const RouterArgs a) {
   const long long row = (long long)blockIdx.x * RT_WARPS + warp;
   if (row >= a.rows) return;
   const float inf = __int_as_float(0x7f800000);
+  const RtLane own(a, lane);
   float v[NV];
-  float m = -inf;
 #pragma unroll
   for (int i = 0; i < NV; ++i) {
-    const int e = rt_expert(a, lane, i);
-    const float z = e >= 0 ? rt_load<T>(a.z, row * a.ld + e) : -inf;
+    const float z = i < own.count ? rt_load<T>(a.z, row * a.ld + own.first + (i << a.log_l)) : -inf;
     v[i] = z > -inf ? z : -inf;   // NaN too
   }
   if (a.avail) {
 #pragma unroll
-    for (int i = 0; i < NV; ++i) {
-      const int e = rt_expert(a, lane, i);
-      if (e >= 0 && !a.avail[e]) v[i] = -inf;
-    }
+    for (int i = 0; i < NV; ++i)
+      if (i < own.count && !a.avail[own.first + (i << a.log_l)]) v[i] = -inf;
   }
+  float m = -inf, sum = 0.0f, tol = 0.0f;
   if (BY_SCORE || (a.softmax && !a.norm)) {
 #pragma unroll
     for (int i = 0; i < NV; ++i) m = fmaxf(m, v[i]);
     m = f32_from_ukey(__reduce_max_sync(0xffffffffu, f32_ukey(m)));
-  }
-  float sum = 0.0f;
-  if (a.softmax && (BY_SCORE || !a.norm)) {
+    if (a.softmax) {
 #pragma unroll
-    for (int i = 0; i < NV; ++i)
-      sum += v[i] == -inf ? 0.0f : v[i] == m ? 1.0f : __expf(v[i] - m);   // all +inf logits share the mass
-    sum = warp_sum_f32(sum);
+      for (int i = 0; i < NV; ++i)   // all +inf logits share the mass
+        sum += v[i] == -inf ? 0.0f : v[i] == m ? 1.0f : __expf(v[i] - m);
+      sum = warp_sum_f32(sum);
+    }
   }
   uint32_t key[NV];
-  bool near = false;
-  float tol = 0.0f;
+  bool in = true;   // the lane's group is kept
   if (BY_SCORE) {
     // |c - exact| <= tol + 2^-24 |c|, tol relative to the row's largest score: __expf
     // is off by 2 + 1.2 |x| ulp and |x| e^x <= 0.4 for x <= 0, so the exponentials
@@ -224,36 +243,26 @@ __global__ void __launch_bounds__(32 * RT_WARPS) k_router(const RouterArgs a) {
     // 5 shuffled adds within 69 * 2^-24 < 5e-6 of itself. Scores below e^-80 are not
     // told apart (1e-30).
     const float inv = a.softmax ? 1.0f / sum : 1.0f;
+    tol = (a.softmax ? 1.6e-5f * inv : 2.0e-6f * rt_sigmoid(m)) + 1e-30f;
     float hi = -inf, lo = -inf;
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
-      const int e = rt_expert(a, lane, i);
-      if (v[i] == -inf) {
-        key[i] = 0;
-        continue;
-      }
-      const float s = a.softmax ? (v[i] == m ? inv : __expf(v[i] - m) * inv)
-                                : rt_sigmoid(v[i]);
-      const float c = a.bias ? s + __ldg(a.bias + e) : s;
-      if (!(c > -inf)) {   // a bias of -inf or NaN takes the expert out
-        key[i] = 0;
-        continue;
-      }
-      key[i] = f32_ukey(a.bias ? c : v[i]);   // without a bias the logits have the scores' order, exactly
-      if (c > hi) { lo = hi; hi = c; }
-      else if (c > lo) lo = c;
+      const float s = a.softmax ? (v[i] == m ? inv : __expf(v[i] - m) * inv) : rt_sigmoid(v[i]);
+      float c = s;
+      if (a.bias) c += i < own.count ? __ldg(a.bias + own.first + (i << a.log_l)) : 0.0f;
+      c = v[i] > -inf && c > -inf ? c : -inf;   // a bias of -inf or NaN takes the expert out
+      lo = fmaxf(lo, fminf(hi, c));
+      hi = fmaxf(hi, c);
+      // without a bias the logits have the scores' order, exactly
+      key[i] = c > -inf ? f32_ukey(a.bias ? c : v[i]) : 0u;
     }
-    const float smax = a.softmax ? inv : rt_sigmoid(m);
-    tol = (a.softmax ? 1.6e-5f : 2.0e-6f) * smax + 1e-30f;
     if (a.G > 1) {
       float far;
-      const bool in = rt_group_kept(a, lane, hi, lo, -inf, &far);
+      in = rt_group_kept(a, lane, hi, lo, -inf, &far);
       const float mag = f32_from_ukey(__reduce_max_sync(0xffffffffu, f32_ukey(hi == -inf ? 0.0f : fabsf(hi))));
-      near = far <= 2.0f * tol + 5.0e-7f * mag;
-      if (!in) {
+      if (far <= 4.0f * tol + 5.0e-7f * mag) in = rt_groups_f64<T>(a, row, lane, (double)m);
 #pragma unroll
-        for (int i = 0; i < NV; ++i) key[i] = 0;
-      }
+      for (int i = 0; i < NV; ++i) key[i] = in ? key[i] : 0u;
     }
   } else {
 #pragma unroll
@@ -262,14 +271,16 @@ __global__ void __launch_bounds__(32 * RT_WARPS) k_router(const RouterArgs a) {
   // The first K (one more where neighbours are compared), descending, ties to the lower id.
   const bool compared = BY_SCORE && a.bias;
   const int places = compared ? a.K + 1 : a.K;
-  int mine = -1;
-  uint32_t my_key = 0;
   uint32_t cur = 0, bound = 0;
 #pragma unroll
   for (int i = 0; i < NV; ++i) cur = max(cur, key[i]);
   for (int j = 0; j < places; ++j) {
     bound = __reduce_max_sync(0xffffffffu, cur);
     if (cur == bound) cur = 0;   // equal lane maxima go together: the bound is lower then, and still one
+  }
+  if (compared && bound > 0) {   // whatever might be as large as the bound in exact arithmetic is a candidate too
+    const float c = f32_from_ukey(bound);
+    bound = f32_ukey(fmaxf(c - 2.0f * tol - 2.5e-7f * fabsf(c), -3.402823466e38f));
   }
   bound = max(bound, 1u);
   int n = 0;
@@ -279,25 +290,26 @@ __global__ void __launch_bounds__(32 * RT_WARPS) k_router(const RouterArgs a) {
     if (who) {
       const int at = n + __popc(who & ((1u << lane) - 1u));
       if (key[i] >= bound && at < 32)
-        cand[warp][at] = ((unsigned long long)key[i] << 32) | (0xFFFFFFFFu - (uint32_t)rt_expert(a, lane, i));
+        cand[warp][at] = ((unsigned long long)key[i] << 32) | (0xFFFFFFFFu - (uint32_t)(own.first + (i << a.log_l)));
       n += __popc(who);
     }
   }
+  int mine = -1;
+  uint32_t my_key = 0;
+  __syncwarp();
   if (n <= 32) {
-    __syncwarp();
-    const unsigned long long own = lane < n ? cand[warp][lane] : 0;
+    const unsigned long long c = lane < n ? cand[warp][lane] : 0;
     int place = 0;
-    for (int q = 0; q < n; ++q) place += cand[warp][q] > own;
+    for (int q = 0; q < n; ++q) place += cand[warp][q] > c;
     __syncwarp();
-    if (lane < n) cand[warp][place] = own;
+    if (lane < n) cand[warp][place] = c;
     __syncwarp();
-    if (lane < min(n, places)) {
-      const unsigned long long c = cand[warp][lane];
-      mine = (int)(0xFFFFFFFFu - (uint32_t)c);
-      my_key = (uint32_t)(c >> 32);
+    if (lane < n) {
+      mine = (int)(0xFFFFFFFFu - (uint32_t)cand[warp][lane]);
+      my_key = (uint32_t)(cand[warp][lane] >> 32);
     }
   } else {
-    // many equal keys, or k near 32: one after another, two redux each
+    // many near keys, or k near 32: one after another, two redux each
     for (int j = 0; j < places; ++j) {
       uint32_t best = 0;
       int bi = 0;
@@ -306,7 +318,7 @@ __global__ void __launch_bounds__(32 * RT_WARPS) k_router(const RouterArgs a) {
         if (key[i] > best) { best = key[i]; bi = i; }
       const uint32_t top = __reduce_max_sync(0xffffffffu, best);
       if (top == 0) break;
-      const int at = best == top ? rt_expert(a, lane, bi) : RT_MAX_E;
+      const int at = best == top ? own.first + (bi << a.log_l) : RT_MAX_E;
       const int id = (int)__reduce_min_sync(0xffffffffu, (unsigned)at);
       if (at == id) {
 #pragma unroll
@@ -317,21 +329,28 @@ __global__ void __launch_bounds__(32 * RT_WARPS) k_router(const RouterArgs a) {
     }
   }
   float z = mine >= 0 ? rt_load<T>(a.z, row * a.ld + mine) : -inf;
-  if (BY_SCORE) {
-    if (compared) {
-      const float b = mine >= 0 ? a.bias[mine] : 0.0f;
-      const int nid = __shfl_down_sync(0xffffffffu, mine, 1);
-      const float nz = __shfl_down_sync(0xffffffffu, z, 1), nb = __shfl_down_sync(0xffffffffu, b, 1);
-      const uint32_t nk = __shfl_down_sync(0xffffffffu, my_key, 1);
-      // equal logits with equal biases are equal in exact arithmetic too, except at the last place: what is
-      // near the first one left out is not looked at
-      if (lane < a.K && mine >= 0 && nid >= 0 && !(z == nz && b == nb && lane < a.K - 1)) {
-        const float c = f32_from_ukey(my_key), nc = f32_from_ukey(nk);
-        near |= c - nc <= 2.0f * tol + 2.5e-7f * fmaxf(fabsf(c), fabsf(nc));
-      }
+  if (compared) {
+    const float b = mine >= 0 ? __ldg(a.bias + mine) : 0.0f;
+    const int nid = __shfl_down_sync(0xffffffffu, mine, 1);
+    const float nz = __shfl_down_sync(0xffffffffu, z, 1), nb = __shfl_down_sync(0xffffffffu, b, 1);
+    const uint32_t nk = __shfl_down_sync(0xffffffffu, my_key, 1);
+    bool near = false;
+    // equal logits with equal biases are equal in exact arithmetic too, except at the last place: what is
+    // near the first one left out is not looked at
+    if (lane < a.K && lane < 31 && mine >= 0 && nid >= 0 && !(z == nz && b == nb && lane < a.K - 1)) {
+      const float c = f32_from_ukey(my_key), nc = f32_from_ukey(nk);
+      near = c - nc <= 2.0f * tol + 2.5e-7f * fmaxf(fabsf(c), fabsf(nc));
     }
     if (__any_sync(0xffffffffu, near)) {
-      mine = rt_choose_f64<T>(a, row, lane, rt_smem + (size_t)warp * a.E);
+      if (n <= 32) {
+        const int place = rt_place_f64<T>(a, row, lane, mine, n, (double)m);
+        __syncwarp();
+        if (lane < n) cand[warp][place] = (unsigned long long)mine;
+        __syncwarp();
+        if (lane < n) mine = (int)cand[warp][lane];
+      } else {
+        mine = rt_choose_f64<T>(a, row, lane, in, (double)m, rt_smem + (size_t)warp * a.E);
+      }
       z = mine >= 0 ? rt_load<T>(a.z, row * a.ld + mine) : -inf;
     }
   }
@@ -341,11 +360,12 @@ __global__ void __launch_bounds__(32 * RT_WARPS) k_router(const RouterArgs a) {
   float w;
   if (a.norm) {
     const float M = f32_from_ukey(__reduce_max_sync(0xffffffffu, f32_ukey(z)));
-    if (a.softmax) w = z == -inf ? 0.0f : z == M ? 1.0f : expf(z - M);
-    else if (M < 0.0f) w = z == -inf ? 0.0f : expf(z - M) / (1.0f + expf(z));
-    else w = z == -inf ? 0.0f : 1.0f / (1.0f + expf(-z));
+    const bool rel = a.softmax || M < 0.0f;
+    const float e = expf(rel ? (z == M ? 0.0f : z - M) : -z);   // z = -inf: 0, or infinity
+    w = a.softmax ? e : __fdividef(rel ? e : 1.0f, 1.0f + (rel ? expf(z) : e));
+    w = z == -inf ? 0.0f : w;
     const float t = warp_sum_f32(w);
-    w = t > 0.0f ? w / t * a.scale : 0.0f;
+    w = t > 0.0f ? __fdividef(w, t) * a.scale : 0.0f;
   } else {
     if (a.softmax) w = z == -inf ? 0.0f : (z == m ? 1.0f : expf(z - m)) / sum * a.scale;
     else w = z == -inf ? 0.0f : 1.0f / (1.0f + expf(-z)) * a.scale;

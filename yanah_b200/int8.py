@@ -21,7 +21,7 @@ from typing import NamedTuple, Optional
 import torch
 
 from . import _lib
-from .launch import DTYPES, check_floats, check_like, elsewhere, row_stride, rows_of, run_there
+from .launch import DTYPES, check_floats, check_like, elsewhere, raw_stream, row_stride, rows_of, run_there
 
 
 class Int8Matrix(NamedTuple):
@@ -47,7 +47,7 @@ def quantize_rows(x: torch.Tensor, stream: Optional[torch.cuda.Stream] = None) -
     scales = torch.empty((rows,), dtype=torch.float32, device=x.device)
     _lib.check(_lib.lib().yn_i8_quant_rows(flat.data_ptr(), DTYPES[x.dtype], row_stride(flat), rows, k, codes.data_ptr(),
                                            codes.stride(0), scales.data_ptr(),
-                                           torch.cuda.current_stream(x.device).cuda_stream))
+                                           raw_stream(x.device)))
     lead = x.shape[:-1]
     return Int8Matrix(codes.view(*lead, codes.shape[-1])[..., :k], scales.view(lead))
 
@@ -93,7 +93,7 @@ def int8_linear(x: torch.Tensor, w: Int8Matrix, out_dtype: Optional[torch.dtype]
     ws = torch.empty(nb, dtype=torch.uint8, device=x.device) if nb else None
     _lib.check(lib.yn_i8_linear(C.byref(m), x.data_ptr(), DTYPES[x.dtype], row_stride(x), rows, y.data_ptr(),
                                 DTYPES[out_dtype], m.rows, None if ws is None else ws.data_ptr(), nb,
-                                torch.cuda.current_stream(x.device).cuda_stream))
+                                raw_stream(x.device)))
     return y
 
 
@@ -139,7 +139,7 @@ def int8_experts(x: torch.Tensor, ids: torch.Tensor, weights: torch.Tensor, gate
                                  None if residual is None else residual.data_ptr(),
                                  0 if residual is None else row_stride(residual), out.data_ptr(), row_stride(out),
                                  ws.data_ptr(), nb,
-                                 torch.cuda.current_stream(x.device).cuda_stream))
+                                 raw_stream(x.device)))
     return out
 
 

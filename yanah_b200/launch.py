@@ -49,6 +49,11 @@ def row_stride(t: torch.Tensor) -> int:
     return t.stride(0) if t.shape[0] > 1 else max(t.stride(0), t.shape[1])
 
 
+def raw_stream(device: torch.device) -> int:
+    """The current stream of a device as the C ABI takes it."""
+    return torch._C._cuda_getCurrentRawStream(device.index)
+
+
 def elsewhere(device: torch.device, stream: Optional[torch.cuda.Stream]) -> bool:
     """Whether a call has to leave the current device or stream."""
     return stream is not None or device.index != torch.cuda.current_device()

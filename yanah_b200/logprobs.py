@@ -12,7 +12,7 @@ from typing import NamedTuple, Optional
 import torch
 
 from . import _lib
-from .launch import DTYPES, check_floats, check_like, elsewhere, row_stride, rows_of, run_there
+from .launch import DTYPES, check_floats, check_like, elsewhere, raw_stream, row_stride, rows_of, run_there
 
 
 class TokenLogprobs(NamedTuple):
@@ -63,7 +63,7 @@ def token_logprobs(logits: torch.Tensor, tokens: Optional[torch.Tensor] = None, 
         logits.data_ptr(), dt, row_stride(logits), rows, vocab, None if tokens is None else tokens.data_ptr(), n_top,
         logprob.data_ptr(), entropy.data_ptr(), rank.data_ptr(), top_ids.data_ptr() if n_top else None,
         top_lp.data_ptr() if n_top else None, None if ws is None else ws.data_ptr(), nb,
-        torch.cuda.current_stream(dev).cuda_stream))
+        raw_stream(dev)))
     if tokens is None:
         logprob = rank = None
     return TokenLogprobs(logprob, rank, entropy, top_ids, top_lp)

@@ -19,7 +19,7 @@ from typing import Optional, Tuple
 import torch
 
 from . import _lib
-from .launch import DTYPES, check_floats, check_like, elsewhere, row_stride, rows_of, run_there
+from .launch import DTYPES, check_floats, check_like, elsewhere, raw_stream, row_stride, rows_of, run_there
 
 SCORES = {"softmax": 0, "sigmoid": 1}
 
@@ -91,5 +91,5 @@ def route_scored(logits: torch.Tensor, rule: RouteRule, bias: Optional[torch.Ten
     _lib.check(_lib.lib().yn_route_scored(
         C.byref(rule.struct(e)), logits.data_ptr(), DTYPES[logits.dtype], row_stride(logits), rows,
         None if bias is None else bias.data_ptr(), None if available is None else available.data_ptr(),
-        ids.data_ptr(), weights.data_ptr(), torch.cuda.current_stream(logits.device).cuda_stream))
+        ids.data_ptr(), weights.data_ptr(), raw_stream(logits.device)))
     return ids, weights
