@@ -515,13 +515,11 @@ int yn_i8_error(void* stream, int32_t* code_out);
  * them alone has log probabilities of -inf and entropy 0. Logits of +inf share
  * the mass. A NaN makes the row's log probabilities and entropy NaN, its rank
  * and ids -1. A token outside [0, vocab) gives NaN and rank -1. tokens, with
- * logprob and rank, may be NULL; so may entropy; top_* with n_top = 0. ws:
- * yn_logprobs_ws_bytes bytes, need not be cleared. Launches one kernel, or two
- * where few rows are split over the device. */
-size_t yn_logprobs_ws_bytes(int64_t rows, int64_t vocab, int32_t dtype, int32_t n_top);
+ * logprob and rank, may be NULL; so may entropy; top_* with n_top = 0. Launches
+ * one kernel. */
 int yn_token_logprobs(const void* logits, int32_t dtype, int64_t row_stride, int64_t rows, int64_t vocab,
                       const int32_t* tokens, int32_t n_top, float* logprob, float* entropy, int32_t* rank,
-                      int32_t* top_ids, float* top_logprobs, void* ws, size_t ws_bytes, void* stream);
+                      int32_t* top_ids, float* top_logprobs, void* stream);
 
 /* ---------------------------------------------------------- slot copies */
 

@@ -39,19 +39,16 @@ def test_route_scored():
         RouteRule(4, "tanh")
 
 
-def logprobs(dtype=0, stride=100, rows=3, vocab=100, tokens=P, n=0, top=P, ws=None, nb=0, logits=P, lp=P):
-    return _lib.lib().yn_token_logprobs(logits, dtype, stride, rows, vocab, tokens, n, lp, P, P, top, top, ws, nb, None)
+def logprobs(dtype=0, stride=100, rows=3, vocab=100, tokens=P, n=0, top=P, logits=P, lp=P):
+    return _lib.lib().yn_token_logprobs(logits, dtype, stride, rows, vocab, tokens, n, lp, P, P, top, top, None)
 
 
 def test_token_logprobs():
     for kw in (dict(dtype=5), dict(stride=99), dict(vocab=0), dict(n=-1), dict(n=65), dict(vocab=3, n=4), dict(n=3, top=None),
-               dict(logits=None), dict(lp=None), dict(rows=-1), dict(logits=C.c_void_p(258)),
-               dict(vocab=100000, stride=100000, ws=None), dict(vocab=100000, stride=100000, ws=P, nb=8)):
+               dict(logits=None), dict(lp=None), dict(rows=-1), dict(logits=C.c_void_p(258))):
         assert logprobs(**kw) == INV, kw
     assert logprobs(vocab=2 ** 31, stride=2 ** 31) == UNS
     assert logprobs(rows=0, logits=None) == _lib.YN_OK
-    assert _lib.lib().yn_logprobs_ws_bytes(1000, 100, 0, 5) == 0
-    assert _lib.lib().yn_logprobs_ws_bytes(1, 151936, 0, 20) > 0
 
 
 def mat(mats=1, rows=32, cols=64, rs=64, ms=2048, ss=32, codes=256, scales=256):

@@ -189,7 +189,7 @@ YN_DEV void i8_ld_wait(int (&v)[16]) {
                : "memory");
 }
 
-constexpr int I8_EPW = 8;                    // epilogue warps (warp % 4: TMEM lanes 32 (warp % 4)..+31)
+constexpr int I8_EPW = 16;                   // epilogue warps (warp % 4: TMEM lanes 32 (warp % 4)..+31)
 constexpr int I8_MW = I8_EPW, I8_LW = I8_EPW + 1;
 constexpr int I8_THREADS = 32 * (I8_EPW + 2);
 constexpr int I8_A_BYTES = 128 * 128;
@@ -261,7 +261,7 @@ __global__ void __launch_bounds__(I8_THREADS, 1) k_i8_gemm(const I8Gemm a, const
   };
 
   if (warp < I8_EPW) {
-    const int m = 32 * (warp & 3) + lane, half = warp >> 2;
+    const int m = 32 * (warp & 3) + lane, part = warp >> 2;
     long long j = 0;
     for (long long ti = blockIdx.x; ti < n_tiles; ti += gridDim.x, ++j) {
       int u0;
@@ -279,7 +279,7 @@ __global__ void __launch_bounds__(I8_THREADS, 1) k_i8_gemm(const I8Gemm a, const
       // channels of every second row (even lanes the even rows).
       const bool odd = lane & 1, two = (r | 1) < a.store_cols;
       const uint32_t sel = odd ? 0x3276u : 0x5410u;
-      for (int c0 = 16 * half; c0 < c.n; c0 += 32) {
+      for (int c0 = 16 * part; c0 < c.n; c0 += 4 * I8_EPW) {
         int v[16], w[16];
         i8_ld16(base + (uint32_t)c0, v);
         if (UP) i8_ld16(base + (uint32_t)(NB + c0), w);

@@ -17,7 +17,9 @@
 // of the n-th largest from below (of its 8 warps' or 256 threads' maxima), and from
 // then on only the threads whose maximum reaches it, a few times n in all, have their
 // elements looked at again (from L2).
-// Rows are split over blocks where there are few; a second kernel joins the parts.
+// Few rows are split over the blocks of a cluster, whose parts the first of them joins
+// through distributed shared memory: one launch, no workspace.
+#include <cooperative_groups.h>
 #include <cuda_runtime.h>
 
 #include <algorithm>
@@ -34,7 +36,7 @@ constexpr int LP_THREADS = 256;
 constexpr int LP_WARPS = LP_THREADS / 32;
 constexpr int LP_MAX_TOP = 64;
 constexpr int LP_CAND = 1024;        // candidates of one chunk that are ranked by counting
-constexpr int LP_MAX_SPLITS = 256;   // blocks of one row: one thread each in the join
+constexpr int LP_MAX_SPLITS = 8;     // blocks of one row: a portable cluster
 constexpr float LP_LOG2E = 1.44269504088896341f;
 constexpr float LP_LN2 = 0.69314718055994531f;
 
@@ -44,12 +46,6 @@ struct LpSums {
   float m, R, D;
   int rank;   // elements of the part that come before the given token
 };
-struct __align__(16) LpPart {
-  LpSums s;
-  int nan;
-  int pad[3];
-};
-
 struct LpArgs {
   const uint8_t* z;
   long long ld, rows;
@@ -60,8 +56,6 @@ struct LpArgs {
   int32_t* rank;
   int32_t* top_ids;
   float* top_lp;
-  LpPart* parts;                 // (rows, splits)
-  unsigned long long* lists;     // (rows, splits, n_top) keys, descending, 0: none
 };
 
 template <typename T>
@@ -244,7 +238,7 @@ YN_DEV unsigned long long lp_block_max(unsigned long long k, unsigned long long*
   return best;
 }
 
-template <typename T, int VPT>
+template <typename T, int VPT, bool SPLIT>
 __global__ void __launch_bounds__(LP_THREADS, 4) k_logprobs(const LpArgs a) {
   using L = LpType<T>;
   constexpr int PER = L::PER;
@@ -255,6 +249,8 @@ __global__ void __launch_bounds__(LP_THREADS, 4) k_logprobs(const LpArgs a) {
   __shared__ int n_cand;
   __shared__ unsigned long long cand[LP_CAND], list[LP_MAX_TOP], buf[2][LP_WARPS];
   __shared__ float log_s_s, m_s;
+  __shared__ LpSums part;
+  __shared__ int part_nan, part_have;
 
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const long long row = blockIdx.x / a.splits;
@@ -436,24 +432,32 @@ __global__ void __launch_bounds__(LP_THREADS, 4) k_logprobs(const LpArgs a) {
       }
     }
     if (a.n_top) {
-      // the elements of every thread of this warp that reaches the bound, one thread's vectors at a
-      // time, one lane per vector
+      // the elements of the warp's threads that reach the bound: 32 / VPT threads at a time, one
+      // lane per vector
       unsigned who = __ballot_sync(0xffffffffu, tk >= thr);
+      const float least = f32_from_ukey(thr);
       while (who) {
-        const int o = __ffs(who) - 1;
-        who &= who - 1;
-        const int at = c0 + lane * LP_THREADS + 32 * warp + o;
-        if (lane < VPT && at < v1) {
+        int o = -1;
+#pragma unroll
+        for (int q = 0; q < 32 / VPT && q < 4; ++q) {
+          if (who && lane / VPT == q) o = __ffs(who) - 1;
+          who &= who - 1;   // 0 stays 0
+        }
+        const int at = c0 + (lane % VPT) * LP_THREADS + 32 * warp + o;
+        if (o >= 0 && at < v1) {
           float f[PER];
           lp_unpack<T>(ldg_nc_v4(base + (size_t)at * 16), f);
-          const long long e0 = (long long)at * PER - lead;
+          unsigned hit = 0;
 #pragma unroll
-          for (int j = 0; j < PER; ++j) {
-            const uint32_t k = f32_ukey(f[j]);
-            if (k >= thr && e0 + j >= 0 && e0 + j < a.V) {
-              const int q = atomicAdd(&n_cand, 1);
-              if (q < LP_CAND) cand[q] = ((unsigned long long)k << 32) | (0xFFFFFFFFu - (uint32_t)(e0 + j));
-            }
+          for (int j = 0; j < PER; ++j) hit |= f[j] >= least ? 1u << j : 0u;
+          while (hit) {
+            const int j = __ffs(hit) - 1;
+            hit &= hit - 1;
+            const long long e = (long long)at * PER - lead + j;
+            if (e < 0 || e >= a.V) continue;
+            const int q = atomicAdd(&n_cand, 1);
+            if (q < LP_CAND)
+              cand[q] = ((unsigned long long)f32_ukey(L::load(p + e * sizeof(T))) << 32) | (0xFFFFFFFFu - (uint32_t)e);
           }
         }
       }
@@ -503,90 +507,92 @@ __global__ void __launch_bounds__(LP_THREADS, 4) k_logprobs(const LpArgs a) {
     have = min(n, a.n_top);
     __syncthreads();
   }
-  if (a.splits > 1) {
-    const long long at = row * a.splits + split;
+  bool row_nan = nan;
+  if constexpr (SPLIT) {
+    namespace cg = cooperative_groups;
+    cg::cluster_group cluster = cg::this_cluster();
     if (tid == 0) {
-      LpPart q = {sums, nan ? 1 : 0, {0, 0, 0}};
-      a.parts[at] = q;
+      part = sums;
+      part_nan = nan;
+      part_have = have;
     }
-    if (tid < a.n_top) a.lists[at * a.n_top + tid] = tid < have ? list[tid] : 0ull;
-    return;
+    cluster.sync();
+    if (split == 0) {
+      if (warp == 0) {
+        LpSums s = {-inf, 0.0f, 0.0f, 0};
+        if (lane < a.splits) {
+          s = *cluster.map_shared_rank(&part, lane);
+          row_nan = *cluster.map_shared_rank(&part_nan, lane) != 0;
+        }
+        sums = lp_warp_join(s);
+      }
+      row_nan = __syncthreads_or(row_nan) != 0;
+      if (a.n_top) {
+        // the parts' lists side by side, then placed as the candidates above
+        for (int i = tid; i < a.splits * a.n_top; i += LP_THREADS) {
+          const int q = i / a.n_top, j = i - q * a.n_top;
+          cand[i] = j < *cluster.map_shared_rank(&part_have, q) ? cluster.map_shared_rank(list, q)[j] : 0ull;
+        }
+        if (tid == 0) n_cand = 0;
+        __syncthreads();
+        for (int i = tid; i < a.splits * a.n_top; i += LP_THREADS) {
+          const unsigned long long k = cand[i];
+          if (!k) continue;
+          atomicAdd(&n_cand, 1);
+          int place = 0;
+          for (int q = 0; q < a.splits * a.n_top; ++q) place += cand[q] > k;
+          if (place < a.n_top) list[place] = k;
+        }
+        __syncthreads();
+        have = min(n_cand, a.n_top);
+      }
+    }
+    cluster.sync();   // no block leaves while its parts are read
+    if (split != 0) return;
   }
   if (tid == 0) {
-    lp_write(a, row, sums, nan, tok, z_tok, &log_s_s);
+    lp_write(a, row, sums, row_nan, tok, z_tok, &log_s_s);
     m_s = sums.m;
   }
   if (a.n_top) {
     __syncthreads();
-    if (tid < a.n_top) lp_write_top(a, row, tid, tid < have ? list[tid] : 0ull, m_s, log_s_s, nan);
+    if (tid < a.n_top) lp_write_top(a, row, tid, tid < have ? list[tid] : 0ull, m_s, log_s_s, row_nan);
   }
 }
 
-// The join of a row's parts, one block per row, one thread per part: sums over the
-// block, then the alternatives as an n_top-step merge of the parts' sorted lists.
-template <typename T>
-__global__ void __launch_bounds__(LP_MAX_SPLITS) k_logprobs_join(const LpArgs a) {
-  using L = LpType<T>;
-  __shared__ unsigned long long buf[2][LP_WARPS];
-  __shared__ LpSums ws[LP_WARPS];
-  __shared__ float log_s_s, m_s;
-  const int tid = threadIdx.x;
-  const long long row = blockIdx.x;
-  const bool on = tid < a.splits;
-  const long long at = row * a.splits + tid;
-  LpSums s = {-__int_as_float(0x7f800000), 0.0f, 0.0f, 0};
-  int bad = 0;
-  if (on) {
-    const LpPart q = a.parts[at];
-    s = q.s;
-    bad = q.nan;
-  }
-  s = lp_warp_join(s);
-  if ((tid & 31) == 0) ws[tid >> 5] = s;
-  const bool nan = __syncthreads_or(bad) != 0;
-  if (tid < 32) {
-    const LpSums none = {-__int_as_float(0x7f800000), 0.0f, 0.0f, 0};
-    s = lp_warp_join(tid < (int)(blockDim.x >> 5) ? ws[tid] : none);
-  }
-  if (tid == 0) {
-    const int tok = a.tokens ? a.tokens[row] : -1;
-    const float z_tok = tok >= 0 && tok < a.V ? L::load(a.z + ((size_t)row * a.ld + tok) * sizeof(T)) : 0.0f;
-    lp_write(a, row, s, nan, tok, z_tok, &log_s_s);
-    m_s = s.m;
-  }
-  if (!a.n_top) return;
-  const unsigned long long* mine = a.lists + at * a.n_top;
-  int next = 0;
-  unsigned long long head = on ? mine[0] : 0ull, win = 0;
-  for (int j = 0; j < a.n_top; ++j) {
-    const unsigned long long best = lp_block_max(head, buf[j & 1]);
-    if (tid == j) win = best;
-    if (best && head == best) head = ++next < a.n_top ? mine[next] : 0ull;
-  }
-  __syncthreads();
-  if (tid < a.n_top) lp_write_top(a, row, tid, win, m_s, log_s_s, nan);
-}
-
-// How a row is split: enough blocks for two waves when the rows alone are fewer,
+// How a row is split: enough blocks for two on every SM when the rows alone are fewer,
 // each with at least one 16-byte load per thread.
-int lp_splits(long long rows, long long vocab, int size) {
-  const long long vecs = (vocab * size + 15) / 16 + 1;
-  if (rows >= 2 * 148) return 1;
-  const long long want = (2 * 148 + rows - 1) / rows, most = (vecs + LP_THREADS - 1) / LP_THREADS;
-  return (int)std::max<long long>(1, std::min<long long>(LP_MAX_SPLITS, std::min(want, most)));
+int lp_splits(long long rows, long long vecs) {
+  int s = 1;
+  while (s < LP_MAX_SPLITS && rows * 2 * s <= 2 * 148 && vecs >= 2 * s * LP_THREADS) s *= 2;
+  return s;
 }
 
-template <typename T>
-void launch_logprobs(const LpArgs& a, cudaStream_t st) {
-  const unsigned grid = (unsigned)(a.rows * a.splits);
-  if (a.split_vecs <= LP_THREADS) k_logprobs<T, 1><<<grid, LP_THREADS, 0, st>>>(a);
-  else if (a.split_vecs <= 2 * LP_THREADS) k_logprobs<T, 2><<<grid, LP_THREADS, 0, st>>>(a);
-  else if (a.split_vecs <= 4 * LP_THREADS) k_logprobs<T, 4><<<grid, LP_THREADS, 0, st>>>(a);
-  else k_logprobs<T, 8><<<grid, LP_THREADS, 0, st>>>(a);
-  if (a.splits > 1) {
-    const int threads = std::max((a.splits + 31) / 32 * 32, a.n_top > 32 ? 64 : 32);
-    k_logprobs_join<T><<<(unsigned)a.rows, threads, 0, st>>>(a);
+template <typename T, int VPT>
+cudaError_t launch_logprobs_vpt(const LpArgs& a, cudaStream_t st) {
+  if (a.splits == 1) {
+    k_logprobs<T, VPT, false><<<(unsigned)a.rows, LP_THREADS, 0, st>>>(a);
+    return cudaGetLastError();
   }
+  cudaLaunchConfig_t c{};
+  c.gridDim = dim3((unsigned)(a.rows * a.splits));
+  c.blockDim = dim3(LP_THREADS);
+  c.stream = st;
+  cudaLaunchAttribute at{};
+  at.id = cudaLaunchAttributeClusterDimension;
+  at.val.clusterDim.x = a.splits;
+  at.val.clusterDim.y = at.val.clusterDim.z = 1;
+  c.attrs = &at;
+  c.numAttrs = 1;
+  return cudaLaunchKernelEx(&c, k_logprobs<T, VPT, true>, a);
+}
+// Pieces per thread: all of a short part at once, else 8.
+template <typename T>
+cudaError_t launch_logprobs(const LpArgs& a, cudaStream_t st) {
+  if (a.split_vecs <= LP_THREADS) return launch_logprobs_vpt<T, 1>(a, st);
+  if (a.split_vecs <= 2 * LP_THREADS) return launch_logprobs_vpt<T, 2>(a, st);
+  if (a.split_vecs <= 4 * LP_THREADS) return launch_logprobs_vpt<T, 4>(a, st);
+  return launch_logprobs_vpt<T, 8>(a, st);
 }
 
 }  // namespace ynb
@@ -597,16 +603,9 @@ namespace {
 int lp_size(int dtype) { return dtype == YN_F32 ? 4 : dtype == YN_BF16 || dtype == YN_F16 ? 2 : 0; }
 }  // namespace
 
-extern "C" size_t yn_logprobs_ws_bytes(int64_t rows, int64_t vocab, int32_t dtype, int32_t n_top) {
-  const int size = lp_size(dtype);
-  if (rows < 1 || vocab < 1 || vocab > 0x7fffff00LL || !size || n_top < 0 || n_top > LP_MAX_TOP) return 0;
-  const long long s = lp_splits(rows, vocab, size);
-  return s == 1 ? 0 : (size_t)(rows * s) * (sizeof(LpPart) + 8 * (size_t)n_top);
-}
-
 extern "C" int yn_token_logprobs(const void* logits, int32_t dtype, int64_t row_stride, int64_t rows, int64_t vocab,
                                  const int32_t* tokens, int32_t n_top, float* logprob, float* entropy, int32_t* rank,
-                                 int32_t* top_ids, float* top_logprobs, void* ws, size_t ws_bytes, void* stream) {
+                                 int32_t* top_ids, float* top_logprobs, void* stream) {
   const int size = lp_size(dtype);
   if (!size) return host_fail(YN_E_INVALID, "unknown dtype");
   if (vocab < 1 || rows < 0 || row_stride < vocab) return host_fail(YN_E_INVALID, "row_stride must be at least vocab, vocab at least 1");
@@ -623,8 +622,8 @@ extern "C" int yn_token_logprobs(const void* logits, int32_t dtype, int64_t row_
   a.rows = rows;
   a.V = (int)vocab;
   a.n_top = n_top;
-  a.splits = lp_splits(rows, vocab, size);
   const long long vecs = (vocab * size + 15) / 16 + 1;   // one more: a row may start inside a vector
+  a.splits = lp_splits(rows, vecs);
   a.split_vecs = (int)((vecs + a.splits - 1) / a.splits);
   a.tokens = tokens;
   a.logprob = logprob;
@@ -632,18 +631,10 @@ extern "C" int yn_token_logprobs(const void* logits, int32_t dtype, int64_t row_
   a.rank = rank;
   a.top_ids = top_ids;
   a.top_lp = top_logprobs;
-  if (a.splits > 1) {
-    const size_t need = yn_logprobs_ws_bytes(rows, vocab, dtype, n_top);
-    if (!ws || ws_bytes < need || reinterpret_cast<uintptr_t>(ws) % 16)
-      return host_fail(YN_E_INVALID, "workspace too small or not 16-byte aligned");
-    a.parts = reinterpret_cast<LpPart*>(ws);
-    a.lists = reinterpret_cast<unsigned long long*>(a.parts + rows * a.splits);
-  }
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
-  if (dtype == YN_F32) launch_logprobs<float>(a, st);
-  else if (dtype == YN_BF16) launch_logprobs<__nv_bfloat16>(a, st);
-  else launch_logprobs<__half>(a, st);
-  const cudaError_t e = cudaGetLastError();
+  const cudaError_t e = dtype == YN_F32    ? launch_logprobs<float>(a, st)
+                        : dtype == YN_BF16 ? launch_logprobs<__nv_bfloat16>(a, st)
+                                           : launch_logprobs<__half>(a, st);
   if (e != cudaSuccess) return host_fail(YN_E_CUDA, std::string("yn_token_logprobs: ") + cudaGetErrorString(e));
   return YN_OK;
 }

@@ -50,20 +50,16 @@ def token_logprobs(logits: torch.Tensor, tokens: Optional[torch.Tensor] = None, 
         raise ValueError("logits must have at least one column")
     if not 0 <= n_top <= min(64, vocab):
         raise ValueError(f"n_top must be in [0, {min(64, vocab)}], not {n_top}")
-    floats = torch.empty((3, rows), dtype=torch.float32, device=dev)
-    logprob, entropy, rank = floats[0], floats[1], floats[2].view(torch.int32)
-    top_ids = top_lp = None
+    entropy = torch.empty(rows, dtype=torch.float32, device=dev)
+    logprob = rank = top_ids = top_lp = None
+    if tokens is not None:
+        logprob = torch.empty_like(entropy)
+        rank = torch.empty_like(tokens)
     if n_top:
-        tops = torch.empty((2, rows, n_top), dtype=torch.float32, device=dev)
-        top_ids, top_lp = tops[0].view(torch.int32), tops[1]
-    lib, dt = _lib.lib(), DTYPES[logits.dtype]
-    nb = int(lib.yn_logprobs_ws_bytes(rows, vocab, dt, n_top))
-    ws = torch.empty(nb, dtype=torch.uint8, device=dev) if nb else None
-    _lib.check(lib.yn_token_logprobs(
-        logits.data_ptr(), dt, row_stride(logits), rows, vocab, None if tokens is None else tokens.data_ptr(), n_top,
-        logprob.data_ptr(), entropy.data_ptr(), rank.data_ptr(), top_ids.data_ptr() if n_top else None,
-        top_lp.data_ptr() if n_top else None, None if ws is None else ws.data_ptr(), nb,
-        raw_stream(dev)))
-    if tokens is None:
-        logprob = rank = None
+        top_ids = torch.empty((rows, n_top), dtype=torch.int32, device=dev)
+        top_lp = torch.empty((rows, n_top), dtype=torch.float32, device=dev)
+    ptr = lambda t: None if t is None else t.data_ptr()  # noqa: E731
+    _lib.check(_lib.lib().yn_token_logprobs(
+        logits.data_ptr(), DTYPES[logits.dtype], row_stride(logits), rows, vocab, ptr(tokens), n_top, ptr(logprob),
+        entropy.data_ptr(), ptr(rank), ptr(top_ids), ptr(top_lp), raw_stream(dev)))
     return TokenLogprobs(logprob, rank, entropy, top_ids, top_lp)
