@@ -26,43 +26,49 @@ YN_DEV void i8_store(int dt, void* p, size_t i, float v) {
 
 // ------------------------------------------------------------- row codes
 constexpr int I8_QT = 128;     // threads of a row
-constexpr int I8_QHOLD = 4;    // 8-element pieces a thread keeps in registers between the two steps
+constexpr long long I8_QWARP = 1184;   // rows from which a warp each fills the device (8 per SM)
 
-// One block per row: the largest magnitude, then the codes. Rows of up to
-// I8_QT * 8 * I8_QHOLD = 4096 elements are read once, longer ones a second time from
-// L2. The codes go to row `to[j]` for each of the `copies` entries of the row's list
-// (or to the row itself): a row's codes are made once for all of its experts.
-template <typename T, bool VEC>
-__global__ void __launch_bounds__(I8_QT) k_i8_quant(const void* x, long long ldx, int K, const int32_t* to, int copies,
-                                                    int8_t* codes, long long ldc, float* scales) {
+// The largest magnitude, then the codes, by N threads per row: a block where there are few
+// rows, a warp where there are many (no barrier, 8 loads in flight per lane). Rows of up to
+// N * 8 * HOLD elements are read once, longer ones a second time from L2. The codes go to row
+// `to[j]` for each of the `copies` entries of the row's list (or to the row itself): a row's
+// codes are made once for all of its experts.
+template <typename T, bool VEC, int N, int HOLD>
+__global__ void __launch_bounds__(I8_QT) k_i8_quant(const void* x, long long ldx, long long rows, int K, const int* n_rows,
+                                                    const int32_t* to, int copies, int8_t* codes, long long ldc,
+                                                    float* scales) {
   __shared__ uint32_t buf[I8_QT / 32];
-  const size_t row = blockIdx.x, base = row * (size_t)ldx;
-  const int tid = threadIdx.x, n8 = VEC ? K / 8 : 0;
-  float f[I8_QHOLD][8];
+  const size_t row = blockIdx.x * (size_t)(I8_QT / N) + threadIdx.x / N, base = row * (size_t)ldx;
+  if (row >= (size_t)(n_rows ? *n_rows : rows)) return;
+  const int tid = threadIdx.x % N, n8 = VEC ? K / 8 : 0;
+  I8Raw<T> raw[HOLD], one;
   uint32_t m = 0;
-#pragma unroll
-  for (int i = 0; i < I8_QHOLD; ++i) {
-    const int at = tid + i * I8_QT;
-    if (at < n8) {
-      i8_load8<T>(x, base + 8 * (size_t)at, f[i]);
-#pragma unroll
-      for (int j = 0; j < 8; ++j) m = max(m, i8_abs_bits(f[i][j]));
-    }
-  }
-  for (int at = tid + I8_QHOLD * I8_QT; at < n8; at += I8_QT) {
+  auto max8 = [&](const I8Raw<T>& r) {
     float g[8];
-    i8_load8<T>(x, base + 8 * (size_t)at, g);
+    r.get(g);
 #pragma unroll
     for (int j = 0; j < 8; ++j) m = max(m, i8_abs_bits(g[j]));
+  };
+#pragma unroll
+  for (int i = 0; i < HOLD; ++i)
+    if (tid + i * N < n8) raw[i].load(x, base + 8 * (size_t)(tid + i * N));
+#pragma unroll
+  for (int i = 0; i < HOLD; ++i)
+    if (tid + i * N < n8) max8(raw[i]);
+  for (int at = tid + HOLD * N; at < n8; at += N) {
+    one.load(x, base + 8 * (size_t)at);
+    max8(one);
   }
-  for (int k = 8 * n8 + tid; k < K; k += I8_QT) m = max(m, i8_abs_bits(I8In<T>::load(x, base + k)));
-  const I8Row q(block_max_u32(m, buf));
+  for (int k = 8 * n8 + tid; k < K; k += N) m = max(m, i8_abs_bits(I8In<T>::load(x, base + k)));
+  const I8Row q(N == 32 ? __reduce_max_sync(0xffffffffu, m) : block_max_u32(m, buf));
   const float scale = q.scale();
   const int n_to = to ? copies : 1;
   auto out = [&](int j) -> long long { return to ? to[row * copies + j] : (long long)row; };
   if (tid < n_to && out(tid) >= 0) scales[out(tid)] = scale;
-  auto put8 = [&](int at, const float (&g)[8]) {
+  auto put8 = [&](int at, const I8Raw<T>& r) {
+    float g[8];
     uint32_t w[2];
+    r.get(g);
     q.codes(g, w);
     const uint2 c = make_uint2(w[0], w[1]);
     for (int j = 0; j < n_to; ++j) {
@@ -71,14 +77,13 @@ __global__ void __launch_bounds__(I8_QT) k_i8_quant(const void* x, long long ldx
     }
   };
 #pragma unroll
-  for (int i = 0; i < I8_QHOLD; ++i)
-    if (tid + i * I8_QT < n8) put8(tid + i * I8_QT, f[i]);
-  for (int at = tid + I8_QHOLD * I8_QT; at < n8; at += I8_QT) {
-    float g[8];
-    i8_load8<T>(x, base + 8 * (size_t)at, g);
-    put8(at, g);
+  for (int i = 0; i < HOLD; ++i)
+    if (tid + i * N < n8) put8(tid + i * N, raw[i]);
+  for (int at = tid + HOLD * N; at < n8; at += N) {
+    one.load(x, base + 8 * (size_t)at);
+    put8(at, one);
   }
-  for (int k = 8 * n8 + tid; k < K; k += I8_QT) {
+  for (int k = 8 * n8 + tid; k < K; k += N) {
     const float g[4] = {I8In<T>::load(x, base + k), 0.0f, 0.0f, 0.0f};
     uint32_t w[1];
     q.codes(g, w);
@@ -88,15 +93,17 @@ __global__ void __launch_bounds__(I8_QT) k_i8_quant(const void* x, long long ldx
   }
 }
 
-int launch_quant(int dt, const void* x, long long ldx, long long rows, int K, const int32_t* to, int copies,
+int launch_quant(int dt, const void* x, long long ldx, long long rows, int K, const int* n_rows, const int32_t* to, int copies,
                  int8_t* codes, long long ldc, float* scales, cudaStream_t st) {
   const size_t size = dt == YN_F32 ? 4 : 2;
   const bool vec = reinterpret_cast<uintptr_t>(x) % 16 == 0 && (ldx * size) % 16 == 0 &&
                    reinterpret_cast<uintptr_t>(codes) % 8 == 0 && ldc % 8 == 0;
-  const dim3 g((unsigned)rows), b(I8_QT);
-#define YN_Q(T)                                                                                            \
-  if (vec) k_i8_quant<T, true><<<g, b, 0, st>>>(x, ldx, K, to, copies, codes, ldc, scales);               \
-  else k_i8_quant<T, false><<<g, b, 0, st>>>(x, ldx, K, to, copies, codes, ldc, scales)
+  const bool warps = vec && rows >= I8_QWARP && K <= 4096;
+  const dim3 g((unsigned)(warps ? (rows + I8_QT / 32 - 1) / (I8_QT / 32) : rows)), b(I8_QT);
+#define YN_Q(T)                                                                                                             \
+  if (warps) k_i8_quant<T, true, 32, sizeof(T) == 4 ? 6 : 8><<<g, b, 0, st>>>(x, ldx, rows, K, n_rows, to, copies, codes, ldc, scales);         \
+  else if (vec) k_i8_quant<T, true, I8_QT, 4><<<g, b, 0, st>>>(x, ldx, rows, K, n_rows, to, copies, codes, ldc, scales);   \
+  else k_i8_quant<T, false, I8_QT, 4><<<g, b, 0, st>>>(x, ldx, rows, K, n_rows, to, copies, codes, ldc, scales)
   if (dt == YN_F32) { YN_Q(float); }
   else if (dt == YN_BF16) { YN_Q(__nv_bfloat16); }
   else { YN_Q(__half); }
@@ -335,32 +342,6 @@ __global__ void __launch_bounds__(I8_PLAN_T) k_i8_plan(const int32_t* ids, int P
     if (pair_of[i] >= 0) pair_of[i] += first[ids[i]];
 }
 
-// The activations' 8-bit codes: one warp per pair, from 16-bit values relative to the
-// largest of each 32 units (the pair's largest is the largest of those).
-__global__ void __launch_bounds__(256) k_i8_act_codes(const int16_t* act, long long lda, const float* bscale, int nb, int I,
-                                                      const int* n_pairs, int8_t* codes, long long ldc, float* scales) {
-  const int lane = threadIdx.x & 31;
-  const long long p = (long long)blockIdx.x * 8 + (threadIdx.x >> 5);
-  if (p >= *n_pairs) return;
-  const float* bs = bscale + p * nb;
-  uint32_t m = 0;
-  for (int b = lane; b < nb; b += 32) m = max(m, __float_as_uint(bs[b]));
-  const I8Row q(__reduce_max_sync(0xffffffffu, m));
-  if (lane == 0) scales[p] = q.scale();
-  const int16_t* a = act + p * lda;
-  for (int u = 8 * lane; u < I; u += 256) {   // lda and ldc are whole 16-byte pieces of 8 values
-    const uint4 v = *reinterpret_cast<const uint4*>(a + u);
-    const uint32_t w[4] = {v.x, v.y, v.z, v.w};
-    const float s = bs[u >> 5] * (1.0f / 32767.0f);
-    float f[8];
-#pragma unroll
-    for (int i = 0; i < 8; ++i) f[i] = (float)(int16_t)(w[i >> 1] >> (16 * (i & 1))) * s;
-    uint32_t c[2];
-    q.codes(f, c);
-    *reinterpret_cast<uint2*>(codes + p * ldc + u) = make_uint2(c[0], c[1]);
-  }
-}
-
 // out[t] = residual[t] + sum_j w_j y[pair_of[t][j]] in fp32, columns in order, rounded once.
 template <typename O, typename Y>
 __global__ void k_i8_combine(const Y* y, long long ldy, const int32_t* pair_of, const float* w, int k, int H,
@@ -397,29 +378,52 @@ __global__ void k_i8_combine(const Y* y, long long ldy, const int32_t* pair_of, 
 // ---------------------------------------------------------------- host side
 size_t up_to(size_t v, size_t m) { return (v + m - 1) / m * m; }
 
-int tmap_2d(CUtensorMap* m, const void* base, long long cols, long long rows, long long stride, int box_rows) {
+int tmap(CUtensorMap* m, const void* base, int rank, const cuuint64_t* dims, const cuuint64_t* strides, const cuuint32_t* box) {
   TmapEncode fn;
   int rc = host_tmap_encode(&fn);
   if (rc) return rc;
-  const cuuint64_t dims[2] = {(cuuint64_t)cols, (cuuint64_t)rows}, strides[1] = {(cuuint64_t)stride};
-  const cuuint32_t box[2] = {128u, (cuuint32_t)box_rows}, one[2] = {1u, 1u};
-  const CUresult r = fn(m, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void*>(base), dims, strides, box, one,
+  const cuuint32_t one[5] = {1u, 1u, 1u, 1u, 1u};
+  const CUresult r = fn(m, CU_TENSOR_MAP_DATA_TYPE_UINT8, rank, const_cast<void*>(base), dims, strides, box, one,
                         CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
                         CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   return r == CUDA_SUCCESS ? YN_OK : host_fail(YN_E_CUDA, "cuTensorMapEncodeTiled failed: " + std::to_string((int)r));
 }
-int tmap_mats(CUtensorMap* m, const yn_i8_mat& w) {
-  TmapEncode fn;
-  int rc = host_tmap_encode(&fn);
-  if (rc) return rc;
+// The rows' codes in boxes of 16, 32, 64 and 128 rows.
+int tmap_rows(I8Maps* maps, const void* base, long long cols, long long rows, long long stride) {
+  for (int i = 0; i < I8_BMAPS; ++i) {
+    const cuuint64_t dims[2] = {(cuuint64_t)cols, (cuuint64_t)rows}, strides[1] = {(cuuint64_t)stride};
+    const cuuint32_t box[2] = {128u, 16u << i};
+    const int rc = tmap(&maps->b[i], base, 2, dims, strides, box);
+    if (rc) return rc;
+  }
+  return YN_OK;
+}
+int tmap_mats(CUtensorMap* m, const yn_i8_mat& w, int box_rows) {
   const cuuint64_t dims[3] = {(cuuint64_t)w.cols, (cuuint64_t)w.rows, (cuuint64_t)w.n_mats};
   const cuuint64_t strides[2] = {(cuuint64_t)w.row_stride,
                                  (cuuint64_t)(w.n_mats > 1 ? w.mat_stride : w.row_stride * (int64_t)w.rows)};
-  const cuuint32_t box[3] = {128u, 128u, 1u}, one[3] = {1u, 1u, 1u};
-  const CUresult r = fn(m, CU_TENSOR_MAP_DATA_TYPE_UINT8, 3, const_cast<void*>(w.codes), dims, strides, box, one,
-                        CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
-                        CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
-  return r == CUDA_SUCCESS ? YN_OK : host_fail(YN_E_CUDA, "cuTensorMapEncodeTiled failed: " + std::to_string((int)r));
+  const cuuint32_t box[3] = {128u, (cuuint32_t)box_rows, 1u};
+  return tmap(m, w.codes, 3, dims, strides, box);
+}
+// Gate and up in one map, (K, 16 rows, 2 matrices, rows / 16, E), where the two are laid out
+// alike and their rows are whole groups of 16: one copy per stage instead of eight (11 -> 16
+// TB/s from L2). Sets `both`; else two maps of 16-row boxes.
+int tmap_gate_up(I8Gemm* g, I8Maps* maps, const yn_i8_mat& gate, const yn_i8_mat& up) {
+  const int64_t delta = reinterpret_cast<int64_t>(up.codes) - reinterpret_cast<int64_t>(gate.codes);
+  const int64_t apart = delta < 0 ? -delta : delta;
+  g->both = gate.rows % 16 == 0 && gate.row_stride == up.row_stride && (gate.n_mats == 1 || gate.mat_stride == up.mat_stride) &&
+            apart > 0 && apart < (1ll << 40);
+  g->swapped = g->both && delta < 0;
+  if (!g->both) {
+    const int rc = tmap_mats(&maps->a, gate, 16);
+    return rc ? rc : tmap_mats(&maps->a_up, up, 16);
+  }
+  const yn_i8_mat& first = g->swapped ? up : gate;
+  const cuuint64_t dims[5] = {(cuuint64_t)gate.cols, 16u, 2u, (cuuint64_t)gate.rows / 16, (cuuint64_t)gate.n_mats};
+  const cuuint64_t strides[4] = {(cuuint64_t)gate.row_stride, (cuuint64_t)apart, (cuuint64_t)gate.row_stride * 16,
+                                 (cuuint64_t)(gate.n_mats > 1 ? gate.mat_stride : gate.row_stride * (int64_t)gate.rows)};
+  const cuuint32_t box[5] = {128u, 16u, 2u, 4u, 1u};
+  return tmap(&maps->a, first.codes, 5, dims, strides, box);
 }
 
 int sm_count(int* out) {
@@ -432,26 +436,25 @@ int sm_count(int* out) {
 template <typename O, bool UP, int NB>
 int launch_gemm(const I8Gemm& a, const I8Maps& maps, long long max_tiles, cudaStream_t st) {
   const void* kern = reinterpret_cast<const void*>(k_i8_gemm<O, UP, NB>);
-  int rc = host_set_smem(kern, I8Cfg<UP, NB>::SMEM), sms = 0;
+  int rc = host_set_smem(kern, I8Cfg<NB>::SMEM), sms = 0;
   if (rc || (rc = sm_count(&sms))) return rc;
-  const unsigned grid = (unsigned)std::max<long long>(1, std::min<long long>(max_tiles, sms));
-  k_i8_gemm<O, UP, NB><<<grid, I8_THREADS, I8Cfg<UP, NB>::SMEM, st>>>(a, maps);
+  const unsigned grid = 2 * (unsigned)std::max<long long>(1, std::min<long long>(max_tiles, sms / 2));
+  k_i8_gemm<O, UP, NB><<<grid, I8_THREADS, I8Cfg<NB>::SMEM, st>>>(a, maps);
   const cudaError_t e = cudaGetLastError();
   return e == cudaSuccess ? YN_OK : host_fail(YN_E_CUDA, std::string("8-bit product: ") + cudaGetErrorString(e));
 }
-template <typename O>
+// Rows per tile: 64 where most tiles have few rows (their time is the weights' way from HBM,
+// and the smaller stages keep more of them in flight), else 256.
+template <typename O, bool UP>
 int launch_gemm_nb(int nb, const I8Gemm& a, const I8Maps& maps, long long max_tiles, cudaStream_t st) {
-  if (nb <= 32) return launch_gemm<O, false, 32>(a, maps, max_tiles, st);
-  if (nb <= 64) return launch_gemm<O, false, 64>(a, maps, max_tiles, st);
-  if (nb <= 128) return launch_gemm<O, false, 128>(a, maps, max_tiles, st);
-  return launch_gemm<O, false, 256>(a, maps, max_tiles, st);
+  if (max_tiles > 0x3fffffff) return host_fail(YN_E_UNSUPPORTED, "more than 2^30 tiles");
+  return nb <= 64 ? launch_gemm<O, UP, 64>(a, maps, max_tiles, st) : launch_gemm<O, UP, 256>(a, maps, max_tiles, st);
 }
 int launch_gemm_out(int odt, int nb, const I8Gemm& a, const I8Maps& maps, long long max_tiles, cudaStream_t st) {
-  if (odt == YN_F32) return launch_gemm_nb<float>(nb, a, maps, max_tiles, st);
-  if (odt == YN_BF16) return launch_gemm_nb<__nv_bfloat16>(nb, a, maps, max_tiles, st);
-  return launch_gemm_nb<__half>(nb, a, maps, max_tiles, st);
+  if (odt == YN_F32) return launch_gemm_nb<float, false>(nb, a, maps, max_tiles, st);
+  if (odt == YN_BF16) return launch_gemm_nb<__nv_bfloat16, false>(nb, a, maps, max_tiles, st);
+  return launch_gemm_nb<__half, false>(nb, a, maps, max_tiles, st);
 }
-int box_rows(int nb) { return nb <= 32 ? 32 : nb <= 64 ? 64 : nb <= 128 ? 128 : 256; }
 
 bool dtype_ok(int dt) { return dt == YN_F32 || dt == YN_BF16 || dt == YN_F16; }
 int dtype_size(int dt) { return dt == YN_F32 ? 4 : 2; }
@@ -492,16 +495,11 @@ int launch_few(int dt, const void* x, long long ldx, int K, const I8Mat& w, int 
 
 // Workspace of the experts' products.
 struct ExpertsWs {
-  size_t n_out, pair_of, chunks, codes, sx, act, bscale, acodes, sa, y, total;
+  size_t n_out, pair_of, chunks, codes, sx, act, acodes, sa, y, total;
   long long ldc, lda, ldac, ldy;
   int nb;
 };
-// Rows per chunk: enough for the mean expert. Small tiles read an expert's weights once per
-// tile (from L2 after the first) but multiply fewer absent rows.
-int chunk_rows(long long pairs, int E) {
-  const long long mean = pairs / std::max(1, E);
-  return mean <= 16 ? 32 : mean <= 48 ? 64 : 128;
-}
+int chunk_rows(long long pairs, int E) { return pairs <= 16ll * E ? 64 : 256; }
 bool experts_few(long long pairs, int k, int H, int I) {
   return pairs <= 40 && up_to(H, I8_GK) <= 96 * 1024 && k * up_to(I, I8_GK) <= 96 * 1024;
 }
@@ -518,7 +516,7 @@ ExpertsWs experts_ws(long long rows, int k, int E, int H, int I, int odt) {
   }
   L.nb = chunk_rows((long long)P, E);
   L.ldc = (long long)up_to(H, 16);
-  L.lda = (long long)up_to(I, 16);
+  L.lda = (long long)up_to(I, 4);
   L.ldac = (long long)up_to(I, 16);
   L.ldy = (long long)up_to(H, 16);
   L.n_out = take(8);
@@ -526,8 +524,7 @@ ExpertsWs experts_ws(long long rows, int k, int E, int H, int I, int odt) {
   L.chunks = take((E + P / L.nb + 1) * sizeof(I8Chunk));
   L.codes = take(P * L.ldc);
   L.sx = take(P * 4);
-  L.act = take(P * L.lda * 2);
-  L.bscale = take(P * (up_to(I, 32) / 32) * 4);
+  L.act = take(P * L.lda * 4);
   L.acodes = take(P * L.ldac);
   L.sa = take(P * 4);
   L.y = take(P * L.ldy * (odt == YN_BF16 ? 2 : 4));
@@ -547,7 +544,7 @@ extern "C" int yn_i8_quant_rows(const void* x, int32_t dtype, int64_t row_stride
   if (rows == 0) return YN_OK;
   if (!x || !codes || !scales) return host_fail(YN_E_INVALID, "null argument");
   if (reinterpret_cast<uintptr_t>(x) % dtype_size(dtype)) return host_fail(YN_E_INVALID, "x must be aligned to its element");
-  return launch_quant(dtype, x, row_stride, rows, cols, nullptr, 1, reinterpret_cast<int8_t*>(codes), code_stride, scales,
+  return launch_quant(dtype, x, row_stride, rows, cols, nullptr, nullptr, 1, reinterpret_cast<int8_t*>(codes), code_stride, scales,
                       reinterpret_cast<cudaStream_t>(stream));
 }
 
@@ -593,7 +590,7 @@ extern "C" int yn_i8_linear(const yn_i8_mat* w, const void* x, int32_t dtype, in
   int8_t* codes = reinterpret_cast<int8_t*>(ws);
   const long long ldc = (long long)up_to(w->cols, 16);
   float* sx = reinterpret_cast<float*>(codes + up_to((size_t)rows * ldc, 256));
-  if ((rc = launch_quant(dtype, x, x_stride, rows, w->cols, nullptr, 1, codes, ldc, sx, st))) return rc;
+  if ((rc = launch_quant(dtype, x, x_stride, rows, w->cols, nullptr, nullptr, 1, codes, ldc, sx, st))) return rc;
   I8Gemm a{};
   a.rows = (int)rows;
   a.channels = w->rows;
@@ -604,10 +601,10 @@ extern "C" int yn_i8_linear(const yn_i8_mat* w, const void* x, int32_t dtype, in
   a.y_stride = y_stride;
   a.store_cols = w->rows;
   a.pairs = reinterpret_cast<uintptr_t>(y) % 4 == 0 && y_stride % 2 == 0;
-  const int nb = box_rows((int)std::min<int64_t>(rows, 256));
+  const int nb = rows <= 64 ? 64 : 256;
   I8Maps maps{};
-  if ((rc = tmap_mats(&maps.a, *w)) || (rc = tmap_2d(&maps.b, codes, w->cols, rows, ldc, nb))) return rc;
-  const long long tiles = (long long)((rows + nb - 1) / nb) * ((w->rows + 127) / 128);
+  if ((rc = tmap_mats(&maps.a, *w, 128)) || (rc = tmap_rows(&maps, codes, w->cols, rows, ldc))) return rc;
+  const long long tiles = (long long)((rows + nb - 1) / nb) * ((w->rows + 255) / 256);
   return launch_gemm_out(y_dtype, nb, a, maps, tiles, st);
 }
 
@@ -662,18 +659,16 @@ extern "C" int yn_i8_experts(const yn_i8_mat* gate, const yn_i8_mat* up, const y
   I8Chunk* chunks = reinterpret_cast<I8Chunk*>(b + L.chunks);
   int8_t* codes = reinterpret_cast<int8_t*>(b + L.codes);
   float* sx = reinterpret_cast<float*>(b + L.sx);
-  int16_t* act = reinterpret_cast<int16_t*>(b + L.act);
-  float* bscale = reinterpret_cast<float*>(b + L.bscale);
+  float* act = reinterpret_cast<float*>(b + L.act);
   int8_t* acodes = reinterpret_cast<int8_t*>(b + L.acodes);
   float* sa = reinterpret_cast<float*>(b + L.sa);
   void* y = b + L.y;
   k_i8_plan<<<1, I8_PLAN_T, 0, st>>>(ids, P, E, L.nb, pair_of, chunks, n_out);
-  if ((rc = launch_quant(dtype, x, x_stride, rows, H, pair_of, top_k, codes, L.ldc, sx, st))) return rc;
+  if ((rc = launch_quant(dtype, x, x_stride, rows, H, nullptr, pair_of, top_k, codes, L.ldc, sx, st))) return rc;
   const long long max_chunks = E + P / L.nb + 1;
   I8Maps maps{};
-  if ((rc = tmap_mats(&maps.a, *gate)) || (rc = tmap_mats(&maps.a_up, *up)) || (rc = tmap_2d(&maps.b, codes, H, P, L.ldc, L.nb)))
-    return rc;
   I8Gemm g{};
+  if ((rc = tmap_gate_up(&g, &maps, *gate, *up)) || (rc = tmap_rows(&maps, codes, H, P, L.ldc))) return rc;
   g.chunks = chunks;
   g.n_chunks = n_out;
   g.rows = P;
@@ -686,16 +681,12 @@ extern "C" int yn_i8_experts(const yn_i8_mat* gate, const yn_i8_mat* up, const y
   g.sw_up_stride = up->scale_stride;
   g.y = act;
   g.y_stride = L.lda;
-  g.bscale = bscale;
-  const long long tu = max_chunks * ((I + 127) / 128), td = max_chunks * ((H + 127) / 128);
-  rc = L.nb == 32   ? launch_gemm<float, true, 32>(g, maps, tu, st)
-       : L.nb == 64 ? launch_gemm<float, true, 64>(g, maps, tu, st)
-                    : launch_gemm<float, true, 128>(g, maps, tu, st);
+  const long long tu = max_chunks * ((I + 127) / 128), td = max_chunks * ((H + 255) / 256);
+  rc = launch_gemm_nb<float, true>(L.nb, g, maps, tu, st);
   if (rc) return rc;
-  const int nbk = (int)up_to(I, 32) / 32;
-  k_i8_act_codes<<<(P + 7) / 8, 256, 0, st>>>(act, L.lda, bscale, nbk, I, n_out + 1, acodes, L.ldac, sa);
+  if ((rc = launch_quant(YN_F32, act, L.lda, P, I, n_out + 1, nullptr, 1, acodes, L.ldac, sa, st))) return rc;
   I8Maps md2{};
-  if ((rc = tmap_mats(&md2.a, *down)) || (rc = tmap_2d(&md2.b, acodes, I, P, L.ldac, L.nb))) return rc;
+  if ((rc = tmap_mats(&md2.a, *down, 128)) || (rc = tmap_rows(&md2, acodes, I, P, L.ldac))) return rc;
   I8Gemm d{};
   d.chunks = chunks;
   d.n_chunks = n_out;

@@ -52,25 +52,34 @@ YN_DEV uint32_t i8_pack2(float lo, float hi) {
   }
 }
 
-// Element by element; 8 at a time where rows are 16-byte aligned.
+// 8 elements as they lie in memory (16-byte aligned), and as fp32.
 template <typename T>
-YN_DEV void i8_load8(const void* p, size_t i, float (&f)[8]) {
-  if constexpr (sizeof(T) == 4) {
-    const float4 a = reinterpret_cast<const float4*>(reinterpret_cast<const float*>(p) + i)[0];
-    const float4 b = reinterpret_cast<const float4*>(reinterpret_cast<const float*>(p) + i)[1];
-    f[0] = a.x; f[1] = a.y; f[2] = a.z; f[3] = a.w;
-    f[4] = b.x; f[5] = b.y; f[6] = b.z; f[7] = b.w;
-  } else {
-    const uint4 v = *reinterpret_cast<const uint4*>(reinterpret_cast<const uint16_t*>(p) + i);
-    const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+struct I8Raw {
+  uint4 v[sizeof(T) / 2];
+  YN_DEV void load(const void* p, size_t i) {
+    const uint4* q = reinterpret_cast<const uint4*>(reinterpret_cast<const T*>(p) + i);
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      const uint16_t h = (uint16_t)(w[j >> 1] >> (16 * (j & 1)));
-      if constexpr (std::is_same_v<T, __half>) f[j] = f16_to_f32(h);
-      else f[j] = bf16_to_f32(h);
+    for (int j = 0; j < (int)sizeof(T) / 2; ++j) v[j] = q[j];
+  }
+  YN_DEV void get(float (&f)[8]) const {
+#pragma unroll
+    for (int j = 0; j < (int)sizeof(T) / 2; ++j) {
+      const uint32_t w[4] = {v[j].x, v[j].y, v[j].z, v[j].w};
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        if constexpr (sizeof(T) == 4) {
+          f[4 * j + i] = __uint_as_float(w[i]);
+        } else if constexpr (std::is_same_v<T, __half>) {
+          f[2 * i] = f16_to_f32((uint16_t)(w[i] & 0xFFFFu));
+          f[2 * i + 1] = f16_to_f32((uint16_t)(w[i] >> 16));
+        } else {
+          f[2 * i] = __uint_as_float(w[i] << 16);
+          f[2 * i + 1] = __uint_as_float(w[i] & 0xFFFF0000u);
+        }
+      }
     }
   }
-}
+};
 
 // A row's quantiser. A row with an infinity or a NaN has a NaN scale and codes of 0, so
 // that its products are NaN and no other row's; a row of zeros has scale 0.
@@ -126,12 +135,17 @@ YN_DEV uint32_t block_max_u32(uint32_t v, uint32_t* buf) {
   return m;
 }
 
-// The tensor-core product. One tile: 128 output channels of one matrix x up to NB rows.
-// A = the channels' codes, B = the rows' codes, both K-major in the 128-byte swizzled
-// layout by TMA, 128 codes of K per stage (four tcgen05.mma kind::i8 of K 32); the
-// accumulator is channels (TMEM lanes) x rows (columns), int32. UP doubles A: the same
-// 128 units of the gate and of the up matrix into two accumulators, so that a thread of
-// the epilogue holds both and SwiGLU needs no exchange.
+// The tensor-core product, by pairs of blocks (a cluster of two SMs, tcgen05 cta_group::2).
+// One tile: 256 channels of one matrix x up to NB rows, each block with 128 of the channels
+// (its own TMEM lanes) and half of the rows' codes in its shared memory; the pair's MMA (M
+// 256, kind::i8) reads both halves, so a row's codes cross from L2 once per pair and a stage
+// moves 32 KB per SM for 512 cycles of MMA. One block alone would move 48 KB, and the 12
+// TB/s that L2 gave here then held the MMA at 62% of its rate (104 us against ... at 4096 x
+// 2048 x 16384).
+// A = the channels' codes, B = the rows' codes, both K-major in the 128-byte swizzled layout
+// by TMA, 128 codes of K per stage (four MMAs of K 32); the accumulator is channels (lanes) x
+// rows (columns), int32. UP interleaves 16 rows of the gate matrix with 16 of the up matrix,
+// so that lanes l and l + 16 of an epilogue warp hold gate and up of the same unit.
 struct I8Chunk {
   int e, p0, n;   // matrix, first row, rows (1..NB)
 };
@@ -144,44 +158,107 @@ struct I8Gemm {
   const float* sw;         // channel scales, sw_stride per matrix
   const float* sw_up;
   long long sw_stride, sw_up_stride;
-  void* y;                 // (rows, y_stride): output, or UP: int16 activations
+  void* y;                 // (rows, y_stride): output, or UP: fp32 activations
   long long y_stride;
   int store_cols;          // columns of a row that may be written: channels, or more where rows are padded
+  bool both, swapped;      // UP: map a holds both matrices; up before gate in it
   bool pairs;              // 16-bit outputs may be written two channels at a time (4-byte aligned rows)
-  float* bscale;           // UP: (rows, ceil(channels / 32)) scales of the activations' blocks
 };
+// Tensor maps. a: the matrices' rows, boxes of 128 (UP: of 16; or, `both`, of 4 x 2 x 16: four times
+// 16 rows of gate and the same of up in one copy). b[i]: the rows' codes, boxes of 16 << i.
+constexpr int I8_BMAPS = 4;
 struct I8Maps {
-  CUtensorMap a, a_up, b;
+  CUtensorMap a, a_up, b[I8_BMAPS];
 };
 
 YN_DEV void i8_mma(uint32_t tmem_d, uint64_t adesc, uint64_t bdesc, uint32_t idesc, uint32_t accumulate) {
   asm volatile(
       "{\n\t.reg .pred p;\n\t"
       "setp.ne.b32 p, %4, 0;\n\t"
-      "tcgen05.mma.cta_group::1.kind::i8 [%0], %1, %2, %3, p;\n\t}"
+      "tcgen05.mma.cta_group::2.kind::i8 [%0], %1, %2, %3, p;\n\t}"
       ::"r"(tmem_d), "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate));
 }
-// int32 accumulate (D format 2 at bits 4-5), signed 8-bit A and B (format 1), both
-// K-major, N >> 3 at bits 17-22, M = 128 at bits 24-28
-YN_DEV uint32_t i8_idesc(int n) {
-  return (2u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)(n >> 3) << 17) | (8u << 24);
-}
-YN_DEV void i8_tma_3d(void* dst, const CUtensorMap* map, int x, int y, int z, uint64_t* bar) {
+// Arrival on the barrier at this offset in both blocks once the MMAs issued so far are done.
+YN_DEV void i8_commit_both(uint64_t* bar) {
   asm volatile(
-      "cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];" ::
-          "r"(smem_u32(dst)), "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(z), "r"(smem_u32(bar))
+      "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(smem_u32(bar)),
+      "h"((uint16_t)3)
       : "memory");
 }
-// 16 consecutive 32-bit columns of this thread's TMEM lane; wait with i8_ld_wait.
+// int32 accumulate (D format 2 at bits 4-5), signed 8-bit A and B (format 1), both
+// K-major, N >> 3 at bits 17-22, M = 256 at bits 24-28
+YN_DEV uint32_t i8_idesc(int n) {
+  return (2u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)(n >> 3) << 17) | (16u << 24);
+}
+YN_DEV uint32_t i8_rank() {
+  uint32_t r;
+  asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+  return r;
+}
+// The address of block 0's copy of a barrier.
+YN_DEV uint32_t i8_leader(uint64_t* bar) {
+  uint32_t a;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, 0;" : "=r"(a) : "r"(smem_u32(bar)));
+  return a;
+}
+YN_DEV void i8_arrive_at(uint32_t cluster_bar) {
+  asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(cluster_bar) : "memory");
+}
+YN_DEV void i8_cluster_sync() {
+  asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+YN_DEV bool i8_try_wait(uint64_t* bar, uint32_t phase) {
+  uint32_t ok;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(ok)
+      : "r"(smem_u32(bar)), "r"(phase)
+      : "memory");
+  return ok != 0;
+}
+// A wait of the whole warp, at most 1 s: on a timeout the error word is set and every role
+// leaves its loop.
+YN_DEV bool i8_wait(uint64_t* bar, uint32_t phase, int* err) {
+  bool ok = i8_try_wait(bar, phase);
+  if (!ok) {
+    const uint64_t t0 = globaltimer_ns();
+    while (!(ok = i8_try_wait(bar, phase)))
+      if (globaltimer_ns() - t0 > 1000000000ull) {
+        raise_error(err, YN_ERR_BULK_TIMEOUT);
+        break;
+      }
+  }
+  return __all_sync(0xffffffffu, ok) != 0;
+}
+// Tile copies of this block whose bytes are counted on a barrier of the pair's first block.
+YN_DEV void i8_tma_3d(void* dst, const CUtensorMap* map, int x, int y, int z, uint32_t cluster_bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.3d.cta_group::2.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];" ::
+          "r"(smem_u32(dst)), "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(z), "r"(cluster_bar)
+      : "memory");
+}
+YN_DEV void i8_tma_5d(void* dst, const CUtensorMap* map, int x, int hi, int z, uint32_t cluster_bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.5d.cta_group::2.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %3, %4, %5}], [%6];" ::
+          "r"(smem_u32(dst)), "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(0), "r"(hi), "r"(z), "r"(cluster_bar)
+      : "memory");
+}
+YN_DEV void i8_tma_2d(void* dst, const CUtensorMap* map, int x, int y, uint32_t cluster_bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];" ::
+          "r"(smem_u32(dst)), "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(cluster_bar)
+      : "memory");
+}
+// 16 consecutive 32-bit columns of this thread's TMEM lane. The wait takes the registers
+// through it, so that nothing reads them before it.
 YN_DEV void i8_ld16(uint32_t taddr, int (&v)[16]) {
   asm volatile(
       "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
       : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7]), "=r"(v[8]),
         "=r"(v[9]), "=r"(v[10]), "=r"(v[11]), "=r"(v[12]), "=r"(v[13]), "=r"(v[14]), "=r"(v[15])
       : "r"(taddr));
-}
-// The wait takes the registers through it, so that nothing reads them before it.
-YN_DEV void i8_ld_wait(int (&v)[16]) {
   asm volatile("tcgen05.wait::ld.sync.aligned;"
                : "+r"(v[0]), "+r"(v[1]), "+r"(v[2]), "+r"(v[3]), "+r"(v[4]), "+r"(v[5]), "+r"(v[6]), "+r"(v[7]),
                  "+r"(v[8]), "+r"(v[9]), "+r"(v[10]), "+r"(v[11]), "+r"(v[12]), "+r"(v[13]), "+r"(v[14]), "+r"(v[15])
@@ -192,28 +269,29 @@ YN_DEV void i8_ld_wait(int (&v)[16]) {
 constexpr int I8_EPW = 16;                   // epilogue warps (warp % 4: TMEM lanes 32 (warp % 4)..+31)
 constexpr int I8_MW = I8_EPW, I8_LW = I8_EPW + 1;
 constexpr int I8_THREADS = 32 * (I8_EPW + 2);
-constexpr int I8_A_BYTES = 128 * 128;
+constexpr int I8_A_BYTES = 128 * 128;        // a block's channels, one stage
 
-template <bool UP, int NB>
+template <int NB>
 struct I8Cfg {
-  static constexpr int STAGE = (UP ? 2 : 1) * I8_A_BYTES + NB * 128;
+  static constexpr int STAGE = I8_A_BYTES + NB / 2 * 128;
   static constexpr int FIT = (224 * 1024) / STAGE;
-  static constexpr int S = FIT < 8 ? FIT : 8;          // stages in flight
-  static constexpr int COLS = (UP ? 2 : 1) * NB;       // TMEM columns of one accumulator, two of them
+  static constexpr int S = FIT < 10 ? FIT : 10;        // stages in flight
   static constexpr int SMEM = 1024 + S * STAGE + (2 * S + 4) * 8 + 16;
-  static_assert(2 * COLS <= 512, "two accumulators have to fit TMEM");
+  static_assert(NB % 32 == 0 && NB <= 256, "two accumulators of NB columns have to fit TMEM");
 };
 
 // SiLU(g) * u in fp32.
 YN_DEV float i8_swiglu(float g, float u) { return __fdividef(g, 1.0f + __expf(-g)) * u; }
 
-// Warp-specialised and persistent: the loader warp fills a ring of stages by TMA, the
-// MMA warp multiplies them into one of two accumulators, the epilogue warps drain the
-// other. Waits are bounded as in the other tensor-core kernels: on a timeout the error
-// word is set and every role leaves its loop.
+// Warp-specialised and persistent: in both blocks a loader warp fills a ring of stages by
+// TMA and epilogue warps drain the accumulators; the first block's MMA warp multiplies for
+// both, into one of two accumulators while the other is drained.
+// full[s] (first block): the bytes of both blocks' stage s; empty[s] (each block): its MMAs
+// are done; acc_full[b] (each block); acc_empty[b] (first block): every epilogue warp of both.
 template <typename O, bool UP, int NB>
-__global__ void __launch_bounds__(I8_THREADS, 1) k_i8_gemm(const I8Gemm a, const __grid_constant__ I8Maps maps) {
-  using F = I8Cfg<UP, NB>;
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(I8_THREADS, 1)
+    k_i8_gemm(const I8Gemm a, const __grid_constant__ I8Maps maps) {
+  using F = I8Cfg<NB>;
   extern __shared__ __align__(1024) uint8_t smem_raw[];
   uint8_t* smem = smem_raw + (((smem_u32(smem_raw) + 1023u) & ~1023u) - smem_u32(smem_raw));
   uint64_t* full = reinterpret_cast<uint64_t*>(smem + F::S * F::STAGE);
@@ -222,11 +300,13 @@ __global__ void __launch_bounds__(I8_THREADS, 1) k_i8_gemm(const I8Gemm a, const
   uint64_t* acc_empty = acc_full + 2;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(acc_empty + 2);
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int rank = (int)i8_rank();
   int* err = &g_i8_err;
 
-  const int UT = (a.channels + 127) / 128;
+  constexpr int TILE = UP ? 128 : 256;   // units or channels of a pair's tile
+  const int UT = (a.channels + TILE - 1) / TILE;
   const int n_chunks = a.chunks ? *a.n_chunks : (a.rows + NB - 1) / NB;
-  const long long n_tiles = (long long)n_chunks * UT;
+  const int n_tiles = n_chunks * UT, step = (int)(gridDim.x >> 1), t0 = (int)(blockIdx.x >> 1);
   const int NK = (a.K + 127) / 128;
   if (tid == 0) {
     for (int s = 0; s < F::S; ++s) {
@@ -235,83 +315,76 @@ __global__ void __launch_bounds__(I8_THREADS, 1) k_i8_gemm(const I8Gemm a, const
     }
     for (int b = 0; b < 2; ++b) {
       mbar_init(&acc_full[b], 1);
-      mbar_init(&acc_empty[b], 32 * I8_EPW);
+      mbar_init(&acc_empty[b], 2 * I8_EPW);
     }
     fence_mbar_init();
   }
   if (warp == I8_MW) {
-    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(smem_u32(tmem_slot)));
-    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
+    asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(smem_u32(tmem_slot)));
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;");
   }
+  tc_fence_before();
   __syncthreads();
+  i8_cluster_sync();
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
   bool ok = true;
   // A list's tiles go unit by unit through a chunk, so that neighbours share the rows; a
-  // single matrix's go chunk by chunk through 128 channels, so that they share the weights.
-  auto tile = [&](long long ti, int& u0) -> I8Chunk {
-    if (a.chunks) {
-      const int c = (int)(ti / UT);
-      u0 = 128 * (int)(ti - (long long)c * UT);
-      return a.chunks[c];
-    }
-    const int u = (int)(ti / n_chunks), c = (int)(ti - (long long)u * n_chunks);
-    u0 = 128 * u;
-    return I8Chunk{0, c * NB, min(NB, a.rows - c * NB)};
+  // single matrix's go chunk by chunk through its channels, so that they share the weights.
+  // Every role looks its next tile up while it works on the current one.
+  struct Tile {
+    I8Chunk c;
+    int u0;
   };
+  auto tile = [&](int ti) -> Tile {
+    if (ti >= n_tiles) return Tile{I8Chunk{0, 0, 0}, 0};
+    if (a.chunks) {
+      const int c = ti / UT;
+      return Tile{a.chunks[c], TILE * (ti - c * UT) + TILE / 2 * rank};
+    }
+    const int u = ti / n_chunks, c = ti - u * n_chunks;
+    return Tile{I8Chunk{0, c * NB, min(NB, a.rows - c * NB)}, TILE * u + TILE / 2 * rank};
+  };
+  Tile next = tile(t0);
 
   if (warp < I8_EPW) {
-    const int m = 32 * (warp & 3) + lane, part = warp >> 2;
+    const int q = warp & 3, part = warp >> 2;
     long long j = 0;
-    for (long long ti = blockIdx.x; ti < n_tiles; ti += gridDim.x, ++j) {
-      int u0;
-      const I8Chunk c = tile(ti, u0);
-      const int b = (int)(j & 1), r = u0 + m;
+    for (int ti = t0; ti < n_tiles; ti += step, ++j) {
+      const I8Chunk c = next.c;
+      const int u0 = next.u0;
+      next = tile(ti + step);
+      const int b = (int)(j & 1), r = UP ? u0 + 16 * q + (lane & 15) : u0 + 32 * q + lane;
       const bool in = r < a.channels;
       const float sw = in ? a.sw[c.e * a.sw_stride + r] : 0.0f;
       const float su = UP && in ? a.sw_up[c.e * a.sw_up_stride + r] : 0.0f;
-      ok = mbar_wait_bounded(&acc_full[b], (uint32_t)(j >> 1) & 1, err);
-      ok = __all_sync(0xffffffffu, ok) != 0;
+      ok = i8_wait(&acc_full[b], (uint32_t)(j >> 1) & 1, err);
       if (!ok) break;
       tc_fence_after();
-      const uint32_t base = tmem + (uint32_t)(b * F::COLS) + ((uint32_t)(32 * (warp & 3)) << 16);
-      // A lane holds one channel of 16 rows: two lanes exchange so that each writes two adjacent
-      // channels of every second row (even lanes the even rows).
-      const bool odd = lane & 1, two = (r | 1) < a.store_cols;
-      const uint32_t sel = odd ? 0x3276u : 0x5410u;
+      const uint32_t base = tmem + (uint32_t)(b * NB) + ((uint32_t)(32 * q) << 16);
       for (int c0 = 16 * part; c0 < c.n; c0 += 4 * I8_EPW) {
-        int v[16], w[16];
-        i8_ld16(base + (uint32_t)c0, v);
-        if (UP) i8_ld16(base + (uint32_t)(NB + c0), w);
         const int left = c.n - c0;
-        const float sx = lane < min(16, left) ? a.sx[c.p0 + c0 + lane] : 0.0f;
-        i8_ld_wait(v);
-        if (UP) i8_ld_wait(w);
         const long long row = c.p0 + c0;
+        const float sx = lane < min(16, left) ? a.sx[row + lane] : 0.0f;
+        int v[16];
+        i8_ld16(base + (uint32_t)c0, v);
         if (UP) {
-          // 16 bits relative to the largest of these 32 units: off by at most 2^-16 of it, 1/516 of
-          // a step of the 8-bit code that follows
-          uint32_t* out = reinterpret_cast<uint32_t*>(reinterpret_cast<int16_t*>(a.y) + (row + odd) * a.y_stride + (r & ~1));
-          float bm = 0.0f;
+          // lanes below 16 take the even rows, the others the odd ones
+          const bool up = lane & 16;
+          const float s_lo = a.swapped ? su : sw, s_hi = a.swapped ? sw : su;
+          float* out = reinterpret_cast<float*>(a.y) + (row + up) * a.y_stride + r;
 #pragma unroll
           for (int k = 0; k < 16; k += 2) {
-            float t[2];
-#pragma unroll
-            for (int i = 0; i < 2; ++i) {
-              const float s = __shfl_sync(0xffffffffu, sx, k + i);
-              const float act = i8_swiglu((float)v[k + i] * s * sw, (float)w[k + i] * s * su);
-              const uint32_t mb = __reduce_max_sync(0xffffffffu, i8_abs_bits(act));
-              const float m = __uint_as_float(mb);
-              if (lane == k + i) bm = m;
-              t[i] = fmaf(act, m > 0.0f ? __fdividef(32767.0f, m) : 0.0f, 12582912.0f);   // the code in the low bits
-            }
-            const uint32_t own = __byte_perm(__float_as_uint(t[0]), __float_as_uint(t[1]), 0x5410);
-            const uint32_t other = __shfl_xor_sync(0xffffffffu, own, 1);
-            if (k + odd < left && (r & ~1) < a.channels) out[(size_t)k * a.y_stride / 2] = __byte_perm(own, other, sel);
+            const int got = __shfl_xor_sync(0xffffffffu, up ? v[k] : v[k + 1], 16);
+            const float s = __shfl_sync(0xffffffffu, sx, k + up);
+            const float lo = (float)(up ? got : v[k]) * s * s_lo, hi = (float)(up ? v[k + 1] : got) * s * s_hi;
+            if (k + up < left && in) out[(size_t)k * a.y_stride] = a.swapped ? i8_swiglu(hi, lo) : i8_swiglu(lo, hi);
           }
-          if (lane < min(16, left) && u0 + 32 * (warp & 3) < a.channels)
-            a.bscale[(row + lane) * ((a.channels + 31) / 32) + (u0 >> 5) + (warp & 3)] = bm;
         } else if (sizeof(O) == 2 && a.pairs) {
+          // two lanes exchange so that each writes two adjacent channels of every second row
+          // (even lanes the even rows)
+          const bool odd = lane & 1, two = (r | 1) < a.store_cols;
+          const uint32_t sel = odd ? 0x3276u : 0x5410u;
           uint32_t* out = reinterpret_cast<uint32_t*>(reinterpret_cast<O*>(a.y) + (row + odd) * a.y_stride + (r & ~1));
 #pragma unroll
           for (int k = 0; k < 16; k += 2) {
@@ -336,58 +409,66 @@ __global__ void __launch_bounds__(I8_THREADS, 1) k_i8_gemm(const I8Gemm a, const
         }
       }
       tc_fence_before();
-      mbar_arrive1(&acc_empty[b]);
+      __syncwarp();
+      if (lane == 0) i8_arrive_at(i8_leader(&acc_empty[b]));
     }
   } else if (warp == I8_MW) {
     long long g = 0, j = 0;
-    for (long long ti = blockIdx.x; ti < n_tiles && ok; ti += gridDim.x, ++j) {
-      int u0;
-      const I8Chunk c = tile(ti, u0);
+    for (int ti = t0; ti < n_tiles && ok && rank == 0; ti += step, ++j) {
+      const I8Chunk c = next.c;
+      next = tile(ti + step);
       const int b = (int)(j & 1);
-      if (j >= 2) ok = mbar_wait_bounded(&acc_empty[b], (uint32_t)((j >> 1) - 1) & 1, err);
-      ok = __all_sync(0xffffffffu, ok) != 0;
+      if (j >= 2) ok = i8_wait(&acc_empty[b], (uint32_t)((j >> 1) - 1) & 1, err);
       if (!ok) break;
       tc_fence_after();
-      const uint32_t idesc = i8_idesc((c.n + 15) & ~15), dcol = tmem + (uint32_t)(b * F::COLS);
+      const uint32_t idesc = i8_idesc((c.n + 31) & ~31), dcol = tmem + (uint32_t)(b * NB);
       for (int kc = 0; kc < NK; ++kc, ++g) {
         const int s = (int)(g % F::S);
-        ok = mbar_wait_bounded(&full[s], (uint32_t)(g / F::S) & 1, err);
-        ok = __all_sync(0xffffffffu, ok) != 0;
+        ok = i8_wait(&full[s], (uint32_t)(g / F::S) & 1, err);
         if (!ok) break;
         tc_fence_after();
         if (lane == 0) {
-          const uint32_t abase = smem_u32(smem + s * F::STAGE), bbase = abase + (UP ? 2 : 1) * I8_A_BYTES;
+          const uint32_t abase = smem_u32(smem + s * F::STAGE), bbase = abase + I8_A_BYTES;
 #pragma unroll
-          for (int k = 0; k < 4; ++k) {
-            const uint32_t acc = kc > 0 || k > 0 ? 1u : 0u;
-            i8_mma(dcol, tc_desc(abase + 32 * k), tc_desc(bbase + 32 * k), idesc, acc);
-            if (UP) i8_mma(dcol + NB, tc_desc(abase + I8_A_BYTES + 32 * k), tc_desc(bbase + 32 * k), idesc, acc);
-          }
-          tc_commit(&empty[s]);
-          if (kc == NK - 1) tc_commit(&acc_full[b]);
+          for (int k = 0; k < 4; ++k)
+            i8_mma(dcol, tc_desc(abase + 32 * k), tc_desc(bbase + 32 * k), idesc, kc > 0 || k > 0 ? 1u : 0u);
+          i8_commit_both(&empty[s]);
+          if (kc == NK - 1) i8_commit_both(&acc_full[b]);
         }
         __syncwarp();
       }
     }
     // the last commits must land before TMEM is released (bounded)
-    if (ok && lane == 0 && j > 0) (void)mbar_wait_bounded(&acc_full[(j - 1) & 1], (uint32_t)((j - 1) >> 1) & 1, err);
-    __syncwarp();
+    if (ok && j > 0) (void)i8_wait(&acc_full[(j - 1) & 1], (uint32_t)((j - 1) >> 1) & 1, err);
   } else {
     long long g = 0;
-    for (long long ti = blockIdx.x; ti < n_tiles && ok; ti += gridDim.x) {
-      int u0;
-      const I8Chunk c = tile(ti, u0);
+    for (int ti = t0; ti < n_tiles && ok; ti += step) {
+      const I8Chunk c = next.c;
+      const int u0 = next.u0;
+      next = tile(ti + step);
+      const int half = ((c.n + 31) & ~31) >> 1, row = c.p0 + rank * half;   // this block's half of the MMA's rows
+      const int bi = half <= 16 ? 0 : half <= 32 ? 1 : half <= 64 ? 2 : 3;
+      const uint32_t bytes = 2u * (I8_A_BYTES + (16u << bi) * 128u);
       for (int kc = 0; kc < NK; ++kc, ++g) {
         const int s = (int)(g % F::S);
-        if (g >= F::S) ok = mbar_wait_bounded(&empty[s], (uint32_t)(g / F::S - 1) & 1, err);
-        ok = __all_sync(0xffffffffu, ok) != 0;
+        if (g >= F::S) ok = i8_wait(&empty[s], (uint32_t)(g / F::S - 1) & 1, err);
         if (!ok) break;
         if (lane == 0) {
           uint8_t* st = smem + s * F::STAGE;
-          mbar_arrive_expect_tx(&full[s], F::STAGE);
-          i8_tma_3d(st, &maps.a, 128 * kc, u0, c.e, &full[s]);
-          if (UP) i8_tma_3d(st + I8_A_BYTES, &maps.a_up, 128 * kc, u0, c.e, &full[s]);
-          tc_tma_rows(st + (UP ? 2 : 1) * I8_A_BYTES, &maps.b, 128 * kc, c.p0, &full[s]);
+          const uint32_t bar = i8_leader(&full[s]);
+          if (rank == 0) mbar_arrive_expect_tx(&full[s], bytes);
+          if (UP && a.both) {
+            i8_tma_5d(st, &maps.a, 128 * kc, u0 >> 4, c.e, bar);
+          } else if (UP) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              i8_tma_3d(st + 4096 * i, &maps.a, 128 * kc, u0 + 16 * i, c.e, bar);
+              i8_tma_3d(st + 4096 * i + 2048, &maps.a_up, 128 * kc, u0 + 16 * i, c.e, bar);
+            }
+          } else {
+            i8_tma_3d(st, &maps.a, 128 * kc, u0, c.e, bar);
+          }
+          i8_tma_2d(st + I8_A_BYTES, &maps.b[bi], 128 * kc, row, bar);
         }
         __syncwarp();
       }
@@ -395,13 +476,14 @@ __global__ void __launch_bounds__(I8_THREADS, 1) k_i8_gemm(const I8Gemm a, const
     // every stage filled must have been read (its copies and MMAs done) before the block ends
     for (int s = 0; s < F::S && ok; ++s) {
       const long long last = g - 1 - ((g - 1 - s) % F::S + F::S) % F::S;   // last stage number in slot s
-      if (last >= 0 && last < g) ok = mbar_wait_bounded(&empty[s], (uint32_t)(last / F::S) & 1, err);
+      if (last >= 0 && last < g) ok = i8_wait(&empty[s], (uint32_t)(last / F::S) & 1, err);
     }
   }
   tc_fence_before();
   __syncthreads();
+  i8_cluster_sync();   // neither block leaves, or gives its TMEM back, while the other may still signal it
   tc_fence_after();
-  if (warp == I8_MW) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem));
+  if (warp == I8_MW) asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, 512;" ::"r"(tmem));
 }
 
 }  // namespace ynb
