@@ -61,35 +61,48 @@ __global__ void __launch_bounds__(I8_QT) k_i8_quant(const void* x, long long ldx
   }
   for (int k = 8 * n8 + tid; k < K; k += N) m = max(m, i8_abs_bits(I8In<T>::load(x, base + k)));
   const I8Row q(N == 32 ? __reduce_max_sync(0xffffffffu, m) : block_max_u32(m, buf));
-  const float scale = q.scale();
-  const int n_to = to ? copies : 1;
-  auto out = [&](int j) -> long long { return to ? to[row * copies + j] : (long long)row; };
-  if (tid < n_to && out(tid) >= 0) scales[out(tid)] = scale;
-  auto put8 = [&](int at, const I8Raw<T>& r) {
+  // lane j of every warp has destination j
+  const int lane = threadIdx.x & 31, n_to = to ? copies : 1;
+  const int dest = lane < n_to ? (to ? to[row * copies + lane] : (int)row) : -1;
+  if (tid < n_to && dest >= 0) scales[dest] = q.scale();
+  auto code8 = [&](const I8Raw<T>& r) {
     float g[8];
     uint32_t w[2];
     r.get(g);
-    q.codes(g, w);
-    const uint2 c = make_uint2(w[0], w[1]);
-    for (int j = 0; j < n_to; ++j) {
-      const long long r = out(j);
-      if (r >= 0) *reinterpret_cast<uint2*>(codes + r * ldc + 8 * at) = c;
-    }
+    q.codes<sizeof(T) == 2>(g, w);
+    return make_uint2(w[0], w[1]);
   };
+  uint2 c[HOLD];
 #pragma unroll
   for (int i = 0; i < HOLD; ++i)
-    if (tid + i * N < n8) put8(tid + i * N, raw[i]);
-  for (int at = tid + HOLD * N; at < n8; at += N) {
-    one.load(x, base + 8 * (size_t)at);
-    put8(at, one);
+    if (tid + i * N < n8) c[i] = code8(raw[i]);
+  for (int j = 0; j < n_to; ++j) {
+    const int r = __shfl_sync(0xffffffffu, dest, j);
+    if (r < 0) continue;
+    uint2* at = reinterpret_cast<uint2*>(codes + (long long)r * ldc) + tid;
+#pragma unroll
+    for (int i = 0; i < HOLD; ++i)
+      if (tid + i * N < n8) at[i * N] = c[i];
+  }
+  for (int i = HOLD * N; i < n8; i += N) {
+    if (i + tid < n8) {
+      one.load(x, base + 8 * (size_t)(i + tid));
+      c[0] = code8(one);
+    }
+    for (int j = 0; j < n_to; ++j) {
+      const int r = __shfl_sync(0xffffffffu, dest, j);
+      if (r >= 0 && i + tid < n8) reinterpret_cast<uint2*>(codes + (long long)r * ldc)[i + tid] = c[0];
+    }
   }
   for (int k = 8 * n8 + tid; k < K; k += N) {
     const float g[4] = {I8In<T>::load(x, base + k), 0.0f, 0.0f, 0.0f};
     uint32_t w[1];
-    q.codes(g, w);
-    const int8_t c = (int8_t)w[0];
-    for (int j = 0; j < n_to; ++j)
-      if (out(j) >= 0) codes[out(j) * ldc + k] = c;
+    q.codes<sizeof(T) == 2>(g, w);
+    const int8_t b = (int8_t)w[0];
+    for (int j = 0; j < n_to; ++j) {
+      const long long r = to ? to[row * copies + j] : (long long)row;
+      if (r >= 0) codes[r * ldc + k] = b;
+    }
   }
 }
 
@@ -148,7 +161,8 @@ YN_DEV void i8_row_smem(int dt, const void* x, size_t base, int K, int KP, int8_
 #pragma unroll
     for (int i = 0; i < 4; ++i) f[i] = k + i < K ? i8_load(dt, x, base + k + i) : 0.0f;
     uint32_t w[1];
-    q.codes(f, w);
+    if (dt == YN_F32) q.codes<false>(f, w);
+    else q.codes<true>(f, w);
     *reinterpret_cast<uint32_t*>(codes + k) = w[0];
   }
 }
@@ -303,12 +317,20 @@ __global__ void __launch_bounds__(I8_PLAN_T) k_i8_plan(const int32_t* ids, int P
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   for (int e = tid; e < I8_MAX_E; e += I8_PLAN_T) cnt[e] = 0;
   __syncthreads();
-  for (int i = tid; i < P; i += I8_PLAN_T) {
-    const int e = ids[i];
-    if (e >= 0 && e < E) pair_of[i] = atomicAdd(&cnt[e], 1);
-    else {
-      pair_of[i] = -1;
-      if (e != -1) raise_error(&g_i8_err, YN_ERR_BAD_EXPERT);
+  // 8 pairs per thread at a time, their loads together
+  for (int i0 = tid; i0 < P; i0 += 8 * I8_PLAN_T) {
+    int e[8];
+#pragma unroll
+    for (int q = 0; q < 8; ++q) e[q] = i0 + q * I8_PLAN_T < P ? ids[i0 + q * I8_PLAN_T] : -1;
+#pragma unroll
+    for (int q = 0; q < 8; ++q) {
+      const int i = i0 + q * I8_PLAN_T;
+      if (i >= P) break;
+      if (e[q] >= 0 && e[q] < E) pair_of[i] = atomicAdd(&cnt[e[q]], 1);
+      else {
+        pair_of[i] = -1;
+        if (e[q] != -1) raise_error(&g_i8_err, YN_ERR_BAD_EXPERT);
+      }
     }
   }
   __syncthreads();
@@ -338,8 +360,18 @@ __global__ void __launch_bounds__(I8_PLAN_T) k_i8_plan(const int32_t* ids, int P
     n_out[1] = all.x;
   }
   __syncthreads();
-  for (int i = tid; i < P; i += I8_PLAN_T)
-    if (pair_of[i] >= 0) pair_of[i] += first[ids[i]];
+  for (int i0 = tid; i0 < P; i0 += 8 * I8_PLAN_T) {
+    int e[8], at[8];
+#pragma unroll
+    for (int q = 0; q < 8; ++q) {
+      const int i = i0 + q * I8_PLAN_T;
+      at[q] = i < P ? pair_of[i] : -1;
+      e[q] = i < P ? ids[i] : 0;
+    }
+#pragma unroll
+    for (int q = 0; q < 8; ++q)
+      if (at[q] >= 0) pair_of[i0 + q * I8_PLAN_T] = at[q] + first[e[q]];
+  }
 }
 
 // out[t] = residual[t] + sum_j w_j y[pair_of[t][j]] in fp32, columns in order, rounded once.

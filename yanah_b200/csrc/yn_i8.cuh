@@ -85,22 +85,23 @@ struct I8Raw {
 // that its products are NaN and no other row's; a row of zeros has scale 0.
 struct I8Row {
   float amax, inv;
-  bool exact;   // 127 / amax outside fp32: every code in fp64
+  bool wide;   // 127 x or 127 / amax outside fp32: every code in fp64
   YN_DEV I8Row(uint32_t amax_bits) {
     amax = __uint_as_float(amax_bits);
-    exact = amax < 1e-30f;
-    inv = amax > 0.0f && amax_bits < 0x7F800000u && !exact ? __fdiv_rn(127.0f, amax) : 0.0f;
-    if (amax_bits >= 0x7F800000u) exact = false;
+    wide = amax < 1e-30f || (amax > 1e36f && amax_bits < 0x7F800000u);
+    inv = amax_bits < 0x7F800000u && !wide ? __fdiv_rn(127.0f, amax) : 0.0f;
   }
   YN_DEV float scale() const {
     return __float_as_uint(amax) >= 0x7F800000u ? __int_as_float(0x7fc00000) : __fdiv_rn(amax, 127.0f);
   }
   // The codes of N values (N a multiple of 4), four to a word. Adding 1.5 * 2^23 rounds y to
-  // the nearest whole number, ties to even, and leaves it in the low bits.
-  template <int N>
+  // the nearest whole number, ties to even, and leaves it in the low bits. Near a tie it is
+  // settled from the remainder 127 x - q amax: for 16-bit inputs (NARROW) both terms have at
+  // most 18 bits and fp32 has it exactly, else fp64.
+  template <bool NARROW, int N>
   YN_DEV void codes(const float (&x)[N], uint32_t (&out)[N / 4]) const {
     float t[N];
-    bool near = exact;
+    bool near = wide;
 #pragma unroll
     for (int i = 0; i < N; ++i) {
       const float y = __fmul_rn(x[i], inv);
@@ -108,11 +109,22 @@ struct I8Row {
       near |= fabsf(__fsub_rn(y, __fsub_rn(t[i], 12582912.0f))) > 0.5f - 6.2e-5f;
     }
     if (near) {
+      if (NARROW && !wide) {
 #pragma unroll
-      for (int i = 0; i < N; ++i) {
-        const float y = __fmul_rn(x[i], inv);
-        if (exact || fabsf(__fsub_rn(y, __fsub_rn(t[i], 12582912.0f))) > 0.5f - 6.2e-5f)
-          t[i] = amax > 0.0f ? __fadd_rn((float)rint(127.0 * (double)x[i] / (double)amax), 12582912.0f) : 12582912.0f;
+        for (int i = 0; i < N; ++i) {
+          const float q = __fsub_rn(t[i], 12582912.0f), d = fmaf(-q, amax, 127.0f * x[i]), a = 2.0f * fabsf(d);
+          if (a > amax || (a == amax && (__float_as_int(t[i]) & 1))) t[i] += copysignf(1.0f, d);
+        }
+      } else {
+#pragma unroll 1
+        for (int k = 0; k < N; ++k) {   // one division in the code, N in a row that needs them
+          float xv = 0.0f;
+#pragma unroll
+          for (int i = 0; i < N; ++i) xv = i == k ? x[i] : xv;
+          const float q = amax > 0.0f ? (float)rint(127.0 * (double)xv / (double)amax) : 0.0f;
+#pragma unroll
+          for (int i = 0; i < N; ++i) t[i] = i == k ? __fadd_rn(q, 12582912.0f) : t[i];
+        }
       }
     }
     const bool none = __float_as_uint(amax) >= 0x7F800000u;   // infinities and NaN stay out of the codes

@@ -14,9 +14,9 @@
 // sums. Only a thread that may hold the row's maximum sums without that element; the
 // others' sums are off by 2^-24 of themselves, of a smaller part of S.
 // The alternatives cost little beside that: in its first pieces a block takes a bound
-// of the n-th largest from below (of its 8 warps' or 256 threads' maxima), and from
-// then on only the threads whose maximum reaches it, a few times n in all, have their
-// elements looked at again (from L2).
+// of the n-th largest from below (the n-th largest of its 32 quarter-warps' maxima, or
+// of its 256 threads'), and from then on only the threads whose maximum reaches it, a
+// few times n in all, have their elements looked at again (from L2).
 // Few rows are split over the blocks of a cluster, whose parts the first of them joins
 // through distributed shared memory: one launch, no workspace.
 #include <cooperative_groups.h>
@@ -189,7 +189,7 @@ YN_DEV void lp_join(LpSums& a, const LpSums& b) {
   const bool up = b.m > a.m;
   const float hm = up ? b.m : a.m, hR = up ? b.R : a.R, hD = up ? b.D : a.D;
   const float lm = up ? a.m : b.m, lR = up ? a.R : b.R, lD = up ? a.D : b.D;
-  const float d = hm == lm ? 0.0f : lm - hm, f = lm == -inf ? 0.0f : expf(d);   // both +inf: d = 0
+  const float d = hm == lm ? 0.0f : lm - hm, f = lm == -inf ? 0.0f : lp_ex2(d * LP_LOG2E);   // both +inf: d = 0
   a.m = hm;
   a.R = fmaf(f, 1.0f + lR, hR);
   a.D = f > 0.0f ? fmaf(f, fmaf(d, 1.0f + lR, lD), hD) : hD;
@@ -209,11 +209,9 @@ YN_DEV LpSums lp_warp_join(const LpSums& s) {
   return o;
 }
 
-// A row's answer from its sums, by one thread. z_tok: the token's logit.
-YN_DEV void lp_write(const LpArgs& a, long long row, const LpSums& s, bool nan, int tok, float z_tok, float* log_s) {
+// A row's answer from its sums and log S, by one thread. z_tok: the token's logit.
+YN_DEV void lp_write(const LpArgs& a, long long row, const LpSums& s, float ls, bool nan, int tok, float z_tok) {
   const float inf = __int_as_float(0x7f800000), none = __int_as_float(0x7fc00000);
-  const float ls = log1pf(s.R);
-  *log_s = nan ? none : ls;
   if (a.entropy) a.entropy[row] = nan ? none : s.m == -inf ? 0.0f : ls - s.D / (1.0f + s.R);
   if (!a.tokens) return;
   const bool ok = !nan && tok >= 0 && tok < a.V;
@@ -243,12 +241,10 @@ __global__ void __launch_bounds__(LP_THREADS, 4) k_logprobs(const LpArgs a) {
   using L = LpType<T>;
   constexpr int PER = L::PER;
   constexpr uint32_t KEY_NEG = 0x007FFFFFu;   // f32_ukey(-inf)
-  __shared__ uint32_t tkey[LP_THREADS], wkey[LP_WARPS];
+  __shared__ uint32_t tkey[LP_THREADS], gkey[32];
   __shared__ LpSums wsum[LP_WARPS];
-  __shared__ uint32_t thr_s;
   __shared__ int n_cand;
   __shared__ unsigned long long cand[LP_CAND], list[LP_MAX_TOP], buf[2][LP_WARPS];
-  __shared__ float log_s_s, m_s;
   __shared__ LpSums part;
   __shared__ int part_nan, part_have;
 
@@ -277,10 +273,15 @@ __global__ void __launch_bounds__(LP_THREADS, 4) k_logprobs(const LpArgs a) {
   if (tid == 0) n_cand = 0;
   for (int c0 = v0; c0 < v1; c0 += LP_THREADS * VPT) {
     uint4 v[VPT];
+    const uint8_t* at0 = base + ((size_t)c0 + tid) * 16;
+    if (c0 + LP_THREADS * VPT <= v1) {
 #pragma unroll
-    for (int i = 0; i < VPT; ++i) {
-      const int at = c0 + i * LP_THREADS + tid;
-      v[i] = at < v1 ? ldg_nc_v4(base + (size_t)at * 16) : make_uint4(L::NEG, L::NEG, L::NEG, L::NEG);
+      for (int i = 0; i < VPT; ++i) v[i] = ldg_nc_v4(at0 + i * (LP_THREADS * 16));
+    } else {
+#pragma unroll
+      for (int i = 0; i < VPT; ++i)
+        v[i] = c0 + i * LP_THREADS + tid < v1 ? ldg_nc_v4(at0 + i * (LP_THREADS * 16))
+                                              : make_uint4(L::NEG, L::NEG, L::NEG, L::NEG);
     }
     if ((c0 == 0 && lead) || c0 + LP_THREADS * VPT >= n_vecs) {  // what lies outside the row reads as -inf
 #pragma unroll
@@ -312,40 +313,39 @@ __global__ void __launch_bounds__(LP_THREADS, 4) k_logprobs(const LpArgs a) {
     bad |= tm != tm;
     const uint32_t tk = f32_ukey(tm);
     if (!known) {
-      __syncthreads();
-      tkey[tid] = tk;
-      const uint32_t wk = __reduce_max_sync(0xffffffffu, tk);
-      if (lane == 0) wkey[warp] = wk;
-      __syncthreads();
-      uint32_t hi = wkey[0], lo = wkey[0];
+      if (c0 != v0) __syncthreads();   // gkey and tkey of the last pieces have been read
+      uint32_t g = tk;
 #pragma unroll
-      for (int w = 1; w < LP_WARPS; ++w) {
-        hi = max(hi, wkey[w]);
-        lo = min(lo, wkey[w]);
-      }
+      for (int o = 4; o > 0; o >>= 1) g = max(g, __shfl_xor_sync(0xffffffffu, g, o));
+      if ((lane & 7) == 0) gkey[tid >> 3] = g;
+      if (a.n_top > 32) tkey[tid] = tk;
+      __syncthreads();
+      g = gkey[lane];
+      const uint32_t hi = __reduce_max_sync(0xffffffffu, g);
       ref = f32_from_ukey(hi);
       known = hi > KEY_NEG;
       if (a.n_top && known) {
-        if (a.n_top <= LP_WARPS && lo > KEY_NEG) {
-          thr = lo;
-        } else {
-          if (warp == 0) {   // the n-th largest thread maximum, its low 16 bits left out (a few more candidates)
-            uint32_t k[LP_WARPS], t = 0;
-#pragma unroll
-            for (int w = 0; w < LP_WARPS; ++w) k[w] = tkey[lane + 32 * w];
-            for (int b = 31; b >= 16; --b) {
-              const uint32_t x = t | (1u << b);
-              int c = 0;
-#pragma unroll
-              for (int w = 0; w < LP_WARPS; ++w) c += k[w] >= x;
-              if (__reduce_add_sync(0xffffffffu, c) >= a.n_top) t = x;
-            }
-            if (lane == 0) thr_s = t;
+        uint32_t t = 0;
+        if (a.n_top <= 32) {
+          // every warp takes the n-th largest of the 32 (equal ones go together: lower, and still a bound)
+          for (int j = 0; j < a.n_top; ++j) {
+            t = __reduce_max_sync(0xffffffffu, g);
+            if (g == t) g = 0;
           }
-          __syncthreads();
-          thr = max(thr_s, KEY_NEG + 1);
-          known = thr > KEY_NEG + 1;   // fewer than n threads with a finite logit: look again in the next pieces
+        } else {
+          uint32_t k[LP_WARPS];   // the n-th largest thread maximum, its low 16 bits left out
+#pragma unroll
+          for (int w = 0; w < LP_WARPS; ++w) k[w] = tkey[lane + 32 * w];
+          for (int b = 31; b >= 16; --b) {
+            const uint32_t x = t | (1u << b);
+            int c = 0;
+#pragma unroll
+            for (int w = 0; w < LP_WARPS; ++w) c += k[w] >= x;
+            if (__reduce_add_sync(0xffffffffu, c) >= a.n_top) t = x;
+          }
         }
+        thr = max(t, KEY_NEG + 1);
+        known = thr > KEY_NEG + 1;   // fewer than n of them with a finite logit: look again in the next pieces
       }
     }
     if (tm > -inf) {
@@ -377,14 +377,19 @@ __global__ void __launch_bounds__(LP_THREADS, 4) k_logprobs(const LpArgs a) {
         c.R = fmaf(f, s, -1.0f);
         c.D = f * fmaf(-del, s, d0 + d1) * LP_LN2;
       } else {
+        // few threads come here: their pieces again, one at a time (a small loop)
         int cnt = 0;
         float d = 0.0f;
-#pragma unroll
+#pragma unroll 1
         for (int i = 0; i < VPT; ++i) {
+          const int at = c0 + i * LP_THREADS + tid;
+          if (at >= v1) break;
           float f[PER];
-          lp_unpack<T>(v[i], f);
+          lp_unpack<T>(ldg_nc_v4(base + (size_t)at * 16), f);
+          const long long e0 = (long long)at * PER - lead;
 #pragma unroll
           for (int j = 0; j < PER; ++j) {
+            if (e0 + j < 0 || e0 + j >= a.V) continue;
             const bool top = f[j] == tm;
             const float y = fmaxf((f[j] - tm) * LP_LOG2E, -200.0f), e = top ? 0.0f : lp_ex2(y);
             cnt += top;
@@ -414,13 +419,14 @@ __global__ void __launch_bounds__(LP_THREADS, 4) k_logprobs(const LpArgs a) {
         sums.rank += L::counted(c);
       } else {
         // a barred token: every logit above -inf, and the barred ones of a lower id
-#pragma unroll
+#pragma unroll 1
         for (int i = 0; i < VPT; ++i) {
           const int at = c0 + i * LP_THREADS + tid;
-          float f[PER];
-          lp_unpack<T>(v[i], f);
-#pragma unroll
-          for (int j = 0; j < PER; ++j) sums.rank += at < v1 && (at < tv ? (at > 0 || j >= lead) : f[j] > -inf);
+          if (at >= v1) break;
+          for (int j = 0; j < PER; ++j) {
+            const long long e = (long long)at * PER + j - lead;
+            if (e >= 0 && e < a.V) sums.rank += at < tv || L::load(p + e * sizeof(T)) > -inf;
+          }
         }
       }
       if (tv >= c0 && tv < min(v1, c0 + LP_THREADS * VPT) && (tv - c0) % LP_THREADS == tid) {
@@ -550,13 +556,10 @@ __global__ void __launch_bounds__(LP_THREADS, 4) k_logprobs(const LpArgs a) {
     cluster.sync();   // no block leaves while its parts are read
     if (split != 0) return;
   }
-  if (tid == 0) {
-    lp_write(a, row, sums, row_nan, tok, z_tok, &log_s_s);
-    m_s = sums.m;
-  }
-  if (a.n_top) {
-    __syncthreads();
-    if (tid < a.n_top) lp_write_top(a, row, tid, tid < have ? list[tid] : 0ull, m_s, log_s_s, row_nan);
+  if (warp == 0) {
+    const float ls = row_nan ? __int_as_float(0x7fc00000) : log1pf(sums.R);
+    if (lane == 0) lp_write(a, row, sums, ls, row_nan, tok, z_tok);
+    for (int j = lane; j < a.n_top; j += 32) lp_write_top(a, row, j, j < have ? list[j] : 0ull, sums.m, ls, row_nan);
   }
 }
 
