@@ -11,12 +11,12 @@
 // registers (all loads in flight at once), takes their maximum and sums their
 // exponentials relative to it, one ex2 per element and two fp32 values per
 // instruction elsewhere (fma.rn.f32x2); pieces and threads are joined by rescaling two
-// sums. Only a thread that may hold the row's maximum sums without that element; the
-// others' sums are off by 2^-24 of themselves, of a smaller part of S.
-// The alternatives cost little beside that: in its first pieces a block takes a bound
-// of the n-th largest from below (the n-th largest of its 32 quarter-warps' maxima, or
-// of its 256 threads'), and from then on only the threads whose maximum reaches it, a
-// few times n in all, have their elements looked at again (from L2).
+// sums. A thread's R is its sum less one, off by 2^-23: where the row's R comes out small
+// one warp sums the pieces of the thread that holds the maximum again without it.
+// The alternatives cost little beside that: the n-th largest of the block's 32
+// quarter-warp maxima (or of its 256 thread maxima) bounds the n-th largest element from
+// below, and only the threads that reach it, little more than n, have their elements
+// looked at again, a warp for each (from L2).
 // Few rows are split over the blocks of a cluster, whose parts the first of them joins
 // through distributed shared memory: one launch, no workspace.
 #include <cooperative_groups.h>
@@ -195,16 +195,19 @@ YN_DEV void lp_join(LpSums& a, const LpSums& b) {
   a.D = f > 0.0f ? fmaf(f, fmaf(d, 1.0f + lR, lD), hD) : hD;
 }
 
-// The join of the 32 lanes' parts, on every lane.
-YN_DEV LpSums lp_warp_join(const LpSums& s) {
+// The join of the 32 lanes' parts, on every lane. own: R and D of the one lane (`first`) whose
+// maximum is taken, which are not in those returned.
+YN_DEV LpSums lp_warp_join(const LpSums& s, float2* own, int* first) {
   const float inf = __int_as_float(0x7f800000);
   LpSums o;
   o.m = f32_from_ukey(__reduce_max_sync(0xffffffffu, f32_ukey(s.m)));
   const bool top = s.m == o.m;
-  const int first = __ffs(__ballot_sync(0xffffffffu, top)) - 1;
-  const float d = top ? 0.0f : s.m - o.m, f = s.m == -inf ? 0.0f : top ? 1.0f : expf(d);
-  o.R = warp_sum_f32((int)(threadIdx.x & 31) == first && s.m > -inf ? s.R : f * (1.0f + s.R));
-  o.D = warp_sum_f32(f > 0.0f ? f * fmaf(d, 1.0f + s.R, s.D) : 0.0f);
+  *first = __ffs(__ballot_sync(0xffffffffu, top)) - 1;
+  const float d = top ? 0.0f : s.m - o.m, f = s.m == -inf ? 0.0f : top ? 1.0f : lp_ex2(d * LP_LOG2E);
+  const bool other = (int)(threadIdx.x & 31) != *first && f > 0.0f;
+  *own = make_float2(__shfl_sync(0xffffffffu, s.R, *first), __shfl_sync(0xffffffffu, s.D, *first));
+  o.R = warp_sum_f32(other ? f * (1.0f + s.R) : 0.0f);
+  o.D = warp_sum_f32(other ? f * fmaf(d, 1.0f + s.R, s.D) : 0.0f);
   o.rank = __reduce_add_sync(0xffffffffu, s.rank);
   return o;
 }
@@ -237,12 +240,14 @@ YN_DEV unsigned long long lp_block_max(unsigned long long k, unsigned long long*
 }
 
 template <typename T, int VPT, bool SPLIT>
-__global__ void __launch_bounds__(LP_THREADS, 4) k_logprobs(const LpArgs a) {
+__global__ void __launch_bounds__(LP_THREADS, 1024 / LP_THREADS) k_logprobs(const LpArgs a) {
   using L = LpType<T>;
   constexpr int PER = L::PER;
   constexpr uint32_t KEY_NEG = 0x007FFFFFu;   // f32_ukey(-inf)
   __shared__ uint32_t tkey[LP_THREADS], gkey[32];
   __shared__ LpSums wsum[LP_WARPS];
+  __shared__ float2 wown[LP_WARPS];
+  __shared__ int wfirst[LP_WARPS];
   __shared__ int n_cand;
   __shared__ unsigned long long cand[LP_CAND], list[LP_MAX_TOP], buf[2][LP_WARPS];
   __shared__ LpSums part;
@@ -266,10 +271,8 @@ __global__ void __launch_bounds__(LP_THREADS, 4) k_logprobs(const LpArgs a) {
   const int tv = ranked ? (int)(((long long)lead + tok) / PER) : 0;
 
   LpSums sums = {-inf, 0.0f, 0.0f, 0};
-  bool bad = false;        // a NaN
-  bool known = false;      // the block has a bound of its n-th largest
-  uint32_t thr = KEY_NEG + 1;
-  float ref = inf;         // threads whose maximum reaches it leave it out of their sums
+  bool bad = false;            // a NaN
+  uint32_t tk = KEY_NEG;       // key of the thread's maximum
   if (tid == 0) n_cand = 0;
   for (int c0 = v0; c0 < v1; c0 += LP_THREADS * VPT) {
     uint4 v[VPT];
@@ -311,47 +314,10 @@ __global__ void __launch_bounds__(LP_THREADS, 4) k_logprobs(const LpArgs a) {
       tm = PER == 4 ? f[0] : (f[0] > f[1] || f[0] != f[0] ? f[0] : f[1]);
     }
     bad |= tm != tm;
-    const uint32_t tk = f32_ukey(tm);
-    if (!known) {
-      if (c0 != v0) __syncthreads();   // gkey and tkey of the last pieces have been read
-      uint32_t g = tk;
-#pragma unroll
-      for (int o = 4; o > 0; o >>= 1) g = max(g, __shfl_xor_sync(0xffffffffu, g, o));
-      if ((lane & 7) == 0) gkey[tid >> 3] = g;
-      if (a.n_top > 32) tkey[tid] = tk;
-      __syncthreads();
-      g = gkey[lane];
-      const uint32_t hi = __reduce_max_sync(0xffffffffu, g);
-      ref = f32_from_ukey(hi);
-      known = hi > KEY_NEG;
-      if (a.n_top && known) {
-        uint32_t t = 0;
-        if (a.n_top <= 32) {
-          // every warp takes the n-th largest of the 32 (equal ones go together: lower, and still a bound)
-          for (int j = 0; j < a.n_top; ++j) {
-            t = __reduce_max_sync(0xffffffffu, g);
-            if (g == t) g = 0;
-          }
-        } else {
-          uint32_t k[LP_WARPS];   // the n-th largest thread maximum, its low 16 bits left out
-#pragma unroll
-          for (int w = 0; w < LP_WARPS; ++w) k[w] = tkey[lane + 32 * w];
-          for (int b = 31; b >= 16; --b) {
-            const uint32_t x = t | (1u << b);
-            int c = 0;
-#pragma unroll
-            for (int w = 0; w < LP_WARPS; ++w) c += k[w] >= x;
-            if (__reduce_add_sync(0xffffffffu, c) >= a.n_top) t = x;
-          }
-        }
-        thr = max(t, KEY_NEG + 1);
-        known = thr > KEY_NEG + 1;   // fewer than n of them with a finite logit: look again in the next pieces
-      }
-    }
     if (tm > -inf) {
       // y is (z - tm) log2(e) + del, del the rounding of tm log2(e), which is taken out of the sums
       LpSums c = {tm, 0.0f, 0.0f, 0};
-      if (tm < ref && fabsf(tm) < 4096.0f) {
+      if (fabsf(tm) < 4096.0f) {
         const float ml = tm * LP_LOG2E, del = fmaf(tm, LP_LOG2E, -ml);
         const uint64_t l2 = lp_pair(LP_LOG2E, LP_LOG2E), ml2 = lp_pair(-ml, -ml);
         uint64_t r2 = 0, d2 = 0;
@@ -377,7 +343,8 @@ __global__ void __launch_bounds__(LP_THREADS, 4) k_logprobs(const LpArgs a) {
         c.R = fmaf(f, s, -1.0f);
         c.D = f * fmaf(-del, s, d0 + d1) * LP_LN2;
       } else {
-        // few threads come here: their pieces again, one at a time (a small loop)
+        // maxima so large that del is not small, or infinite: the pieces again, one at a time, the
+        // subtraction first
         int cnt = 0;
         float d = 0.0f;
 #pragma unroll 1
@@ -401,6 +368,7 @@ __global__ void __launch_bounds__(LP_THREADS, 4) k_logprobs(const LpArgs a) {
         c.D = d * LP_LN2;
       }
       lp_join(sums, c);
+      tk = max(tk, f32_ukey(tm));
     }
     if (ranked && tm >= z_tok) {
       if (z_tok > -inf) {
@@ -437,45 +405,102 @@ __global__ void __launch_bounds__(LP_THREADS, 4) k_logprobs(const LpArgs a) {
         }
       }
     }
-    if (a.n_top) {
-      // the elements of the warp's threads that reach the bound: 32 / VPT threads at a time, one
-      // lane per vector
-      unsigned who = __ballot_sync(0xffffffffu, tk >= thr);
-      const float least = f32_from_ukey(thr);
-      while (who) {
-        int o = -1;
+  }
+  {
+    float2 own;
+    int first;
+    sums = lp_warp_join(sums, &own, &first);
+    if (lane == 0) {
+      wsum[warp] = sums;
+      wown[warp] = own;
+      wfirst[warp] = first;
+    }
+    uint32_t g = tk;
 #pragma unroll
-        for (int q = 0; q < 32 / VPT && q < 4; ++q) {
-          if (who && lane / VPT == q) o = __ffs(who) - 1;
-          who &= who - 1;   // 0 stays 0
-        }
-        const int at = c0 + (lane % VPT) * LP_THREADS + 32 * warp + o;
-        if (o >= 0 && at < v1) {
-          float f[PER];
-          lp_unpack<T>(ldg_nc_v4(base + (size_t)at * 16), f);
-          unsigned hit = 0;
+    for (int o = LP_THREADS / 64; o > 0; o >>= 1) g = max(g, __shfl_xor_sync(0xffffffffu, g, o));
+    if (tid % (LP_THREADS / 32) == 0) gkey[tid / (LP_THREADS / 32)] = g;
+    if (a.n_top > 32) tkey[tid] = tk;
+  }
+  const bool nan = __syncthreads_or(bad) != 0;
+  if (a.n_top) {
+    uint32_t t = 0;
+    if (a.n_top <= 32) {
+      // every warp takes the n-th largest of the 32 (equal ones go together: lower, and still a bound)
+      uint32_t g = gkey[lane];
+      for (int j = 0; j < a.n_top; ++j) {
+        t = __reduce_max_sync(0xffffffffu, g);
+        if (g == t) g = 0;
+      }
+    } else {
+      uint32_t k[LP_WARPS];   // the n-th largest thread maximum, its low 16 bits left out
 #pragma unroll
-          for (int j = 0; j < PER; ++j) hit |= f[j] >= least ? 1u << j : 0u;
-          while (hit) {
-            const int j = __ffs(hit) - 1;
-            hit &= hit - 1;
-            const long long e = (long long)at * PER - lead + j;
-            if (e < 0 || e >= a.V) continue;
-            const int q = atomicAdd(&n_cand, 1);
-            if (q < LP_CAND)
-              cand[q] = ((unsigned long long)f32_ukey(L::load(p + e * sizeof(T))) << 32) | (0xFFFFFFFFu - (uint32_t)e);
-          }
-        }
+      for (int w = 0; w < LP_WARPS; ++w) k[w] = tkey[lane + 32 * w];
+      for (int b = 31; b >= 16; --b) {
+        const uint32_t x = t | (1u << b);
+        int c = 0;
+#pragma unroll
+        for (int w = 0; w < LP_WARPS; ++w) c += k[w] >= x;
+        if (__reduce_add_sync(0xffffffffu, c) >= a.n_top) t = x;
       }
     }
+    t = max(t, KEY_NEG + 1);
+    const float least = f32_from_ukey(t);
+    // the elements of each of the warp's threads that reach the bound, a lane per vector
+    for (unsigned who = __ballot_sync(0xffffffffu, tk >= t); who; who &= who - 1) {
+      for (int at = v0 + 32 * warp + __ffs(who) - 1 + lane * LP_THREADS; at < v1; at += 32 * LP_THREADS) {
+        const uint4 q = ldg_nc_v4(base + (size_t)at * 16);
+        const uint32_t w = L::max_nan(L::max_nan(q.x, q.y), L::max_nan(q.z, q.w));
+        float f[PER];
+        L::unpack(w, f);
+        if (at > 0 && at < n_vecs - 1 && !(f[0] >= least || (PER == 8 && f[1] >= least))) continue;
+        lp_unpack<T>(q, f);
+        const long long e0 = (long long)at * PER - lead;
+#pragma unroll
+        for (int j = 0; j < PER; ++j)
+          if (f[j] >= least && e0 + j >= 0 && e0 + j < a.V) {
+            const int n = atomicAdd(&n_cand, 1);
+            if (n < LP_CAND) cand[n] = ((unsigned long long)f32_ukey(f[j]) << 32) | (0xFFFFFFFFu - (uint32_t)(e0 + j));
+          }
+      }
+      __syncwarp();
+    }
   }
-  sums = lp_warp_join(sums);
-  if (lane == 0) wsum[warp] = sums;
-  const bool nan = __syncthreads_or(bad) != 0;
   if (warp == 0) {
     const LpSums none = {-inf, 0.0f, 0.0f, 0};
-    sums = lp_warp_join(lane < LP_WARPS ? wsum[lane] : none);
+    // a warp's sums are whole where another warp has the maximum
+    LpSums s = lane < LP_WARPS ? wsum[lane] : none;
+    const float2 own = lane < LP_WARPS ? wown[lane] : make_float2(0.0f, 0.0f), apart = make_float2(s.R, s.D);
+    s.R += own.x;
+    s.D += own.y;
+    float2 whole;
+    int w0;
+    sums = lp_warp_join(s, &whole, &w0);
+    float2 rest = wown[w0];   // of the thread that holds the maximum
+    sums.R += __shfl_sync(0xffffffffu, apart.x, w0);
+    sums.D += __shfl_sync(0xffffffffu, apart.y, w0);
+    if (sums.R + rest.x < 0.25f && fabsf(sums.m) < inf) {
+      float r = 0.0f, d = 0.0f;
+      int cnt = 0;
+      for (int at = v0 + 32 * w0 + wfirst[w0] + lane * LP_THREADS; at < v1; at += 32 * LP_THREADS) {
+        float f[PER];
+        lp_unpack<T>(ldg_nc_v4(base + (size_t)at * 16), f);
+#pragma unroll
+        for (int j = 0; j < PER; ++j) {
+          const long long e = (long long)at * PER + j - lead;
+          if (e < 0 || e >= a.V) continue;
+          const float y = fmaxf((f[j] - sums.m) * LP_LOG2E, -200.0f), x = f[j] == sums.m ? 0.0f : lp_ex2(y);
+          cnt += f[j] == sums.m;
+          r += x;
+          d = fmaf(x, y, d);
+        }
+      }
+      rest.x = warp_sum_f32(r) + (float)(__reduce_add_sync(0xffffffffu, cnt) - 1);
+      rest.y = warp_sum_f32(d) * LP_LN2;
+    }
+    sums.R += rest.x;
+    sums.D += rest.y;
   }
+  if (a.n_top) __syncthreads();
   int have = 0;
   if (a.n_top) {
     int n = n_cand;
@@ -530,7 +555,11 @@ __global__ void __launch_bounds__(LP_THREADS, 4) k_logprobs(const LpArgs a) {
           s = *cluster.map_shared_rank(&part, lane);
           row_nan = *cluster.map_shared_rank(&part_nan, lane) != 0;
         }
-        sums = lp_warp_join(s);
+        float2 own;
+        int first;
+        sums = lp_warp_join(s, &own, &first);
+        sums.R += own.x;
+        sums.D += own.y;
       }
       row_nan = __syncthreads_or(row_nan) != 0;
       if (a.n_top) {
