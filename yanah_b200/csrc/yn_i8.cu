@@ -145,27 +145,56 @@ YN_DEV uint4 i8_codes16(const int8_t* row, int off, int K) {
   return make_uint4(w[0], w[1], w[2], w[3]);
 }
 
-// Codes and scale of one row of K elements into shared memory by `n` threads (the
-// whole block, or one warp), zero up to KP.
-template <bool BLOCK>
-YN_DEV void i8_row_smem(int dt, const void* x, size_t base, int K, int KP, int8_t* codes, float* scale, uint32_t* buf) {
+// Codes and scale of one row of K elements into shared memory by `n` threads (the whole
+// block, or one warp), zero up to KP. The elements are read twice (from L1 or L2 the second
+// time): rows are a few KB.
+template <bool BLOCK, typename T>
+YN_DEV void i8_row_smem_t(const void* x, size_t base, int K, int KP, int8_t* codes, float* scale, uint32_t* buf) {
   const int at = BLOCK ? threadIdx.x : threadIdx.x & 31, n = BLOCK ? (int)blockDim.x : 32;
+  const bool vec = (reinterpret_cast<uintptr_t>(reinterpret_cast<const T*>(x) + base) & 15u) == 0;
+  const int n8 = vec ? K / 8 : 0;
   uint32_t m = 0;
-  for (int k = at; k < K; k += n) m = max(m, i8_abs_bits(i8_load(dt, x, base + k)));
+#pragma unroll 2
+  for (int i = at; i < n8; i += n) {
+    I8Raw<T> r;
+    float f[8];
+    r.load(x, base + 8 * (size_t)i);
+    r.get(f);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) m = max(m, i8_abs_bits(f[j]));
+  }
+  for (int k = 8 * n8 + at; k < K; k += n) m = max(m, i8_abs_bits(I8In<T>::load(x, base + k)));
   if (BLOCK) m = block_max_u32(m, buf);
   else m = __reduce_max_sync(0xffffffffu, m);
   const I8Row q(m);
   if (at == 0) *scale = q.scale();
-  for (int k = 4 * at; k < KP; k += 4 * n) {
-    float f[4];
+#pragma unroll 2
+  for (int i = at; i < KP / 8; i += n) {
+    I8Raw<T> r;
+    float f[8];
+    if (i < n8) {
+      r.load(x, base + 8 * (size_t)i);
+      r.get(f);
+    } else {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) f[i] = k + i < K ? i8_load(dt, x, base + k + i) : 0.0f;
-    uint32_t w[1];
-    if (dt == YN_F32) q.codes<false>(f, w);
-    else q.codes<true>(f, w);
-    *reinterpret_cast<uint32_t*>(codes + k) = w[0];
+      for (int j = 0; j < 8; ++j) f[j] = 8 * i + j < K ? I8In<T>::load(x, base + 8 * i + j) : 0.0f;
+    }
+    uint32_t w[2];
+    q.codes<sizeof(T) == 2>(f, w);
+    *reinterpret_cast<uint2*>(codes + 8 * i) = make_uint2(w[0], w[1]);
   }
 }
+template <bool BLOCK>
+YN_DEV void i8_row_smem(int dt, const void* x, size_t base, int K, int KP, int8_t* codes, float* scale, uint32_t* buf) {
+  if (dt == YN_F32) i8_row_smem_t<BLOCK, float>(x, base, K, KP, codes, scale, buf);
+  else if (dt == YN_BF16) i8_row_smem_t<BLOCK, __nv_bfloat16>(x, base, K, KP, codes, scale, buf);
+  else i8_row_smem_t<BLOCK, __half>(x, base, K, KP, codes, scale, buf);
+}
+
+// The second of two kernels starts while the first still runs (programmatic launch); what it
+// reads of the first it reads after the wait.
+YN_DEV void i8_launch_next() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+YN_DEV void i8_wait_previous() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 
 struct I8Mat {
   const int8_t* codes;
@@ -210,31 +239,89 @@ YN_DEV void i8_dots(const int8_t* const (&w)[R], const int8_t* xs, int KP, int K
 
 // y (T, N) of T <= 8 rows: every block makes the rows' codes itself (they are a few KB),
 // then its warps take 4 output channels at a time through the matrix, which is read once:
-// bound by that read.
+// bound by that read. A lane copies its own 16 codes of 4 channels per step into a ring of
+// its warp (cp.async, I8_FS steps deep, 160 KB in flight per SM) and reads them back itself,
+// so that neither the products nor the sums over lanes stop the copies and no thread waits
+// for another. Loads into registers instead (8 per lane in flight) took 25 us for 1 x 2048 x
+// 65536 and 71 us for 5 x 2048 x 151936, twice as many of them 32 and 91 us.
+constexpr int I8_FR = 4;    // channels per step
+constexpr int I8_FS = 6;    // steps in the ring
+constexpr int I8_FRING = I8_FS * I8_FR * I8_GK;   // bytes per warp
+
+YN_DEV void i8_copy16(uint32_t dst, const void* src, int bytes) {   // bytes past `bytes` become 0
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
+}
+
 template <int T>
-__global__ void __launch_bounds__(I8_GT) k_i8_few(int dt, const void* x, long long ldx, int K, int KP, const I8Mat w,
-                                                  int N, int odt, void* y, long long ldy) {
-  extern __shared__ __align__(16) int8_t xs[];
+__global__ void __launch_bounds__(I8_GT, 2) k_i8_few(int dt, const void* x, long long ldx, int K, int KP, const I8Mat w,
+                                                     int N, int odt, void* y, long long ldy) {
+  extern __shared__ __align__(16) int8_t few_smem[];   // rings, then the rows' codes
   __shared__ float sx[T];
   __shared__ uint32_t buf[I8_GW];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  int8_t* xs = few_smem + I8_GW * I8_FRING;
+  const uint32_t ring = smem_u32(few_smem + warp * I8_FRING) + 16 * lane;
+  const int NC = KP / I8_GK;
+  const long long stride = (long long)gridDim.x * I8_GW * I8_FR, n_first = ((long long)blockIdx.x * I8_GW + warp) * I8_FR;
+  // the step that is copied next
+  long long cn = n_first;
+  int cc = 0, cslot = 0;
+  auto copy = [&]() {
+    if (cn < N) {
+      const int off = cc * I8_GK + 16 * lane, bytes = min(16, max(0, K - off));
+#pragma unroll
+      for (int r = 0; r < I8_FR; ++r) {
+        const long long n = cn + r < N ? cn + r : (long long)N - 1;
+        i8_copy16(ring + cslot * (I8_FR * I8_GK) + r * I8_GK, w.codes + n * w.row_stride + (bytes ? off : 0), bytes);
+      }
+      cslot = cslot + 1 < I8_FS ? cslot + 1 : 0;
+      if (++cc == NC) {
+        cc = 0;
+        cn += stride;
+      }
+    }
+    asm volatile("cp.async.commit_group;" ::: "memory");
+  };
+#pragma unroll
+  for (int i = 0; i < I8_FS - 1; ++i) copy();
   if (T == 1) i8_row_smem<true>(dt, x, 0, K, KP, xs, sx, buf);
   else if (warp < T) i8_row_smem<false>(dt, x, (size_t)warp * ldx, K, KP, xs + warp * KP, sx + warp, buf);
   __syncthreads();
-  constexpr int R = 4;
-  for (long long n0 = ((long long)blockIdx.x * I8_GW + warp) * R; n0 < N; n0 += (long long)gridDim.x * I8_GW * R) {
-    const int8_t* rows[R];
+  int slot = 0;
+  for (long long n0 = n_first; n0 < N; n0 += stride) {
+    int acc[I8_FR][T];
 #pragma unroll
-    for (int r = 0; r < R; ++r) rows[r] = w.codes + (n0 + r < N ? n0 + r : (long long)N - 1) * w.row_stride;
-    int acc[R][T];
-    i8_dots<R, T, 2>(rows, xs, KP, K, lane, acc);
+    for (int r = 0; r < I8_FR; ++r)
 #pragma unroll
-    for (int r = 0; r < R; ++r)
+      for (int t = 0; t < T; ++t) acc[r][t] = 0;
+    for (int c = 0; c < NC; ++c) {
+      asm volatile("cp.async.wait_group %0;" ::"n"(I8_FS - 2) : "memory");
+      uint4 a[I8_FR];
 #pragma unroll
-      for (int t = 0; t < T; ++t)
-        if (lane == r * T + t && n0 + r < N)
-          i8_store(odt, y, (size_t)t * ldy + n0 + r, (float)acc[r][t] * sx[t] * w.scales[n0 + r]);
+      for (int r = 0; r < I8_FR; ++r)
+        a[r] = *reinterpret_cast<const uint4*>(few_smem + warp * I8_FRING + slot * (I8_FR * I8_GK) + r * I8_GK + 16 * lane);
+      slot = slot + 1 < I8_FS ? slot + 1 : 0;
+#pragma unroll
+      for (int t = 0; t < T; ++t) {
+        const uint4 q = *reinterpret_cast<const uint4*>(xs + t * KP + c * I8_GK + 16 * lane);
+#pragma unroll
+        for (int r = 0; r < I8_FR; ++r) acc[r][t] = dot16(a[r], q, acc[r][t]);
+      }
+      copy();   // into the slot read one step ago
+    }
+    // every lane gets all sums; lane r * T + t (for T = 8 all 32) writes one
+    float out = 0.0f;
+#pragma unroll
+    for (int r = 0; r < I8_FR; ++r)
+#pragma unroll
+      for (int t = 0; t < T; ++t) {
+        const int v = __reduce_add_sync(0xffffffffu, acc[r][t]);
+        if (lane == r * T + t) out = (float)v;
+      }
+    const int r = lane / T, t = lane - r * T;
+    if (r < I8_FR && n0 + r < N) i8_store(odt, y, (size_t)t * ldy + n0 + r, out * sx[t] * __ldg(w.scales + n0 + r));
   }
+  asm volatile("cp.async.wait_group 0;" ::: "memory");
 }
 
 // Few (row, expert) pairs: gate and up of 2 units per warp, the pair's row codes made by
@@ -245,6 +332,7 @@ __global__ void __launch_bounds__(I8_GT) k_i8_up_few(int dt, const void* x, long
   __shared__ float sx;
   __shared__ uint32_t buf[I8_GW];
   const int p = blockIdx.y, e = ids[p], warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  i8_launch_next();
   if (e < 0 || e >= E) {
     if (e != -1 && threadIdx.x == 0 && blockIdx.x == 0) raise_error(&g_i8_err, YN_ERR_BAD_EXPERT);
     return;
@@ -269,33 +357,66 @@ __global__ void __launch_bounds__(I8_GT) k_i8_up_few(int dt, const void* x, long
 }
 
 // The down products of a row's experts and their weighted sum: a block makes the codes of
-// the row's k activations, its warps take 2 outputs each through all k experts.
+// the row's k activations, its warps take 2 outputs each through all k experts, 4 experts'
+// rows in flight at a time, the first of them before the activations are there.
+constexpr int I8_DJ = 4;
 __global__ void __launch_bounds__(I8_GT) k_i8_down_few(const float* act, int I, int IP, const int32_t* ids, const float* wts,
                                                        int k, int E, const I8Mat down, int H, int odt, const void* res,
                                                        long long ldr, void* out, long long ldo) {
   extern __shared__ __align__(16) int8_t as[];
   __shared__ float sa[32];
   const int t = blockIdx.y, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int h0 = 2 * (blockIdx.x * I8_GW + warp), h1 = h0 + 1 < H ? h0 + 1 : h0;
+  const bool work = h0 < H;
+  const int mine = lane < k ? ids[(size_t)t * k + lane] : -1;   // lane j: the row's expert j
+  const float w_mine = lane < k ? wts[(size_t)t * k + lane] : 0.0f;
+  uint4 a[I8_DJ][2];
+  // rows of experts j0.. from column off on
+  auto load = [&](int j0, int off) {
+#pragma unroll
+    for (int q = 0; q < I8_DJ; ++q) {
+      const int e = __shfl_sync(0xffffffffu, mine, (j0 + q) & 31);
+      const bool on = work && j0 + q < k && e >= 0 && e < E && off < I;
+      const int8_t* d = down.codes + (on ? e * down.mat_stride : 0);
+      a[q][0] = on ? i8_codes16(d + h0 * down.row_stride, off, I) : make_uint4(0, 0, 0, 0);
+      a[q][1] = on ? i8_codes16(d + h1 * down.row_stride, off, I) : make_uint4(0, 0, 0, 0);
+    }
+  };
+  load(0, 16 * lane);
+  i8_wait_previous();
   for (int j = warp; j < k; j += I8_GW) {
-    const int e = ids[(size_t)t * k + j];
-    if (e >= 0 && e < E)
-      i8_row_smem<false>(YN_F32, act, ((size_t)t * k + j) * I, I, IP, as + j * IP, sa + j, nullptr);
+    const int e = __shfl_sync(0xffffffffu, mine, j);
+    if (e >= 0 && e < E) i8_row_smem_t<false, float>(act, ((size_t)t * k + j) * I, I, IP, as + j * IP, sa + j, nullptr);
   }
   __syncthreads();
-  const int h0 = 2 * (blockIdx.x * I8_GW + warp);
-  if (h0 >= H) return;
-  const int h1 = h0 + 1 < H ? h0 + 1 : h0;
+  if (!work) return;
   float sum = 0.0f;   // of output h0 + (lane & 1)
-  for (int j = 0; j < k; ++j) {
-    const int e = ids[(size_t)t * k + j];
-    if (e < 0 || e >= E) continue;
-    const int8_t* d = down.codes + e * down.mat_stride;
-    const int8_t* rows[2] = {d + h0 * down.row_stride, d + h1 * down.row_stride};
-    int acc[2][1];
-    i8_dots<2, 1, 1>(rows, as + j * IP, IP, I, lane, acc);
-    const int h = lane & 1 ? h1 : h0;
-    sum = fmaf(wts[(size_t)t * k + j],
-               (float)(lane & 1 ? acc[1][0] : acc[0][0]) * sa[j] * down.scales[e * down.scale_stride + h], sum);
+  for (int j0 = 0; j0 < k; j0 += I8_DJ) {
+    int acc[I8_DJ][2];
+#pragma unroll
+    for (int q = 0; q < I8_DJ; ++q) acc[q][0] = acc[q][1] = 0;
+    for (int k0 = 0; k0 < I; k0 += I8_GK) {
+      const int off = k0 + 16 * lane;
+      if (j0 + k0 > 0) load(j0, off);
+      if (off < I) {
+#pragma unroll
+        for (int q = 0; q < I8_DJ; ++q) {
+          if (j0 + q >= k) break;
+          const uint4 x = *reinterpret_cast<const uint4*>(as + (j0 + q) * IP + off);
+          acc[q][0] = dot16(a[q][0], x, acc[q][0]);
+          acc[q][1] = dot16(a[q][1], x, acc[q][1]);
+        }
+      }
+      __syncwarp();
+    }
+#pragma unroll
+    for (int q = 0; q < I8_DJ; ++q) {
+      const int e = __shfl_sync(0xffffffffu, mine, (j0 + q) & 31);
+      const float w = __shfl_sync(0xffffffffu, w_mine, (j0 + q) & 31);
+      const int d0 = __reduce_add_sync(0xffffffffu, acc[q][0]), d1 = __reduce_add_sync(0xffffffffu, acc[q][1]);
+      if (j0 + q >= k || e < 0 || e >= E) continue;
+      sum = fmaf(w, (float)(lane & 1 ? d1 : d0) * sa[j0 + q] * __ldg(down.scales + e * down.scale_stride + (lane & 1 ? h1 : h0)), sum);
+    }
   }
   if (lane < 2 && h0 + lane < H) {
     const size_t h = h0 + lane;
@@ -516,10 +637,10 @@ template <int T>
 int launch_few(int dt, const void* x, long long ldx, int K, const I8Mat& w, int N, int odt, void* y, long long ldy, int sms,
                cudaStream_t st) {
   const int KP = (int)up_to(K, I8_GK);
-  const size_t smem = (size_t)T * KP;
-  int rc = host_set_smem(reinterpret_cast<const void*>(k_i8_few<T>), 96 * 1024);
+  const size_t smem = (size_t)T * KP + I8_GW * I8_FRING;
+  const int rc = host_set_smem(reinterpret_cast<const void*>(k_i8_few<T>), 96 * 1024 + I8_GW * I8_FRING);
   if (rc) return rc;
-  const int grid = std::min((N + 4 * I8_GW - 1) / (4 * I8_GW), 3 * sms);
+  const int grid = std::min((N + I8_FR * I8_GW - 1) / (I8_FR * I8_GW), 2 * sms);
   k_i8_few<T><<<grid, I8_GT, smem, st>>>(dt, x, ldx, K, KP, w, N, odt, y, ldy);
   const cudaError_t e = cudaGetLastError();
   return e == cudaSuccess ? YN_OK : host_fail(YN_E_CUDA, std::string("8-bit product: ") + cudaGetErrorString(e));
@@ -676,13 +797,24 @@ extern "C" int yn_i8_experts(const yn_i8_mat* gate, const yn_i8_mat* up, const y
   if (experts_few(P, top_k, H, I)) {
     float* act = reinterpret_cast<float*>(b + L.act);
     const int HP = (int)up_to(H, I8_GK), IP = (int)up_to(I, I8_GK);
-    if ((rc = host_set_smem(reinterpret_cast<const void*>(k_i8_up_few), 96 * 1024)) ||
-        (rc = host_set_smem(reinterpret_cast<const void*>(k_i8_down_few), 96 * 1024)))
+    const size_t ds = (size_t)top_k * IP;
+    if ((HP > 48 * 1024 && (rc = host_set_smem(reinterpret_cast<const void*>(k_i8_up_few), 96 * 1024))) ||
+        (ds > 40 * 1024 && (rc = host_set_smem(reinterpret_cast<const void*>(k_i8_down_few), 96 * 1024))))
       return rc;
     k_i8_up_few<<<dim3((I + 2 * I8_GW - 1) / (2 * I8_GW), P), I8_GT, HP, st>>>(dtype, x, x_stride, H, HP, ids, top_k, E, mg, mu,
                                                                              I, act);
-    k_i8_down_few<<<dim3((H + 2 * I8_GW - 1) / (2 * I8_GW), (unsigned)rows), I8_GT, (size_t)top_k * IP, st>>>(
-        act, I, IP, ids, weights, top_k, E, md, H, dtype, residual, res_stride, out, out_stride);
+    cudaLaunchAttribute at{};
+    at.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    at.val.programmaticStreamSerializationAllowed = 1;
+    cudaLaunchConfig_t lc{};
+    lc.gridDim = dim3((H + 2 * I8_GW - 1) / (2 * I8_GW), (unsigned)rows);
+    lc.blockDim = dim3(I8_GT);
+    lc.dynamicSmemBytes = ds;
+    lc.stream = st;
+    lc.attrs = &at;
+    lc.numAttrs = 1;
+    (void)cudaLaunchKernelEx(&lc, k_i8_down_few, (const float*)act, I, IP, ids, weights, (int)top_k, E, md, H, (int)dtype,
+                             residual, (long long)res_stride, out, (long long)out_stride);
     const cudaError_t e = cudaGetLastError();
     return e == cudaSuccess ? YN_OK : host_fail(YN_E_CUDA, std::string("experts: ") + cudaGetErrorString(e));
   }

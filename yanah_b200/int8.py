@@ -54,19 +54,20 @@ def quantize_rows(x: torch.Tensor, stream: Optional[torch.cuda.Stream] = None) -
 
 def _mat(w: Int8Matrix, like: torch.Tensor, what: str) -> _lib.I8Mat:
     codes, scales = w
-    if codes.dtype != torch.int8 or scales.dtype != torch.float32:
+    shape, strides, device = codes.shape, codes.stride(), like.device
+    if codes.dtype is not torch.int8 or scales.dtype is not torch.float32:
         raise TypeError(f"{what} must have int8 codes and float32 scales")
-    if codes.dim() not in (2, 3) or scales.shape != codes.shape[:-1]:
+    if len(shape) not in (2, 3) or scales.shape != shape[:-1]:
         raise ValueError(f"{what}: codes (N, K) or (E, N, K) with scales (N) or (E, N)")
-    if codes.device != like.device or scales.device != like.device:
-        raise ValueError(f"{what} is not on {like.device}")
-    n, k = codes.shape[-2:]
-    e = codes.shape[0] if codes.dim() == 3 else 1
-    if (k > 1 and codes.stride(-1) != 1) or (n > 1 and scales.stride(-1) != 1):
+    if codes.device != device or scales.device != device:
+        raise ValueError(f"{what} is not on {device}")
+    n, k = shape[-2:]
+    e = shape[0] if len(shape) == 3 else 1
+    if (k > 1 and strides[-1] != 1) or (n > 1 and scales.stride(-1) != 1):
         raise ValueError(f"{what}: a row's codes and a matrix's scales must be adjacent")
-    rs = codes.stride(-2) if n > 1 else (k + 15) // 16 * 16
-    many = codes.dim() == 3 and e > 1
-    return _lib.I8Mat(codes.data_ptr(), scales.data_ptr(), rs, codes.stride(0) if many else rs * n,
+    rs = strides[-2] if n > 1 else (k + 15) // 16 * 16
+    many = e > 1
+    return _lib.I8Mat(codes.data_ptr(), scales.data_ptr(), rs, strides[0] if many else rs * n,
                       scales.stride(0) if many else n, e, n, k)
 
 

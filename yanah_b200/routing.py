@@ -13,8 +13,8 @@ route their layers by such a rule; the ids and weights are those that
 from __future__ import annotations
 
 import ctypes as C
-from dataclasses import dataclass
-from typing import Optional, Tuple
+from functools import lru_cache
+from typing import NamedTuple, Optional, Tuple
 
 import torch
 
@@ -24,8 +24,8 @@ from .launch import DTYPES, check_floats, check_like, elsewhere, raw_stream, row
 SCORES = {"softmax": 0, "sigmoid": 1}
 
 
-@dataclass(frozen=True)
-class RouteRule:
+class RouteRule(NamedTuple("RouteRule", [("top_k", int), ("score", str), ("n_groups", int), ("top_groups", int),
+                                        ("group_top", int), ("norm_topk", bool), ("scale", float)])):
     """How a row chooses its experts.
 
     top_k: experts per row (<= 31). score: "softmax" or "sigmoid". n_groups: the
@@ -33,26 +33,19 @@ class RouteRule:
     ``top_groups`` best; a group's score is the sum of its ``group_top`` (1 or 2)
     largest choice values. norm_topk: divide the weights by their sum. scale:
     factor of the weights."""
-    top_k: int
-    score: str = "softmax"
-    n_groups: int = 1
-    top_groups: int = 1
-    group_top: int = 2
-    norm_topk: bool = True
-    scale: float = 1.0
+    __slots__ = ()
 
-    def __post_init__(self):
-        if self.score not in SCORES:
-            raise ValueError(f"score must be 'softmax' or 'sigmoid', not {self.score!r}")
-        object.__setattr__(self, "_structs", {})
+    def __new__(cls, top_k: int, score: str = "softmax", n_groups: int = 1, top_groups: int = 1, group_top: int = 2,
+                norm_topk: bool = True, scale: float = 1.0):
+        if score not in SCORES:
+            raise ValueError(f"score must be 'softmax' or 'sigmoid', not {score!r}")
+        return tuple.__new__(cls, (top_k, score, n_groups, top_groups, group_top, norm_topk, scale))
 
-    def struct(self, n_experts: int) -> _lib.RouteRuleStruct:
-        s = self._structs.get(n_experts)
-        if s is None:
-            s = self._structs[n_experts] = _lib.RouteRuleStruct(
-                n_experts, self.top_k, SCORES[self.score], self.n_groups, self.top_groups, self.group_top,
-                int(self.norm_topk), self.scale)
-        return s
+
+@lru_cache(maxsize=256)
+def _rule_struct(rule: RouteRule, n_experts: int) -> _lib.RouteRuleStruct:
+    return _lib.RouteRuleStruct(n_experts, rule.top_k, SCORES[rule.score], rule.n_groups, rule.top_groups,
+                                rule.group_top, int(rule.norm_topk), rule.scale)
 
 
 def route_scored(logits: torch.Tensor, rule: RouteRule, bias: Optional[torch.Tensor] = None,
@@ -89,7 +82,7 @@ def route_scored(logits: torch.Tensor, rule: RouteRule, bias: Optional[torch.Ten
         if not (ids.is_contiguous() and weights.is_contiguous()):
             raise ValueError("out must be contiguous")
     _lib.check(_lib.lib().yn_route_scored(
-        C.byref(rule.struct(e)), logits.data_ptr(), DTYPES[logits.dtype], row_stride(logits), rows,
+        C.byref(_rule_struct(rule, e)), logits.data_ptr(), DTYPES[logits.dtype], row_stride(logits), rows,
         None if bias is None else bias.data_ptr(), None if available is None else available.data_ptr(),
         ids.data_ptr(), weights.data_ptr(), raw_stream(logits.device)))
     return ids, weights
