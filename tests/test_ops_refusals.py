@@ -68,7 +68,7 @@ def test_int8_linear():
                dict(rows=20), dict(rows=20, ws=P, nb=64)):
         assert linear(mat(), **kw) == INV, kw
     assert linear(mat(), rows=0, x=None) == _lib.YN_OK
-    assert _lib.lib().yn_i8_linear_ws_bytes(8, 2048) == 0 and _lib.lib().yn_i8_linear_ws_bytes(9, 2048) >= 9 * 2048
+    assert _lib.lib().yn_i8_linear_ws_bytes(1, 2048) == 0 and _lib.lib().yn_i8_linear_ws_bytes(9, 2048) >= 9 * 2048
     q = _lib.lib().yn_i8_quant_rows
     assert q(P, 0, 63, 2, 64, P, 64, P, None) == INV and q(P, 0, 64, 2, 64, P, 63, P, None) == INV
     assert q(P, 9, 64, 2, 64, P, 64, P, None) == INV and q(None, 0, 64, 2, 64, P, 64, P, None) == INV

@@ -237,15 +237,16 @@ YN_DEV void i8_dots(const int8_t* const (&w)[R], const int8_t* xs, int KP, int K
     for (int t = 0; t < T; ++t) acc[r][t] = __reduce_add_sync(0xffffffffu, acc[r][t]);
 }
 
-// y (T, N) of T <= 8 rows: every block makes the rows' codes itself (they are a few KB),
+// y (T, N) of T <= 5 rows: every block makes the rows' codes itself (they are a few KB),
 // then its warps take 4 output channels at a time through the matrix, which is read once:
-// bound by that read. A lane copies its own 16 codes of 4 channels per step into a ring of
-// its warp (cp.async, I8_FS steps deep, 160 KB in flight per SM) and reads them back itself,
+// bound by that read with one row (2048 x 151936: 47.5 us, 6.57 TB/s), with five by the
+// products too (58 us). A lane copies its own 16 codes of 4 channels per step into a ring of
+// its warp (cp.async, I8_FS steps deep, 144 KB in flight per SM) and reads them back itself,
 // so that neither the products nor the sums over lanes stop the copies and no thread waits
-// for another. Loads into registers instead (8 per lane in flight) took 25 us for 1 x 2048 x
-// 65536 and 71 us for 5 x 2048 x 151936, twice as many of them 32 and 91 us.
+// for another. Loads into registers instead (8 per lane in flight) took 71 us for five rows,
+// twice as many of them 91 us.
 constexpr int I8_FR = 4;    // channels per step
-constexpr int I8_FS = 6;    // steps in the ring
+constexpr int I8_FS = 4;    // steps in the ring
 constexpr int I8_FRING = I8_FS * I8_FR * I8_GK;   // bytes per warp
 
 YN_DEV void i8_copy16(uint32_t dst, const void* src, int bytes) {   // bytes past `bytes` become 0
@@ -253,7 +254,7 @@ YN_DEV void i8_copy16(uint32_t dst, const void* src, int bytes) {   // bytes pas
 }
 
 template <int T>
-__global__ void __launch_bounds__(I8_GT, 2) k_i8_few(int dt, const void* x, long long ldx, int K, int KP, const I8Mat w,
+__global__ void __launch_bounds__(I8_GT, 3) k_i8_few(int dt, const void* x, long long ldx, int K, int KP, const I8Mat w,
                                                      int N, int odt, void* y, long long ldy) {
   extern __shared__ __align__(16) int8_t few_smem[];   // rings, then the rows' codes
   __shared__ float sx[T];
@@ -309,7 +310,7 @@ __global__ void __launch_bounds__(I8_GT, 2) k_i8_few(int dt, const void* x, long
       }
       copy();   // into the slot read one step ago
     }
-    // every lane gets all sums; lane r * T + t (for T = 8 all 32) writes one
+    // every lane gets all sums; lane r * T + t writes one
     float out = 0.0f;
 #pragma unroll
     for (int r = 0; r < I8_FR; ++r)
@@ -616,7 +617,9 @@ I8Mat mat_of(const yn_i8_mat& w) {
 }
 
 constexpr int I8_MAX_K = 131072;   // 127^2 * 131072 < 2^31
-constexpr int I8_FEW = 8;          // rows of a product on dp4a
+// Rows of a product on dp4a. Six rows of 2048 x 151936 take 72 us so, and 66 us on the tensor
+// cores with their codes made first.
+constexpr int I8_FEW = 5;
 
 int check_mat(const yn_i8_mat& w, const char* what) {
   const std::string n(what);
@@ -640,7 +643,7 @@ int launch_few(int dt, const void* x, long long ldx, int K, const I8Mat& w, int 
   const size_t smem = (size_t)T * KP + I8_GW * I8_FRING;
   const int rc = host_set_smem(reinterpret_cast<const void*>(k_i8_few<T>), 96 * 1024 + I8_GW * I8_FRING);
   if (rc) return rc;
-  const int grid = std::min((N + I8_FR * I8_GW - 1) / (I8_FR * I8_GW), 2 * sms);
+  const int grid = std::min((N + I8_FR * I8_GW - 1) / (I8_FR * I8_GW), 3 * sms);
   k_i8_few<T><<<grid, I8_GT, smem, st>>>(dt, x, ldx, K, KP, w, N, odt, y, ldy);
   const cudaError_t e = cudaGetLastError();
   return e == cudaSuccess ? YN_OK : host_fail(YN_E_CUDA, std::string("8-bit product: ") + cudaGetErrorString(e));
@@ -732,9 +735,6 @@ extern "C" int yn_i8_linear(const yn_i8_mat* w, const void* x, int32_t dtype, in
       YN_FEW(3);
       YN_FEW(4);
       YN_FEW(5);
-      YN_FEW(6);
-      YN_FEW(7);
-      YN_FEW(8);
     }
 #undef YN_FEW
   }
