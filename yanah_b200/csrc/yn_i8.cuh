@@ -288,8 +288,10 @@ struct I8Cfg {
   static constexpr int STAGE = I8_A_BYTES + NB / 2 * 128;
   static constexpr int FIT = (224 * 1024) / STAGE;
   static constexpr int S = FIT < 10 ? FIT : 10;        // stages in flight
-  static constexpr int SMEM = 1024 + S * STAGE + (2 * S + 4) * 8 + 16;
-  static_assert(NB % 32 == 0 && NB <= 256, "two accumulators of NB columns have to fit TMEM");
+  static constexpr int ACC = 512 / NB < 4 ? 512 / NB : 4;   // accumulators of NB columns in TMEM
+  static constexpr int PARTS = (NB + 4 * I8_EPW - 1) / (4 * I8_EPW);   // 16-column pieces of an epilogue warp
+  static constexpr int SMEM = 1024 + S * STAGE + (2 * S + 2 * ACC) * 8 + 16;
+  static_assert(NB % 32 == 0 && NB <= 256, "two accumulators have to fit TMEM");
 };
 
 // SiLU(g) * u in fp32.
@@ -297,7 +299,7 @@ YN_DEV float i8_swiglu(float g, float u) { return __fdividef(g, 1.0f + __expf(-g
 
 // Warp-specialised and persistent: in both blocks a loader warp fills a ring of stages by
 // TMA and epilogue warps drain the accumulators; the first block's MMA warp multiplies for
-// both, into one of two accumulators while the other is drained.
+// both, into one of the accumulators while the others are drained.
 // full[s] (first block): the bytes of both blocks' stage s; empty[s] (each block): its MMAs
 // are done; acc_full[b] (each block); acc_empty[b] (first block): every epilogue warp of both.
 template <typename O, bool UP, int NB>
@@ -309,8 +311,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(I8_THREADS, 1)
   uint64_t* full = reinterpret_cast<uint64_t*>(smem + F::S * F::STAGE);
   uint64_t* empty = full + F::S;
   uint64_t* acc_full = empty + F::S;
-  uint64_t* acc_empty = acc_full + 2;
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(acc_empty + 2);
+  uint64_t* acc_empty = acc_full + F::ACC;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(acc_empty + F::ACC);
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int rank = (int)i8_rank();
   int* err = &g_i8_err;
@@ -325,7 +327,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(I8_THREADS, 1)
       mbar_init(&full[s], 1);
       mbar_init(&empty[s], 1);
     }
-    for (int b = 0; b < 2; ++b) {
+    for (int b = 0; b < F::ACC; ++b) {
       mbar_init(&acc_full[b], 1);
       mbar_init(&acc_empty[b], 2 * I8_EPW);
     }
@@ -343,7 +345,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(I8_THREADS, 1)
   bool ok = true;
   // A list's tiles go unit by unit through a chunk, so that neighbours share the rows; a
   // single matrix's go chunk by chunk through its channels, so that they share the weights.
-  // Every role looks its next tile up while it works on the current one.
+  // Every role looks its tiles up two ahead.
   struct Tile {
     I8Chunk c;
     int u0;
@@ -357,27 +359,52 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(I8_THREADS, 1)
     const int u = ti / n_chunks, c = ti - u * n_chunks;
     return Tile{I8Chunk{0, c * NB, min(NB, a.rows - c * NB)}, TILE * u + TILE / 2 * rank};
   };
-  Tile next = tile(t0);
+  Tile next = tile(t0), after = tile(t0 + step);
 
   if (warp < I8_EPW) {
-    const int q = warp & 3, part = warp >> 2;
-    long long j = 0;
+    const int q = warp & 3, part = warp >> 2, r_in = UP ? 16 * q + (lane & 15) : 32 * q + lane;
+    // A tile's scales are loaded while the tile before it is drained, its chunk one earlier still:
+    // under a saturated memory each such load takes longer than a short tile.
+    struct Scales {
+      float sw, su, sx[F::PARTS];
+    };
+    auto scales = [&](const Tile& t) -> Scales {
+      Scales o;
+      const int r = t.u0 + r_in;
+      const bool in = r < a.channels && t.c.n > 0;
+      o.sw = in ? a.sw[t.c.e * a.sw_stride + r] : 0.0f;
+      o.su = UP && in ? a.sw_up[t.c.e * a.sw_up_stride + r] : 0.0f;
+#pragma unroll
+      for (int i = 0; i < F::PARTS; ++i) {
+        const int col = 16 * part + 4 * I8_EPW * i + lane;
+        o.sx[i] = lane < 16 && col < t.c.n ? a.sx[t.c.p0 + col] : 0.0f;
+      }
+      return o;
+    };
+    Scales sc = scales(next);
+    int j = 0;
     for (int ti = t0; ti < n_tiles; ti += step, ++j) {
       const I8Chunk c = next.c;
-      const int u0 = next.u0;
-      next = tile(ti + step);
-      const int b = (int)(j & 1), r = UP ? u0 + 16 * q + (lane & 15) : u0 + 32 * q + lane;
+      const int u0 = next.u0, b = j % F::ACC, r = u0 + r_in;
+      const float sw = sc.sw, su = sc.su;
+      float sxs[F::PARTS];
+#pragma unroll
+      for (int i = 0; i < F::PARTS; ++i) sxs[i] = sc.sx[i];
+      next = after;
+      after = tile(ti + 2 * step);
+      sc = scales(next);
       const bool in = r < a.channels;
-      const float sw = in ? a.sw[c.e * a.sw_stride + r] : 0.0f;
-      const float su = UP && in ? a.sw_up[c.e * a.sw_up_stride + r] : 0.0f;
-      ok = i8_wait(&acc_full[b], (uint32_t)(j >> 1) & 1, err);
+      ok = i8_wait(&acc_full[b], (uint32_t)(j / F::ACC) & 1, err);
       if (!ok) break;
       tc_fence_after();
       const uint32_t base = tmem + (uint32_t)(b * NB) + ((uint32_t)(32 * q) << 16);
-      for (int c0 = 16 * part; c0 < c.n; c0 += 4 * I8_EPW) {
+#pragma unroll
+      for (int i = 0; i < F::PARTS; ++i) {
+        const int c0 = 16 * part + 4 * I8_EPW * i;
+        if (c0 >= c.n) break;
         const int left = c.n - c0;
         const long long row = c.p0 + c0;
-        const float sx = lane < min(16, left) ? a.sx[row + lane] : 0.0f;
+        const float sx = sxs[i];
         int v[16];
         i8_ld16(base + (uint32_t)c0, v);
         if (UP) {
@@ -425,12 +452,14 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(I8_THREADS, 1)
       if (lane == 0) i8_arrive_at(i8_leader(&acc_empty[b]));
     }
   } else if (warp == I8_MW) {
-    long long g = 0, j = 0;
+    long long g = 0;
+    int j = 0;
     for (int ti = t0; ti < n_tiles && ok && rank == 0; ti += step, ++j) {
       const I8Chunk c = next.c;
-      next = tile(ti + step);
-      const int b = (int)(j & 1);
-      if (j >= 2) ok = i8_wait(&acc_empty[b], (uint32_t)((j >> 1) - 1) & 1, err);
+      next = after;
+      after = tile(ti + 2 * step);
+      const int b = j % F::ACC;
+      if (j >= F::ACC) ok = i8_wait(&acc_empty[b], (uint32_t)(j / F::ACC - 1) & 1, err);
       if (!ok) break;
       tc_fence_after();
       const uint32_t idesc = i8_idesc((c.n + 31) & ~31), dcol = tmem + (uint32_t)(b * NB);
@@ -451,13 +480,14 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(I8_THREADS, 1)
       }
     }
     // the last commits must land before TMEM is released (bounded)
-    if (ok && j > 0) (void)i8_wait(&acc_full[(j - 1) & 1], (uint32_t)((j - 1) >> 1) & 1, err);
+    if (ok && j > 0) (void)i8_wait(&acc_full[(j - 1) % F::ACC], (uint32_t)((j - 1) / F::ACC) & 1, err);
   } else {
     long long g = 0;
     for (int ti = t0; ti < n_tiles && ok; ti += step) {
       const I8Chunk c = next.c;
       const int u0 = next.u0;
-      next = tile(ti + step);
+      next = after;
+      after = tile(ti + 2 * step);
       const int half = ((c.n + 31) & ~31) >> 1, row = c.p0 + rank * half;   // this block's half of the MMA's rows
       const int bi = half <= 16 ? 0 : half <= 32 ? 1 : half <= 64 ? 2 : 3;
       const uint32_t bytes = 2u * (I8_A_BYTES + (16u << bi) * 128u);
