@@ -287,9 +287,11 @@ template <int NB>
 struct I8Cfg {
   static constexpr int STAGE = I8_A_BYTES + NB / 2 * 128;
   static constexpr int FIT = (224 * 1024) / STAGE;
-  static constexpr int S = FIT < 10 ? FIT : 10;        // stages in flight
+  static constexpr int S = FIT < 8 ? FIT : 8;          // stages in flight: with 8 of 18 KB HBM is as fast as it gets
   static constexpr int ACC = 512 / NB < 4 ? 512 / NB : 4;   // accumulators of NB columns in TMEM
-  static constexpr int PARTS = (NB + 4 * I8_EPW - 1) / (4 * I8_EPW);   // 16-column pieces of an epilogue warp
+  static constexpr int GROUPS = NB <= 64 ? ACC : 1;         // groups of epilogue warps, a tile each
+  static constexpr int SPLIT = I8_EPW / 4 / GROUPS;         // warps of a group on the same 32 lanes
+  static constexpr int PIECES = NB / (16 * SPLIT);          // 16-column pieces of such a warp
   static constexpr int SMEM = 1024 + S * STAGE + (2 * S + 2 * ACC) * 8 + 16;
   static_assert(NB % 32 == 0 && NB <= 256, "two accumulators have to fit TMEM");
 };
@@ -301,7 +303,7 @@ YN_DEV float i8_swiglu(float g, float u) { return __fdividef(g, 1.0f + __expf(-g
 // TMA and epilogue warps drain the accumulators; the first block's MMA warp multiplies for
 // both, into one of the accumulators while the others are drained.
 // full[s] (first block): the bytes of both blocks' stage s; empty[s] (each block): its MMAs
-// are done; acc_full[b] (each block); acc_empty[b] (first block): every epilogue warp of both.
+// are done; acc_full[b] (each block); acc_empty[b] (first block): the accumulator's epilogue warps of both.
 template <typename O, bool UP, int NB>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(I8_THREADS, 1)
     k_i8_gemm(const I8Gemm a, const __grid_constant__ I8Maps maps) {
@@ -329,7 +331,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(I8_THREADS, 1)
     }
     for (int b = 0; b < F::ACC; ++b) {
       mbar_init(&acc_full[b], 1);
-      mbar_init(&acc_empty[b], 2 * I8_EPW);
+      mbar_init(&acc_empty[b], 2 * I8_EPW / F::GROUPS);
     }
     fence_mbar_init();
   }
@@ -362,11 +364,15 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(I8_THREADS, 1)
   Tile next = tile(t0), after = tile(t0 + step);
 
   if (warp < I8_EPW) {
-    const int q = warp & 3, part = warp >> 2, r_in = UP ? 16 * q + (lane & 15) : 32 * q + lane;
-    // A tile's scales are loaded while the tile before it is drained, its chunk one earlier still:
-    // under a saturated memory each such load takes longer than a short tile.
+    // Tiles of few rows are short (4 stages of K 512 come in 1.6 us) and draining one is a chain of
+    // TMEM loads, exchanges and stores that takes longer: every accumulator has warps of its own then,
+    // which take every 4th tile (2048 x 512 experts, 166 MB: 49 -> 41 us). All warps on each tile
+    // is better for long ones (4096 x 2048 x 16384: 115 us, 121 us in groups). A tile's scales are
+    // loaded while the group's tile before it is drained.
+    const int q = warp & 3, group = (warp >> 2) % F::GROUPS, part = (warp >> 2) / F::GROUPS;
+    const int r_in = UP ? 16 * q + (lane & 15) : 32 * q + lane, ahead = F::GROUPS * step;
     struct Scales {
-      float sw, su, sx[F::PARTS];
+      float sw, su, sx[F::PIECES];
     };
     auto scales = [&](const Tile& t) -> Scales {
       Scales o;
@@ -375,23 +381,25 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(I8_THREADS, 1)
       o.sw = in ? a.sw[t.c.e * a.sw_stride + r] : 0.0f;
       o.su = UP && in ? a.sw_up[t.c.e * a.sw_up_stride + r] : 0.0f;
 #pragma unroll
-      for (int i = 0; i < F::PARTS; ++i) {
-        const int col = 16 * part + 4 * I8_EPW * i + lane;
+      for (int i = 0; i < F::PIECES; ++i) {
+        const int col = 16 * (part + F::SPLIT * i) + lane;
         o.sx[i] = lane < 16 && col < t.c.n ? a.sx[t.c.p0 + col] : 0.0f;
       }
       return o;
     };
+    next = tile(t0 + group * step);
+    after = tile(t0 + group * step + ahead);
     Scales sc = scales(next);
-    int j = 0;
-    for (int ti = t0; ti < n_tiles; ti += step, ++j) {
+    int j = group;
+    for (int ti = t0 + group * step; ti < n_tiles; ti += ahead, j += F::GROUPS) {
       const I8Chunk c = next.c;
-      const int u0 = next.u0, b = j % F::ACC, r = u0 + r_in;
+      const int u0 = next.u0, r = u0 + r_in, b = j % F::ACC;
       const float sw = sc.sw, su = sc.su;
-      float sxs[F::PARTS];
+      float sxs[F::PIECES];
 #pragma unroll
-      for (int i = 0; i < F::PARTS; ++i) sxs[i] = sc.sx[i];
+      for (int i = 0; i < F::PIECES; ++i) sxs[i] = sc.sx[i];
       next = after;
-      after = tile(ti + 2 * step);
+      after = tile(ti + 2 * ahead);
       sc = scales(next);
       const bool in = r < a.channels;
       ok = i8_wait(&acc_full[b], (uint32_t)(j / F::ACC) & 1, err);
@@ -399,8 +407,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(I8_THREADS, 1)
       tc_fence_after();
       const uint32_t base = tmem + (uint32_t)(b * NB) + ((uint32_t)(32 * q) << 16);
 #pragma unroll
-      for (int i = 0; i < F::PARTS; ++i) {
-        const int c0 = 16 * part + 4 * I8_EPW * i;
+      for (int i = 0; i < F::PIECES; ++i) {
+        const int c0 = 16 * (part + F::SPLIT * i);
         if (c0 >= c.n) break;
         const int left = c.n - c0;
         const long long row = c.p0 + c0;
