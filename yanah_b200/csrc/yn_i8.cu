@@ -1,6 +1,7 @@
 // Rows in 8-bit integers, the products of few rows (dp4a), the grouping and the
 // joining of the experts' products, and the C ABI of all of it. The tensor-core
 // product of many rows is in yn_i8.cuh.
+#include <cooperative_groups.h>
 #include <cuda.h>
 #include <cuda_runtime.h>
 
@@ -427,36 +428,52 @@ __global__ void __launch_bounds__(I8_GT) k_i8_down_few(const float* act, int I, 
 
 // --------------------------------------------- many rows: grouping, joining
 constexpr int I8_PLAN_T = 1024;
+constexpr int I8_PLAN_B = 8;     // blocks, one cluster
+constexpr int I8_PLAN_Q = 4;     // pairs that a thread has in registers at a time
 constexpr int I8_MAX_E = 1024;
 
 // Pairs of one expert made contiguous and cut into chunks of at most NB rows. Which place
 // a pair takes inside its expert does not change its product. pair_of: (row, column) ->
-// pair, -1 where there is no expert. n_out[0] = chunks, [1] = pairs.
-__global__ void __launch_bounds__(I8_PLAN_T) k_i8_plan(const int32_t* ids, int P, int E, int NB, int32_t* pair_of,
-                                                       I8Chunk* chunks, int* n_out) {
-  __shared__ int cnt[I8_MAX_E], first[I8_MAX_E];
+// pair, -1 where there is no expert. n_out[0] = chunks, [1] = pairs. The blocks of a
+// cluster count a part of the pairs each, read one another's counts through distributed
+// shared memory, and all make the same scan over the experts (16384 pairs: one block alone
+// took 11 us, most of it atomics on popular experts).
+__global__ void __cluster_dims__(I8_PLAN_B, 1, 1) __launch_bounds__(I8_PLAN_T)
+    k_i8_plan(const int32_t* ids, int P, int E, int NB, int32_t* pair_of, I8Chunk* chunks, int* n_out) {
+  namespace cg = cooperative_groups;
+  cg::cluster_group cluster = cg::this_cluster();
+  __shared__ int cnt[I8_MAX_E], base_of[I8_MAX_E];
   __shared__ int2 ws[I8_PLAN_T / 32];
-  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  for (int e = tid; e < I8_MAX_E; e += I8_PLAN_T) cnt[e] = 0;
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, me = (int)cluster.block_rank();
+  cnt[tid] = 0;
   __syncthreads();
-  // 8 pairs per thread at a time, their loads together
-  for (int i0 = tid; i0 < P; i0 += 8 * I8_PLAN_T) {
-    int e[8];
+  // part of the pairs: rounds of I8_PLAN_B * I8_PLAN_T * Q
+  const int round = I8_PLAN_B * I8_PLAN_T * I8_PLAN_Q, rounds = (P + round - 1) / round;
+  for (int k = 0; k < rounds; ++k) {
+    const int i0 = k * round + me * (I8_PLAN_T * I8_PLAN_Q) + tid;
+    int e[I8_PLAN_Q];
 #pragma unroll
-    for (int q = 0; q < 8; ++q) e[q] = i0 + q * I8_PLAN_T < P ? ids[i0 + q * I8_PLAN_T] : -1;
+    for (int q = 0; q < I8_PLAN_Q; ++q) e[q] = i0 + q * I8_PLAN_T < P ? ids[i0 + q * I8_PLAN_T] : -1;
 #pragma unroll
-    for (int q = 0; q < 8; ++q) {
+    for (int q = 0; q < I8_PLAN_Q; ++q) {
       const int i = i0 + q * I8_PLAN_T;
       if (i >= P) break;
-      if (e[q] >= 0 && e[q] < E) pair_of[i] = atomicAdd(&cnt[e[q]], 1);
+      if (e[q] >= 0 && e[q] < E) pair_of[i] = atomicAdd(&cnt[e[q]], 1);   // place inside this block's share
       else {
         pair_of[i] = -1;
         if (e[q] != -1) raise_error(&g_i8_err, YN_ERR_BAD_EXPERT);
       }
     }
   }
-  __syncthreads();
-  const int c = tid < E ? cnt[tid] : 0, nc = (c + NB - 1) / NB;
+  cluster.sync();
+  int c = 0, before = 0;   // expert tid: pairs of all blocks, and of those before this one
+#pragma unroll
+  for (int b = 0; b < I8_PLAN_B; ++b) {
+    const int v = *cluster.map_shared_rank(&cnt[tid], b);
+    c += v;
+    before += b < me ? v : 0;
+  }
+  const int nc = (c + NB - 1) / NB;
   int2 inc = make_int2(c, nc);
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
@@ -465,68 +482,104 @@ __global__ void __launch_bounds__(I8_PLAN_T) k_i8_plan(const int32_t* ids, int P
   }
   if (lane == 31) ws[warp] = inc;
   __syncthreads();
-  int2 base = make_int2(0, 0), all = make_int2(0, 0);
-  for (int w = 0; w < I8_PLAN_T / 32; ++w) {
-    const int2 q = ws[w];
-    if (w < warp) { base.x += q.x; base.y += q.y; }
-    all.x += q.x;
-    all.y += q.y;
-  }
+  // the warps before: every warp sums its own
+  int2 v = ws[lane];
+  int2 base = lane < warp ? v : make_int2(0, 0);
+  base.x = __reduce_add_sync(0xffffffffu, base.x);
+  base.y = __reduce_add_sync(0xffffffffu, base.y);
   const int start = base.x + inc.x - c, at = base.y + inc.y - nc;
-  if (tid < E) {
-    first[tid] = start;
+  base_of[tid] = start + before;
+  if (me == tid % I8_PLAN_B)   // the blocks share the writing of the list
     for (int i = 0; i < nc; ++i) chunks[at + i] = I8Chunk{tid, start + i * NB, min(NB, c - i * NB)};
-  }
-  if (tid == 0) {
-    n_out[0] = all.y;
-    n_out[1] = all.x;
+  if (me == 0 && tid == I8_PLAN_T - 1) {
+    n_out[0] = at + nc;
+    n_out[1] = start + c;
   }
   __syncthreads();
-  for (int i0 = tid; i0 < P; i0 += 8 * I8_PLAN_T) {
-    int e[8], at[8];
+  for (int k = 0; k < rounds; ++k) {
+    const int i0 = k * round + me * (I8_PLAN_T * I8_PLAN_Q) + tid;
+    int e[I8_PLAN_Q], place[I8_PLAN_Q];
 #pragma unroll
-    for (int q = 0; q < 8; ++q) {
+    for (int q = 0; q < I8_PLAN_Q; ++q) {
       const int i = i0 + q * I8_PLAN_T;
-      at[q] = i < P ? pair_of[i] : -1;
+      place[q] = i < P ? pair_of[i] : -1;
       e[q] = i < P ? ids[i] : 0;
     }
 #pragma unroll
-    for (int q = 0; q < 8; ++q)
-      if (at[q] >= 0) pair_of[i0 + q * I8_PLAN_T] = at[q] + first[e[q]];
+    for (int q = 0; q < I8_PLAN_Q; ++q)
+      if (place[q] >= 0) pair_of[i0 + q * I8_PLAN_T] = place[q] + base_of[e[q]];
   }
+  cluster.sync();   // no block leaves while its counts are read
 }
 
 // out[t] = residual[t] + sum_j w_j y[pair_of[t][j]] in fp32, columns in order, rounded once.
-template <typename O, typename Y>
-__global__ void k_i8_combine(const Y* y, long long ldy, const int32_t* pair_of, const float* w, int k, int H,
-                             const void* res, long long ldr, void* out, long long ldo) {
-  const size_t t = blockIdx.y;
-  const int h = 4 * (blockIdx.x * blockDim.x + threadIdx.x);
-  if (h >= H) return;
-  float acc[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-  for (int j = 0; j < k; ++j) {
-    const int p = pair_of[t * k + j];
-    if (p < 0) continue;
-    const float wj = w[t * k + j];
-    const Y* row = y + (size_t)p * ldy + h;   // rows of y are padded to whole vectors
-    float v[4];
-    if constexpr (sizeof(Y) == 4) {
-      const float4 q = *reinterpret_cast<const float4*>(row);
-      v[0] = q.x; v[1] = q.y; v[2] = q.z; v[3] = q.w;
-    } else {
-      const uint2 q = *reinterpret_cast<const uint2*>(row);
-      v[0] = bf16_to_f32((uint16_t)(q.x & 0xFFFFu)); v[1] = bf16_to_f32((uint16_t)(q.x >> 16));
-      v[2] = bf16_to_f32((uint16_t)(q.y & 0xFFFFu)); v[3] = bf16_to_f32((uint16_t)(q.y >> 16));
+// One row of the batch per blockIdx.x, 8 outputs per thread; VEC: residual and out in 16-byte pieces.
+template <typename O, typename Y, bool VEC>
+__global__ void __launch_bounds__(128) k_i8_combine(const Y* y, long long ldy, const int32_t* pair_of, const float* w, int k,
+                                                    int H, const void* res, long long ldr, void* out, long long ldo) {
+  const size_t t = blockIdx.x;
+  const int lane = threadIdx.x & 31, h = 8 * (blockIdx.y * 128 + threadIdx.x);
+  const int p_mine = lane < k ? pair_of[t * k + lane] : -1;   // lane j: the row's pair j
+  const float w_mine = lane < k ? w[t * k + lane] : 0.0f;
+  float acc[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) acc[i] = 0.0f;
+  const bool on = h < H;
+  for (int j0 = 0; j0 < k; j0 += 4) {
+    I8Raw<Y> r[4];
+    float wj[4];
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {   // 4 rows of y in flight
+      const int p = __shfl_sync(0xffffffffu, p_mine, (j0 + q) & 31);
+      wj[q] = __shfl_sync(0xffffffffu, w_mine, (j0 + q) & 31);
+      if (j0 + q >= k || p < 0) wj[q] = 0.0f;
+      if (on && j0 + q < k && p >= 0) r[q].load(y, (size_t)p * ldy + h);   // rows of y are padded to whole pieces
+      else r[q] = I8Raw<Y>{};
     }
 #pragma unroll
-    for (int i = 0; i < 4; ++i) acc[i] = fmaf(wj, v[i], acc[i]);
+    for (int q = 0; q < 4; ++q) {
+      float v[8];
+      r[q].get(v);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) acc[i] = fmaf(wj[q], v[i], acc[i]);
+    }
+  }
+  if (!on) return;
+  if (VEC && h + 8 <= H) {
+    if (res) {
+      I8Raw<O> r;
+      float v[8];
+      r.load(res, t * ldr + h);
+      r.get(v);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) acc[i] += v[i];
+    }
+    uint4* o = reinterpret_cast<uint4*>(reinterpret_cast<O*>(out) + t * ldo + h);
+    if constexpr (sizeof(O) == 4) {
+      o[0] = make_uint4(__float_as_uint(acc[0]), __float_as_uint(acc[1]), __float_as_uint(acc[2]), __float_as_uint(acc[3]));
+      o[1] = make_uint4(__float_as_uint(acc[4]), __float_as_uint(acc[5]), __float_as_uint(acc[6]), __float_as_uint(acc[7]));
+    } else {
+      o[0] = make_uint4(i8_pack2<O>(acc[0], acc[1]), i8_pack2<O>(acc[2], acc[3]), i8_pack2<O>(acc[4], acc[5]),
+                        i8_pack2<O>(acc[6], acc[7]));
+    }
+    return;
   }
 #pragma unroll
-  for (int i = 0; i < 4; ++i)
+  for (int i = 0; i < 8; ++i)
     if (h + i < H) {
       const float r = res ? I8In<O>::load(res, t * ldr + h + i) : 0.0f;
       reinterpret_cast<O*>(out)[t * ldo + h + i] = i8_out<O>(r + acc[i]);
     }
+}
+template <typename O, typename Y>
+void launch_combine(const void* y, long long ldy, const int32_t* pair_of, const float* w, int k, int H, long long rows,
+                    const void* res, long long ldr, void* out, long long ldo, cudaStream_t st) {
+  const bool vec = reinterpret_cast<uintptr_t>(out) % 16 == 0 && (ldo * sizeof(O)) % 16 == 0 &&
+                   reinterpret_cast<uintptr_t>(res) % 16 == 0 && (ldr * sizeof(O)) % 16 == 0;
+  const dim3 g((unsigned)rows, (H + 1023) / 1024);
+  const Y* yy = reinterpret_cast<const Y*>(y);
+  if (vec) k_i8_combine<O, Y, true><<<g, 128, 0, st>>>(yy, ldy, pair_of, w, k, H, res, ldr, out, ldo);
+  else k_i8_combine<O, Y, false><<<g, 128, 0, st>>>(yy, ldy, pair_of, w, k, H, res, ldr, out, ldo);
 }
 
 // ---------------------------------------------------------------- host side
@@ -827,7 +880,7 @@ extern "C" int yn_i8_experts(const yn_i8_mat* gate, const yn_i8_mat* up, const y
   int8_t* acodes = reinterpret_cast<int8_t*>(b + L.acodes);
   float* sa = reinterpret_cast<float*>(b + L.sa);
   void* y = b + L.y;
-  k_i8_plan<<<1, I8_PLAN_T, 0, st>>>(ids, P, E, L.nb, pair_of, chunks, n_out);
+  k_i8_plan<<<I8_PLAN_B, I8_PLAN_T, 0, st>>>(ids, P, E, L.nb, pair_of, chunks, n_out);
   if ((rc = launch_quant(dtype, x, x_stride, rows, H, nullptr, pair_of, top_k, codes, L.ldc, sx, st))) return rc;
   const long long max_chunks = E + P / L.nb + 1;
   I8Maps maps{};
@@ -866,16 +919,11 @@ extern "C" int yn_i8_experts(const yn_i8_mat* gate, const yn_i8_mat* up, const y
   d.pairs = true;
   const bool yb = dtype == YN_BF16;
   if ((rc = launch_gemm_out(yb ? YN_BF16 : YN_F32, L.nb, d, md2, td, st))) return rc;
-  const dim3 cg((H + 4 * 128 - 1) / (4 * 128), (unsigned)rows);
   if (yb)
-    k_i8_combine<__nv_bfloat16, uint16_t><<<cg, 128, 0, st>>>(reinterpret_cast<const uint16_t*>(y), L.ldy, pair_of, weights,
-                                                              top_k, H, residual, res_stride, out, out_stride);
+    launch_combine<__nv_bfloat16, __nv_bfloat16>(y, L.ldy, pair_of, weights, top_k, H, rows, residual, res_stride, out, out_stride, st);
   else if (dtype == YN_F16)
-    k_i8_combine<__half, float><<<cg, 128, 0, st>>>(reinterpret_cast<const float*>(y), L.ldy, pair_of, weights, top_k, H,
-                                                    residual, res_stride, out, out_stride);
-  else
-    k_i8_combine<float, float><<<cg, 128, 0, st>>>(reinterpret_cast<const float*>(y), L.ldy, pair_of, weights, top_k, H,
-                                                   residual, res_stride, out, out_stride);
+    launch_combine<__half, float>(y, L.ldy, pair_of, weights, top_k, H, rows, residual, res_stride, out, out_stride, st);
+  else launch_combine<float, float>(y, L.ldy, pair_of, weights, top_k, H, rows, residual, res_stride, out, out_stride, st);
   const cudaError_t e = cudaGetLastError();
   return e == cudaSuccess ? YN_OK : host_fail(YN_E_CUDA, std::string("experts: ") + cudaGetErrorString(e));
 }
