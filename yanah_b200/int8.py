@@ -21,7 +21,7 @@ from typing import NamedTuple, Optional
 import torch
 
 from . import _lib
-from .launch import DTYPES, check_floats, check_like, elsewhere, raw_stream, row_stride, rows_of, run_there
+from .launch import DTYPES, check_floats, check_like, elsewhere, raw_stream, rows_of, run_there
 
 
 class Int8Matrix(NamedTuple):
@@ -35,66 +35,63 @@ class Int8Matrix(NamedTuple):
 def quantize_rows(x: torch.Tensor, stream: Optional[torch.cuda.Stream] = None) -> Int8Matrix:
     """Rows (..., K) as 8-bit codes with one scale each: activations per token, weights
     per output channel. A row with an infinity or a NaN gets a NaN scale."""
-    check_floats(x, "x")
-    if elsewhere(x.device, stream):
+    dtype, dev = check_floats(x, "x"), x.get_device()
+    if elsewhere(dev, stream):
         return run_there(lambda: quantize_rows(x), x.device, stream, (x,))
     if x.dim() < 1 or x.shape[-1] < 1:
         raise ValueError("x must have at least one column")
-    k = x.shape[-1]
-    flat = rows_of(x.reshape(-1, k), "x")
-    rows = flat.shape[0]
-    codes = torch.empty((rows, (k + 15) // 16 * 16), dtype=torch.int8, device=x.device)
-    scales = torch.empty((rows,), dtype=torch.float32, device=x.device)
-    _lib.check(_lib.lib().yn_i8_quant_rows(flat.data_ptr(), DTYPES[x.dtype], row_stride(flat), rows, k, codes.data_ptr(),
-                                           codes.stride(0), scales.data_ptr(),
-                                           raw_stream(x.device)))
-    lead = x.shape[:-1]
-    return Int8Matrix(codes.view(*lead, codes.shape[-1])[..., :k], scales.view(lead))
+    lead, k = x.shape[:-1], x.shape[-1]
+    flat, rows, k, stride = rows_of(x.reshape(-1, k), "x")
+    pitch = (k + 15) // 16 * 16
+    codes = x.new_empty((rows, pitch), dtype=torch.int8)
+    scales = x.new_empty((rows,), dtype=torch.float32)
+    _lib.check(_lib.lib().yn_i8_quant_rows(flat.data_ptr(), dtype, stride, rows, k, codes.data_ptr(), pitch,
+                                           scales.data_ptr(), raw_stream(dev)))
+    return Int8Matrix(codes.view(*lead, pitch)[..., :k], scales.view(lead))
 
 
-def _mat(w: Int8Matrix, like: torch.Tensor, what: str) -> _lib.I8Mat:
+def _mat(w: Int8Matrix, index: int, what: str) -> _lib.I8Mat:
     codes, scales = w
-    shape, strides, device = codes.shape, codes.stride(), like.device
+    shape, strides = codes.shape, codes.stride()
     if codes.dtype is not torch.int8 or scales.dtype is not torch.float32:
         raise TypeError(f"{what} must have int8 codes and float32 scales")
     if len(shape) not in (2, 3) or scales.shape != shape[:-1]:
         raise ValueError(f"{what}: codes (N, K) or (E, N, K) with scales (N) or (E, N)")
-    if codes.device != device or scales.device != device:
-        raise ValueError(f"{what} is not on {device}")
+    if codes.get_device() != index or scales.get_device() != index:
+        raise ValueError(f"{what} is not on cuda:{index}")
     n, k = shape[-2:]
-    e = shape[0] if len(shape) == 3 else 1
-    if (k > 1 and strides[-1] != 1) or (n > 1 and scales.stride(-1) != 1):
+    s_strides = scales.stride()
+    if (k > 1 and strides[-1] != 1) or (n > 1 and s_strides[-1] != 1):
         raise ValueError(f"{what}: a row's codes and a matrix's scales must be adjacent")
     rs = strides[-2] if n > 1 else (k + 15) // 16 * 16
-    many = e > 1
-    return _lib.I8Mat(codes.data_ptr(), scales.data_ptr(), rs, strides[0] if many else rs * n,
-                      scales.stride(0) if many else n, e, n, k)
+    if len(shape) == 3 and shape[0] > 1:
+        return _lib.I8Mat(codes.data_ptr(), scales.data_ptr(), rs, strides[0], s_strides[0], shape[0], n, k)
+    return _lib.I8Mat(codes.data_ptr(), scales.data_ptr(), rs, rs * n, n, shape[0] if len(shape) == 3 else 1, n, k)
 
 
 def int8_linear(x: torch.Tensor, w: Int8Matrix, out_dtype: Optional[torch.dtype] = None,
                 stream: Optional[torch.cuda.Stream] = None) -> torch.Tensor:
     """x (T, K) in fp32, bf16 or fp16 times the transpose of w (N, K): (T, N) in
     ``out_dtype`` (default: that of x), rounded once from fp32. Any number of rows."""
-    check_floats(x, "x")
-    if elsewhere(x.device, stream):
+    dtype, dev = check_floats(x, "x"), x.get_device()
+    if elsewhere(dev, stream):
         return run_there(lambda: int8_linear(x, w, out_dtype), x.device, stream, (x, *w))
-    x = rows_of(x, "x")
+    x, rows, k, stride = rows_of(x, "x")
     if w.codes.dim() != 2:
         raise ValueError("w must be one matrix (N, K)")
-    m = _mat(w, x, "w")
-    if x.shape[1] != m.cols:
-        raise ValueError(f"x has {x.shape[1]} columns, w {m.cols}")
+    m = _mat(w, dev, "w")
+    if k != m.cols:
+        raise ValueError(f"x has {k} columns, w {m.cols}")
     out_dtype = out_dtype or x.dtype
     if out_dtype not in DTYPES:
         raise TypeError(f"out_dtype must be float32, bfloat16 or float16, not {out_dtype}")
-    rows = x.shape[0]
-    y = torch.empty((rows, m.rows), dtype=out_dtype, device=x.device)
+    n = m.rows
+    y = x.new_empty((rows, n), dtype=out_dtype)
     lib = _lib.lib()
-    nb = int(lib.yn_i8_linear_ws_bytes(rows, m.cols))
-    ws = torch.empty(nb, dtype=torch.uint8, device=x.device) if nb else None
-    _lib.check(lib.yn_i8_linear(C.byref(m), x.data_ptr(), DTYPES[x.dtype], row_stride(x), rows, y.data_ptr(),
-                                DTYPES[out_dtype], m.rows, None if ws is None else ws.data_ptr(), nb,
-                                raw_stream(x.device)))
+    nb = lib.yn_i8_linear_ws_bytes(rows, k)
+    ws = x.new_empty((nb,), dtype=torch.uint8) if nb else None
+    _lib.check(lib.yn_i8_linear(C.byref(m), x.data_ptr(), dtype, stride, rows, y.data_ptr(), DTYPES[out_dtype], n,
+                                None if ws is None else ws.data_ptr(), nb, raw_stream(dev)))
     return y
 
 
@@ -108,39 +105,38 @@ def int8_experts(x: torch.Tensor, ids: torch.Tensor, weights: torch.Tensor, gate
     reported by ``check_error``). gate, up: (E, I, H); down: (E, H, I). The activations
     are quantised per (row, expert), the sum is fp32 and rounded once to the type of x.
     ``out``: (T, H) to write, rows of adjacent elements; it may be the residual."""
-    check_floats(x, "x")
-    if elsewhere(x.device, stream):
+    dtype, dev = check_floats(x, "x"), x.get_device()
+    if elsewhere(dev, stream):
         return run_there(lambda: int8_experts(x, ids, weights, gate, up, down, residual, out=out), x.device, stream,
                          (x, ids, weights, residual, out, *gate, *up, *down))
-    x = rows_of(x, "x")
-    rows, h = x.shape
+    x, rows, h, stride = rows_of(x, "x")
     if ids.dim() != 2:
         raise ValueError("ids must be (T, k)")
     k = ids.shape[1]
-    check_like(ids, x, (rows, k), (torch.int32,), "ids")
-    check_like(weights, x, (rows, k), (torch.float32,), "weights")
-    g, u, d = _mat(gate, x, "gate"), _mat(up, x, "up"), _mat(down, x, "down")
+    check_like(ids, dev, (rows, k), (torch.int32,), "ids")
+    check_like(weights, dev, (rows, k), (torch.float32,), "weights")
+    g, u, d = _mat(gate, dev, "gate"), _mat(up, dev, "up"), _mat(down, dev, "down")
     if g.cols != h:
         raise ValueError(f"x has {h} columns, gate {g.cols}")
     ids, weights = ids.contiguous(), weights.contiguous()
+    p_res, res_stride, out_stride = None, 0, h
     if residual is not None:
-        check_like(residual, x, (rows, h), (x.dtype,), "residual")
-        residual = rows_of(residual, "residual")
+        check_like(residual, dev, (rows, h), (x.dtype,), "residual")
+        residual, _, _, res_stride = rows_of(residual, "residual")
+        p_res = residual.data_ptr()
     if out is None:
-        out = torch.empty((rows, h), dtype=x.dtype, device=x.device)
+        out = x.new_empty((rows, h))
     else:
-        check_like(out, x, (rows, h), (x.dtype,), "out")
-        if rows_of(out, "out") is not out:
+        check_like(out, dev, (rows, h), (x.dtype,), "out")
+        same, _, _, out_stride = rows_of(out, "out")
+        if same is not out:
             raise ValueError("out must have rows of adjacent elements that do not overlap")
-    lib, dt = _lib.lib(), DTYPES[x.dtype]
-    nb = int(lib.yn_i8_experts_ws_bytes(rows, k, g.n_mats, h, g.rows, dt))
-    ws = torch.empty(nb, dtype=torch.uint8, device=x.device)
-    _lib.check(lib.yn_i8_experts(C.byref(g), C.byref(u), C.byref(d), x.data_ptr(), dt, row_stride(x), rows,
-                                 ids.data_ptr(), weights.data_ptr(), k,
-                                 None if residual is None else residual.data_ptr(),
-                                 0 if residual is None else row_stride(residual), out.data_ptr(), row_stride(out),
-                                 ws.data_ptr(), nb,
-                                 raw_stream(x.device)))
+    lib = _lib.lib()
+    nb = lib.yn_i8_experts_ws_bytes(rows, k, g.n_mats, h, g.rows, dtype)
+    ws = x.new_empty((nb,), dtype=torch.uint8)
+    _lib.check(lib.yn_i8_experts(C.byref(g), C.byref(u), C.byref(d), x.data_ptr(), dtype, stride, rows, ids.data_ptr(),
+                                 weights.data_ptr(), k, p_res, res_stride, out.data_ptr(), out_stride, ws.data_ptr(), nb,
+                                 raw_stream(dev)))
     return out
 
 

@@ -7,7 +7,7 @@ have no gradients: an argument that requires one is refused while gradients are 
 """
 from __future__ import annotations
 
-from typing import Optional
+from typing import Optional, Tuple
 
 import torch
 
@@ -15,48 +15,50 @@ import torch
 DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
 
 
-def check_floats(t: torch.Tensor, what: str) -> None:
-    """A CUDA tensor of fp32, bf16 or fp16 without a gradient."""
-    if t.dtype not in DTYPES:
+# A call of a few rows takes the host longer than the device: these checks ask a tensor for
+# as little as they can (each attribute costs 0.1 to 0.3 us).
+def check_floats(t: torch.Tensor, what: str) -> int:
+    """A CUDA tensor of fp32, bf16 or fp16 without a gradient; returns the C ABI's code of its type."""
+    code = DTYPES.get(t.dtype)
+    if code is None:
         raise TypeError(f"{what} must be float32, bfloat16 or float16, not {t.dtype}")
     if not t.is_cuda:
         raise ValueError(f"{what} must be a CUDA tensor")
     if t.requires_grad and torch.is_grad_enabled():
         raise RuntimeError(f"{what} requires a gradient: this operator has none (call it under torch.no_grad())")
+    return code
 
 
-def check_like(t: torch.Tensor, like: torch.Tensor, shape: tuple, dtypes: tuple, what: str) -> None:
-    """`t` on the device of `like`, of this shape and one of these types."""
-    if tuple(t.shape) != tuple(shape):
+def check_like(t: torch.Tensor, index: int, shape: tuple, dtypes: tuple, what: str) -> None:
+    """`t` on CUDA device `index`, of this shape and one of these types."""
+    if t.shape != shape:
         raise ValueError(f"{what} must have shape {tuple(shape)}, not {tuple(t.shape)}")
     if t.dtype not in dtypes:
         raise TypeError(f"{what} must be {' or '.join(str(d) for d in dtypes)}, not {t.dtype}")
-    if t.device != like.device:
-        raise ValueError(f"{what} is on {t.device}, not on {like.device}")
+    if t.get_device() != index:
+        raise ValueError(f"{what} is on {t.device}, not on cuda:{index}")
 
 
-def rows_of(t: torch.Tensor, what: str) -> torch.Tensor:
-    """`t` as rows whose elements are adjacent and which do not overlap; copied where it is laid out otherwise."""
+def rows_of(t: torch.Tensor, what: str) -> Tuple[torch.Tensor, int, int, int]:
+    """`t` as rows whose elements are adjacent and which do not overlap (copied where it is laid out otherwise),
+    their number, length and stride."""
     if t.dim() != 2:
         raise ValueError(f"{what} must have two dimensions, not {t.dim()}")
     n, c = t.shape
-    if (c > 1 and t.stride(1) != 1) or (n > 1 and t.stride(0) < c):
-        return t.contiguous()
-    return t
+    s0, s1 = t.stride()
+    if (c > 1 and s1 != 1) or (n > 1 and s0 < c):
+        return t.contiguous(), n, c, c
+    return t, n, c, s0 if n > 1 else c
 
 
-def row_stride(t: torch.Tensor) -> int:
-    return t.stride(0) if t.shape[0] > 1 else max(t.stride(0), t.shape[1])
+def raw_stream(index: int) -> int:
+    """The current stream of CUDA device `index` as the C ABI takes it."""
+    return torch._C._cuda_getCurrentRawStream(index)
 
 
-def raw_stream(device: torch.device) -> int:
-    """The current stream of a device as the C ABI takes it."""
-    return torch._C._cuda_getCurrentRawStream(device.index)
-
-
-def elsewhere(device: torch.device, stream: Optional[torch.cuda.Stream]) -> bool:
+def elsewhere(index: int, stream: Optional[torch.cuda.Stream]) -> bool:
     """Whether a call has to leave the current device or stream."""
-    return stream is not None or device.index != torch.cuda.current_device()
+    return stream is not None or index != torch.cuda.current_device()
 
 
 def run_there(fn, device: torch.device, stream: Optional[torch.cuda.Stream], tensors):

@@ -12,7 +12,7 @@ from typing import NamedTuple, Optional
 import torch
 
 from . import _lib
-from .launch import DTYPES, check_floats, check_like, elsewhere, raw_stream, row_stride, rows_of, run_there
+from .launch import check_floats, check_like, elsewhere, raw_stream, rows_of, run_there
 
 
 class TokenLogprobs(NamedTuple):
@@ -37,29 +37,26 @@ def token_logprobs(logits: torch.Tensor, tokens: Optional[torch.Tensor] = None, 
     of -inf alone has log probabilities of -inf and entropy 0, one with a NaN has NaN
     and ranks and ids of -1. A token outside [0, V), as padded rows have, gives NaN
     and rank -1. n_top <= 64."""
-    check_floats(logits, "logits")
-    if elsewhere(logits.device, stream):
+    dtype, dev = check_floats(logits, "logits"), logits.get_device()
+    if elsewhere(dev, stream):
         return run_there(lambda: token_logprobs(logits, tokens, n_top), logits.device, stream, (logits, tokens))
-    logits = rows_of(logits, "logits")
-    rows, vocab = logits.shape
-    dev = logits.device
-    if tokens is not None:
-        check_like(tokens, logits, (rows,), (torch.int32,), "tokens")
-        tokens = tokens.contiguous()
+    logits, rows, vocab, stride = rows_of(logits, "logits")
     if vocab < 1:
         raise ValueError("logits must have at least one column")
     if not 0 <= n_top <= min(64, vocab):
         raise ValueError(f"n_top must be in [0, {min(64, vocab)}], not {n_top}")
-    entropy = torch.empty(rows, dtype=torch.float32, device=dev)
+    new, f32, i32 = logits.new_empty, torch.float32, torch.int32
+    entropy = new((rows,), dtype=f32)
     logprob = rank = top_ids = top_lp = None
+    p_tokens = p_logprob = p_rank = p_ids = p_top = None
     if tokens is not None:
-        logprob = torch.empty_like(entropy)
-        rank = torch.empty_like(tokens)
+        check_like(tokens, dev, (rows,), (i32,), "tokens")
+        tokens = tokens.contiguous()
+        logprob, rank = new((rows,), dtype=f32), new((rows,), dtype=i32)
+        p_tokens, p_logprob, p_rank = tokens.data_ptr(), logprob.data_ptr(), rank.data_ptr()
     if n_top:
-        top_ids = torch.empty((rows, n_top), dtype=torch.int32, device=dev)
-        top_lp = torch.empty((rows, n_top), dtype=torch.float32, device=dev)
-    ptr = lambda t: None if t is None else t.data_ptr()  # noqa: E731
-    _lib.check(_lib.lib().yn_token_logprobs(
-        logits.data_ptr(), DTYPES[logits.dtype], row_stride(logits), rows, vocab, ptr(tokens), n_top, ptr(logprob),
-        entropy.data_ptr(), ptr(rank), ptr(top_ids), ptr(top_lp), raw_stream(dev)))
+        top_ids, top_lp = new((rows, n_top), dtype=i32), new((rows, n_top), dtype=f32)
+        p_ids, p_top = top_ids.data_ptr(), top_lp.data_ptr()
+    _lib.check(_lib.lib().yn_token_logprobs(logits.data_ptr(), dtype, stride, rows, vocab, p_tokens, n_top, p_logprob,
+                                            entropy.data_ptr(), p_rank, p_ids, p_top, raw_stream(dev)))
     return TokenLogprobs(logprob, rank, entropy, top_ids, top_lp)

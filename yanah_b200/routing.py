@@ -19,7 +19,7 @@ from typing import NamedTuple, Optional, Tuple
 import torch
 
 from . import _lib
-from .launch import DTYPES, check_floats, check_like, elsewhere, raw_stream, row_stride, rows_of, run_there
+from .launch import check_floats, check_like, elsewhere, raw_stream, rows_of, run_there
 
 SCORES = {"softmax": 0, "sigmoid": 1}
 
@@ -60,29 +60,28 @@ def route_scored(logits: torch.Tensor, rule: RouteRule, bias: Optional[torch.Ten
     ``available`` (E) (bool or uint8) is false or its logit is -inf or NaN; rows with
     fewer than k experts left end in ids of -1 with weight 0. Any number of rows.
     ``out``: contiguous ids and weights to write."""
-    check_floats(logits, "logits")
-    if elsewhere(logits.device, stream):
+    dtype, dev = check_floats(logits, "logits"), logits.get_device()
+    if elsewhere(dev, stream):
         return run_there(lambda: route_scored(logits, rule, bias, available, out=out), logits.device, stream,
                          (logits, bias, available, *(out or ())))
-    logits = rows_of(logits, "logits")
-    rows, e = logits.shape
+    logits, rows, e, stride = rows_of(logits, "logits")
     if bias is not None:
-        check_like(bias, logits, (e,), (torch.float32,), "bias")
+        check_like(bias, dev, (e,), (torch.float32,), "bias")
         bias = bias.contiguous()
     if available is not None:
-        check_like(available, logits, (e,), (torch.bool, torch.uint8), "available")
+        check_like(available, dev, (e,), (torch.bool, torch.uint8), "available")
         available = available.contiguous()
     if out is None:
-        ids = torch.empty((rows, rule.top_k), dtype=torch.int32, device=logits.device)
-        weights = torch.empty((rows, rule.top_k), dtype=torch.float32, device=logits.device)
+        ids = logits.new_empty((rows, rule.top_k), dtype=torch.int32)
+        weights = logits.new_empty((rows, rule.top_k), dtype=torch.float32)
     else:
         ids, weights = out
-        check_like(ids, logits, (rows, rule.top_k), (torch.int32,), "out ids")
-        check_like(weights, logits, (rows, rule.top_k), (torch.float32,), "out weights")
+        check_like(ids, dev, (rows, rule.top_k), (torch.int32,), "out ids")
+        check_like(weights, dev, (rows, rule.top_k), (torch.float32,), "out weights")
         if not (ids.is_contiguous() and weights.is_contiguous()):
             raise ValueError("out must be contiguous")
     _lib.check(_lib.lib().yn_route_scored(
-        C.byref(_rule_struct(rule, e)), logits.data_ptr(), DTYPES[logits.dtype], row_stride(logits), rows,
+        C.byref(_rule_struct(rule, e)), logits.data_ptr(), dtype, stride, rows,
         None if bias is None else bias.data_ptr(), None if available is None else available.data_ptr(),
-        ids.data_ptr(), weights.data_ptr(), raw_stream(logits.device)))
+        ids.data_ptr(), weights.data_ptr(), raw_stream(dev)))
     return ids, weights
