@@ -103,8 +103,8 @@ YN_DEV float warp_max_redux(float v) {
 // Unsigned key whose order is the order of the floats, infinities included (-0 as +0;
 // every float that is not NaN has a key above 0), and back.
 YN_DEV uint32_t f32_ukey(float f) {
-  const uint32_t b = __float_as_uint(__fadd_rn(f, 0.0f));
-  return (b & 0x80000000u) ? ~b : (b | 0x80000000u);
+  const int b = __float_as_int(__fadd_rn(f, 0.0f));
+  return (uint32_t)(b ^ ((b >> 31) | (int)0x80000000u));
 }
 YN_DEV float f32_from_ukey(uint32_t k) { return __uint_as_float((k & 0x80000000u) ? (k & 0x7FFFFFFFu) : ~k); }
 YN_DEV float warp_sum_f32(float v) {

@@ -71,10 +71,16 @@ YN_DEV double warp_sum_f64(double v) {
   for (int m = 16; m > 0; m >>= 1) v += __shfl_xor_sync(0xffffffffu, v, m);
   return v;
 }
-// 1 / (1 + e^-z) by two approximations of 1 and 2 ulp (z above -80).
+// 2^x and 1 / (1 + e^-z) by the hardware's approximations (2 and 1 ulp; 0 below 2^-126).
+YN_DEV float rt_ex2(float x) {
+  float r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+  return r;
+}
+constexpr float RT_LOG2E = 1.44269504088896341f;
 YN_DEV float rt_sigmoid(float z) {
   float r;
-  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(1.0f + __expf(fminf(-z, 80.0f))));
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(1.0f + rt_ex2(-RT_LOG2E * z)));
   return r;
 }
 
@@ -230,24 +236,24 @@ __global__ void __launch_bounds__(32 * RT_WARPS) k_router(const RouterArgs a) {
     if (a.softmax) {
 #pragma unroll
       for (int i = 0; i < NV; ++i)   // all +inf logits share the mass
-        sum += v[i] == -inf ? 0.0f : v[i] == m ? 1.0f : __expf(v[i] - m);
+        sum += v[i] == -inf ? 0.0f : v[i] == m ? 1.0f : rt_ex2((v[i] - m) * RT_LOG2E);
       sum = warp_sum_f32(sum);
     }
   }
   uint32_t key[NV];
   bool in = true;   // the lane's group is kept
   if (BY_SCORE) {
-    // |c - exact| <= tol + 2^-24 |c|, tol relative to the row's largest score: __expf
-    // is off by 2 + 1.2 |x| ulp and |x| e^x <= 0.4 for x <= 0, so the exponentials
-    // stay within 2^-21 of the largest; the softmax sum of at most 64 terms a lane and
-    // 5 shuffled adds within 69 * 2^-24 < 5e-6 of itself. Scores below e^-80 are not
-    // told apart (1e-30).
+    // |c - exact| <= tol + 2^-24 |c|, tol relative to the row's largest score: e^x as
+    // 2^(x log2 e) is off by 2 ulp and the rounding of its exponent, 1.2 |x| ulp, and |x| e^x
+    // <= 0.4 for x <= 0, so the exponentials stay within 2^-21 of the largest; the softmax sum
+    // of at most 64 terms a lane and 5 shuffled adds within 69 * 2^-24 < 5e-6 of itself. Scores
+    // below 1e-30 are not told apart.
     const float inv = a.softmax ? 1.0f / sum : 1.0f;
     tol = (a.softmax ? 1.6e-5f * inv : 2.0e-6f * rt_sigmoid(m)) + 1e-30f;
     float hi = -inf, lo = -inf;
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
-      const float s = a.softmax ? (v[i] == m ? inv : __expf(v[i] - m) * inv) : rt_sigmoid(v[i]);
+      const float s = a.softmax ? (v[i] == m ? inv : rt_ex2((v[i] - m) * RT_LOG2E) * inv) : rt_sigmoid(v[i]);
       float c = s;
       if (a.bias) c += i < own.count ? __ldg(a.bias + own.first + (i << a.log_l)) : 0.0f;
       c = v[i] > -inf && c > -inf ? c : -inf;   // a bias of -inf or NaN takes the expert out
@@ -283,16 +289,23 @@ __global__ void __launch_bounds__(32 * RT_WARPS) k_router(const RouterArgs a) {
     bound = f32_ukey(fmaxf(c - 2.0f * tol - 2.5e-7f * fabsf(c), -3.402823466e38f));
   }
   bound = max(bound, 1u);
-  int n = 0;
+  // one lane's candidates side by side, the lanes one after another (their order does not matter)
+  int own_n = 0;
 #pragma unroll
-  for (int i = 0; i < NV; ++i) {
-    const unsigned who = __ballot_sync(0xffffffffu, key[i] >= bound);
-    if (who) {
-      const int at = n + __popc(who & ((1u << lane) - 1u));
-      if (key[i] >= bound && at < 32)
-        cand[warp][at] = ((unsigned long long)key[i] << 32) | (0xFFFFFFFFu - (uint32_t)(own.first + (i << a.log_l)));
-      n += __popc(who);
-    }
+  for (int i = 0; i < NV; ++i) own_n += key[i] >= bound;
+  const unsigned below = (1u << lane) - 1u;
+  const unsigned b1 = __ballot_sync(0xffffffffu, own_n > 0), b2 = __ballot_sync(0xffffffffu, own_n > 1);
+  int at = __popc(b1 & below) + __popc(b2 & below), n = __popc(b1) + __popc(b2);
+  for (int q = 2; __any_sync(0xffffffffu, own_n > q); ++q) {   // three or more in one lane: seldom
+    const unsigned bq = __ballot_sync(0xffffffffu, own_n > q);
+    at += __popc(bq & below);
+    n += __popc(bq);
+  }
+  if (n <= 32) {
+#pragma unroll
+    for (int i = 0; i < NV; ++i)
+      if (key[i] >= bound)
+        cand[warp][at++] = ((unsigned long long)key[i] << 32) | (0xFFFFFFFFu - (uint32_t)(own.first + (i << a.log_l)));
   }
   int mine = -1;
   uint32_t my_key = 0;
@@ -300,6 +313,7 @@ __global__ void __launch_bounds__(32 * RT_WARPS) k_router(const RouterArgs a) {
   if (n <= 32) {
     const unsigned long long c = lane < n ? cand[warp][lane] : 0;
     int place = 0;
+#pragma unroll 4
     for (int q = 0; q < n; ++q) place += cand[warp][q] > c;
     __syncwarp();
     if (lane < n) cand[warp][place] = c;
@@ -318,9 +332,9 @@ __global__ void __launch_bounds__(32 * RT_WARPS) k_router(const RouterArgs a) {
         if (key[i] > best) { best = key[i]; bi = i; }
       const uint32_t top = __reduce_max_sync(0xffffffffu, best);
       if (top == 0) break;
-      const int at = best == top ? own.first + (bi << a.log_l) : RT_MAX_E;
-      const int id = (int)__reduce_min_sync(0xffffffffu, (unsigned)at);
-      if (at == id) {
+      const int e = best == top ? own.first + (bi << a.log_l) : RT_MAX_E;
+      const int id = (int)__reduce_min_sync(0xffffffffu, (unsigned)e);
+      if (e == id) {
 #pragma unroll
         for (int i = 0; i < NV; ++i)
           if (i == bi) key[i] = 0;
