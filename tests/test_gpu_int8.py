@@ -271,6 +271,89 @@ def test_two_streams_and_graphs():
         assert torch.equal(out[0], ref[0]) and torch.equal(out[1], ref[1])
 
 
+@pytest.mark.parametrize("T", [1, 4])
+def test_few_pairs_on_streams_and_in_graphs(T):
+    # the two kernels of few pairs overlap (programmatic launch): back to back calls on changing inputs, on two
+    # streams, and replays, with the routing made just before on the same stream
+    from yanah_b200.routing import RouteRule, route_scored
+    x, _, _, mats, res = setup(16, 96, 256, T, 4, seed=30)
+    rule = RouteRule(4)
+
+    def run(rows, logits):
+        ids, w = route_scored(logits, rule)
+        return int8_experts(rows, ids, w, *mats, residual=res)
+
+    ins = [(normal(T, 256, seed=40 + i, dtype=x.dtype), normal(T, 16, seed=60 + i)) for i in range(12)]
+    want = [run(*i) for i in ins]
+    torch.cuda.synchronize()
+    for i, w in zip(ins, want):
+        ids, weights = route_scored(i[1], rule)
+        m = [(np64(a.codes), np64(a.scales)) for a in mats]
+        ref = ref64.experts(np64(i[0]), ids.cpu().numpy(), np64(weights), *m, residual=np64(res))
+        assert np.linalg.norm(np64(w) - ref) <= (4e-3 + 2 ** -8) * np.linalg.norm(ref)
+    for _ in range(3):
+        assert all(torch.equal(run(*i), w) for i, w in zip(ins, want))
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    for s in streams:
+        s.wait_stream(torch.cuda.current_stream())
+    got = []
+    for n, i in enumerate(ins):
+        with torch.cuda.stream(streams[n % 2]):
+            got.append(run(*i))
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+    bx, bl = ins[0][0].clone(), ins[0][1].clone()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        first = run(bx, bl)
+        second = run(first, bl)
+    for i, w in zip(ins, want):
+        bx.copy_(i[0])
+        bl.copy_(i[1])
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(first, w) and torch.equal(second, run(w, i[1]))
+
+
+def test_offsets_past_32_bits():
+    # an output of more than 2^31 elements, and matrices of more than 2^31 bytes
+    x = normal(14500, 32, seed=70, dtype=torch.bfloat16)
+    w = matrix(151936, cols=32, seed=71)
+    y = int8_linear(x, w)
+    some = torch.tensor([0, 7000, 14499])
+    want = ref64.linear(np64(x[some]), np64(w.codes[-500:]), np64(w.scales[-500:]))
+    got = np64(y[some][:, -500:])
+    assert np.all(np.abs(got - want) <= (2 ** -8 + 2 ** -21) * np.abs(want))
+    del y
+    E, I, H = 1024, 1088, 2048
+    g = torch.Generator(device="cuda").manual_seed(72)
+    codes = [torch.randint(-127, 128, s, generator=g, device="cuda", dtype=torch.int8) for s in ((E, I, H), (E, I, H), (E, H, I))]
+    mats = [Int8Matrix(c, torch.full(c.shape[:2], 2e-4, device="cuda")) for c in codes]
+    assert codes[0].numel() > 2 ** 31
+    for T in (2, 60):
+        x, res = normal(T, H, seed=73, dtype=torch.bfloat16), normal(T, H, seed=74, dtype=torch.bfloat16)
+        ids = torch.full((T, 2), 1023, dtype=torch.int32, device="cuda")
+        ids[:, 1] = 1000
+        w = torch.full((T, 2), 0.5, device="cuda")
+        out = int8_experts(x, ids, w, *mats, residual=res)
+        m = [({1023: np64(a.codes[1023]), 1000: np64(a.codes[1000])}, np64(a.scales)) for a in mats]
+
+        class At:   # the two experts that are used, by id
+            shape = (E,)
+
+            def __init__(self, d):
+                self.d = d
+
+            def __getitem__(self, e):
+                return self.d[e]
+
+        want = ref64.experts(np64(x[-2:]), ids[-2:].cpu().numpy(), np64(w[-2:]), *[(At(d), s) for d, s in m],
+                             residual=np64(res[-2:]))
+        got = np64(out[-2:])
+        part = want - np64(res[-2:])
+        assert np.linalg.norm(got - want) <= 4e-3 * np.linalg.norm(part) + 2 ** -8 * np.linalg.norm(want)
+
+
 def test_refusals():
     x, ids, w, mats, res = setup(8, 64, 128, 4, 2, seed=12)
     lin = matrix(32, cols=128)

@@ -708,9 +708,16 @@ struct ExpertsWs {
   long long ldc, lda, ldac, ldy;
   int nb;
 };
-int chunk_rows(long long pairs, int E) { return pairs <= 16ll * E ? 64 : 256; }
+// Rows per chunk of an expert, by the pairs per expert (see launch_gemm_nb). On 512 experts of 3 MB 64
+// and 256 rows take 129 and 136 us at 5 pairs per expert, 176 and 183 at 10, 248 and 241 at 20; on 64
+// experts of 9 MB 105 and 108 us at 7.5, 126 and 122 at 12.5, 174 and 149 at 38.
+int chunk_rows(long long pairs, int E) { return pairs <= 10ll * E ? 64 : 256; }
+// Pairs that go to the dp4a kernels: two launches instead of six, but they read an expert's matrices
+// for every pair. The two ways meet at about 190 MB of such reads: 60 pairs on 3 MB experts take 41
+// us so and 46 us grouped (80: 53 and 47), 20 pairs on 9 MB experts 44 and 47 us (32: 61 and 54).
 bool experts_few(long long pairs, int k, int H, int I) {
-  return pairs <= 40 && up_to(H, I8_GK) <= 96 * 1024 && k * up_to(I, I8_GK) <= 96 * 1024;
+  return (pairs <= 8 || (pairs <= 64 && pairs * 3 * H * I <= 192000000ll)) && up_to(H, I8_GK) <= 96 * 1024 &&
+         k * up_to(I, I8_GK) <= 96 * 1024;
 }
 
 ExpertsWs experts_ws(long long rows, int k, int E, int H, int I, int odt) {
@@ -851,7 +858,7 @@ extern "C" int yn_i8_experts(const yn_i8_mat* gate, const yn_i8_mat* up, const y
     float* act = reinterpret_cast<float*>(b + L.act);
     const int HP = (int)up_to(H, I8_GK), IP = (int)up_to(I, I8_GK);
     const size_t ds = (size_t)top_k * IP;
-    if ((HP > 48 * 1024 && (rc = host_set_smem(reinterpret_cast<const void*>(k_i8_up_few), 96 * 1024))) ||
+    if ((HP > 40 * 1024 && (rc = host_set_smem(reinterpret_cast<const void*>(k_i8_up_few), 96 * 1024))) ||
         (ds > 40 * 1024 && (rc = host_set_smem(reinterpret_cast<const void*>(k_i8_down_few), 96 * 1024))))
       return rc;
     k_i8_up_few<<<dim3((I + 2 * I8_GW - 1) / (2 * I8_GW), P), I8_GT, HP, st>>>(dtype, x, x_stride, H, HP, ids, top_k, E, mg, mu,
