@@ -230,20 +230,20 @@ YN_DEV bool i8_try_wait(uint64_t* bar, uint32_t phase) {
       : "memory");
   return ok != 0;
 }
-// A wait of the whole warp, at most 1 s: on a timeout the error word is set and every role
-// leaves its loop.
-YN_DEV bool i8_wait(uint64_t* bar, uint32_t phase, int* err) {
-  bool ok = i8_try_wait(bar, phase);
-  if (!ok) {
-    const uint64_t t0 = globaltimer_ns();
-    while (!(ok = i8_try_wait(bar, phase)))
-      if (globaltimer_ns() - t0 > 1000000000ull) {
-        raise_error(err, YN_ERR_BULK_TIMEOUT);
-        break;
-      }
-  }
-  return __all_sync(0xffffffffu, ok) != 0;
+// A wait of one thread, at most 1 s: on a timeout the error word is set and every role leaves
+// its loop.
+YN_DEV bool i8_wait1(uint64_t* bar, uint32_t phase, int* err) {
+  if (i8_try_wait(bar, phase)) return true;
+  const uint64_t t0 = globaltimer_ns();
+  while (!i8_try_wait(bar, phase))
+    if (globaltimer_ns() - t0 > 1000000000ull) {
+      raise_error(err, YN_ERR_BULK_TIMEOUT);
+      return false;
+    }
+  return true;
 }
+// The same of a whole warp.
+YN_DEV bool i8_wait(uint64_t* bar, uint32_t phase, int* err) { return __all_sync(0xffffffffu, i8_wait1(bar, phase, err)) != 0; }
 // Tile copies of this block whose bytes are counted on a barrier of the pair's first block.
 YN_DEV void i8_tma_3d(void* dst, const CUtensorMap* map, int x, int y, int z, uint32_t cluster_bar) {
   asm volatile(
@@ -460,50 +460,53 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(I8_THREADS, 1)
       if (lane == 0) i8_arrive_at(i8_leader(&acc_empty[b]));
     }
   } else if (warp == I8_MW) {
-    long long g = 0;
-    int j = 0;
-    for (int ti = t0; ti < n_tiles && ok && rank == 0; ti += step, ++j) {
-      const I8Chunk c = next.c;
-      next = after;
-      after = tile(ti + 2 * step);
-      const int b = j % F::ACC;
-      if (j >= F::ACC) ok = i8_wait(&acc_empty[b], (uint32_t)(j / F::ACC - 1) & 1, err);
-      if (!ok) break;
-      tc_fence_after();
-      const uint32_t idesc = i8_idesc((c.n + 31) & ~31), dcol = tmem + (uint32_t)(b * NB);
-      for (int kc = 0; kc < NK; ++kc, ++g) {
-        const int s = (int)(g % F::S);
-        ok = i8_wait(&full[s], (uint32_t)(g / F::S) & 1, err);
-        if (!ok) break;
+    // One thread: few MMAs wait in the tensor core's queue, so what it does between them counts.
+    if (lane == 0 && rank == 0) {
+      int j = 0, s = 0;
+      uint32_t full_phase = 0;
+      const uint64_t a0 = tc_desc(smem_u32(smem)), b0 = tc_desc(smem_u32(smem) + I8_A_BYTES);
+      for (int ti = t0; ti < n_tiles && ok; ti += step, ++j) {
+        const int n = next.c.n, b = j % F::ACC;
+        next = after;
+        after = tile(ti + 2 * step);
+        if (j >= F::ACC) ok = i8_wait1(&acc_empty[b], (uint32_t)(j / F::ACC - 1) & 1, err);
         tc_fence_after();
-        if (lane == 0) {
-          const uint32_t abase = smem_u32(smem + s * F::STAGE), bbase = abase + I8_A_BYTES;
+        const uint32_t idesc = i8_idesc((n + 31) & ~31), dcol = tmem + (uint32_t)(b * NB);
+        for (int kc = 0; kc < NK && ok; ++kc) {
+          ok = i8_wait1(&full[s], full_phase, err);
+          if (!ok) break;
+          tc_fence_after();
+          const uint64_t ad = a0 + (uint32_t)(s * (F::STAGE >> 4)), bd = b0 + (uint32_t)(s * (F::STAGE >> 4));
 #pragma unroll
-          for (int k = 0; k < 4; ++k)
-            i8_mma(dcol, tc_desc(abase + 32 * k), tc_desc(bbase + 32 * k), idesc, kc > 0 || k > 0 ? 1u : 0u);
+          for (int k = 0; k < 4; ++k) i8_mma(dcol, ad + 2 * k, bd + 2 * k, idesc, kc > 0 || k > 0 ? 1u : 0u);
           i8_commit_both(&empty[s]);
           if (kc == NK - 1) i8_commit_both(&acc_full[b]);
+          if (++s == F::S) {
+            s = 0;
+            full_phase ^= 1;
+          }
         }
-        __syncwarp();
       }
+      // the last commits must land before TMEM is released (bounded)
+      if (ok && j > 0) (void)i8_wait1(&acc_full[(j - 1) % F::ACC], (uint32_t)((j - 1) / F::ACC) & 1, err);
     }
-    // the last commits must land before TMEM is released (bounded)
-    if (ok && j > 0) (void)i8_wait(&acc_full[(j - 1) % F::ACC], (uint32_t)((j - 1) / F::ACC) & 1, err);
+    __syncwarp();
   } else {
-    long long g = 0;
-    for (int ti = t0; ti < n_tiles && ok; ti += step) {
-      const I8Chunk c = next.c;
-      const int u0 = next.u0;
-      next = after;
-      after = tile(ti + 2 * step);
-      const int half = ((c.n + 31) & ~31) >> 1, row = c.p0 + rank * half;   // this block's half of the MMA's rows
-      const int bi = half <= 16 ? 0 : half <= 32 ? 1 : half <= 64 ? 2 : 3;
-      const uint32_t bytes = 2u * (I8_A_BYTES + (16u << bi) * 128u);
-      for (int kc = 0; kc < NK; ++kc, ++g) {
-        const int s = (int)(g % F::S);
-        if (g >= F::S) ok = i8_wait(&empty[s], (uint32_t)(g / F::S - 1) & 1, err);
-        if (!ok) break;
-        if (lane == 0) {
+    if (lane == 0) {
+      int s = 0, used = 0;
+      uint32_t empty_phase = 1;   // the first round finds the ring empty
+      for (int ti = t0; ti < n_tiles && ok; ti += step) {
+        const I8Chunk c = next.c;
+        const int u0 = next.u0;
+        next = after;
+        after = tile(ti + 2 * step);
+        const int half = ((c.n + 31) & ~31) >> 1, row = c.p0 + rank * half;   // this block's half of the MMA's rows
+        const int bi = half <= 16 ? 0 : half <= 32 ? 1 : half <= 64 ? 2 : 3;
+        const uint32_t bytes = 2u * (I8_A_BYTES + (16u << bi) * 128u);
+        for (int kc = 0; kc < NK; ++kc) {
+          if (used == F::S) ok = i8_wait1(&empty[s], empty_phase, err);
+          else ++used;
+          if (!ok) break;
           uint8_t* st = smem + s * F::STAGE;
           const uint32_t bar = i8_leader(&full[s]);
           if (rank == 0) mbar_arrive_expect_tx(&full[s], bytes);
@@ -519,15 +522,27 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(I8_THREADS, 1)
             i8_tma_3d(st, &maps.a, 128 * kc, u0, c.e, bar);
           }
           i8_tma_2d(st + I8_A_BYTES, &maps.b[bi], 128 * kc, row, bar);
+          if (++s == F::S) {
+            s = 0;
+            empty_phase ^= 1;
+          }
         }
-        __syncwarp();
+      }
+      // every stage filled must have been read (its copies and MMAs done) before the block ends: the
+      // ring's `used` slots, the oldest first
+      if (used < F::S) {
+        s = 0;
+        empty_phase = 0;
+      }
+      for (int i = 0; i < used && ok; ++i) {
+        ok = i8_wait1(&empty[s], empty_phase, err);
+        if (++s == F::S) {
+          s = 0;
+          empty_phase ^= 1;
+        }
       }
     }
-    // every stage filled must have been read (its copies and MMAs done) before the block ends
-    for (int s = 0; s < F::S && ok; ++s) {
-      const long long last = g - 1 - ((g - 1 - s) % F::S + F::S) % F::S;   // last stage number in slot s
-      if (last >= 0 && last < g) ok = i8_wait(&empty[s], (uint32_t)(last / F::S) & 1, err);
-    }
+    __syncwarp();
   }
   tc_fence_before();
   __syncthreads();
