@@ -39,6 +39,8 @@ __global__ void __launch_bounds__(I8_QT) k_i8_quant(const void* x, long long ldx
                                                     const int32_t* to, int copies, int8_t* codes, long long ldc,
                                                     float* scales) {
   __shared__ uint32_t buf[I8_QT / 32];
+  i8_launch_next();
+  i8_wait_previous();
   const size_t row = blockIdx.x * (size_t)(I8_QT / N) + threadIdx.x / N, base = row * (size_t)ldx;
   if (row >= (size_t)(n_rows ? *n_rows : rows)) return;
   const int tid = threadIdx.x % N, n8 = VEC ? K / 8 : 0;
@@ -107,17 +109,38 @@ __global__ void __launch_bounds__(I8_QT) k_i8_quant(const void* x, long long ldx
   }
 }
 
+// Kernels of one call follow one another without a gap (programmatic launch): all but the first
+// are launched with this. Each waits for the one before it itself.
+template <typename... P, typename... A>
+void launch_after(void (*kern)(P...), dim3 grid, unsigned block, size_t smem, cudaStream_t st, A... args) {
+  cudaLaunchAttribute at{};
+  at.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  at.val.programmaticStreamSerializationAllowed = 1;
+  cudaLaunchConfig_t lc{};
+  lc.gridDim = grid;
+  lc.blockDim = dim3(block);
+  lc.dynamicSmemBytes = smem;
+  lc.stream = st;
+  lc.attrs = &at;
+  lc.numAttrs = 1;
+  (void)cudaLaunchKernelEx(&lc, kern, static_cast<P>(args)...);   // its error is the caller's cudaGetLastError
+}
+
 int launch_quant(int dt, const void* x, long long ldx, long long rows, int K, const int* n_rows, const int32_t* to, int copies,
-                 int8_t* codes, long long ldc, float* scales, cudaStream_t st) {
+                 int8_t* codes, long long ldc, float* scales, bool first, cudaStream_t st) {
   const size_t size = dt == YN_F32 ? 4 : 2;
   const bool vec = reinterpret_cast<uintptr_t>(x) % 16 == 0 && (ldx * size) % 16 == 0 &&
                    reinterpret_cast<uintptr_t>(codes) % 8 == 0 && ldc % 8 == 0;
   const bool warps = vec && rows >= I8_QWARP && K <= 4096;
-  const dim3 g((unsigned)(warps ? (rows + I8_QT / 32 - 1) / (I8_QT / 32) : rows)), b(I8_QT);
-#define YN_Q(T)                                                                                                             \
-  if (warps) k_i8_quant<T, true, 32, sizeof(T) == 4 ? 6 : 8><<<g, b, 0, st>>>(x, ldx, rows, K, n_rows, to, copies, codes, ldc, scales);         \
-  else if (vec) k_i8_quant<T, true, I8_QT, 4><<<g, b, 0, st>>>(x, ldx, rows, K, n_rows, to, copies, codes, ldc, scales);   \
-  else k_i8_quant<T, false, I8_QT, 4><<<g, b, 0, st>>>(x, ldx, rows, K, n_rows, to, copies, codes, ldc, scales)
+  const dim3 g((unsigned)(warps ? (rows + I8_QT / 32 - 1) / (I8_QT / 32) : rows));
+  auto go = [&](auto kern) {
+    if (first) kern<<<g, I8_QT, 0, st>>>(x, ldx, rows, K, n_rows, to, copies, codes, ldc, scales);
+    else launch_after(kern, g, I8_QT, 0, st, x, ldx, rows, K, n_rows, to, copies, codes, ldc, scales);
+  };
+#define YN_Q(T)                                                       \
+  if (warps) go(k_i8_quant<T, true, 32, sizeof(T) == 4 ? 6 : 8>);     \
+  else if (vec) go(k_i8_quant<T, true, I8_QT, 4>);                    \
+  else go(k_i8_quant<T, false, I8_QT, 4>)
   if (dt == YN_F32) { YN_Q(float); }
   else if (dt == YN_BF16) { YN_Q(__nv_bfloat16); }
   else { YN_Q(__half); }
@@ -191,11 +214,6 @@ YN_DEV void i8_row_smem(int dt, const void* x, size_t base, int K, int KP, int8_
   else if (dt == YN_BF16) i8_row_smem_t<BLOCK, __nv_bfloat16>(x, base, K, KP, codes, scale, buf);
   else i8_row_smem_t<BLOCK, __half>(x, base, K, KP, codes, scale, buf);
 }
-
-// The second of two kernels starts while the first still runs (programmatic launch); what it
-// reads of the first it reads after the wait.
-YN_DEV void i8_launch_next() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
-YN_DEV void i8_wait_previous() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 
 struct I8Mat {
   const int8_t* codes;
@@ -445,6 +463,7 @@ __global__ void __cluster_dims__(I8_PLAN_B, 1, 1) __launch_bounds__(I8_PLAN_T)
   __shared__ int cnt[I8_MAX_E], base_of[I8_MAX_E];
   __shared__ int2 ws[I8_PLAN_T / 32];
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, me = (int)cluster.block_rank();
+  i8_launch_next();
   cnt[tid] = 0;
   __syncthreads();
   // part of the pairs: rounds of I8_PLAN_B * I8_PLAN_T * Q
@@ -517,6 +536,7 @@ __global__ void __cluster_dims__(I8_PLAN_B, 1, 1) __launch_bounds__(I8_PLAN_T)
 template <typename O, typename Y, bool VEC>
 __global__ void __launch_bounds__(128) k_i8_combine(const Y* y, long long ldy, const int32_t* pair_of, const float* w, int k,
                                                     int H, const void* res, long long ldr, void* out, long long ldo) {
+  i8_wait_previous();
   const size_t t = blockIdx.x;
   const int lane = threadIdx.x & 31, h = 8 * (blockIdx.y * 128 + threadIdx.x);
   const int p_mine = lane < k ? pair_of[t * k + lane] : -1;   // lane j: the row's pair j
@@ -578,8 +598,8 @@ void launch_combine(const void* y, long long ldy, const int32_t* pair_of, const 
                    reinterpret_cast<uintptr_t>(res) % 16 == 0 && (ldr * sizeof(O)) % 16 == 0;
   const dim3 g((unsigned)rows, (H + 1023) / 1024);
   const Y* yy = reinterpret_cast<const Y*>(y);
-  if (vec) k_i8_combine<O, Y, true><<<g, 128, 0, st>>>(yy, ldy, pair_of, w, k, H, res, ldr, out, ldo);
-  else k_i8_combine<O, Y, false><<<g, 128, 0, st>>>(yy, ldy, pair_of, w, k, H, res, ldr, out, ldo);
+  if (vec) launch_after(k_i8_combine<O, Y, true>, g, 128, 0, st, yy, ldy, pair_of, w, k, H, res, ldr, out, ldo);
+  else launch_after(k_i8_combine<O, Y, false>, g, 128, 0, st, yy, ldy, pair_of, w, k, H, res, ldr, out, ldo);
 }
 
 // ---------------------------------------------------------------- host side
@@ -646,7 +666,7 @@ int launch_gemm(const I8Gemm& a, const I8Maps& maps, long long max_tiles, cudaSt
   int rc = host_set_smem(kern, I8Cfg<NB>::SMEM), sms = 0;
   if (rc || (rc = sm_count(&sms))) return rc;
   const unsigned grid = 2 * (unsigned)std::max<long long>(1, std::min<long long>(max_tiles, sms / 2));
-  k_i8_gemm<O, UP, NB><<<grid, I8_THREADS, I8Cfg<NB>::SMEM, st>>>(a, maps);
+  launch_after(k_i8_gemm<O, UP, NB>, grid, I8_THREADS, I8Cfg<NB>::SMEM, st, a, maps);   // after the rows' codes
   const cudaError_t e = cudaGetLastError();
   return e == cudaSuccess ? YN_OK : host_fail(YN_E_CUDA, std::string("8-bit product: ") + cudaGetErrorString(e));
 }
@@ -760,7 +780,7 @@ extern "C" int yn_i8_quant_rows(const void* x, int32_t dtype, int64_t row_stride
   if (rows == 0) return YN_OK;
   if (!x || !codes || !scales) return host_fail(YN_E_INVALID, "null argument");
   if (reinterpret_cast<uintptr_t>(x) % dtype_size(dtype)) return host_fail(YN_E_INVALID, "x must be aligned to its element");
-  return launch_quant(dtype, x, row_stride, rows, cols, nullptr, nullptr, 1, reinterpret_cast<int8_t*>(codes), code_stride, scales,
+  return launch_quant(dtype, x, row_stride, rows, cols, nullptr, nullptr, 1, reinterpret_cast<int8_t*>(codes), code_stride, scales, true,
                       reinterpret_cast<cudaStream_t>(stream));
 }
 
@@ -803,7 +823,7 @@ extern "C" int yn_i8_linear(const yn_i8_mat* w, const void* x, int32_t dtype, in
   int8_t* codes = reinterpret_cast<int8_t*>(ws);
   const long long ldc = (long long)up_to(w->cols, 16);
   float* sx = reinterpret_cast<float*>(codes + up_to((size_t)rows * ldc, 256));
-  if ((rc = launch_quant(dtype, x, x_stride, rows, w->cols, nullptr, nullptr, 1, codes, ldc, sx, st))) return rc;
+  if ((rc = launch_quant(dtype, x, x_stride, rows, w->cols, nullptr, nullptr, 1, codes, ldc, sx, true, st))) return rc;
   I8Gemm a{};
   a.rows = (int)rows;
   a.channels = w->rows;
@@ -863,18 +883,8 @@ extern "C" int yn_i8_experts(const yn_i8_mat* gate, const yn_i8_mat* up, const y
       return rc;
     k_i8_up_few<<<dim3((I + 2 * I8_GW - 1) / (2 * I8_GW), P), I8_GT, HP, st>>>(dtype, x, x_stride, H, HP, ids, top_k, E, mg, mu,
                                                                              I, act);
-    cudaLaunchAttribute at{};
-    at.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    at.val.programmaticStreamSerializationAllowed = 1;
-    cudaLaunchConfig_t lc{};
-    lc.gridDim = dim3((H + 2 * I8_GW - 1) / (2 * I8_GW), (unsigned)rows);
-    lc.blockDim = dim3(I8_GT);
-    lc.dynamicSmemBytes = ds;
-    lc.stream = st;
-    lc.attrs = &at;
-    lc.numAttrs = 1;
-    (void)cudaLaunchKernelEx(&lc, k_i8_down_few, (const float*)act, I, IP, ids, weights, (int)top_k, E, md, H, (int)dtype,
-                             residual, (long long)res_stride, out, (long long)out_stride);
+    launch_after(k_i8_down_few, dim3((H + 2 * I8_GW - 1) / (2 * I8_GW), (unsigned)rows), I8_GT, ds, st, act, I, IP, ids, weights,
+                 top_k, E, md, H, dtype, residual, res_stride, out, out_stride);
     const cudaError_t e = cudaGetLastError();
     return e == cudaSuccess ? YN_OK : host_fail(YN_E_CUDA, std::string("experts: ") + cudaGetErrorString(e));
   }
@@ -888,7 +898,7 @@ extern "C" int yn_i8_experts(const yn_i8_mat* gate, const yn_i8_mat* up, const y
   float* sa = reinterpret_cast<float*>(b + L.sa);
   void* y = b + L.y;
   k_i8_plan<<<I8_PLAN_B, I8_PLAN_T, 0, st>>>(ids, P, E, L.nb, pair_of, chunks, n_out);
-  if ((rc = launch_quant(dtype, x, x_stride, rows, H, nullptr, pair_of, top_k, codes, L.ldc, sx, st))) return rc;
+  if ((rc = launch_quant(dtype, x, x_stride, rows, H, nullptr, pair_of, top_k, codes, L.ldc, sx, false, st))) return rc;
   const long long max_chunks = E + P / L.nb + 1;
   I8Maps maps{};
   I8Gemm g{};
@@ -908,7 +918,7 @@ extern "C" int yn_i8_experts(const yn_i8_mat* gate, const yn_i8_mat* up, const y
   const long long tu = max_chunks * ((I + 127) / 128), td = max_chunks * ((H + 255) / 256);
   rc = launch_gemm_nb<float, true>(L.nb, g, maps, tu, st);
   if (rc) return rc;
-  if ((rc = launch_quant(YN_F32, act, L.lda, P, I, n_out + 1, nullptr, 1, acodes, L.ldac, sa, st))) return rc;
+  if ((rc = launch_quant(YN_F32, act, L.lda, P, I, n_out + 1, nullptr, 1, acodes, L.ldac, sa, false, st))) return rc;
   I8Maps md2{};
   if ((rc = tmap_mats(&md2.a, *down, 128)) || (rc = tmap_rows(&md2, acodes, I, P, L.ldac))) return rc;
   I8Gemm d{};

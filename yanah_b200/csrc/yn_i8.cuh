@@ -151,9 +151,11 @@ YN_DEV uint32_t block_max_u32(uint32_t v, uint32_t* buf) {
 // One tile: 256 channels of one matrix x up to NB rows, each block with 128 of the channels
 // (its own TMEM lanes) and half of the rows' codes in its shared memory; the pair's MMA (M
 // 256, kind::i8) reads both halves, so a row's codes cross from L2 once per pair and a stage
-// moves 32 KB per SM for 512 cycles of MMA. One block alone would move 48 KB, and the 12
-// TB/s that L2 gave here then held the MMA at 62% of its rate (104 us against ... at 4096 x
-// 2048 x 16384).
+// moves 32 KB per SM for 512 cycles of MMA where one block alone would move 48 KB (4096 rows
+// of 64 experts: 334 us, 346 with single blocks). 4096 x 2048 x 16384 takes 108 us in single
+// launches, 82 at the tensor cores' nominal rate; without its loads it takes 102 us, without
+// its epilogue 91, without both 86. Run after run the card's power limit holds it (1.55 GHz of
+// 1.97 at 956 W; operands of zeros run at the full clock and take 15% less).
 // A = the channels' codes, B = the rows' codes, both K-major in the 128-byte swizzled layout
 // by TMA, 128 codes of K per stage (four MMAs of K 32); the accumulator is channels (lanes) x
 // rows (columns), int32. UP interleaves 16 rows of the gate matrix with 16 of the up matrix,
@@ -182,6 +184,12 @@ constexpr int I8_BMAPS = 4;
 struct I8Maps {
   CUtensorMap a, a_up, b[I8_BMAPS];
 };
+
+// A kernel of a call may be launched while the one before it runs (launch_after): it sets itself
+// up, then waits until that one is done and its writes can be seen. Every thread of it waits, so
+// that a kernel that is done has all before it done.
+YN_DEV void i8_launch_next() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+YN_DEV void i8_wait_previous() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 
 YN_DEV void i8_mma(uint32_t tmem_d, uint64_t adesc, uint64_t bdesc, uint32_t idesc, uint32_t accumulate) {
   asm volatile(
@@ -294,6 +302,7 @@ struct I8Cfg {
   static constexpr int PIECES = NB / (16 * SPLIT);          // 16-column pieces of such a warp
   static constexpr int SMEM = 1024 + S * STAGE + (2 * S + 2 * ACC) * 8 + 16;
   static_assert(NB % 32 == 0 && NB <= 256, "two accumulators have to fit TMEM");
+  static_assert(2 * SMEM > 228 * 1024, "each block takes an SM's whole TMEM: no two may share one");
 };
 
 // SiLU(g) * u in fp32.
@@ -321,9 +330,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(I8_THREADS, 1)
 
   constexpr int TILE = UP ? 128 : 256;   // units or channels of a pair's tile
   const int UT = (a.channels + TILE - 1) / TILE;
-  const int n_chunks = a.chunks ? *a.n_chunks : (a.rows + NB - 1) / NB;
-  const int n_tiles = n_chunks * UT, step = (int)(gridDim.x >> 1), t0 = (int)(blockIdx.x >> 1);
-  const int NK = (a.K + 127) / 128;
+  const int step = (int)(gridDim.x >> 1), t0 = (int)(blockIdx.x >> 1), NK = (a.K + 127) / 128;
+  i8_launch_next();
   if (tid == 0) {
     for (int s = 0; s < F::S; ++s) {
       mbar_init(&full[s], 1);
@@ -345,6 +353,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(I8_THREADS, 1)
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
   bool ok = true;
+  i8_wait_previous();
+  const int n_chunks = a.chunks ? *a.n_chunks : (a.rows + NB - 1) / NB, n_tiles = n_chunks * UT;
   // A list's tiles go unit by unit through a chunk, so that neighbours share the rows; a
   // single matrix's go chunk by chunk through its channels, so that they share the weights.
   // Every role looks its tiles up two ahead.
@@ -460,7 +470,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(I8_THREADS, 1)
       if (lane == 0) i8_arrive_at(i8_leader(&acc_empty[b]));
     }
   } else if (warp == I8_MW) {
-    // One thread: few MMAs wait in the tensor core's queue, so what it does between them counts.
+    // One thread: few MMAs wait in the tensor core's queue, so what it does between them counts
+    // (whole warps that elected a lane for each step took 116 us, this 108, at 4096 x 2048 x 16384).
     if (lane == 0 && rank == 0) {
       int j = 0, s = 0;
       uint32_t full_phase = 0;
