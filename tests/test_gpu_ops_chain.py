@@ -19,7 +19,7 @@ from tests import ref64
 from tests.gpu_helpers import bf16_dev, bf16_np, hidden_rows, rel_l2, small_config
 from yanah_b200 import _lib
 from yanah_b200.device import stream_ptr
-from yanah_b200.int8 import int8_linear, quantize_rows
+from yanah_b200.int8 import int8_experts, int8_linear, quantize_rows
 from yanah_b200.logprobs import token_logprobs
 from yanah_b200.prefill import PrefillStack
 from yanah_b200.routing import RouteRule
@@ -177,3 +177,51 @@ def test_a_prompt_pass_answers_in_one_graph():
         torch.cuda.synchronize()
         assert all(torch.equal(a, b) for a, b in zip(want, out))
     assert st.check_error() == 0
+
+
+@pytest.mark.parametrize("experts", ["records", "int8"])
+def test_rule_that_leaves_rows_short(experts):
+    # a bias of -inf takes all experts but one, or all, out: the columns without an expert add nothing
+    cfg, T = config(), 37
+    bias = torch.full((cfg.n_layers, cfg.n_experts), -float("inf"), device="cuda")
+    bias[0, 5] = 0.25
+    st = PrefillStack(cfg, max_rows=T, rule=RouteRule(2, "sigmoid", scale=2.0), choice_bias=bias, experts=experts)
+    h = bf16_dev(hidden_rows(cfg, T, stream=6))
+    out = torch.full_like(h, float("nan"))
+    for buf in (st.pair_of, st.pair_row):
+        buf.fill_(0x7fffffff)       # what an allocation may hold
+    st.layer(1, h, out)
+    torch.cuda.synchronize()
+    assert (st.ids[:T] == -1).all() and (st.w[:T] == 0).all() and torch.equal(out, h)
+    st.layer(0, h, out)
+    torch.cuda.synchronize()
+    assert (st.ids[:T, 0] == 5).all() and (st.ids[:T, 1] == -1).all()
+    # the weight: a quotient by a hardware reciprocal, 2 ulp, and its product with the scale
+    assert ((st.w[:T, 0] - 2).abs() <= 4e-6).all() and (st.w[:T, 1] == 0).all() and st.check_error() == 0
+    # expert 5 twice with weight 1 is the same sum (a + a = 2 a exactly)
+    want = torch.empty_like(h)
+    five, ones = torch.full((T, 2), 5, dtype=torch.int32, device="cuda"), torch.ones(T, 2, device="cuda")
+    if experts == "int8":
+        int8_experts(st.x[:T], five, ones, *st.int8[0], residual=h, out=want)
+        torch.cuda.synchronize()
+        # the same bf16 products, fp32 sums off by the weight's 2e-6, and the two roundings of half a step each
+        a, b = out.double(), want.double()
+        assert ((a - b).abs() <= 2 ** -7 * b.abs() + 4e-6 * (b - h.double()).abs()).all()
+    else:
+        y = cpu.OracleStack(cfg, threads=8)
+        x = y.post_attention(0, bf16_np(h))["x"]
+        for t in (0, T - 1):
+            ref = cpu.bf16_to_f32(bf16_np(h)[t]) + 2.0 * cpu.bf16_to_f32(y.expert(0, 5, x[t])[1])
+            got = out[t].double().cpu().numpy()
+            assert np.linalg.norm(got - ref) <= 1e-2 * np.linalg.norm(ref)
+
+
+def test_backend_refuses_rows_left_short():
+    from yanah_b200.backend import CudaMoEBackend
+    cfg = config()
+    bias = torch.full((cfg.n_layers, cfg.n_experts), -float("inf"), device="cuda")
+    be = CudaMoEBackend(cfg, "cuda", rule=RouteRule(2, "sigmoid"), choice_bias=bias)
+    for T in (1, 40):
+        be.pre_moe(0, bf16_dev(hidden_rows(cfg, T, stream=5)))
+        with pytest.raises(RuntimeError, match="fewer than top_k"):
+            be.route(None)

@@ -265,6 +265,7 @@ class CudaMoEBackend:
             ids, w = self._pre["rows"]
             with torch.cuda.stream(self.stream):
                 ids_np = ids.cpu().numpy().astype(np.int64)      # the routing sync
+            self._check_routed(ids_np)
             return ids_np, w, None
         lib, st = _lib.lib(), self._st()
         ids = self.ws.tensor("ids", (T, K), torch.int32)
@@ -275,8 +276,14 @@ class CudaMoEBackend:
             _lib.check(lib.yn_memcpy_async(self._fp_host.data_ptr(), fp.data_ptr(), fp.numel() * 4, st))
         self.stream.synchronize()                                 # the routing sync
         ids_np = self._ids_np[:T * K].reshape(T, K).astype(np.int64)
+        self._check_routed(ids_np)
         fp_np = self._fp_np[:n_fp * self.cfg.n_experts].reshape(n_fp, -1) if n_fp else None
         return ids_np, self.ws.tensor("weights", (T, K), torch.float32), fp_np
+
+    def _check_routed(self, ids: np.ndarray) -> None:
+        # the pool has no slot for "no expert"
+        if self.rule is not None and ids.size and ids.min() < 0:
+            raise RuntimeError("the rule left a row fewer than top_k experts: its logits or biases are -inf or NaN")
 
     def route(self, logits):
         """Routing of the last `pre_moe` (computed there on the device)."""

@@ -715,7 +715,8 @@ namespace ynb {
 // 1024 threads): counts per expert, a block scan over experts (ascending id),
 // pair placement (pairs of one expert contiguous; their order inside an
 // expert does not change any pair's result), then per expert ceil(n / 256)
-// row chunks x (I / 64) gate/up tiles and x (H / 128) down tiles.
+// row chunks x (I / 64) gate/up tiles and x (H / 128) down tiles. An id of -1 (a rule that
+// leaves a row fewer than k experts) has no pair; any other outside [0, E) is an error.
 // n_tiles[0], n_tiles[1] = gate/up and down tiles written.
 constexpr int PLAN_THREADS = 1024;
 
@@ -781,7 +782,7 @@ __global__ void __launch_bounds__(PLAN_THREADS) k_prefill_plan(const PrefillPlan
   for (int i = tid; i < Pw; i += PLAN_THREADS) {
     const int e = i < P ? a.ids[i] : -1;
     const bool valid = e >= 0 && e < a.E;
-    if (i < P && !valid) raise_error(a.err, YN_ERR_BAD_EXPERT);
+    if (i < P && !valid && e != -1) raise_error(a.err, YN_ERR_BAD_EXPERT);
     agg_atomic_add(cnt, valid ? e : 0, valid);
   }
   __syncthreads();
@@ -800,8 +801,11 @@ __global__ void __launch_bounds__(PLAN_THREADS) k_prefill_plan(const PrefillPlan
     if (valid) {
       a.pair_row[start[e] + pos] = i / a.K;
       a.pair_of[i] = start[e] + pos;
+    } else if (i < P) {
+      a.pair_of[i] = -1;
     }
   }
+  for (int i = tot.x + tid; i < P; i += PLAN_THREADS) a.pair_row[i] = 0;  // gathered, in no tile
   // chunks of at most TC_NMAX pairs per expert, then every tile in parallel
   if (tid < a.E && c) {
     for (int k = 0; k * TC_NMAX < c; ++k) {

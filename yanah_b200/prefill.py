@@ -97,8 +97,8 @@ class PrefillStack:
     """Resident experts and dense weights of `layers` of `cfg`, and the
     buffers for prompts of up to `max_rows` rows in total. A layer runs
     entirely on the device (routing, grouping, GEMMs, combine): no host
-    synchronisation. rule / choice_bias: route by a rule, with a bias (layers, E)
-    fp32 on its choice. experts: "records" (4-bit codes as they are) or "int8"."""
+    synchronisation. rule / choice_bias: route by a rule, with a bias (layers of the
+    stack, E) fp32 on its choice. experts: "records" (4-bit codes as they are) or "int8"."""
 
     def __init__(self, cfg: StackConfig, max_rows: int, device: str = "cuda",
                  layers: Optional[Sequence[int]] = None, rule: Optional[RouteRule] = None,
