@@ -438,7 +438,7 @@ typedef struct yn_route_rule {
  * (E) fp32 or NULL); the top_groups groups with the best scores are kept, and
  * of their experts the k with the largest choice values are chosen, in
  * descending order, ties to the lower id (groups alike). The order is that of
- * exact arithmetic; without a bias it is the order of the logits. weights: s
+ * 64-bit arithmetic; without a bias it is the order of the logits. weights: s
  * of the chosen (without the bias), renormalised if asked, times `scale`, in
  * fp32. An expert does not take part (it has no share of a softmax either)
  * where `available` ((E) bytes, NULL: all) is 0, its logit is -inf or NaN; one

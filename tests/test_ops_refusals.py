@@ -107,3 +107,18 @@ def test_tensors_of_the_cpu_are_refused():
         verify_rows(z, w, torch.zeros(4, dtype=torch.int32))
     with pytest.raises(ValueError):
         verify_rows(z, w, torch.zeros(1, dtype=torch.int32), n_top=0)
+
+
+def test_arguments_that_require_a_gradient_are_refused():
+    # no operator has a backward pass: a gradient is refused, not dropped (-1: the index of the CPU)
+    from yanah_b200.int8 import _mat
+    from yanah_b200.launch import check_like
+    w = torch.zeros(3, 2, requires_grad=True)
+    with pytest.raises(RuntimeError, match="weights requires a gradient"):
+        check_like(w, -1, (3, 2), (torch.float32,), "weights")
+    m = Int8Matrix(torch.zeros(8, 64, dtype=torch.int8), torch.zeros(8, requires_grad=True))
+    with pytest.raises(RuntimeError, match="w's scales requires a gradient"):
+        _mat(m, -1, "w")
+    with torch.no_grad():
+        check_like(w, -1, (3, 2), (torch.float32,), "weights")
+        assert _mat(m, -1, "w").rows == 8

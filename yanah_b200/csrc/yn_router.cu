@@ -8,7 +8,7 @@
 // its `group_top` largest c; the k largest c inside the `top_groups` best groups
 // are chosen (ties: lower id first) and weighted by s, not c.
 //
-// The order is that of exact arithmetic. Without a bias and groups c is a
+// The order is that of exact arithmetic, as far as 64 bits have it. Without a bias and groups c is a
 // monotone function of z, so the logits themselves are compared. Otherwise the
 // row is ordered in fp32, whose error on c is bounded (below); only where two
 // neighbours of the chosen order, or the last group in and the first one out,

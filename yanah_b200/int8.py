@@ -21,7 +21,7 @@ from typing import NamedTuple, Optional
 import torch
 
 from . import _lib
-from .launch import DTYPES, check_floats, check_like, elsewhere, raw_stream, rows_of, run_there
+from .launch import DTYPES, check_floats, check_like, check_no_grad, elsewhere, raw_stream, rows_of, run_there
 
 
 class Int8Matrix(NamedTuple):
@@ -59,6 +59,8 @@ def _mat(w: Int8Matrix, index: int, what: str) -> _lib.I8Mat:
         raise ValueError(f"{what}: codes (N, K) or (E, N, K) with scales (N) or (E, N)")
     if codes.get_device() != index or scales.get_device() != index:
         raise ValueError(f"{what} is not on cuda:{index}")
+    if scales.requires_grad:
+        check_no_grad(f"{what}'s scales")
     n, k = shape[-2:]
     s_strides = scales.stride()
     if (k > 1 and strides[-1] != 1) or (n > 1 and s_strides[-1] != 1):

@@ -24,9 +24,15 @@ def check_floats(t: torch.Tensor, what: str) -> int:
         raise TypeError(f"{what} must be float32, bfloat16 or float16, not {t.dtype}")
     if not t.is_cuda:
         raise ValueError(f"{what} must be a CUDA tensor")
-    if t.requires_grad and torch.is_grad_enabled():
-        raise RuntimeError(f"{what} requires a gradient: this operator has none (call it under torch.no_grad())")
+    if t.requires_grad:
+        check_no_grad(what)
     return code
+
+
+def check_no_grad(what: str) -> None:
+    """For an argument that requires a gradient."""
+    if torch.is_grad_enabled():
+        raise RuntimeError(f"{what} requires a gradient: this operator has none (call it under torch.no_grad())")
 
 
 def check_like(t: torch.Tensor, index: int, shape: tuple, dtypes: tuple, what: str) -> None:
@@ -37,6 +43,8 @@ def check_like(t: torch.Tensor, index: int, shape: tuple, dtypes: tuple, what: s
         raise TypeError(f"{what} must be {' or '.join(str(d) for d in dtypes)}, not {t.dtype}")
     if t.get_device() != index:
         raise ValueError(f"{what} is on {t.device}, not on cuda:{index}")
+    if t.requires_grad:
+        check_no_grad(what)
 
 
 def rows_of(t: torch.Tensor, what: str) -> Tuple[torch.Tensor, int, int, int]:

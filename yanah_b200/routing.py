@@ -55,7 +55,7 @@ def route_scored(logits: torch.Tensor, rule: RouteRule, bias: Optional[torch.Ten
     fp32, bf16 or fp16.
 
     The choice value of an expert is its score plus ``bias`` (E) fp32; ids are in
-    descending order of it, equal ones by id; the order is that of exact arithmetic.
+    descending order of it, equal ones by id; the order is that of 64-bit arithmetic.
     The weights are the scores of the chosen. An expert does not take part where
     ``available`` (E) (bool or uint8) is false or its logit is -inf or NaN; rows with
     fewer than k experts left end in ids of -1 with weight 0. Any number of rows.
