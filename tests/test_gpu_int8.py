@@ -3,12 +3,12 @@
 Codes are compared for equality, scales to one rounding (2^-24). A linear product: the
 sum is exact, its conversion and two factors (one of them a rounded quotient) are four
 roundings of 2^-24, and the output's rounding eps / 2: eps / 2 + 2^-21 of the value is
-asked. Experts: the activations a carry errors of at most 2^-16 of the largest of their
-32 units (many rows) plus a few fp32 ulp of the exponential; where that moves one over
-the border between two codes the code is off by one, so a product's error is at most
-sum_u |sd qd| sa over the moved ones. Expected share of moved codes: the error in steps,
-below 127 * 2^-16 / 2 = 1e-3. Asked of the whole output: relative 2-norm 4e-3 * (share of
-the experts' part in it <= 1) + eps / 2.
+asked. Experts: the activations a are fp32 values of a hardware exponential and
+reciprocal (a few ulp); where that moves one over the border between two codes the code is
+off by one, so a product's error is at most sum_u |sd qd| sa over the moved ones. Expected
+share of moved codes: the error in steps, below 127 * 8 * 2^-23 = 1.3e-4. The products'
+rounding to bf16 before they are summed is half a step, 2^-8 = 3.9e-3, of each. Asked of
+the whole output: relative 2-norm 4e-3 * (share of the experts' part in it <= 1) + eps / 2.
 """
 from __future__ import annotations
 

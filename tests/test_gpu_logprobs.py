@@ -130,6 +130,21 @@ def test_strides_and_alignment(dtype):
     check(whole[:, 3:1000], tok[:4], 4)
 
 
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("T", [2, 300])
+def test_signed_zeros_are_equal_and_denormals_are_not(dtype, T):
+    V = 5000
+    z = torch.full((T, V), -1.0, dtype=dtype, device="cuda")
+    tiny = torch.finfo(dtype).tiny * torch.finfo(dtype).eps       # the smallest value of the type
+    z[:, 100] = -0.0
+    z[:, 3000] = 0.0
+    z[:, 3001] = -tiny
+    z[:, 4999] = tiny
+    z[1::2, 4999] = -2 * tiny
+    for t in (100, 3000, 3001, 4999):
+        check(z, torch.full((T,), t, dtype=torch.int32, device="cuda"), 6)
+
+
 def test_large_offsets():
     # element offsets past 2^31
     V, T = 151936, 14200

@@ -74,6 +74,22 @@ def test_masks(score):
     check(z, RouteRule(k, score), bias=bias)
 
 
+@pytest.mark.parametrize("score", ["softmax", "sigmoid"])
+def test_signed_zeros_are_equal(score):
+    z = torch.full((3, 64), -1.0, device="cuda")
+    z[:, 5] = -0.0
+    z[:, 40] = 0.0
+    z[1, 63] = 1e-45
+    z[2, 0] = -1e-45
+    bias = torch.zeros(64, device="cuda")
+    bias[40] = -0.0
+    for rule in (RouteRule(4, score), RouteRule(4, score, 8, 3), RouteRule(4, score, 8, 3, 1)):
+        check(z, rule)
+    # (with a bias the order is that of scores in 64 bits, where 1e-45 is nothing: rows of zeros alone)
+    check(z[:1], RouteRule(4, score), bias=bias)
+    check(z[:1], RouteRule(4, score, 8, 3), bias=bias)
+
+
 def test_poisoned_places_do_not_leak():
     # infinities and NaN at experts that are away change nothing
     E = 128

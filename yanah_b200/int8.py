@@ -74,7 +74,8 @@ def _mat(w: Int8Matrix, index: int, what: str) -> _lib.I8Mat:
 def int8_linear(x: torch.Tensor, w: Int8Matrix, out_dtype: Optional[torch.dtype] = None,
                 stream: Optional[torch.cuda.Stream] = None) -> torch.Tensor:
     """x (T, K) in fp32, bf16 or fp16 times the transpose of w (N, K): (T, N) in
-    ``out_dtype`` (default: that of x), rounded once from fp32. Any number of rows."""
+    ``out_dtype`` (default: that of x), rounded once from fp32: the sum times the row's
+    scale, times the channel's. Any number of rows."""
     dtype, dev = check_floats(x, "x"), x.get_device()
     if elsewhere(dev, stream):
         return run_there(lambda: int8_linear(x, w, out_dtype), x.device, stream, (x, *w))
