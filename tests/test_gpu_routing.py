@@ -122,6 +122,18 @@ def test_near_ties_follow_exact_arithmetic(score):
     check(logits(50, E, torch.bfloat16, seed=13).round(), RouteRule(8, score, 4, 2), bias=zero)
 
 
+@pytest.mark.parametrize("G,kept", [(32, 5), (8, 3)])
+def test_group_scores_with_large_biases(G, kept):
+    # a group's second value far below its first: its rounding to fp32 (2^-24 of 1000) is larger than the
+    # distance of many groups' scores, which the order has to settle all the same
+    E, T = 64, 700
+    z = logits(T, E, seed=G, std=0.01)
+    bias = torch.full((E,), -1000.0, device="cuda")
+    bias[::E // G] = 0.25
+    check(z, RouteRule(3, "sigmoid", G, kept), bias=bias)
+    check(z, RouteRule(3, "softmax", G, kept), bias=bias)
+
+
 def test_strides_alignment_and_many_rows():
     E = 48
     base = logits(70, 2 * E + 3, torch.bfloat16, seed=6)

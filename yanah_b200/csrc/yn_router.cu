@@ -265,7 +265,9 @@ __global__ void __launch_bounds__(32 * RT_WARPS) k_router(const RouterArgs a) {
     if (a.G > 1) {
       float far;
       in = rt_group_kept(a, lane, hi, lo, -inf, &far);
-      const float mag = f32_from_ukey(__reduce_max_sync(0xffffffffu, f32_ukey(hi == -inf ? 0.0f : fabsf(hi))));
+      // the largest of the lanes' two values: a score's terms are rounded by 2^-24 of theirs
+      const float mag = f32_from_ukey(
+          __reduce_max_sync(0xffffffffu, f32_ukey(hi == -inf ? 0.0f : lo == -inf ? fabsf(hi) : fmaxf(fabsf(hi), fabsf(lo)))));
       if (far <= 4.0f * tol + 5.0e-7f * mag) in = rt_groups_f64<T>(a, row, lane, (double)m);
 #pragma unroll
       for (int i = 0; i < NV; ++i) key[i] = in ? key[i] : 0u;
