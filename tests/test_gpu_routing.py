@@ -151,6 +151,20 @@ def test_strides_alignment_and_many_rows():
     assert ids.shape == (0, 2) and w.shape == (0, 2)
 
 
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("E,G", [(64, 1), (128, 4), (256, 8), (512, 16), (1024, 32)])
+def test_rows_that_start_anywhere(dtype, E, G):
+    # aligned rows of whole lanes are read in wide pieces, others one by one: both against the plain form
+    wide = logits(6, E + 8, dtype, seed=E)
+    bias = 0.2 * logits(1, E + 4, seed=3)[0]
+    avail = torch.rand(E, generator=torch.Generator().manual_seed(1)).cuda() < 0.8
+    for off in (0, 1, 2, 8):
+        z = wide[:, off:off + E]
+        for rule in (RouteRule(6, "sigmoid", G, max(1, G // 2), scale=2.5), RouteRule(6, "softmax", G, max(1, G // 2), 1, False)):
+            check(z, rule)
+            check(z, rule, bias=bias[off // 2:off // 2 + E], available=avail)
+
+
 def test_streams_and_graphs():
     z = logits(300, 256, seed=8)
     rule = RouteRule(8, "sigmoid", 8, 4, scale=2.5)

@@ -16,14 +16,19 @@
 //
 // One warp per row, keys in registers: L = 32 / (groups rounded up to a power of
 // two) lanes hold one group, element i of a lane being expert
-// (lane / L) * per_group + lane % L + i * L. A row is at most 4 KB, so the kernel
-// is bound by issuing instructions, not by memory. The choice takes few of them: the
+// (lane / L) * per_group + lane % L + i * L; where the groups fill their lanes and the
+// row is aligned, a lane has consecutive experts instead, read in wide pieces (16384 x
+// 256 in 8 groups, bias: 19.5 us, 24.0 one by one with the groups ranked by shuffles).
+// A row is at most 4 KB, so the kernel is bound by issuing instructions (three quarters
+// of all cycles, 1.4 us of memory traffic), not by memory, and more warps per SM change
+// nothing (10 or 12 blocks: 24.0 and 24.8 us then). The choice takes few of them: the
 // k-th largest of the 32 lane maxima (k redux) bounds the k-th largest key from
 // below; the keys that reach it, little more than k, are gathered one per lane and
 // placed by counting the larger ones.
 #include <cuda_runtime.h>
 
 #include <string>
+#include <type_traits>
 
 #include "yanah_b200.h"
 #include "yn_common.cuh"
@@ -34,6 +39,7 @@ namespace ynb {
 constexpr int RT_WARPS = 4;          // rows per block
 constexpr int RT_MAX_E = 1024;
 constexpr int RT_MAX_K = 31;         // lane k holds the first expert not chosen
+constexpr uint32_t RT_NONE = 0x007FFFFFu;   // f32_ukey(-inf): experts that take no part
 
 struct RouterArgs {
   const void* z;
@@ -59,6 +65,31 @@ YN_DEV float rt_load<__nv_bfloat16>(const void* z, long long i) {
 template <>
 YN_DEV float rt_load<__half>(const void* z, long long i) {
   return f16_to_f32(__ldg(reinterpret_cast<const uint16_t*>(z) + i));
+}
+
+// N consecutive values in pieces of up to 16 bytes.
+template <int N, typename T>
+YN_DEV void rt_load_wide(const T* p, float (&v)[N]) {
+  constexpr int W = N * sizeof(T) < 16 ? N * sizeof(T) / 4 : 4, PER = 4 / sizeof(T);   // words of a piece, values of a word
+#pragma unroll
+  for (int i = 0; i < N; i += W * PER) {
+    uint32_t w[W];
+    if constexpr (W == 1) {
+      w[0] = __ldg(reinterpret_cast<const uint32_t*>(p + i));
+    } else if constexpr (W == 2) {
+      const uint2 q = __ldg(reinterpret_cast<const uint2*>(p + i));
+      w[0] = q.x, w[1] = q.y;
+    } else {
+      const uint4 q = __ldg(reinterpret_cast<const uint4*>(p + i));
+      w[0] = q.x, w[1] = q.y, w[2] = q.z, w[3] = q.w;
+    }
+#pragma unroll
+    for (int j = 0; j < W * PER; ++j) {
+      if constexpr (sizeof(T) == 4) v[i + j] = __uint_as_float(w[j]);
+      else if constexpr (std::is_same_v<T, __half>) v[i + j] = f16_to_f32((uint16_t)(w[j / 2] >> (16 * (j & 1))));
+      else v[i + j] = __uint_as_float(j & 1 ? w[j / 2] & 0xFFFF0000u : w[j / 2] << 16);
+    }
+  }
 }
 
 YN_DEV double warp_max_f64(double v) {
@@ -94,32 +125,41 @@ struct RtLane {
   }
 };
 
-// Whether the lane's group is among the `kept` best: hi, lo are the two largest values of
-// the lane, merged over the L lanes of its group; the group's rank is by score, ties to
-// the lower group. far, or null: the smallest distance between a group that is in and one
-// that is out, for the caller's check in fp32.
+// The two largest values of the lane, merged over the L lanes of its group, as the group's score.
 template <typename F>
-YN_DEV bool rt_group_kept(const RouterArgs& a, int lane, F hi, F lo, F none, float* far) {
+YN_DEV F rt_group_score(const RouterArgs& a, F hi, F lo, F none) {
   for (int m = 1; m < a.L; m <<= 1) {
     const F h2 = __shfl_xor_sync(0xffffffffu, hi, m), l2 = __shfl_xor_sync(0xffffffffu, lo, m);
     const F mn = hi < h2 ? hi : h2, mx = hi < h2 ? h2 : hi, l = lo < l2 ? l2 : lo;
     hi = mx;
     lo = mn < l ? l : mn;
   }
-  const F score = a.group_top > 1 && lo != none ? hi + lo : hi;
+  return a.group_top > 1 && lo != none ? hi + lo : hi;
+}
+// Whether the lane's group is among the `kept` best by score, ties to the lower group.
+YN_DEV bool rt_group_kept_f64(const RouterArgs& a, int lane, double score) {
   const int g = lane >> a.log_l;
   int rank = 0;
   for (int o = 0; o < a.G; ++o) {
-    const F s = __shfl_sync(0xffffffffu, score, o << a.log_l);
+    const double s = __shfl_sync(0xffffffffu, score, o << a.log_l);
     rank += s > score || (s == score && o < g);
   }
-  const bool in = g < a.G && rank < a.kept;
-  if (far) {
-    const float lowest_in = f32_from_ukey(__reduce_min_sync(0xffffffffu, in && score != none ? f32_ukey((float)score) : ~0u));
-    const float best_out = f32_from_ukey(__reduce_max_sync(0xffffffffu, f32_ukey(!in && g < a.G ? (float)score : (float)none)));
-    *far = best_out == (float)none ? -(float)none : lowest_in - best_out;
+  return g < a.G && rank < a.kept;
+}
+// The same in fp32, a redux per kept group. far: the distance between the last group in and the
+// first one out.
+YN_DEV bool rt_group_kept(const RouterArgs& a, int lane, float score, float* far) {
+  const int g = lane >> a.log_l;
+  uint32_t k = g < a.G && (lane & (a.L - 1)) == 0 ? f32_ukey(score) : 0u, top = 0, groups = 0;
+  for (int j = 0; j < a.kept; ++j) {
+    top = __reduce_max_sync(0xffffffffu, k);
+    const int w = __ffs(__ballot_sync(0xffffffffu, k == top)) - 1;
+    groups |= 1u << (w >> a.log_l);
+    if (lane == w) k = 0;
   }
-  return in;
+  const uint32_t out = __reduce_max_sync(0xffffffffu, k);
+  *far = out <= RT_NONE ? __int_as_float(0x7f800000) : f32_from_ukey(top) - f32_from_ukey(out);
+  return (groups >> g) & 1u;
 }
 
 // A row's scores in fp64: 1 / sum exp(z - m) of a softmax (1 for sigmoids).
@@ -158,7 +198,7 @@ __device__ __noinline__ bool rt_groups_f64(const RouterArgs& a, long long row, i
     if (c > hi) { lo = hi; hi = c; }
     else if (c > lo) lo = c;
   }
-  return rt_group_kept(a, lane, hi, lo, none, (float*)nullptr);
+  return rt_group_kept_f64(a, lane, rt_group_score(a, hi, lo, none));
 }
 
 // The place of this lane's candidate (id, or -1) among the n <= 32 candidates, by fp64.
@@ -208,7 +248,9 @@ __device__ __noinline__ int rt_choose_f64(const RouterArgs& a, long long row, in
 
 // NV: elements per lane. BY_SCORE: the order needs the scores (a bias or groups);
 // otherwise the logits order the experts.
-template <typename T, int NV, bool BY_SCORE>
+// WHOLE: the row has 32 * NV experts, whose groups fill their lanes, and is aligned: a lane
+// takes NV consecutive ones in wide loads and asks for no bounds.
+template <typename T, int NV, bool BY_SCORE, bool WHOLE>
 __global__ void __launch_bounds__(32 * RT_WARPS) k_router(const RouterArgs a) {
   extern __shared__ double rt_smem[];   // BY_SCORE: E doubles per warp
   __shared__ unsigned long long cand[RT_WARPS][32];
@@ -217,16 +259,22 @@ __global__ void __launch_bounds__(32 * RT_WARPS) k_router(const RouterArgs a) {
   if (row >= a.rows) return;
   const float inf = __int_as_float(0x7f800000);
   const RtLane own(a, lane);
+  const int first = WHOLE ? NV * lane : own.first;
+  auto expert = [&](int i) { return WHOLE ? first + i : first + (i << a.log_l); };
+  auto there = [&](int i) { return WHOLE || i < own.count; };
   float v[NV];
+  if (WHOLE) {
+    rt_load_wide<NV>(reinterpret_cast<const T*>(a.z) + row * a.ld + first, v);
+  } else {
 #pragma unroll
-  for (int i = 0; i < NV; ++i) {
-    const float z = i < own.count ? rt_load<T>(a.z, row * a.ld + own.first + (i << a.log_l)) : -inf;
-    v[i] = z > -inf ? z : -inf;   // NaN too
+    for (int i = 0; i < NV; ++i) v[i] = there(i) ? rt_load<T>(a.z, row * a.ld + expert(i)) : -inf;
   }
+#pragma unroll
+  for (int i = 0; i < NV; ++i) v[i] = fmaxf(v[i], -inf);   // NaN too
   if (a.avail) {
 #pragma unroll
     for (int i = 0; i < NV; ++i)
-      if (i < own.count && !a.avail[own.first + (i << a.log_l)]) v[i] = -inf;
+      if (there(i) && !a.avail[expert(i)]) v[i] = -inf;
   }
   float m = -inf, sum = 0.0f, tol = 0.0f;
   if (BY_SCORE || (a.softmax && !a.norm)) {
@@ -250,31 +298,33 @@ __global__ void __launch_bounds__(32 * RT_WARPS) k_router(const RouterArgs a) {
     // below 1e-30 are not told apart.
     const float inv = a.softmax ? 1.0f / sum : 1.0f;
     tol = (a.softmax ? 1.6e-5f * inv : 2.0e-6f * rt_sigmoid(m)) + 1e-30f;
-    float hi = -inf, lo = -inf;
+    float hi = -inf, lo = -inf, b[NV];
+    if (WHOLE && a.bias) {
+      rt_load_wide<NV>(a.bias + first, b);
+    } else {
+#pragma unroll
+      for (int i = 0; i < NV; ++i) b[i] = a.bias && there(i) ? __ldg(a.bias + expert(i)) : 0.0f;
+    }
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
       const float s = a.softmax ? (v[i] == m ? inv : rt_ex2((v[i] - m) * RT_LOG2E) * inv) : rt_sigmoid(v[i]);
-      float c = s;
-      if (a.bias) c += i < own.count ? __ldg(a.bias + own.first + (i << a.log_l)) : 0.0f;
-      c = v[i] > -inf && c > -inf ? c : -inf;   // a bias of -inf or NaN takes the expert out
+      const float c = v[i] > -inf ? fmaxf(s + b[i], -inf) : -inf;   // a bias of -inf or NaN takes the expert out
       lo = fmaxf(lo, fminf(hi, c));
       hi = fmaxf(hi, c);
       // without a bias the logits have the scores' order, exactly
-      key[i] = c > -inf ? f32_ukey(a.bias ? c : v[i]) : 0u;
+      key[i] = f32_ukey(a.bias ? c : v[i]);
     }
     if (a.G > 1) {
       float far;
-      in = rt_group_kept(a, lane, hi, lo, -inf, &far);
+      in = rt_group_kept(a, lane, rt_group_score(a, hi, lo, -inf), &far);
       // the largest of the lanes' two values: a score's terms are rounded by 2^-24 of theirs
-      const float mag = f32_from_ukey(
-          __reduce_max_sync(0xffffffffu, f32_ukey(hi == -inf ? 0.0f : lo == -inf ? fabsf(hi) : fmaxf(fabsf(hi), fabsf(lo)))));
+      const float mag = __uint_as_float(__reduce_max_sync(
+          0xffffffffu, __float_as_uint(hi == -inf ? 0.0f : lo == -inf ? fabsf(hi) : fmaxf(fabsf(hi), fabsf(lo)))));
       if (far <= 4.0f * tol + 5.0e-7f * mag) in = rt_groups_f64<T>(a, row, lane, (double)m);
-#pragma unroll
-      for (int i = 0; i < NV; ++i) key[i] = in ? key[i] : 0u;
     }
   } else {
 #pragma unroll
-    for (int i = 0; i < NV; ++i) key[i] = v[i] == -inf ? 0u : f32_ukey(v[i]);
+    for (int i = 0; i < NV; ++i) key[i] = f32_ukey(v[i]);
   }
   // The first K (one more where neighbours are compared), descending, ties to the lower id.
   const bool compared = BY_SCORE && a.bias;
@@ -282,15 +332,16 @@ __global__ void __launch_bounds__(32 * RT_WARPS) k_router(const RouterArgs a) {
   uint32_t cur = 0, bound = 0;
 #pragma unroll
   for (int i = 0; i < NV; ++i) cur = max(cur, key[i]);
+  cur = in ? cur : 0u;
   for (int j = 0; j < places; ++j) {
     bound = __reduce_max_sync(0xffffffffu, cur);
     if (cur == bound) cur = 0;   // equal lane maxima go together: the bound is lower then, and still one
   }
-  if (compared && bound > 0) {   // whatever might be as large as the bound in exact arithmetic is a candidate too
+  if (compared && bound > RT_NONE) {   // whatever might be as large as the bound in exact arithmetic is a candidate too
     const float c = f32_from_ukey(bound);
     bound = f32_ukey(fmaxf(c - 2.0f * tol - 2.5e-7f * fabsf(c), -3.402823466e38f));
   }
-  bound = max(bound, 1u);
+  bound = in ? max(bound, RT_NONE + 1u) : ~0u;
   // one lane's candidates side by side, the lanes one after another (their order does not matter)
   int own_n = 0;
 #pragma unroll
@@ -307,7 +358,7 @@ __global__ void __launch_bounds__(32 * RT_WARPS) k_router(const RouterArgs a) {
 #pragma unroll
     for (int i = 0; i < NV; ++i)
       if (key[i] >= bound)
-        cand[warp][at++] = ((unsigned long long)key[i] << 32) | (0xFFFFFFFFu - (uint32_t)(own.first + (i << a.log_l)));
+        cand[warp][at++] = ((unsigned long long)key[i] << 32) | (0xFFFFFFFFu - (uint32_t)expert(i));
   }
   int mine = -1;
   uint32_t my_key = 0;
@@ -327,14 +378,14 @@ __global__ void __launch_bounds__(32 * RT_WARPS) k_router(const RouterArgs a) {
   } else {
     // many near keys, or k near 32: one after another, two redux each
     for (int j = 0; j < places; ++j) {
-      uint32_t best = 0;
+      uint32_t best = RT_NONE;
       int bi = 0;
 #pragma unroll
       for (int i = 0; i < NV; ++i)
-        if (key[i] > best) { best = key[i]; bi = i; }
+        if (in && key[i] > best) { best = key[i]; bi = i; }
       const uint32_t top = __reduce_max_sync(0xffffffffu, best);
-      if (top == 0) break;
-      const int e = best == top ? own.first + (bi << a.log_l) : RT_MAX_E;
+      if (top == RT_NONE) break;
+      const int e = best == top ? expert(bi) : RT_MAX_E;
       const int id = (int)__reduce_min_sync(0xffffffffu, (unsigned)e);
       if (e == id) {
 #pragma unroll
@@ -346,16 +397,16 @@ __global__ void __launch_bounds__(32 * RT_WARPS) k_router(const RouterArgs a) {
   }
   float z = mine >= 0 ? rt_load<T>(a.z, row * a.ld + mine) : -inf;
   if (compared) {
-    const float b = mine >= 0 ? __ldg(a.bias + mine) : 0.0f;
     const int nid = __shfl_down_sync(0xffffffffu, mine, 1);
-    const float nz = __shfl_down_sync(0xffffffffu, z, 1), nb = __shfl_down_sync(0xffffffffu, b, 1);
     const uint32_t nk = __shfl_down_sync(0xffffffffu, my_key, 1);
     bool near = false;
-    // equal logits with equal biases are equal in exact arithmetic too, except at the last place: what is
-    // near the first one left out is not looked at
-    if (lane < a.K && lane < 31 && mine >= 0 && nid >= 0 && !(z == nz && b == nb && lane < a.K - 1)) {
+    if (lane < a.K && mine >= 0 && nid >= 0) {   // K < 32: lane K has the first one left out
       const float c = f32_from_ukey(my_key), nc = f32_from_ukey(nk);
       near = c - nc <= 2.0f * tol + 2.5e-7f * fmaxf(fabsf(c), fabsf(nc));
+      // equal logits with equal biases are equal in exact arithmetic too, except at the last place: what is
+      // near the first one left out is not looked at
+      if (near && lane < a.K - 1)
+        near = z != rt_load<T>(a.z, row * a.ld + nid) || __ldg(a.bias + mine) != __ldg(a.bias + nid);
     }
     if (__any_sync(0xffffffffu, near)) {
       if (n <= 32) {
@@ -392,17 +443,32 @@ __global__ void __launch_bounds__(32 * RT_WARPS) k_router(const RouterArgs a) {
   }
 }
 
+template <typename T, int NV, bool BY_SCORE>
+void launch_router_nv(const RouterArgs& a, dim3 grid, size_t smem, cudaStream_t st) {
+  const dim3 b(32 * RT_WARPS);
+  constexpr size_t ZA = NV * sizeof(T) < 16 ? NV * sizeof(T) : 16, BA = NV * 4 < 16 ? NV * 4 : 16;
+  // groups that are a power of two fill their lanes
+  const bool whole = a.E == 32 * NV && a.G * a.L == 32 && reinterpret_cast<uintptr_t>(a.z) % ZA == 0 &&
+                     (a.ld * sizeof(T)) % ZA == 0 && reinterpret_cast<uintptr_t>(a.bias) % BA == 0;
+  if constexpr (NV <= 32) {
+    if (whole) {
+      k_router<T, NV, BY_SCORE, true><<<grid, b, smem, st>>>(a);
+      return;
+    }
+  }
+  k_router<T, NV, BY_SCORE, false><<<grid, b, smem, st>>>(a);
+}
+
 template <typename T, bool BY_SCORE>
 void launch_router(const RouterArgs& a, int nv, cudaStream_t st) {
   const unsigned grid = (unsigned)((a.rows + RT_WARPS - 1) / RT_WARPS);
   const size_t smem = BY_SCORE ? (size_t)RT_WARPS * a.E * sizeof(double) : 0;
-  const dim3 b(32 * RT_WARPS);
-  if (nv <= 2) k_router<T, 2, BY_SCORE><<<grid, b, smem, st>>>(a);
-  else if (nv <= 4) k_router<T, 4, BY_SCORE><<<grid, b, smem, st>>>(a);
-  else if (nv <= 8) k_router<T, 8, BY_SCORE><<<grid, b, smem, st>>>(a);
-  else if (nv <= 16) k_router<T, 16, BY_SCORE><<<grid, b, smem, st>>>(a);
-  else if (nv <= 32) k_router<T, 32, BY_SCORE><<<grid, b, smem, st>>>(a);
-  else k_router<T, 64, BY_SCORE><<<grid, b, smem, st>>>(a);
+  if (nv <= 2) launch_router_nv<T, 2, BY_SCORE>(a, grid, smem, st);
+  else if (nv <= 4) launch_router_nv<T, 4, BY_SCORE>(a, grid, smem, st);
+  else if (nv <= 8) launch_router_nv<T, 8, BY_SCORE>(a, grid, smem, st);
+  else if (nv <= 16) launch_router_nv<T, 16, BY_SCORE>(a, grid, smem, st);
+  else if (nv <= 32) launch_router_nv<T, 32, BY_SCORE>(a, grid, smem, st);
+  else launch_router_nv<T, 64, BY_SCORE>(a, grid, smem, st);
 }
 
 }  // namespace ynb
