@@ -43,8 +43,8 @@ def quantize_rows(x: torch.Tensor, stream: Optional[torch.cuda.Stream] = None) -
     lead, k = x.shape[:-1], x.shape[-1]
     flat, rows, k, stride = rows_of(x.reshape(-1, k), "x")
     pitch = (k + 15) // 16 * 16
-    codes = x.new_empty((rows, pitch), dtype=torch.int8)
-    scales = x.new_empty((rows,), dtype=torch.float32)
+    codes = x.new_empty(rows, pitch, dtype=torch.int8)
+    scales = x.new_empty(rows, dtype=torch.float32)
     _lib.check(_lib.lib().yn_i8_quant_rows(flat.data_ptr(), dtype, stride, rows, k, codes.data_ptr(), pitch,
                                            scales.data_ptr(), raw_stream(dev)))
     return Int8Matrix(codes.view(*lead, pitch)[..., :k], scales.view(lead))
@@ -89,10 +89,10 @@ def int8_linear(x: torch.Tensor, w: Int8Matrix, out_dtype: Optional[torch.dtype]
     if out_dtype not in DTYPES:
         raise TypeError(f"out_dtype must be float32, bfloat16 or float16, not {out_dtype}")
     n = m.rows
-    y = x.new_empty((rows, n), dtype=out_dtype)
+    y = x.new_empty(rows, n, dtype=out_dtype)
     lib = _lib.lib()
     nb = lib.yn_i8_linear_ws_bytes(rows, k)
-    ws = x.new_empty((nb,), dtype=torch.uint8) if nb else None
+    ws = x.new_empty(nb, dtype=torch.uint8) if nb else None
     _lib.check(lib.yn_i8_linear(C.byref(m), x.data_ptr(), dtype, stride, rows, y.data_ptr(), DTYPES[out_dtype], n,
                                 None if ws is None else ws.data_ptr(), nb, raw_stream(dev)))
     return y
@@ -128,7 +128,7 @@ def int8_experts(x: torch.Tensor, ids: torch.Tensor, weights: torch.Tensor, gate
         residual, _, _, res_stride = rows_of(residual, "residual")
         p_res = residual.data_ptr()
     if out is None:
-        out = x.new_empty((rows, h))
+        out = x.new_empty(rows, h)
     else:
         check_like(out, dev, (rows, h), (x.dtype,), "out")
         same, _, _, out_stride = rows_of(out, "out")
@@ -136,7 +136,7 @@ def int8_experts(x: torch.Tensor, ids: torch.Tensor, weights: torch.Tensor, gate
             raise ValueError("out must have rows of adjacent elements that do not overlap")
     lib = _lib.lib()
     nb = lib.yn_i8_experts_ws_bytes(rows, k, g.n_mats, h, g.rows, dtype)
-    ws = x.new_empty((nb,), dtype=torch.uint8)
+    ws = x.new_empty(nb, dtype=torch.uint8)
     _lib.check(lib.yn_i8_experts(C.byref(g), C.byref(u), C.byref(d), x.data_ptr(), dtype, stride, rows, ids.data_ptr(),
                                  weights.data_ptr(), k, p_res, res_stride, out.data_ptr(), out_stride, ws.data_ptr(), nb,
                                  raw_stream(dev)))

@@ -45,17 +45,18 @@ def token_logprobs(logits: torch.Tensor, tokens: Optional[torch.Tensor] = None, 
         raise ValueError("logits must have at least one column")
     if not 0 <= n_top <= min(64, vocab):
         raise ValueError(f"n_top must be in [0, {min(64, vocab)}], not {n_top}")
-    new, f32, i32 = logits.new_empty, torch.float32, torch.int32
-    entropy = new((rows,), dtype=f32)
+    f32, i32, like = torch.float32, torch.int32, torch.empty_like
+    entropy = logits.new_empty(rows, dtype=f32)
     logprob = rank = top_ids = top_lp = None
     p_tokens = p_logprob = p_rank = p_ids = p_top = None
     if tokens is not None:
         check_like(tokens, dev, (rows,), (i32,), "tokens")
         tokens = tokens.contiguous()
-        logprob, rank = new((rows,), dtype=f32), new((rows,), dtype=i32)
+        logprob, rank = like(entropy), like(entropy, dtype=i32)
         p_tokens, p_logprob, p_rank = tokens.data_ptr(), logprob.data_ptr(), rank.data_ptr()
     if n_top:
-        top_ids, top_lp = new((rows, n_top), dtype=i32), new((rows, n_top), dtype=f32)
+        top_ids = logits.new_empty(rows, n_top, dtype=i32)
+        top_lp = like(top_ids, dtype=f32)
         p_ids, p_top = top_ids.data_ptr(), top_lp.data_ptr()
     _lib.check(_lib.lib().yn_token_logprobs(logits.data_ptr(), dtype, stride, rows, vocab, p_tokens, n_top, p_logprob,
                                             entropy.data_ptr(), p_rank, p_ids, p_top, raw_stream(dev)))

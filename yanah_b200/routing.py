@@ -72,8 +72,8 @@ def route_scored(logits: torch.Tensor, rule: RouteRule, bias: Optional[torch.Ten
         check_like(available, dev, (e,), (torch.bool, torch.uint8), "available")
         available = available.contiguous()
     if out is None:
-        ids = logits.new_empty((rows, rule.top_k), dtype=torch.int32)
-        weights = logits.new_empty((rows, rule.top_k), dtype=torch.float32)
+        ids = logits.new_empty(rows, rule.top_k, dtype=torch.int32)
+        weights = torch.empty_like(ids, dtype=torch.float32)
     else:
         ids, weights = out
         check_like(ids, dev, (rows, rule.top_k), (torch.int32,), "out ids")
