@@ -52,23 +52,29 @@ def quantize_rows(x: torch.Tensor, stream: Optional[torch.cuda.Stream] = None) -
 
 def _mat(w: Int8Matrix, index: int, what: str) -> _lib.I8Mat:
     codes, scales = w
-    shape, strides = codes.shape, codes.stride()
+    shape, strides, s_strides = codes.shape, codes.stride(), scales.stride()
     if codes.dtype is not torch.int8 or scales.dtype is not torch.float32:
         raise TypeError(f"{what} must have int8 codes and float32 scales")
-    if len(shape) not in (2, 3) or scales.shape != shape[:-1]:
+    if len(shape) == 3:
+        mats, n, k = shape
+        alike = scales.shape == (mats, n)
+    elif len(shape) == 2:
+        mats, (n, k) = 1, shape
+        alike = scales.shape == (n,)
+    else:
+        alike = False
+    if not alike:
         raise ValueError(f"{what}: codes (N, K) or (E, N, K) with scales (N) or (E, N)")
     if codes.get_device() != index or scales.get_device() != index:
         raise ValueError(f"{what} is not on cuda:{index}")
     if scales.requires_grad:
         check_no_grad(f"{what}'s scales")
-    n, k = shape[-2:]
-    s_strides = scales.stride()
     if (k > 1 and strides[-1] != 1) or (n > 1 and s_strides[-1] != 1):
         raise ValueError(f"{what}: a row's codes and a matrix's scales must be adjacent")
     rs = strides[-2] if n > 1 else (k + 15) // 16 * 16
-    if len(shape) == 3 and shape[0] > 1:
-        return _lib.I8Mat(codes.data_ptr(), scales.data_ptr(), rs, strides[0], s_strides[0], shape[0], n, k)
-    return _lib.I8Mat(codes.data_ptr(), scales.data_ptr(), rs, rs * n, n, shape[0] if len(shape) == 3 else 1, n, k)
+    if mats > 1:
+        return _lib.I8Mat(codes.data_ptr(), scales.data_ptr(), rs, strides[0], s_strides[0], mats, n, k)
+    return _lib.I8Mat(codes.data_ptr(), scales.data_ptr(), rs, rs * n, n, mats, n, k)
 
 
 def int8_linear(x: torch.Tensor, w: Int8Matrix, out_dtype: Optional[torch.dtype] = None,
