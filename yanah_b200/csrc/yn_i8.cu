@@ -258,8 +258,8 @@ YN_DEV void i8_dots(const int8_t* const (&w)[R], const int8_t* xs, int KP, int K
 
 // y (T, N) of T <= 5 rows: every block makes the rows' codes itself (they are a few KB),
 // then its warps take 4 output channels at a time through the matrix, which is read once:
-// bound by that read with one row (2048 x 151936: 47.5 us, 6.57 TB/s), with five by the
-// products too (58 us). A lane copies its own 16 codes of 4 channels per step into a ring of
+// bound by that read with one row (2048 x 151936: 47.4 us, 6.57 TB/s), with five by the
+// products too (59 us). A lane copies its own 16 codes of 4 channels per step into a ring of
 // its warp (cp.async, I8_FS steps deep, 144 KB in flight per SM) and reads them back itself,
 // so that neither the products nor the sums over lanes stop the copies and no thread waits
 // for another. Loads into registers instead (8 per lane in flight) took 71 us for five rows,
@@ -690,8 +690,8 @@ I8Mat mat_of(const yn_i8_mat& w) {
 }
 
 constexpr int I8_MAX_K = 131072;   // 127^2 * 131072 < 2^31
-// Rows of a product on dp4a. Six rows of 2048 x 151936 take 72 us so, and 66 us on the tensor
-// cores with their codes made first.
+// Rows of a product on dp4a. One row of 2048 x 151936 takes 47 us so, five 59 and six 72; any of
+// them 58 us on the tensor cores with their codes made first (2048 x 4096: 4.0, 6.7 and 10.6 us).
 constexpr int I8_FEW = 5;
 
 int check_mat(const yn_i8_mat& w, const char* what) {
@@ -729,12 +729,12 @@ struct ExpertsWs {
   int nb;
 };
 // Rows per chunk of an expert, by the pairs per expert (see launch_gemm_nb). On 512 experts of 3 MB 64
-// and 256 rows take 129 and 136 us at 5 pairs per expert, 176 and 183 at 10, 248 and 241 at 20; on 64
-// experts of 9 MB 105 and 108 us at 7.5, 126 and 122 at 12.5, 174 and 149 at 38.
+// and 256 rows take 126 and 132 us at 5 pairs per expert, 167 and 175 at 10, 235 and 229 at 20; on 64
+// experts of 9 MB 103 and 102 us at 7.5, 120 and 119 at 12.5, 166 and 143 at 38.
 int chunk_rows(long long pairs, int E) { return pairs <= 10ll * E ? 64 : 256; }
 // Pairs that go to the dp4a kernels: two launches instead of six, but they read an expert's matrices
 // for every pair. The two ways meet at about 190 MB of such reads: 60 pairs on 3 MB experts take 41
-// us so and 46 us grouped (80: 53 and 47), 20 pairs on 9 MB experts 44 and 47 us (32: 61 and 54).
+// us so and 43 us grouped (80: 52 and 44), 16 pairs on 9 MB experts 36 and 35 us (20: 44 and 41).
 bool experts_few(long long pairs, int k, int H, int I) {
   return (pairs <= 8 || (pairs <= 64 && pairs * 3 * H * I <= 192000000ll)) && up_to(H, I8_GK) <= 96 * 1024 &&
          k * up_to(I, I8_GK) <= 96 * 1024;
