@@ -33,14 +33,15 @@ constexpr long long I8_QWARP = 1184;   // rows from which a warp each fills the 
 // rows, a warp where there are many (no barrier, 8 loads in flight per lane). Rows of up to
 // N * 8 * HOLD elements are read once, longer ones a second time from L2. The codes go to row
 // `to[j]` for each of the `copies` entries of the row's list (or to the row itself): a row's
-// codes are made once for all of its experts.
+// codes are made once for all of its experts. late: the kernel before makes the lists, not the
+// rows, and is waited for when the codes are made.
 template <typename T, bool VEC, int N, int HOLD>
 __global__ void __launch_bounds__(I8_QT) k_i8_quant(const void* x, long long ldx, long long rows, int K, const int* n_rows,
                                                     const int32_t* to, int copies, int8_t* codes, long long ldc,
-                                                    float* scales) {
+                                                    float* scales, bool late) {
   __shared__ uint32_t buf[I8_QT / 32];
   i8_launch_next();
-  i8_wait_previous();
+  if (!late) i8_wait_previous();
   const size_t row = blockIdx.x * (size_t)(I8_QT / N) + threadIdx.x / N, base = row * (size_t)ldx;
   if (row >= (size_t)(n_rows ? *n_rows : rows)) return;
   const int tid = threadIdx.x % N, n8 = VEC ? K / 8 : 0;
@@ -64,10 +65,6 @@ __global__ void __launch_bounds__(I8_QT) k_i8_quant(const void* x, long long ldx
   }
   for (int k = 8 * n8 + tid; k < K; k += N) m = max(m, i8_abs_bits(I8In<T>::load(x, base + k)));
   const I8Row q(N == 32 ? __reduce_max_sync(0xffffffffu, m) : block_max_u32(m, buf));
-  // lane j of every warp has destination j
-  const int lane = threadIdx.x & 31, n_to = to ? copies : 1;
-  const int dest = lane < n_to ? (to ? to[row * copies + lane] : (int)row) : -1;
-  if (tid < n_to && dest >= 0) scales[dest] = q.scale();
   auto code8 = [&](const I8Raw<T>& r) {
     float g[8];
     uint32_t w[2];
@@ -79,6 +76,11 @@ __global__ void __launch_bounds__(I8_QT) k_i8_quant(const void* x, long long ldx
 #pragma unroll
   for (int i = 0; i < HOLD; ++i)
     if (tid + i * N < n8) c[i] = code8(raw[i]);
+  if (late) i8_wait_previous();
+  // lane j of every warp has destination j
+  const int lane = threadIdx.x & 31, n_to = to ? copies : 1;
+  const int dest = lane < n_to ? (to ? to[row * copies + lane] : (int)row) : -1;
+  if (tid < n_to && dest >= 0) scales[dest] = q.scale();
   for (int j = 0; j < n_to; ++j) {
     const int r = __shfl_sync(0xffffffffu, dest, j);
     if (r < 0) continue;
@@ -134,8 +136,8 @@ int launch_quant(int dt, const void* x, long long ldx, long long rows, int K, co
   const bool warps = vec && rows >= I8_QWARP && K <= 4096;
   const dim3 g((unsigned)(warps ? (rows + I8_QT / 32 - 1) / (I8_QT / 32) : rows));
   auto go = [&](auto kern) {
-    if (first) kern<<<g, I8_QT, 0, st>>>(x, ldx, rows, K, n_rows, to, copies, codes, ldc, scales);
-    else launch_after(kern, g, I8_QT, 0, st, x, ldx, rows, K, n_rows, to, copies, codes, ldc, scales);
+    if (first) kern<<<g, I8_QT, 0, st>>>(x, ldx, rows, K, n_rows, to, copies, codes, ldc, scales, false);
+    else launch_after(kern, g, I8_QT, 0, st, x, ldx, rows, K, n_rows, to, copies, codes, ldc, scales, to != nullptr);
   };
 #define YN_Q(T)                                                       \
   if (warps) go(k_i8_quant<T, true, 32, sizeof(T) == 4 ? 6 : 8>);     \

@@ -5,8 +5,9 @@
 //
 // Row codes: a = max |x|, scale = a / 127, q = the whole number nearest to 127 x / a,
 // ties to even. The nearest one exactly: x with an 8- or 11-bit mantissa meets ties
-// often (x = a / 2), so quotients within 2^-14 of a tie are taken again in fp64, where
-// neither product nor quotient can reach or leave a tie by rounding.
+// often (x = a / 2), so quotients within 2^-14 of a tie are settled by the remainder 127 x -
+// q a, which fp32 holds exactly for 16-bit inputs, or for fp32 inputs taken again in fp64,
+// where neither product nor quotient can reach or leave a tie by rounding.
 #pragma once
 #include <type_traits>
 
@@ -377,7 +378,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(I8_THREADS, 1)
     // Tiles of few rows are short (4 stages of K 512 come in 1.6 us) and draining one is a chain of
     // TMEM loads, exchanges and stores that takes longer: every accumulator has warps of its own then,
     // which take every 4th tile (2048 x 512 experts, 166 MB: 49 -> 41 us). All warps on each tile
-    // is better for long ones (4096 x 2048 x 16384: 115 us, 121 us in groups). A tile's scales are
+    // is better for long ones (4096 x 2048 x 16384: 115 us, 121 us in groups, when measured). A tile's scales are
     // loaded while the group's tile before it is drained.
     const int q = warp & 3, group = (warp >> 2) % F::GROUPS, part = (warp >> 2) / F::GROUPS;
     const int r_in = UP ? 16 * q + (lane & 15) : 32 * q + lane, ahead = F::GROUPS * step;
