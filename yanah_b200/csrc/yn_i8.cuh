@@ -153,10 +153,8 @@ YN_DEV uint32_t block_max_u32(uint32_t v, uint32_t* buf) {
 // (its own TMEM lanes) and half of the rows' codes in its shared memory; the pair's MMA (M
 // 256, kind::i8) reads both halves, so a row's codes cross from L2 once per pair and a stage
 // moves 32 KB per SM for 512 cycles of MMA where one block alone would move 48 KB (4096 rows
-// of 64 experts: 334 us, 346 with single blocks). 4096 x 2048 x 16384 takes 108 us in single
-// launches, 82 at the tensor cores' nominal rate; without its loads it takes 102 us, without
-// its epilogue 91, without both 86. Run after run the card's power limit holds it (1.55 GHz of
-// 1.97 at 956 W; operands of zeros run at the full clock and take 15% less).
+// of 64 experts: 334 us, 346 with single blocks). 4096 x 2048 x 16384 takes 92 us in single
+// launches, 66 without its loads and its epilogue. Run after run the card's power limit holds it.
 // A = the channels' codes, B = the rows' codes, both K-major in the 128-byte swizzled layout
 // by TMA, 128 codes of K per stage (four MMAs of K 32); the accumulator is channels (lanes) x
 // rows (columns), int32. UP interleaves 16 rows of the gate matrix with 16 of the up matrix,
@@ -211,6 +209,13 @@ YN_DEV void i8_commit_both(uint64_t* bar) {
 YN_DEV uint32_t i8_idesc(int n) {
   return (2u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)(n >> 3) << 17) | (16u << 24);
 }
+// One thread of a converged warp. Under its predicate the compiler keeps the operands of copies and
+// products in uniform registers; under `lane == 0` it moves each of them there for every instruction.
+YN_DEV bool i8_elect() {
+  uint32_t one;
+  asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(one));
+  return one != 0;
+}
 YN_DEV uint32_t i8_rank() {
   uint32_t r;
   asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
@@ -228,23 +233,36 @@ YN_DEV void i8_arrive_at(uint32_t cluster_bar) {
 YN_DEV void i8_cluster_sync() {
   asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
+// Copies and commits complete a barrier of this block by themselves; only where threads of the other
+// block arrive does a wait have to acquire from the cluster, which costs far more.
+template <bool CLUSTER>
 YN_DEV bool i8_try_wait(uint64_t* bar, uint32_t phase) {
   uint32_t ok;
-  asm volatile(
-      "{\n\t.reg .pred p;\n\t"
-      "mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n\t"
-      "selp.u32 %0, 1, 0, p;\n\t}"
-      : "=r"(ok)
-      : "r"(smem_u32(bar)), "r"(phase)
-      : "memory");
+  if (CLUSTER)
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t}"
+        : "=r"(ok)
+        : "r"(smem_u32(bar)), "r"(phase)
+        : "memory");
+  else
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "mbarrier.try_wait.parity.acquire.cta.shared::cta.b64 p, [%1], %2;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t}"
+        : "=r"(ok)
+        : "r"(smem_u32(bar)), "r"(phase)
+        : "memory");
   return ok != 0;
 }
 // A wait of one thread, at most 1 s: on a timeout the error word is set and every role leaves
 // its loop.
+template <bool CLUSTER = false>
 YN_DEV bool i8_wait1(uint64_t* bar, uint32_t phase, int* err) {
-  if (i8_try_wait(bar, phase)) return true;
+  if (i8_try_wait<CLUSTER>(bar, phase)) return true;
   const uint64_t t0 = globaltimer_ns();
-  while (!i8_try_wait(bar, phase))
+  while (!i8_try_wait<CLUSTER>(bar, phase))
     if (globaltimer_ns() - t0 > 1000000000ull) {
       raise_error(err, YN_ERR_BULK_TIMEOUT);
       return false;
@@ -471,9 +489,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(I8_THREADS, 1)
       if (lane == 0) i8_arrive_at(i8_leader(&acc_empty[b]));
     }
   } else if (warp == I8_MW) {
-    // One thread: few MMAs wait in the tensor core's queue, so what it does between them counts
-    // (whole warps that elected a lane for each step took 116 us, this 108, at 4096 x 2048 x 16384).
-    if (lane == 0 && rank == 0) {
+    // One elected thread: few MMAs wait in the tensor core's queue, so what it does between them
+    // counts (4096 x 2048 x 16384: 92 us; 104 by lane 0, 116 by whole warps that elected one per step).
+    if (i8_elect() && rank == 0) {
       int j = 0, s = 0;
       uint32_t full_phase = 0;
       const uint64_t a0 = tc_desc(smem_u32(smem)), b0 = tc_desc(smem_u32(smem) + I8_A_BYTES);
@@ -481,7 +499,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(I8_THREADS, 1)
         const int n = next.c.n, b = j % F::ACC;
         next = after;
         after = tile(ti + 2 * step);
-        if (j >= F::ACC) ok = i8_wait1(&acc_empty[b], (uint32_t)(j / F::ACC - 1) & 1, err);
+        if (j >= F::ACC) ok = i8_wait1<true>(&acc_empty[b], (uint32_t)(j / F::ACC - 1) & 1, err);
         tc_fence_after();
         const uint32_t idesc = i8_idesc((n + 31) & ~31), dcol = tmem + (uint32_t)(b * NB);
         for (int kc = 0; kc < NK && ok; ++kc) {
@@ -504,7 +522,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(I8_THREADS, 1)
     }
     __syncwarp();
   } else {
-    if (lane == 0) {
+    if (i8_elect()) {
       int s = 0, used = 0;
       uint32_t empty_phase = 1;   // the first round finds the ring empty
       for (int ti = t0; ti < n_tiles && ok; ti += step) {
