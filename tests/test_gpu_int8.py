@@ -106,6 +106,15 @@ def test_linear(dtype, T, K, N):
     check_linear(x, matrix(N, cols=K, seed=N), torch.float32)
 
 
+@pytest.mark.parametrize("T", [1, 3, 4, 5, 6])
+def test_linear_few_rows_of_a_large_matrix(T):
+    # above 16 M codes four rows and more run on the tensor cores
+    w = matrix(8200, cols=2048, seed=2)
+    x = normal(T, 2048, seed=T, dtype=torch.bfloat16)
+    y = check_linear(x, w, torch.float32)
+    assert torch.equal(int8_linear(torch.cat((x, x)), w, torch.float32), torch.cat((y, y)))
+
+
 @pytest.mark.parametrize("T", [1, 8, 9, 70])
 @pytest.mark.parametrize("K,N", [(1, 1), (16, 1), (15, 130), (4096, 64), (4111, 5), (30000, 17), (131072, 3)])
 def test_linear_edges(T, K, N):

@@ -258,7 +258,7 @@ YN_DEV void i8_dots(const int8_t* const (&w)[R], const int8_t* xs, int KP, int K
     for (int t = 0; t < T; ++t) acc[r][t] = __reduce_add_sync(0xffffffffu, acc[r][t]);
 }
 
-// y (T, N) of T <= 5 rows: every block makes the rows' codes itself (they are a few KB),
+// y (T, N) of T <= 5 rows (linear_few): every block makes the rows' codes itself (they are a few KB),
 // then its warps take 4 output channels at a time through the matrix, which is read once:
 // bound by that read with one row (2048 x 151936: 47.4 us, 6.57 TB/s), with five by the
 // products too (59 us). A lane copies its own 16 codes of 4 channels per step into a ring of
@@ -692,9 +692,11 @@ I8Mat mat_of(const yn_i8_mat& w) {
 }
 
 constexpr int I8_MAX_K = 131072;   // 127^2 * 131072 < 2^31
-// Rows of a product on dp4a. One row of 2048 x 151936 takes 47 us so, five 59 and six 72; any of
-// them 58 us on the tensor cores with their codes made first (2048 x 4096: 4.0, 6.7 and 10.6 us).
-constexpr int I8_FEW = 5;
+// Rows of a product on dp4a: three, or five of a small matrix, where a launch counts. 2048 x 151936:
+// 47 us one row, 51.5 three, 53.6 four, 58.7 five; on the tensor cores, codes made first, 51 to 53.6.
+// 2048 x 16384: 6.4, 8.9, 9.8, 11.3 and 8.3; 2048 x 4096: 4.0, 5.6, 5.8, 6.6 and 8.0.
+constexpr int I8_FEW = 3, I8_FEW_SMALL = 5;
+constexpr long long I8_SMALL = 16ll << 20;   // codes
 
 int check_mat(const yn_i8_mat& w, const char* what) {
   const std::string n(what);
@@ -709,7 +711,9 @@ int check_mat(const yn_i8_mat& w, const char* what) {
   return YN_OK;
 }
 
-bool linear_few(long long rows, long long k) { return rows <= I8_FEW && rows * (long long)up_to(k, I8_GK) <= 96 * 1024; }
+bool linear_few(long long rows, long long k, long long n) {
+  return rows <= (n * k <= I8_SMALL ? I8_FEW_SMALL : I8_FEW) && rows * (long long)up_to(k, I8_GK) <= 96 * 1024;
+}
 
 template <int T>
 int launch_few(int dt, const void* x, long long ldx, int K, const I8Mat& w, int N, int odt, void* y, long long ldy, int sms,
@@ -731,14 +735,14 @@ struct ExpertsWs {
   int nb;
 };
 // Rows per chunk of an expert, by the pairs per expert (see launch_gemm_nb). On 512 experts of 3 MB 64
-// and 256 rows take 126 and 132 us at 5 pairs per expert, 167 and 175 at 10, 235 and 229 at 20; on 64
-// experts of 9 MB 103 and 102 us at 7.5, 120 and 119 at 12.5, 166 and 143 at 38.
-int chunk_rows(long long pairs, int E) { return pairs <= 10ll * E ? 64 : 256; }
+// and 256 rows take 111 and 126 us at 5 pairs per expert, 141 and 167 at 10, 196 and 218 at 20; on 64
+// experts of 9 MB 92 and 93 us at 7.5, 117 and 121 at 19, 136 and 132 at 38, 173 and 159 at 75.
+int chunk_rows(long long pairs, int E) { return pairs <= 24ll * E ? 64 : 256; }
 // Pairs that go to the dp4a kernels: two launches instead of six, but they read an expert's matrices
-// for every pair. The two ways meet at about 190 MB of such reads: 60 pairs on 3 MB experts take 41
-// us so and 43 us grouped (80: 52 and 44), 16 pairs on 9 MB experts 36 and 35 us (20: 44 and 41).
+// for every pair. The two ways meet at about 120 MB of such reads: 30 pairs on 3 MB experts take 26 us so
+// and 32 us grouped (40: 30 and 31, 50: 39 and 34), 8 pairs on 9 MB experts 21.5 and 27 us (16: 36 and 28).
 bool experts_few(long long pairs, int k, int H, int I) {
-  return (pairs <= 8 || (pairs <= 64 && pairs * 3 * H * I <= 192000000ll)) && up_to(H, I8_GK) <= 96 * 1024 &&
+  return (pairs <= 8 || (pairs <= 64 && pairs * 3 * H * I <= 120000000ll)) && up_to(H, I8_GK) <= 96 * 1024 &&
          k * up_to(I, I8_GK) <= 96 * 1024;
 }
 
@@ -787,7 +791,7 @@ extern "C" int yn_i8_quant_rows(const void* x, int32_t dtype, int64_t row_stride
 }
 
 extern "C" size_t yn_i8_linear_ws_bytes(int64_t rows, int32_t cols) {
-  if (rows < 1 || cols < 1 || linear_few(rows, cols)) return 0;
+  if (rows < 1 || cols < 1 || linear_few(rows, cols, I8_SMALL + 1)) return 0;   // for any number of channels
   return up_to((size_t)rows * up_to(cols, 16), 256) + (size_t)rows * 4;
 }
 
@@ -805,7 +809,7 @@ extern "C" int yn_i8_linear(const yn_i8_mat* w, const void* x, int32_t dtype, in
   if (reinterpret_cast<uintptr_t>(x) % dtype_size(dtype) || reinterpret_cast<uintptr_t>(y) % dtype_size(y_dtype))
     return host_fail(YN_E_INVALID, "x and y must be aligned to their elements");
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
-  if (linear_few(rows, w->cols)) {
+  if (linear_few(rows, w->cols, w->rows)) {
     const I8Mat m = mat_of(*w);
     int sms = 0;
     if ((rc = sm_count(&sms))) return rc;
