@@ -834,16 +834,27 @@ extern "C" int yn_i8_linear(const yn_i8_mat* w, const void* x, int32_t dtype, in
   a.rows = (int)rows;
   a.channels = w->rows;
   a.K = w->cols;
+  a.half = 128;
   a.sx = sx;
   a.sw = w->scales;
   a.y = y;
   a.y_stride = y_stride;
   a.store_cols = w->rows;
   a.pairs = reinterpret_cast<uintptr_t>(y) % 4 == 0 && y_stride % 2 == 0;
-  const int nb = rows <= 64 ? 64 : 256;
+  // 33 to 64 rows are the same on either tile where the weights' way counts (2048 x 151936: 57.2 and 57.7
+  // us), and faster on the larger one elsewhere (2048 x 16384, 64 rows: 11.5 and 9.7)
+  const int nb = rows <= 32 ? 64 : 256;
+  int sms = 0;
+  if ((rc = sm_count(&sms))) return rc;
+  const long long pairs = std::max(1, sms / 2), rounds = (w->rows + 256 * pairs - 1) / (256 * pairs);
+  if (nb == 64 && rounds > 1) {
+    // bound by the weights' way from HBM: tiles that come out even over the pairs of SMs (6 rows of
+    // 2048 x 151936: 53.6 -> 52.8 us, of 2048 x 65536 27.7 -> 26.2)
+    a.half = (int)(up_to((size_t)((w->rows + rounds * pairs - 1) / (rounds * pairs)), 4) / 2);
+  }
   I8Maps maps{};
-  if ((rc = tmap_mats(&maps.a, *w, 128)) || (rc = tmap_rows(&maps, codes, w->cols, rows, ldc))) return rc;
-  const long long tiles = (long long)((rows + nb - 1) / nb) * ((w->rows + 255) / 256);
+  if ((rc = tmap_mats(&maps.a, *w, a.half)) || (rc = tmap_rows(&maps, codes, w->cols, rows, ldc))) return rc;
+  const long long tiles = (long long)((rows + nb - 1) / nb) * ((w->rows + 2 * a.half - 1) / (2 * a.half));
   return launch_gemm_out(y_dtype, nb, a, maps, tiles, st);
 }
 
@@ -933,6 +944,7 @@ extern "C" int yn_i8_experts(const yn_i8_mat* gate, const yn_i8_mat* up, const y
   d.rows = P;
   d.channels = H;
   d.K = I;
+  d.half = 128;
   d.sx = sa;
   d.sw = down->scales;
   d.sw_stride = down->scale_stride;

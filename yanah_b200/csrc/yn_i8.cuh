@@ -167,6 +167,7 @@ struct I8Gemm {
   const I8Chunk* chunks;   // null: one matrix, chunk c = rows [c * NB, ...) of `rows`
   const int* n_chunks;     // device count of `chunks`
   int rows, channels, K;
+  int half;                // channels of a block's tile, even, 128 at most (UP: 64 units)
   const float* sx;         // (rows) row scales
   const float* sw;         // channel scales, sw_stride per matrix
   const float* sw_up;
@@ -347,7 +348,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(I8_THREADS, 1)
   const int rank = (int)i8_rank();
   int* err = &g_i8_err;
 
-  constexpr int TILE = UP ? 128 : 256;   // units or channels of a pair's tile
+  const int tile_half = UP ? 64 : a.half, TILE = 2 * tile_half;   // units or channels of a block's and of a pair's tile
   const int UT = (a.channels + TILE - 1) / TILE;
   const int step = (int)(gridDim.x >> 1), t0 = (int)(blockIdx.x >> 1), NK = (a.K + 127) / 128;
   i8_launch_next();
@@ -385,10 +386,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(I8_THREADS, 1)
     if (ti >= n_tiles) return Tile{I8Chunk{0, 0, 0}, 0};
     if (a.chunks) {
       const int c = ti / UT;
-      return Tile{a.chunks[c], TILE * (ti - c * UT) + TILE / 2 * rank};
+      return Tile{a.chunks[c], TILE * (ti - c * UT) + tile_half * rank};
     }
     const int u = ti / n_chunks, c = ti - u * n_chunks;
-    return Tile{I8Chunk{0, c * NB, min(NB, a.rows - c * NB)}, TILE * u + TILE / 2 * rank};
+    return Tile{I8Chunk{0, c * NB, min(NB, a.rows - c * NB)}, TILE * u + tile_half * rank};
   };
   Tile next = tile(t0), after = tile(t0 + step);
 
@@ -430,7 +431,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(I8_THREADS, 1)
       next = after;
       after = tile(ti + 2 * ahead);
       sc = scales(next);
-      const bool in = r < a.channels;
+      const bool mine = UP || r_in < tile_half, in = mine && r < a.channels;
       ok = i8_wait(&acc_full[b], (uint32_t)(j / F::ACC) & 1, err);
       if (!ok) break;
       tc_fence_after();
@@ -469,7 +470,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(I8_THREADS, 1)
             const uint32_t own = i8_pack2<O>(f0, f1);
             const uint32_t other = __shfl_xor_sync(0xffffffffu, own, 1);
             const uint32_t pk = __byte_perm(own, other, sel);
-            if (k + odd < left) {
+            if (k + odd < left && mine) {
               if (two) out[(size_t)k * a.y_stride / 2] = pk;
               else if ((r & ~1) < a.channels)
                 reinterpret_cast<uint16_t*>(out)[(size_t)k * a.y_stride] = (uint16_t)pk;
@@ -532,7 +533,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(I8_THREADS, 1)
         after = tile(ti + 2 * step);
         const int half = ((c.n + 31) & ~31) >> 1, row = c.p0 + rank * half;   // this block's half of the MMA's rows
         const int bi = half <= 16 ? 0 : half <= 32 ? 1 : half <= 64 ? 2 : 3;
-        const uint32_t bytes = 2u * (I8_A_BYTES + (16u << bi) * 128u);
+        const uint32_t bytes = 2u * ((UP ? 128u : (uint32_t)tile_half) + (16u << bi)) * 128u;
         for (int kc = 0; kc < NK; ++kc) {
           if (used == F::S) ok = i8_wait1(&empty[s], empty_phase, err);
           else ++used;
