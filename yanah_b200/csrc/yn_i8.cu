@@ -533,10 +533,12 @@ __global__ void __cluster_dims__(I8_PLAN_B, 1, 1) __launch_bounds__(I8_PLAN_T)
   cluster.sync();   // no block leaves while its counts are read
 }
 
-// out[t] = residual[t] + sum_j w_j y[pair_of[t][j]] in fp32, columns in order, rounded once.
+// out[t] = residual[t] + sum_j w_j y[pair_of[t][j]] in fp32, columns in order, rounded once: the
+// products y stay fp32 until then, as they do in k_i8_down_few, so that a row comes out the same
+// in a batch of any size.
 // One row of the batch per blockIdx.x, 8 outputs per thread; VEC: residual and out in 16-byte pieces.
-template <typename O, typename Y, bool VEC>
-__global__ void __launch_bounds__(128) k_i8_combine(const Y* y, long long ldy, const int32_t* pair_of, const float* w, int k,
+template <typename O, bool VEC>
+__global__ void __launch_bounds__(128) k_i8_combine(const float* y, long long ldy, const int32_t* pair_of, const float* w, int k,
                                                     int H, const void* res, long long ldr, void* out, long long ldo) {
   i8_wait_previous();
   const size_t t = blockIdx.x;
@@ -548,7 +550,7 @@ __global__ void __launch_bounds__(128) k_i8_combine(const Y* y, long long ldy, c
   for (int i = 0; i < 8; ++i) acc[i] = 0.0f;
   const bool on = h < H;
   for (int j0 = 0; j0 < k; j0 += 4) {
-    I8Raw<Y> r[4];
+    I8Raw<float> r[4];
     float wj[4];
 #pragma unroll
     for (int q = 0; q < 4; ++q) {   // 4 rows of y in flight
@@ -556,7 +558,7 @@ __global__ void __launch_bounds__(128) k_i8_combine(const Y* y, long long ldy, c
       wj[q] = __shfl_sync(0xffffffffu, w_mine, (j0 + q) & 31);
       if (j0 + q >= k || p < 0) wj[q] = 0.0f;
       if (on && j0 + q < k && p >= 0) r[q].load(y, (size_t)p * ldy + h);   // rows of y are padded to whole pieces
-      else r[q] = I8Raw<Y>{};
+      else r[q] = I8Raw<float>{};
     }
 #pragma unroll
     for (int q = 0; q < 4; ++q) {
@@ -593,15 +595,14 @@ __global__ void __launch_bounds__(128) k_i8_combine(const Y* y, long long ldy, c
       reinterpret_cast<O*>(out)[t * ldo + h + i] = i8_out<O>(r + acc[i]);
     }
 }
-template <typename O, typename Y>
-void launch_combine(const void* y, long long ldy, const int32_t* pair_of, const float* w, int k, int H, long long rows,
+template <typename O>
+void launch_combine(const float* y, long long ldy, const int32_t* pair_of, const float* w, int k, int H, long long rows,
                     const void* res, long long ldr, void* out, long long ldo, cudaStream_t st) {
   const bool vec = reinterpret_cast<uintptr_t>(out) % 16 == 0 && (ldo * sizeof(O)) % 16 == 0 &&
                    reinterpret_cast<uintptr_t>(res) % 16 == 0 && (ldr * sizeof(O)) % 16 == 0;
   const dim3 g((unsigned)rows, (H + 1023) / 1024);
-  const Y* yy = reinterpret_cast<const Y*>(y);
-  if (vec) launch_after(k_i8_combine<O, Y, true>, g, 128, 0, st, yy, ldy, pair_of, w, k, H, res, ldr, out, ldo);
-  else launch_after(k_i8_combine<O, Y, false>, g, 128, 0, st, yy, ldy, pair_of, w, k, H, res, ldr, out, ldo);
+  if (vec) launch_after(k_i8_combine<O, true>, g, 128, 0, st, y, ldy, pair_of, w, k, H, res, ldr, out, ldo);
+  else launch_after(k_i8_combine<O, false>, g, 128, 0, st, y, ldy, pair_of, w, k, H, res, ldr, out, ldo);
 }
 
 // ---------------------------------------------------------------- host side
@@ -746,7 +747,7 @@ bool experts_few(long long pairs, int k, int H, int I) {
          k * up_to(I, I8_GK) <= 96 * 1024;
 }
 
-ExpertsWs experts_ws(long long rows, int k, int E, int H, int I, int odt) {
+ExpertsWs experts_ws(long long rows, int k, int E, int H, int I) {
   ExpertsWs L{};
   size_t o = 0;
   auto take = [&](size_t b) { const size_t at = o; o = up_to(o + b, 256); return at; };
@@ -769,7 +770,7 @@ ExpertsWs experts_ws(long long rows, int k, int E, int H, int I, int odt) {
   L.act = take(P * L.lda * 4);
   L.acodes = take(P * L.ldac);
   L.sa = take(P * 4);
-  L.y = take(P * L.ldy * (odt == YN_BF16 ? 2 : 4));
+  L.y = take(P * L.ldy * 4);
   L.total = o;
   return L;
 }
@@ -839,7 +840,6 @@ extern "C" int yn_i8_linear(const yn_i8_mat* w, const void* x, int32_t dtype, in
   a.sw = w->scales;
   a.y = y;
   a.y_stride = y_stride;
-  a.store_cols = w->rows;
   a.pairs = reinterpret_cast<uintptr_t>(y) % 4 == 0 && y_stride % 2 == 0;
   // 33 to 64 rows are the same on either tile where the weights' way counts (2048 x 151936: 57.2 and 57.7
   // us), and faster on the larger one elsewhere (2048 x 16384, 64 rows: 11.5 and 9.7)
@@ -861,7 +861,7 @@ extern "C" int yn_i8_linear(const yn_i8_mat* w, const void* x, int32_t dtype, in
 extern "C" size_t yn_i8_experts_ws_bytes(int64_t rows, int32_t top_k, int32_t n_experts, int32_t hidden, int32_t inter,
                                          int32_t dtype) {
   if (rows < 1 || top_k < 1 || n_experts < 1 || hidden < 1 || inter < 1 || !dtype_ok(dtype)) return 0;
-  return experts_ws(rows, top_k, n_experts, hidden, inter, dtype).total;
+  return experts_ws(rows, top_k, n_experts, hidden, inter).total;
 }
 
 extern "C" int yn_i8_experts(const yn_i8_mat* gate, const yn_i8_mat* up, const yn_i8_mat* down, const void* x, int32_t dtype,
@@ -884,7 +884,7 @@ extern "C" int yn_i8_experts(const yn_i8_mat* gate, const yn_i8_mat* up, const y
   if (reinterpret_cast<uintptr_t>(x) % size || reinterpret_cast<uintptr_t>(out) % size ||
       (residual && reinterpret_cast<uintptr_t>(residual) % size))
     return host_fail(YN_E_INVALID, "rows must be aligned to their element");
-  const ExpertsWs L = experts_ws(rows, top_k, E, H, I, dtype);
+  const ExpertsWs L = experts_ws(rows, top_k, E, H, I);
   if (ws_bytes < L.total || reinterpret_cast<uintptr_t>(ws) % 256)
     return host_fail(YN_E_INVALID, "workspace too small or not 256-byte aligned");
   uint8_t* b = reinterpret_cast<uint8_t*>(ws);
@@ -913,7 +913,7 @@ extern "C" int yn_i8_experts(const yn_i8_mat* gate, const yn_i8_mat* up, const y
   float* act = reinterpret_cast<float*>(b + L.act);
   int8_t* acodes = reinterpret_cast<int8_t*>(b + L.acodes);
   float* sa = reinterpret_cast<float*>(b + L.sa);
-  void* y = b + L.y;
+  float* y = reinterpret_cast<float*>(b + L.y);
   k_i8_plan<<<I8_PLAN_B, I8_PLAN_T, 0, st>>>(ids, P, E, L.nb, pair_of, chunks, n_out);
   if ((rc = launch_quant(dtype, x, x_stride, rows, H, nullptr, pair_of, top_k, codes, L.ldc, sx, false, st))) return rc;
   const long long max_chunks = E + P / L.nb + 1;
@@ -950,15 +950,12 @@ extern "C" int yn_i8_experts(const yn_i8_mat* gate, const yn_i8_mat* up, const y
   d.sw_stride = down->scale_stride;
   d.y = y;
   d.y_stride = L.ldy;
-  d.store_cols = (int)L.ldy;
-  d.pairs = true;
-  const bool yb = dtype == YN_BF16;
-  if ((rc = launch_gemm_out(yb ? YN_BF16 : YN_F32, L.nb, d, md2, td, st))) return rc;
-  if (yb)
-    launch_combine<__nv_bfloat16, __nv_bfloat16>(y, L.ldy, pair_of, weights, top_k, H, rows, residual, res_stride, out, out_stride, st);
+  if ((rc = launch_gemm_nb<float, false>(L.nb, d, md2, td, st))) return rc;
+  if (dtype == YN_BF16)
+    launch_combine<__nv_bfloat16>(y, L.ldy, pair_of, weights, top_k, H, rows, residual, res_stride, out, out_stride, st);
   else if (dtype == YN_F16)
-    launch_combine<__half, float>(y, L.ldy, pair_of, weights, top_k, H, rows, residual, res_stride, out, out_stride, st);
-  else launch_combine<float, float>(y, L.ldy, pair_of, weights, top_k, H, rows, residual, res_stride, out, out_stride, st);
+    launch_combine<__half>(y, L.ldy, pair_of, weights, top_k, H, rows, residual, res_stride, out, out_stride, st);
+  else launch_combine<float>(y, L.ldy, pair_of, weights, top_k, H, rows, residual, res_stride, out, out_stride, st);
   const cudaError_t e = cudaGetLastError();
   return e == cudaSuccess ? YN_OK : host_fail(YN_E_CUDA, std::string("experts: ") + cudaGetErrorString(e));
 }

@@ -174,7 +174,6 @@ struct I8Gemm {
   long long sw_stride, sw_up_stride;
   void* y;                 // (rows, y_stride): output, or UP: fp32 activations
   long long y_stride;
-  int store_cols;          // columns of a row that may be written: channels, or more where rows are padded
   bool both, swapped;      // UP: map a holds both matrices; up before gate in it
   bool pairs;              // 16-bit outputs may be written two channels at a time (4-byte aligned rows)
 };
@@ -460,7 +459,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(I8_THREADS, 1)
         } else if (sizeof(O) == 2 && a.pairs) {
           // two lanes exchange so that each writes two adjacent channels of every second row
           // (even lanes the even rows)
-          const bool odd = lane & 1, two = (r | 1) < a.store_cols;
+          const bool odd = lane & 1, two = (r | 1) < a.channels;
           const uint32_t sel = odd ? 0x3276u : 0x5410u;
           uint32_t* out = reinterpret_cast<uint32_t*>(reinterpret_cast<O*>(a.y) + (row + odd) * a.y_stride + (r & ~1));
 #pragma unroll
