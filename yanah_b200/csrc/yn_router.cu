@@ -294,10 +294,12 @@ __global__ void __launch_bounds__(32 * RT_WARPS) k_router(const RouterArgs a) {
     // |c - exact| <= tol + 2^-24 |c|, tol relative to the row's largest score: e^x as
     // 2^(x log2 e) is off by 2 ulp and the rounding of its exponent, 1.2 |x| ulp, and |x| e^x
     // <= 0.4 for x <= 0, so the exponentials stay within 2^-21 of the largest; the softmax sum
-    // of at most 64 terms a lane and 5 shuffled adds within 69 * 2^-24 < 5e-6 of itself. Scores
-    // below 1e-30 are not told apart.
+    // of at most 64 terms a lane and 5 shuffled adds within 69 * 2^-24 < 5e-6 of itself. Sigmoids of
+    // a row whose largest logit m is far below 0 are e^z too, relative to a largest score of e^m: the
+    // exponent's rounding and that of log2 e are 7.3e-8 |z| of e^z, which is largest at m (|z| e^z
+    // falls from z = -1 on; 0.4 is its maximum). Scores below 1e-30 are not told apart.
     const float inv = a.softmax ? 1.0f / sum : 1.0f;
-    tol = (a.softmax ? 1.6e-5f * inv : 2.0e-6f * rt_sigmoid(m)) + 1e-30f;
+    tol = (a.softmax ? 1.6e-5f * inv : (2.0e-6f + 1.0e-7f * fminf(fmaxf(-m, 0.0f), 100.0f)) * rt_sigmoid(m)) + 1e-30f;
     float hi = -inf, lo = -inf, b[NV];
     if (WHOLE && a.bias) {
       rt_load_wide<NV>(a.bias + first, b);
