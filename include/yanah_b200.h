@@ -381,11 +381,17 @@ int yn_gather_f16_kperm(const void* x, const int32_t* row_of, int64_t rows, int3
  * synchronisation: pairs of each expert made contiguous (pair_row: pair ->
  * row, pair_of: t * k + j -> pair), then the gate/up and down tiles of every
  * expert (n_tiles[0], n_tiles[1] on the device; pass them to yn_tc_experts
- * as n_tiles_dev with grids of max_up / max_dn from yn_prefill_max_tiles). */
+ * as n_tiles_dev with grids of max_up / max_dn from yn_prefill_max_tiles). An
+ * id outside [0, E) sets `err`; its pair_of is -1 and no tile has it. */
 int yn_prefill_max_tiles(const yn_dims* dims, int32_t T, int32_t* max_up, int32_t* max_dn);
 int yn_prefill_plan(const yn_dims* dims, const int32_t* ids, int32_t T, int32_t* pair_row, int32_t* pair_of,
                     yn_tc_tile* tiles_up, int32_t max_up, yn_tc_tile* tiles_dn, int32_t max_dn, int32_t* n_tiles,
                     int32_t* err, void* stream);
+/* The same for ids of yn_route_scored, whose rows may end in -1 (no expert is
+ * left): such a column has no pair, and is no error. */
+int yn_prefill_plan_by_rule(const yn_dims* dims, const int32_t* ids, int32_t T, int32_t* pair_row, int32_t* pair_of,
+                            yn_tc_tile* tiles_up, int32_t max_up, yn_tc_tile* tiles_dn, int32_t max_dn,
+                            int32_t* n_tiles, int32_t* err, void* stream);
 
 /* Combine of T rows (mlx_backend.py:409/:420, :438-440; orchestrator.py:287):
  * out[t] = h_res[t] + (sum_j bf16(y[pair_of[t][j]] * w[t][j]) in column order

@@ -139,6 +139,7 @@ _SIGS = {
     "yn_gather_f16_kperm": (C.c_int, [_P, _P, C.c_int64, _I, _P, _P]),
     "yn_prefill_max_tiles": (C.c_int, [C.POINTER(Dims), _I, C.POINTER(C.c_int32), C.POINTER(C.c_int32)]),
     "yn_prefill_plan": (C.c_int, [C.POINTER(Dims), _P, _I, _P, _P, _P, _I, _P, _I, _P, _P, _P]),
+    "yn_prefill_plan_by_rule": (C.c_int, [C.POINTER(Dims), _P, _I, _P, _P, _P, _I, _P, _I, _P, _P, _P]),
     "yn_pairs_combine": (C.c_int, [C.POINTER(Dims), _P, _P, _P, _P, _P, _I, _P, _P]),
     "yn_gather_kperm": (C.c_int, [_P, _P, C.c_int64, _I, _I, _I, _P, _P]),
     "yn_scale_rows": (C.c_int, [_P, _P, C.c_int64, _I, _P, _P]),

@@ -296,9 +296,10 @@ extern "C" int yn_prefill_max_tiles(const yn_dims* dims, int32_t T, int32_t* max
   return YN_OK;
 }
 
-extern "C" int yn_prefill_plan(const yn_dims* dims, const int32_t* ids, int32_t T, int32_t* pair_row, int32_t* pair_of,
-                               yn_tc_tile* tiles_up, int32_t max_up, yn_tc_tile* tiles_dn, int32_t max_dn,
-                               int32_t* n_tiles, int32_t* err, void* stream) {
+namespace {
+int prefill_plan(const yn_dims* dims, const int32_t* ids, int32_t T, int32_t* pair_row, int32_t* pair_of,
+                 yn_tc_tile* tiles_up, int32_t max_up, yn_tc_tile* tiles_dn, int32_t max_dn, int32_t* n_tiles,
+                 int32_t* err, bool absent, void* stream) {
   if (!dims || !ids || !pair_row || !pair_of || !tiles_up || !tiles_dn || !n_tiles || !err)
     return host_fail(YN_E_INVALID, "null argument");
   if (T < 1 || (long long)T * dims->top_k > 65536) return host_fail(YN_E_UNSUPPORTED, "T * top_k must be in [1, 65536]");
@@ -318,7 +319,21 @@ extern "C" int yn_prefill_plan(const yn_dims* dims, const int32_t* ids, int32_t 
   a.max_dn = max_dn;
   a.n_tiles = n_tiles;
   a.err = err;
+  a.absent = absent;
   k_prefill_plan<<<1, PLAN_THREADS, 0, as_st(stream)>>>(a);
   YN_CUDA_T(cudaGetLastError());
   return YN_OK;
+}
+}  // namespace
+
+extern "C" int yn_prefill_plan(const yn_dims* dims, const int32_t* ids, int32_t T, int32_t* pair_row, int32_t* pair_of,
+                               yn_tc_tile* tiles_up, int32_t max_up, yn_tc_tile* tiles_dn, int32_t max_dn,
+                               int32_t* n_tiles, int32_t* err, void* stream) {
+  return prefill_plan(dims, ids, T, pair_row, pair_of, tiles_up, max_up, tiles_dn, max_dn, n_tiles, err, false, stream);
+}
+
+extern "C" int yn_prefill_plan_by_rule(const yn_dims* dims, const int32_t* ids, int32_t T, int32_t* pair_row,
+                                       int32_t* pair_of, yn_tc_tile* tiles_up, int32_t max_up, yn_tc_tile* tiles_dn,
+                                       int32_t max_dn, int32_t* n_tiles, int32_t* err, void* stream) {
+  return prefill_plan(dims, ids, T, pair_row, pair_of, tiles_up, max_up, tiles_dn, max_dn, n_tiles, err, true, stream);
 }

@@ -715,8 +715,8 @@ namespace ynb {
 // 1024 threads): counts per expert, a block scan over experts (ascending id),
 // pair placement (pairs of one expert contiguous; their order inside an
 // expert does not change any pair's result), then per expert ceil(n / 256)
-// row chunks x (I / 64) gate/up tiles and x (H / 128) down tiles. An id of -1 (a rule that
-// leaves a row fewer than k experts) has no pair; any other outside [0, E) is an error.
+// row chunks x (I / 64) gate/up tiles and x (H / 128) down tiles. An id outside [0, E) has no
+// pair and is an error, but for -1 where `absent` allows it (a rule leaves a row fewer than k experts).
 // n_tiles[0], n_tiles[1] = gate/up and down tiles written.
 constexpr int PLAN_THREADS = 1024;
 
@@ -731,6 +731,7 @@ struct PrefillPlanArgs {
   int max_dn;
   int* n_tiles;        // [2]
   int* err;
+  bool absent;         // ids of -1 are no error
 };
 
 YN_DEV int2 block_scan2(int2 v, int2* total) {
@@ -782,7 +783,7 @@ __global__ void __launch_bounds__(PLAN_THREADS) k_prefill_plan(const PrefillPlan
   for (int i = tid; i < Pw; i += PLAN_THREADS) {
     const int e = i < P ? a.ids[i] : -1;
     const bool valid = e >= 0 && e < a.E;
-    if (i < P && !valid && e != -1) raise_error(a.err, YN_ERR_BAD_EXPERT);
+    if (i < P && !valid && !(a.absent && e == -1)) raise_error(a.err, YN_ERR_BAD_EXPERT);
     agg_atomic_add(cnt, valid ? e : 0, valid);
   }
   __syncthreads();

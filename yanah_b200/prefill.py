@@ -7,7 +7,7 @@ bit-identical to the single-row path); the rows' fp16 K-permuted copy
 the reference's prefill sweep plans its staging groups (sweep.py:80-138); the grouped gate/up + SwiGLU and down GEMMs
 (`yn_tc_experts`, 128 weight rows x up to 256 rows per tile); the combine in
 column order plus the residual (`yn_pairs_combine`). The grouping runs on the
-device (`yn_prefill_plan`); `plan_prefill` is its host restatement.
+device (`yn_prefill_plan`, by a rule `yn_prefill_plan_by_rule`); `plan_prefill` is its host restatement.
 
 Two things can be chosen: `rule` routes by a `routing.RouteRule` instead of the
 softmax top-k (the logits of `yn_rows_route` through `yn_route_scored`), and
@@ -172,9 +172,10 @@ class PrefillStack:
         if self.int8 is not None:
             int8_experts(self.x[:T], self.ids[:T], self.w[:T], *self.int8[i], residual=h, stream=stream, out=out)
             return
-        _lib.check(lib.yn_prefill_plan(D, self.ids.data_ptr(), T, self.pair_row.data_ptr(), self.pair_of.data_ptr(),
-                                       self.tiles_up.data_ptr(), self.max_up, self.tiles_dn.data_ptr(), self.max_dn,
-                                       self.n_tiles.data_ptr(), self.err.data_ptr(), st))
+        plan = lib.yn_prefill_plan if self.rule is None else lib.yn_prefill_plan_by_rule
+        _lib.check(plan(D, self.ids.data_ptr(), T, self.pair_row.data_ptr(), self.pair_of.data_ptr(),
+                        self.tiles_up.data_ptr(), self.max_up, self.tiles_dn.data_ptr(), self.max_dn,
+                        self.n_tiles.data_ptr(), self.err.data_ptr(), st))
         P = T * cfg.top_k
         _lib.check(lib.yn_gather_f16_kperm(self.x.data_ptr(), self.pair_row.data_ptr(), P, H, self.x16.data_ptr(), st))
         if gemm_events is not None:
