@@ -502,8 +502,16 @@ int yn_i8_experts(const yn_i8_mat* gate, const yn_i8_mat* up, const yn_i8_mat* d
                   int64_t x_stride, int64_t rows, const int32_t* ids, const float* weights, int32_t top_k,
                   const void* residual, int64_t res_stride, void* out, int64_t out_stride, void* ws, size_t ws_bytes,
                   void* stream);
-/* Read and clear the current device's error word of these entry points
- * (synchronises the stream). */
+/* The same with an error word of the caller's own (device memory, written only where
+ * it is 0; NULL: the device's, which all other calls share). */
+int yn_i8_experts_err(const yn_i8_mat* gate, const yn_i8_mat* up, const yn_i8_mat* down, const void* x, int32_t dtype,
+                      int64_t x_stride, int64_t rows, const int32_t* ids, const float* weights, int32_t top_k,
+                      const void* residual, int64_t res_stride, void* out, int64_t out_stride, void* ws,
+                      size_t ws_bytes, int32_t* err, void* stream);
+/* Read and clear the current device's error word of these entry points, which all
+ * callers without a word of their own share (synchronises the stream). Besides bad
+ * ids it reports a wait inside a tensor-core product that ran out (1 s; the call's
+ * output is wrong then). */
 int yn_i8_error(void* stream, int32_t* code_out);
 
 /* --------------------------------------------- token log probabilities */

@@ -151,6 +151,8 @@ _SIGS = {
     "yn_i8_experts_ws_bytes": (C.c_size_t, [C.c_int64, _I, _I, _I, _I, _I]),
     "yn_i8_experts": (C.c_int, [C.POINTER(I8Mat), C.POINTER(I8Mat), C.POINTER(I8Mat), _P, _I, C.c_int64, C.c_int64, _P,
                                 _P, _I, _P, C.c_int64, _P, C.c_int64, _P, C.c_size_t, _P]),
+    "yn_i8_experts_err": (C.c_int, [C.POINTER(I8Mat), C.POINTER(I8Mat), C.POINTER(I8Mat), _P, _I, C.c_int64, C.c_int64,
+                                    _P, _P, _I, _P, C.c_int64, _P, C.c_int64, _P, C.c_size_t, _P, _P]),
     "yn_i8_error": (C.c_int, [_P, C.POINTER(C.c_int32)]),
     "yn_token_logprobs": (C.c_int, [_P, _I, C.c_int64, C.c_int64, C.c_int64, _P, _I, _P, _P, _P, _P, _P, _P]),
     "yn_rows_route_shared": (C.c_int, [C.POINTER(Dims), _I, _P, C.POINTER(C.c_void_p), C.POINTER(C.c_void_p)]),

@@ -349,14 +349,15 @@ __global__ void __launch_bounds__(I8_GT, 3) k_i8_few(int dt, const void* x, long
 // Few (row, expert) pairs: gate and up of 2 units per warp, the pair's row codes made by
 // every block, SwiGLU in fp32 to act (pairs, I).
 __global__ void __launch_bounds__(I8_GT) k_i8_up_few(int dt, const void* x, long long ldx, int H, int HP, const int32_t* ids,
-                                                     int k, int E, const I8Mat gate, const I8Mat up, int I, float* act) {
+                                                     int k, int E, const I8Mat gate, const I8Mat up, int I, float* act,
+                                                    int* err) {
   extern __shared__ __align__(16) int8_t xs[];
   __shared__ float sx;
   __shared__ uint32_t buf[I8_GW];
   const int p = blockIdx.y, e = ids[p], warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   i8_launch_next();
   if (e < 0 || e >= E) {
-    if (e != -1 && threadIdx.x == 0 && blockIdx.x == 0) raise_error(&g_i8_err, YN_ERR_BAD_EXPERT);
+    if (e != -1 && threadIdx.x == 0 && blockIdx.x == 0) raise_error(i8_err(err), YN_ERR_BAD_EXPERT);
     return;
   }
   i8_row_smem<true>(dt, x, (size_t)(p / k) * ldx, H, HP, xs, &sx, buf);
@@ -459,7 +460,7 @@ constexpr int I8_MAX_E = 1024;
 // shared memory, and all make the same scan over the experts (16384 pairs: one block alone
 // took 11 us, most of it atomics on popular experts).
 __global__ void __cluster_dims__(I8_PLAN_B, 1, 1) __launch_bounds__(I8_PLAN_T)
-    k_i8_plan(const int32_t* ids, int P, int E, int NB, int32_t* pair_of, I8Chunk* chunks, int* n_out) {
+    k_i8_plan(const int32_t* ids, int P, int E, int NB, int32_t* pair_of, I8Chunk* chunks, int* n_out, int* err) {
   namespace cg = cooperative_groups;
   cg::cluster_group cluster = cg::this_cluster();
   __shared__ int cnt[I8_MAX_E], base_of[I8_MAX_E];
@@ -482,7 +483,7 @@ __global__ void __cluster_dims__(I8_PLAN_B, 1, 1) __launch_bounds__(I8_PLAN_T)
       if (e[q] >= 0 && e[q] < E) pair_of[i] = atomicAdd(&cnt[e[q]], 1);   // place inside this block's share
       else {
         pair_of[i] = -1;
-        if (e[q] != -1) raise_error(&g_i8_err, YN_ERR_BAD_EXPERT);
+        if (e[q] != -1) raise_error(i8_err(err), YN_ERR_BAD_EXPERT);
       }
     }
   }
@@ -868,6 +869,14 @@ extern "C" int yn_i8_experts(const yn_i8_mat* gate, const yn_i8_mat* up, const y
                              int64_t x_stride, int64_t rows, const int32_t* ids, const float* weights, int32_t top_k,
                              const void* residual, int64_t res_stride, void* out, int64_t out_stride, void* ws,
                              size_t ws_bytes, void* stream) {
+  return yn_i8_experts_err(gate, up, down, x, dtype, x_stride, rows, ids, weights, top_k, residual, res_stride, out,
+                           out_stride, ws, ws_bytes, nullptr, stream);
+}
+
+extern "C" int yn_i8_experts_err(const yn_i8_mat* gate, const yn_i8_mat* up, const yn_i8_mat* down, const void* x,
+                                 int32_t dtype, int64_t x_stride, int64_t rows, const int32_t* ids, const float* weights,
+                                 int32_t top_k, const void* residual, int64_t res_stride, void* out, int64_t out_stride,
+                                 void* ws, size_t ws_bytes, int32_t* err, void* stream) {
   if (!gate || !up || !down) return host_fail(YN_E_INVALID, "null argument");
   int rc = check_mat(*gate, "gate");
   if (rc || (rc = check_mat(*up, "up")) || (rc = check_mat(*down, "down"))) return rc;
@@ -899,7 +908,7 @@ extern "C" int yn_i8_experts(const yn_i8_mat* gate, const yn_i8_mat* up, const y
         (ds > 40 * 1024 && (rc = host_set_smem(reinterpret_cast<const void*>(k_i8_down_few), 96 * 1024))))
       return rc;
     k_i8_up_few<<<dim3((I + 2 * I8_GW - 1) / (2 * I8_GW), P), I8_GT, HP, st>>>(dtype, x, x_stride, H, HP, ids, top_k, E, mg, mu,
-                                                                             I, act);
+                                                                             I, act, err);
     launch_after(k_i8_down_few, dim3((H + 2 * I8_GW - 1) / (2 * I8_GW), (unsigned)rows), I8_GT, ds, st, act, I, IP, ids, weights,
                  top_k, E, md, H, dtype, residual, res_stride, out, out_stride);
     const cudaError_t e = cudaGetLastError();
@@ -914,13 +923,14 @@ extern "C" int yn_i8_experts(const yn_i8_mat* gate, const yn_i8_mat* up, const y
   int8_t* acodes = reinterpret_cast<int8_t*>(b + L.acodes);
   float* sa = reinterpret_cast<float*>(b + L.sa);
   float* y = reinterpret_cast<float*>(b + L.y);
-  k_i8_plan<<<I8_PLAN_B, I8_PLAN_T, 0, st>>>(ids, P, E, L.nb, pair_of, chunks, n_out);
+  k_i8_plan<<<I8_PLAN_B, I8_PLAN_T, 0, st>>>(ids, P, E, L.nb, pair_of, chunks, n_out, err);
   if ((rc = launch_quant(dtype, x, x_stride, rows, H, nullptr, pair_of, top_k, codes, L.ldc, sx, false, st))) return rc;
   const long long max_chunks = E + P / L.nb + 1;
   I8Maps maps{};
   I8Gemm g{};
   if ((rc = tmap_gate_up(&g, &maps, *gate, *up)) || (rc = tmap_rows(&maps, codes, H, P, L.ldc))) return rc;
   g.chunks = chunks;
+  g.err = err;
   g.n_chunks = n_out;
   g.rows = P;
   g.channels = I;
@@ -940,6 +950,7 @@ extern "C" int yn_i8_experts(const yn_i8_mat* gate, const yn_i8_mat* up, const y
   if ((rc = tmap_mats(&md2.a, *down, 128)) || (rc = tmap_rows(&md2, acodes, I, P, L.ldac))) return rc;
   I8Gemm d{};
   d.chunks = chunks;
+  d.err = err;
   d.n_chunks = n_out;
   d.rows = P;
   d.channels = H;

@@ -16,8 +16,9 @@
 
 namespace ynb {
 
-// Error word of these kernels, one per device: first error wins (yn_i8_error).
+// Error word of the calls that were given none of their own, one per device: first error wins (yn_i8_error).
 __device__ int g_i8_err;
+YN_DEV int* i8_err(int* own) { return own ? own : &g_i8_err; }
 
 template <typename T>
 struct I8In;
@@ -174,6 +175,7 @@ struct I8Gemm {
   long long sw_stride, sw_up_stride;
   void* y;                 // (rows, y_stride): output, or UP: fp32 activations
   long long y_stride;
+  int* err;                // error word, null: the device's
   bool both, swapped;      // UP: map a holds both matrices; up before gate in it
   bool pairs;              // 16-bit outputs may be written two channels at a time (4-byte aligned rows)
 };
@@ -345,7 +347,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(I8_THREADS, 1)
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(acc_empty + F::ACC);
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int rank = (int)i8_rank();
-  int* err = &g_i8_err;
+  int* err = i8_err(a.err);
 
   const int tile_half = UP ? 64 : a.half, TILE = 2 * tile_half;   // units or channels of a block's and of a pair's tile
   const int UT = (a.channels + TILE - 1) / TILE;

@@ -81,7 +81,8 @@ def int8_linear(x: torch.Tensor, w: Int8Matrix, out_dtype: Optional[torch.dtype]
                 stream: Optional[torch.cuda.Stream] = None) -> torch.Tensor:
     """x (T, K) in fp32, bf16 or fp16 times the transpose of w (N, K): (T, N) in
     ``out_dtype`` (default: that of x), rounded once from fp32: the sum times the row's
-    scale, times the channel's. Any number of rows."""
+    scale, times the channel's. Any number of rows. ``check_error`` reports a product that
+    did not finish."""
     dtype, dev = check_floats(x, "x"), x.get_device()
     if elsewhere(dev, stream):
         return run_there(lambda: int8_linear(x, w, out_dtype), x.device, stream, (x, *w))
@@ -106,18 +107,19 @@ def int8_linear(x: torch.Tensor, w: Int8Matrix, out_dtype: Optional[torch.dtype]
 
 def int8_experts(x: torch.Tensor, ids: torch.Tensor, weights: torch.Tensor, gate: Int8Matrix, up: Int8Matrix,
                  down: Int8Matrix, residual: Optional[torch.Tensor] = None,
-                 stream: Optional[torch.cuda.Stream] = None, out: Optional[torch.Tensor] = None) -> torch.Tensor:
+                 stream: Optional[torch.cuda.Stream] = None, out: Optional[torch.Tensor] = None,
+                 err: Optional[torch.Tensor] = None) -> torch.Tensor:
     """residual + sum over a row's experts of weight * down(silu(gate x) * up x).
 
     x (T, H); ids (T, k) int32 and weights (T, k) fp32 as ``routing.route_scored``
     returns them: an id of -1 has no expert (any other id outside [0, E) is left out and
-    reported by ``check_error``). gate, up: (E, I, H); down: (E, H, I). The activations
+    reported by ``check_error``, or in ``err``, (1) int32, an error word of the caller's own). gate, up: (E, I, H); down: (E, H, I). The activations
     are quantised per (row, expert), the sum is fp32 and rounded once to the type of x.
     ``out``: (T, H) to write, rows of adjacent elements; it may be the residual."""
     dtype, dev = check_floats(x, "x"), x.get_device()
     if elsewhere(dev, stream):
-        return run_there(lambda: int8_experts(x, ids, weights, gate, up, down, residual, out=out), x.device, stream,
-                         (x, ids, weights, residual, out, *gate, *up, *down))
+        return run_there(lambda: int8_experts(x, ids, weights, gate, up, down, residual, out=out, err=err), x.device,
+                         stream, (x, ids, weights, residual, out, err, *gate, *up, *down))
     x, rows, h, stride = rows_of(x, "x")
     if ids.dim() != 2:
         raise ValueError("ids must be (T, k)")
@@ -140,18 +142,22 @@ def int8_experts(x: torch.Tensor, ids: torch.Tensor, weights: torch.Tensor, gate
         same, _, _, out_stride = rows_of(out, "out")
         if same is not out:
             raise ValueError("out must have rows of adjacent elements that do not overlap")
+    if err is not None:
+        check_like(err, dev, (1,), (torch.int32,), "err")
     lib = _lib.lib()
     nb = lib.yn_i8_experts_ws_bytes(rows, k, g.n_mats, h, g.rows, dtype)
     ws = x.new_empty(nb, dtype=torch.uint8)
-    _lib.check(lib.yn_i8_experts(C.byref(g), C.byref(u), C.byref(d), x.data_ptr(), dtype, stride, rows, ids.data_ptr(),
-                                 weights.data_ptr(), k, p_res, res_stride, out.data_ptr(), out_stride, ws.data_ptr(), nb,
-                                 raw_stream(dev)))
+    _lib.check(lib.yn_i8_experts_err(C.byref(g), C.byref(u), C.byref(d), x.data_ptr(), dtype, stride, rows,
+                                     ids.data_ptr(), weights.data_ptr(), k, p_res, res_stride, out.data_ptr(), out_stride,
+                                     ws.data_ptr(), nb, None if err is None else err.data_ptr(), raw_stream(dev)))
     return out
 
 
 def check_error(device=None) -> int:
     """Read and clear the error word of the 8-bit products on a device (synchronises its
-    current stream): 0, or a code as ``CudaMoEBackend.check_error`` returns."""
+    current stream): 0, or a code as ``CudaMoEBackend.check_error`` returns, of an id outside
+    the experts or a wait inside a product that ran out (1 s: that call's output is wrong). All
+    calls on the device share the word, but for those of ``int8_experts`` with one of their own."""
     code = C.c_int32(0)
     with torch.cuda.device(device):
         _lib.check(_lib.lib().yn_i8_error(torch.cuda.current_stream().cuda_stream, C.byref(code)))

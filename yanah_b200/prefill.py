@@ -26,7 +26,6 @@ from . import _lib
 from .device import DeviceLayer, ExpertArena, dims_struct, fill_synthetic_experts, stream_ptr
 from .formats import RecordSpec
 from .int8 import Int8Matrix, int8_experts, quantize_rows
-from .int8 import check_error as int8_error
 from .routing import RouteRule, route_scored
 from .synthetic import StackConfig, dense_layer
 
@@ -170,7 +169,8 @@ class PrefillStack:
                          None if self.choice_bias is None else self.choice_bias[i], stream=stream,
                          out=(self.ids[:T], self.w[:T]))
         if self.int8 is not None:
-            int8_experts(self.x[:T], self.ids[:T], self.w[:T], *self.int8[i], residual=h, stream=stream, out=out)
+            int8_experts(self.x[:T], self.ids[:T], self.w[:T], *self.int8[i], residual=h, stream=stream, out=out,
+                         err=self.err)
             return
         plan = lib.yn_prefill_plan if self.rule is None else lib.yn_prefill_plan_by_rule
         _lib.check(plan(D, self.ids.data_ptr(), T, self.pair_row.data_ptr(), self.pair_of.data_ptr(),
@@ -215,7 +215,7 @@ class PrefillStack:
         _lib.check(_lib.lib().yn_route_error(self.route_ws.data_ptr(), C.byref(self.dims), stream_ptr(),
                                              C.byref(rc)))
         self.err.zero_()
-        return code or rc.value or (int8_error(self.device) if self.int8 is not None else 0)
+        return code or rc.value
 
 
 def kperm_inverse(a: np.ndarray) -> np.ndarray:
