@@ -56,3 +56,19 @@ def test_an_error_word_of_the_callers_own(T):
     for bad in (mine.long(), torch.zeros(2, dtype=torch.int32, device="cuda"), mine.cpu()):
         with pytest.raises((TypeError, ValueError)):
             bad_call(T, err=bad)
+
+
+def test_no_error_is_lost_between_reading_and_clearing():
+    # a check on one stream while a call on another sets the word: the check, or the one after it, has it
+    x, ids, w, mats, res = setup(16, 96, 256, 2, 4, seed=3)
+    ids[1, 2] = 16
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    assert check_error() == 0
+    for n in range(1500):
+        with torch.cuda.stream(side):
+            torch.cuda._sleep(20000 + 1000 * (n % 100))   # 10 to 60 us, so that the call meets every part of the check
+            int8_experts(x, ids, w, *mats, residual=res)
+        seen = check_error()
+        side.synchronize()
+        assert seen == BAD_EXPERT or check_error() == BAD_EXPERT, n

@@ -6,6 +6,7 @@
 #include <cuda_runtime.h>
 
 #include <algorithm>
+#include <mutex>
 #include <string>
 
 #include "yanah_b200.h"
@@ -973,11 +974,16 @@ extern "C" int yn_i8_experts_err(const yn_i8_mat* gate, const yn_i8_mat* up, con
 
 extern "C" int yn_i8_error(void* stream, int32_t* code_out) {
   if (!code_out) return host_fail(YN_E_INVALID, "null argument");
+  // A word that reads 0 is not cleared: a kernel of another stream may set it meanwhile. One that does not
+  // read 0 takes no further error until it is cleared, and one caller at a time does that.
+  static std::mutex mu;
+  std::lock_guard<std::mutex> lock(mu);
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
   void* p = nullptr;
   cudaError_t e = cudaGetSymbolAddress(&p, g_i8_err);
   if (e == cudaSuccess) e = cudaMemcpyAsync(code_out, p, 4, cudaMemcpyDeviceToHost, st);
-  if (e == cudaSuccess) e = cudaMemsetAsync(p, 0, 4, st);
+  if (e == cudaSuccess) e = cudaStreamSynchronize(st);
+  if (e == cudaSuccess && *code_out) e = cudaMemsetAsync(p, 0, 4, st);
   if (e == cudaSuccess) e = cudaStreamSynchronize(st);
   return e == cudaSuccess ? YN_OK : host_fail(YN_E_CUDA, std::string("yn_i8_error: ") + cudaGetErrorString(e));
 }
