@@ -1,0 +1,50 @@
+"""Options of the stacks that are refused where they are given, before any device work (these run
+without a GPU), and the ones that a stack of some layers takes."""
+from __future__ import annotations
+
+import pytest
+
+torch = pytest.importorskip("torch")
+
+from tests.gpu_helpers import bf16_dev, hidden_rows, small_config
+from yanah_b200.prefill import PrefillStack
+from yanah_b200.routing import RouteRule
+
+RULE = RouteRule(2, "sigmoid")
+
+
+def config(shared=0):
+    return small_config(bits=(4, 4, 4, 4), gs=64, hidden=512, n_experts=16, top_k=2, inter=512, shared=shared, seed=7)
+
+
+def test_a_bias_has_a_row_for_each_layer():
+    from yanah_b200.backend import CudaMoEBackend
+    cfg = config()
+    E = cfg.n_experts
+    for make in (lambda bias, rule=RULE: PrefillStack(cfg, max_rows=4, layers=[1, 3], rule=rule, choice_bias=bias),
+                 lambda bias, rule=RULE: CudaMoEBackend(cfg, rule=rule, choice_bias=bias)):
+        for shape in ((3, E), (E,), (2, E + 1), (1, 2, E)):
+            with pytest.raises(ValueError, match="choice_bias"):
+                make(torch.zeros(shape))
+        with pytest.raises(ValueError, match="needs a rule"):
+            make(torch.zeros(2, E), None)
+    # the model's biases are not those of a stack of two of its layers
+    with pytest.raises(ValueError, match="row for each layer"):
+        PrefillStack(cfg, max_rows=4, layers=[1, 3], rule=RULE, choice_bias=torch.zeros(cfg.n_layers, E))
+    with pytest.raises(TypeError, match="choice_bias"):
+        PrefillStack(cfg, max_rows=4, layers=[1, 3], rule=RULE, choice_bias=torch.zeros(2, E, dtype=torch.float64))
+
+
+@pytest.mark.gpu
+def test_the_biases_of_some_layers():
+    cfg, T = config(), 9
+    bias = 0.3 * torch.randn(cfg.n_layers, cfg.n_experts, generator=torch.Generator().manual_seed(2)).cuda()
+    every = PrefillStack(cfg, max_rows=T, rule=RULE, choice_bias=bias)
+    some = PrefillStack(cfg, max_rows=T, layers=[3, 1], rule=RULE, choice_bias=bias[[3, 1]])
+    h = bf16_dev(hidden_rows(cfg, T, stream=4))
+    a, b = torch.empty_like(h), torch.empty_like(h)
+    for i, layer in enumerate((3, 1)):
+        every.layer(layer, h, a)
+        some.layer(i, h, b)
+        torch.cuda.synchronize()
+        assert torch.equal(every.ids[:T], some.ids[:T]) and torch.equal(every.w[:T], some.w[:T]) and torch.equal(a, b)

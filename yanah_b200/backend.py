@@ -50,7 +50,7 @@ import torch
 from . import _lib
 from .device import DeviceLayer, ExpertArena, Workspace, dims_struct, record_struct, stream_ptr
 from .formats import ExpertLayout, ModelGeometry, RecordSpec
-from .routing import RouteRule, route_scored
+from .routing import RouteRule, check_choice_bias, route_scored
 from .synthetic import StackConfig, dense_layer
 
 
@@ -102,10 +102,9 @@ class CudaMoEBackend:
                  rule: Optional[RouteRule] = None, choice_bias: Optional[torch.Tensor] = None):
         if rule is not None and rule.top_k != cfg.top_k:
             raise ValueError(f"the rule chooses {rule.top_k} experts, the configuration {cfg.top_k}")
-        if choice_bias is not None and rule is None:
-            raise ValueError("choice_bias needs a rule")
+        check_choice_bias(choice_bias, rule, cfg.n_layers, cfg.n_experts)
         self.cfg = cfg
-        self.rule, self.choice_bias = rule, choice_bias      # choice_bias: (layers, E) fp32
+        self.rule, self.choice_bias = rule, choice_bias      # choice_bias: (n_layers, E) fp32
         self.device = torch.device(device)
         self.stream = stream or torch.cuda.current_stream(self.device)
         self.geometry = ModelGeometry(n_layers=cfg.n_layers, n_mtp_layers=0, n_experts=cfg.n_experts,

@@ -26,7 +26,7 @@ from . import _lib
 from .device import DeviceLayer, ExpertArena, dims_struct, fill_synthetic_experts, stream_ptr
 from .formats import RecordSpec
 from .int8 import Int8Matrix, int8_experts, quantize_rows
-from .routing import RouteRule, route_scored
+from .routing import RouteRule, check_choice_bias, route_scored
 from .synthetic import StackConfig, dense_layer
 
 TILE_ROWS = 256      # token rows per tile
@@ -96,8 +96,8 @@ class PrefillStack:
     """Resident experts and dense weights of `layers` of `cfg`, and the
     buffers for prompts of up to `max_rows` rows in total. A layer runs
     entirely on the device (routing, grouping, GEMMs, combine): no host
-    synchronisation. rule / choice_bias: route by a rule, with a bias (layers of the
-    stack, E) fp32 on its choice. experts: "records" (4-bit codes as they are) or "int8"."""
+    synchronisation. rule / choice_bias: route by a rule, with a bias fp32 on its choice,
+    (len(layers), E): row i is that of ``layers[i]``. experts: "records" (4-bit codes as they are) or "int8"."""
 
     def __init__(self, cfg: StackConfig, max_rows: int, device: str = "cuda",
                  layers: Optional[Sequence[int]] = None, rule: Optional[RouteRule] = None,
@@ -106,13 +106,12 @@ class PrefillStack:
             raise ValueError(f"experts must be 'records' or 'int8', not {experts!r}")
         if rule is not None and rule.top_k != cfg.top_k:
             raise ValueError(f"the rule chooses {rule.top_k} experts, the configuration {cfg.top_k}")
-        if choice_bias is not None and rule is None:
-            raise ValueError("choice_bias needs a rule")
         self.cfg = cfg
+        self.layer_ids = list(range(cfg.n_layers)) if layers is None else list(layers)
+        check_choice_bias(choice_bias, rule, len(self.layer_ids), cfg.n_experts)
         self.rule, self.choice_bias = rule, choice_bias
         self.int8: Optional[List[Tuple[Int8Matrix, Int8Matrix, Int8Matrix]]] = [] if experts == "int8" else None
         self.device = torch.device(device)
-        self.layer_ids = list(range(cfg.n_layers)) if layers is None else list(layers)
         self.dims = dims_struct(cfg)
         self.arenas: List[ExpertArena] = []
         self.layers: List[DeviceLayer] = []

@@ -42,6 +42,18 @@ class RouteRule(NamedTuple("RouteRule", [("top_k", int), ("score", str), ("n_gro
         return tuple.__new__(cls, (top_k, score, n_groups, top_groups, group_top, norm_topk, scale))
 
 
+def check_choice_bias(bias: Optional[torch.Tensor], rule: Optional[RouteRule], layers: int, n_experts: int) -> None:
+    """The biases of a stack of layers: a row of fp32 for each of its layers."""
+    if bias is None:
+        return
+    if rule is None:
+        raise ValueError("choice_bias needs a rule")
+    if tuple(bias.shape) != (layers, n_experts):
+        raise ValueError(f"choice_bias must have a row for each layer, ({layers}, {n_experts}), not {tuple(bias.shape)}")
+    if bias.dtype is not torch.float32:
+        raise TypeError(f"choice_bias must be torch.float32, not {bias.dtype}")
+
+
 @lru_cache(maxsize=256)
 def _rule_struct(rule: RouteRule, n_experts: int) -> _lib.RouteRuleStruct:
     return _lib.RouteRuleStruct(n_experts, rule.top_k, SCORES[rule.score], rule.n_groups, rule.top_groups,
