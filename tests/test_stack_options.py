@@ -35,6 +35,11 @@ def test_a_bias_has_a_row_for_each_layer():
         PrefillStack(cfg, max_rows=4, layers=[1, 3], rule=RULE, choice_bias=torch.zeros(2, E, dtype=torch.float64))
 
 
+def test_8_bit_experts_refuse_a_configuration_with_a_shared_one():
+    with pytest.raises(NotImplementedError, match="shared"):
+        PrefillStack(config(shared=512), max_rows=4, experts="int8")
+
+
 @pytest.mark.gpu
 def test_the_biases_of_some_layers():
     cfg, T = config(), 9

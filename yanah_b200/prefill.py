@@ -96,7 +96,9 @@ class PrefillStack:
     """Resident experts and dense weights of `layers` of `cfg`, and the
     buffers for prompts of up to `max_rows` rows in total. A layer runs
     entirely on the device (routing, grouping, GEMMs, combine): no host
-    synchronisation. rule / choice_bias: route by a rule, with a bias fp32 on its choice,
+    synchronisation. A layer's output is the residual and the routed experts: a shared
+    expert is not in it (the backend's prompt pass has one), and ``experts="int8"`` refuses a
+    configuration that has one. rule / choice_bias: route by a rule, with a bias fp32 on its choice,
     (len(layers), E): row i is that of ``layers[i]``. experts: "records" (4-bit codes as they are) or "int8"."""
 
     def __init__(self, cfg: StackConfig, max_rows: int, device: str = "cuda",
@@ -104,6 +106,8 @@ class PrefillStack:
                  choice_bias: Optional[torch.Tensor] = None, experts: str = "records"):
         if experts not in ("records", "int8"):
             raise ValueError(f"experts must be 'records' or 'int8', not {experts!r}")
+        if experts == "int8" and cfg.shared_inter:
+            raise NotImplementedError("experts='int8' runs the routed experts only: the configuration has a shared one")
         if rule is not None and rule.top_k != cfg.top_k:
             raise ValueError(f"the rule chooses {rule.top_k} experts, the configuration {cfg.top_k}")
         self.cfg = cfg
