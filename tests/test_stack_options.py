@@ -53,3 +53,19 @@ def test_the_biases_of_some_layers():
         some.layer(i, h, b)
         torch.cuda.synchronize()
         assert torch.equal(every.ids[:T], some.ids[:T]) and torch.equal(every.w[:T], some.w[:T]) and torch.equal(a, b)
+
+
+@pytest.mark.gpu
+def test_8_bit_experts_refuse_events():
+    # the list would stay empty
+    cfg = config()
+    st = PrefillStack(cfg, max_rows=4, layers=[0], experts="int8")
+    h = bf16_dev(hidden_rows(cfg, 4, stream=4))
+    for call in (lambda e: st.prefill(h, gemm_events=e), lambda e: st.layer(0, h, torch.empty_like(h), gemm_events=e)):
+        with pytest.raises(ValueError, match="gemm_events"):
+            call([])
+    st.prefill(h)
+    events = []
+    PrefillStack(cfg, max_rows=4, layers=[0]).prefill(h, gemm_events=events)
+    torch.cuda.synchronize()
+    assert len(events) == 1 and events[0][0].elapsed_time(events[0][1]) > 0

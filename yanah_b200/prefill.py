@@ -158,11 +158,13 @@ class PrefillStack:
     def layer(self, i: int, h: torch.Tensor, out: torch.Tensor, stream=None, gemm_events=None) -> None:
         """Layer i (index into `layer_ids`) of T = h.shape[0] rows. gemm_events:
         optional list that receives (start, end) CUDA events around the two
-        grouped GEMM launches."""
+        grouped GEMM launches (of the records; the 8-bit experts are one call)."""
         lib, cfg = _lib.lib(), self.cfg
         T, H = h.shape[0], cfg.hidden
         if T > self.max_rows:
             raise ValueError("more rows than the buffers hold")
+        if self.int8 is not None and gemm_events is not None:
+            raise ValueError("gemm_events: the 8-bit experts have no events between their kernels")
         st = stream_ptr(stream)
         D, L = C.byref(self.dims), C.byref(self.structs[i])
         _lib.check(lib.yn_rows_route(D, L, h.data_ptr(), T, self.x.data_ptr(), self.ids.data_ptr(), self.w.data_ptr(),
