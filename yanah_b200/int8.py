@@ -21,7 +21,7 @@ from typing import NamedTuple, Optional
 import torch
 
 from . import _lib
-from .launch import DTYPES, check_floats, check_like, check_no_grad, elsewhere, raw_stream, rows_of, run_there
+from .launch import DTYPES, check_constant, check_floats, check_like, elsewhere, raw_stream, rows_of, run_there
 
 
 class Int8Matrix(NamedTuple):
@@ -67,8 +67,7 @@ def _mat(w: Int8Matrix, index: int, what: str) -> _lib.I8Mat:
         raise ValueError(f"{what}: codes (N, K) or (E, N, K) with scales (N) or (E, N)")
     if codes.get_device() != index or scales.get_device() != index:
         raise ValueError(f"{what} is not on cuda:{index}")
-    if scales.requires_grad:
-        check_no_grad(f"{what}'s scales")
+    check_constant(scales, f"{what}'s scales")
     if (k > 1 and strides[-1] != 1) or (n > 1 and s_strides[-1] != 1):
         raise ValueError(f"{what}: a row's codes and a matrix's scales must be adjacent")
     rs = strides[-2] if n > 1 else (k + 15) // 16 * 16

@@ -3,13 +3,15 @@ of their tensor arguments, and running on a given stream or another device.
 
 They allocate their outputs and workspaces with torch on the stream they run on, so
 two calls never share memory, on one stream or on several, eager or captured. They
-have no gradients: an argument that requires one is refused while gradients are on.
+have no gradients: an argument that requires one is refused while gradients are on, and
+so is one with a tangent (forward mode).
 """
 from __future__ import annotations
 
 from typing import Optional, Tuple
 
 import torch
+from torch.autograd import forward_ad
 
 # element types of the C ABI (YN_F32, YN_BF16, YN_F16)
 DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
@@ -25,9 +27,17 @@ def check_floats(t: torch.Tensor, what: str) -> int:
         raise TypeError(f"{what} must be float32, bfloat16 or float16, not {t.dtype}")
     if not t.is_cuda:
         raise ValueError(f"{what} must be a CUDA tensor")
+    check_constant(t, what)
+    return code
+
+
+def check_constant(t: torch.Tensor, what: str) -> None:
+    """A tensor that no derivative is asked of."""
     if t.requires_grad:
         check_no_grad(what)
-    return code
+    # only inside forward_ad.dual_level() has a tensor a tangent
+    if forward_ad._current_level >= 0 and forward_ad.unpack_dual(t).tangent is not None:
+        raise RuntimeError(f"{what} has a tangent: this operator has no derivative")
 
 
 def check_no_grad(what: str) -> None:
@@ -44,8 +54,7 @@ def check_like(t: torch.Tensor, index: int, shape: tuple, dtypes: tuple, what: s
         raise TypeError(f"{what} must be {' or '.join(str(d) for d in dtypes)}, not {t.dtype}")
     if t.get_device() != index:
         raise ValueError(f"{what} is on {t.device}, not on cuda:{index}")
-    if t.requires_grad:
-        check_no_grad(what)
+    check_constant(t, what)
 
 
 def rows_of(t: torch.Tensor, what: str) -> Tuple[torch.Tensor, int, int, int]:
