@@ -886,7 +886,7 @@ extern "C" int yn_i8_experts_err(const yn_i8_mat* gate, const yn_i8_mat* up, con
     return host_fail(YN_E_INVALID, "gate and up are (E, I, H), down is (E, H, I)");
   if (E > I8_MAX_E || top_k < 1 || top_k > 32) return host_fail(YN_E_UNSUPPORTED, "at most 1024 experts, top_k in [1, 32]");
   if (!dtype_ok(dtype)) return host_fail(YN_E_INVALID, "unknown dtype");
-  if (rows < 0 || rows * top_k > (1 << 22) || x_stride < H || out_stride < H || (residual && res_stride < H))
+  if (rows < 0 || rows > (1 << 22) / top_k || x_stride < H || out_stride < H || (residual && res_stride < H))
     return host_fail(YN_E_INVALID, "rows * top_k must be in [0, 2^22], strides at least hidden");
   if (rows == 0) return YN_OK;
   if (!x || !ids || !weights || !out || !ws) return host_fail(YN_E_INVALID, "null argument");
