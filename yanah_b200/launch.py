@@ -89,6 +89,6 @@ def run_there(fn, device: torch.device, stream: Optional[torch.cuda.Stream], ten
             return fn()
         with torch.cuda.stream(stream):
             for t in tensors:
-                if t is not None:
+                if t is not None and t.is_cuda:   # fn refuses others
                     t.record_stream(stream)
             return fn()
