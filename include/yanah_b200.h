@@ -480,9 +480,9 @@ int yn_i8_quant_rows(const void* x, int32_t dtype, int64_t row_stride, int64_t r
 /* y (rows, w->rows) = x (rows, w->cols) times the transpose of w, the rows of x
  * as above, sums exact in 32 bits, then * row scale * channel scale in fp32 and
  * one rounding to y_dtype (QuantizedLinear's counterpart, mlx_backend.py:305-306,
- * for matrices with channel scales). Up to 3 rows (5 of a small matrix) run on dp4a
- * in one kernel that makes the codes itself; more on the tensor cores (tcgen05,
- * kind::i8). ws: yn_i8_linear_ws_bytes bytes, 256-byte aligned, need not be cleared. */
+ * for matrices with channel scales). A row, or a few (up to 3 short ones, up to 5 of a
+ * small matrix), run on dp4a in one kernel that makes the codes itself; more on the
+ * tensor cores (tcgen05, kind::i8). ws: yn_i8_linear_ws_bytes bytes, 256-byte aligned, need not be cleared. */
 size_t yn_i8_linear_ws_bytes(int64_t rows, int32_t cols);
 int yn_i8_linear(const yn_i8_mat* w, const void* x, int32_t dtype, int64_t x_stride, int64_t rows, void* y,
                  int32_t y_dtype, int64_t y_stride, void* ws, size_t ws_bytes, void* stream);

@@ -261,12 +261,12 @@ YN_DEV void i8_dots(const int8_t* const (&w)[R], const int8_t* xs, int KP, int K
 
 // y (T, N) of T <= 5 rows (linear_few): every block makes the rows' codes itself (they are a few KB),
 // then its warps take 4 output channels at a time through the matrix, which is read once:
-// bound by that read with one row (2048 x 151936: 47.4 us, 6.57 TB/s), with five by the
-// products too (59 us). A lane copies its own 16 codes of 4 channels per step into a ring of
+// bound by that read with one row (2048 x 151936: 47.6 us, 6.54 TB/s), with more by the
+// products too (three rows 51.8 us). A lane copies its own 16 codes of 4 channels per step into a ring of
 // its warp (cp.async, I8_FS steps deep, 144 KB in flight per SM) and reads them back itself,
 // so that neither the products nor the sums over lanes stop the copies and no thread waits
-// for another. Loads into registers instead (8 per lane in flight) took 71 us for five rows,
-// twice as many of them 91 us.
+// for another. With five rows the ring took 59 us, loads into registers instead (8 per lane in
+// flight) 71 us, twice as many of them 91 us.
 constexpr int I8_FR = 4;    // channels per step
 constexpr int I8_FS = 4;    // steps in the ring
 constexpr int I8_FRING = I8_FS * I8_FR * I8_GK;   // bytes per warp
@@ -695,11 +695,18 @@ I8Mat mat_of(const yn_i8_mat& w) {
 }
 
 constexpr int I8_MAX_K = 131072;   // 127^2 * 131072 < 2^31
-// Rows of a product on dp4a: three, or five of a small matrix, where a launch counts. 2048 x 151936:
-// 47 us one row, 51.5 three, 53.6 four, 58.7 five; on the tensor cores, codes made first, 51 to 53.6.
-// 2048 x 16384: 6.4, 8.9, 9.8, 11.3 and 8.3; 2048 x 4096: 4.0, 5.6, 5.8, 6.6 and 8.0.
-constexpr int I8_FEW = 3, I8_FEW_SMALL = 5;
-constexpr long long I8_SMALL = 16ll << 20;   // codes
+// Rows of a product on dp4a: one row of any matrix that fits, and a few where a launch counts (small
+// matrices) or where every block's work on their codes does not (short rows). K x N, us with 1 to 5 rows
+// on dp4a and, with any of them, on the tensor cores, which have the codes made first:
+//   2048 x 4096     5.0   6.2   6.4   7.0   7.4   |  8.4      4096 x 4096    6.9   9.7  10.2  10.3  11.2  | 11.1
+//   2048 x 8192     6.6   7.8   8.4   8.7   9.7   |  9.2      8192 x 1024    8.3  14.4  14.7  19.0  21.2  | 17.2
+//   2048 x 16384    8.5  10.5  11.0  11.9  13.1   | 10.9      8192 x 2048    8.9  15.0  15.3  19.3  21.5  | 17.5
+//   2048 x 65536   22.7  24.8  26.0  28.0  30.5   | 26.2     16384 x 1024   13.0  33.4  35.0  35     38   | 29.9
+//   2048 x 151936  47.6  50.8  51.8  55    62     | 51 to 52  2560 x 40000  17.8  20.6  21.8  23.5  29    | 21.2
+//   1536 x 40000   12.2  13.4  14.2  16.0  17.5   | 14.8      4096 x 16384  13.4  17.2  21.3  23    25    | 15.6
+constexpr int I8_FEW = 3, I8_FEW_MEDIUM = 4, I8_FEW_SMALL = 5;
+constexpr long long I8_SMALL = 8ll << 20, I8_MEDIUM = 16ll << 20;   // codes of the matrix
+constexpr long long I8_FEW_CODES = 6 * 1024, I8_FEW_CODES_MEDIUM = 24 * 1024;   // codes of the rows
 
 int check_mat(const yn_i8_mat& w, const char* what) {
   const std::string n(what);
@@ -715,7 +722,9 @@ int check_mat(const yn_i8_mat& w, const char* what) {
 }
 
 bool linear_few(long long rows, long long k, long long n) {
-  return rows <= (n * k <= I8_SMALL ? I8_FEW_SMALL : I8_FEW) && rows * (long long)up_to(k, I8_GK) <= 96 * 1024;
+  if (rows == 1) return up_to(k, I8_GK) <= 96 * 1024;
+  if (n * k > I8_MEDIUM) return rows <= I8_FEW && rows * k <= I8_FEW_CODES;
+  return rows <= (n * k <= I8_SMALL ? I8_FEW_SMALL : I8_FEW_MEDIUM) && rows * k <= I8_FEW_CODES_MEDIUM;
 }
 
 template <int T>
@@ -794,7 +803,7 @@ extern "C" int yn_i8_quant_rows(const void* x, int32_t dtype, int64_t row_stride
 }
 
 extern "C" size_t yn_i8_linear_ws_bytes(int64_t rows, int32_t cols) {
-  if (rows < 1 || cols < 1 || linear_few(rows, cols, I8_SMALL + 1)) return 0;   // for any number of channels
+  if (rows < 1 || cols < 1 || linear_few(rows, cols, I8_MEDIUM + 1)) return 0;   // few rows of a large matrix are few of any
   return up_to((size_t)rows * up_to(cols, 16), 256) + (size_t)rows * 4;
 }
 
