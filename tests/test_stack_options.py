@@ -69,3 +69,23 @@ def test_8_bit_experts_refuse_events():
     PrefillStack(cfg, max_rows=4, layers=[0]).prefill(h, gemm_events=events)
     torch.cuda.synchronize()
     assert len(events) == 1 and events[0][0].elapsed_time(events[0][1]) > 0
+
+
+@pytest.mark.gpu
+def test_8_bit_experts_hold_no_buffers_of_the_records():
+    cfg, T = config(), 2048
+    K, H, I = cfg.top_k, cfg.hidden, cfg.moe_inter
+
+    def asked():
+        # what was asked of the allocator; memory_allocated counts its blocks, of which a large one may have up to 1 MiB more
+        return torch.cuda.memory_stats()["requested_bytes.all.current"]
+
+    def held(experts):
+        before = asked()
+        st = PrefillStack(cfg, max_rows=T, layers=[0], experts=experts)
+        weights = sum(m.codes.untyped_storage().nbytes() + 4 * m.scales.numel() for m in st.int8[0]) if experts == "int8" \
+            else st.arenas[0].buf.numel()
+        return asked() - before - weights
+
+    # x16 and y (pairs, H) and act (pairs, I), 16 bits each
+    assert held("records") - held("int8") >= 2 * T * K * (2 * H + I)

@@ -141,17 +141,19 @@ class PrefillStack:
         mu, md = C.c_int32(0), C.c_int32(0)
         _lib.check(lib.yn_prefill_max_tiles(C.byref(self.dims), max_rows, C.byref(mu), C.byref(md)))
         self.max_up, self.max_dn = mu.value, md.value
-        self.tiles_up = torch.empty((self.max_up, 4), dtype=torch.int32, device=dev)
-        self.tiles_dn = torch.empty((self.max_dn, 4), dtype=torch.int32, device=dev)
         self.n_tiles = torch.zeros(2, dtype=torch.int32, device=dev)
         self.pair_row = torch.empty(P, dtype=torch.int32, device=dev)
         self.pair_of = torch.empty(P, dtype=torch.int32, device=dev)
         self.x = torch.empty((T, H), dtype=torch.bfloat16, device=dev)
-        self.x16 = torch.empty((P, H), dtype=torch.float16, device=dev)  # rows in pair order
         self.ids = torch.empty((T, K), dtype=torch.int32, device=dev)
         self.w = torch.empty((T, K), dtype=torch.float32, device=dev)
-        self.act = torch.empty((P, I), dtype=torch.bfloat16, device=dev)
-        self.y = torch.empty((P, H), dtype=torch.bfloat16, device=dev)
+        self.tiles_up = self.tiles_dn = self.x16 = self.act = self.y = None
+        if self.int8 is None:      # what the record experts need; int8_experts takes a workspace of its own
+            self.tiles_up = torch.empty((self.max_up, 4), dtype=torch.int32, device=dev)
+            self.tiles_dn = torch.empty((self.max_dn, 4), dtype=torch.int32, device=dev)
+            self.x16 = torch.empty((P, H), dtype=torch.float16, device=dev)  # rows in pair order
+            self.act = torch.empty((P, I), dtype=torch.bfloat16, device=dev)
+            self.y = torch.empty((P, H), dtype=torch.bfloat16, device=dev)
         self.err = torch.zeros(1, dtype=torch.int32, device=dev)
         self.ping = torch.empty((2, T, H), dtype=torch.bfloat16, device=dev)
 
