@@ -63,3 +63,18 @@ def test_products_that_cancel(T, dtype):
     assert np.linalg.norm(want) <= 2e-4 * np.linalg.norm(one[0])
     norm = np.linalg.norm
     assert norm(got - want) <= (4e-3 + torch.finfo(dtype).eps / 2) * norm(want) + 2.0 ** -20 * norm(size)
+
+
+@pytest.mark.parametrize("dtype", DTS)
+@pytest.mark.parametrize("T", [3, 60])
+def test_the_output_may_be_the_residual(T, dtype):
+    x, ids, w, mats, res = setup(16, 96, 257, T, 4, dtype, seed=34)
+    want = int8_experts(x, ids, w, *mats, residual=res)
+    wide = torch.full((T, 300), 7.0, dtype=dtype, device="cuda")
+    for place in (wide[:, 8:265], wide[:, 5:262], res):
+        place.copy_(res)
+        assert int8_experts(x, ids, w, *mats, residual=place, out=place) is place
+        assert torch.equal(place, want)
+        if place is not res:
+            place.fill_(7.0)
+            assert (wide == 7.0).all()

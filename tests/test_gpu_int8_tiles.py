@@ -91,3 +91,13 @@ def test_gate_and_up_in_either_order(I, H, T, k, dtype):
     assert torch.equal(int8_experts(x, ids, w, gate, Int8Matrix(wide[..., :H], up.scales), down, residual=res), want)
     assert torch.equal(int8_experts(x, ids, w, Int8Matrix(wide[..., :H], up.scales), up, down, residual=res),
                        int8_experts(x, ids, w, up, up, down, residual=res))
+
+
+@pytest.mark.parametrize("dtype", DTS)
+@pytest.mark.parametrize("k,rows", [(1, (119, 120, 121)), (2, (59, 60, 61)), (3, (39, 40, 41))])
+def test_chunks_of_either_size(k, rows, dtype):
+    # 3 experts: up to 120 pairs are cut into chunks of 64 rows, more into chunks of 256
+    x, ids, w, mats, res = setup(3, 100, 136, 200, k, dtype, seed=60 + k)
+    whole = check_experts(x, ids, w, mats, res)
+    for n in rows:
+        assert torch.equal(int8_experts(x[:n], ids[:n], w[:n], *mats, residual=res[:n]), whole[:n])

@@ -747,9 +747,10 @@ struct ExpertsWs {
   int nb;
 };
 // Rows per chunk of an expert, by the pairs per expert (see launch_gemm_nb). On 512 experts of 3 MB 64
-// and 256 rows take 111 and 126 us at 5 pairs per expert, 141 and 167 at 10, 196 and 218 at 20; on 64
-// experts of 9 MB 92 and 93 us at 7.5, 117 and 121 at 19, 136 and 132 at 38, 173 and 159 at 75.
-int chunk_rows(long long pairs, int E) { return pairs <= 24ll * E ? 64 : 256; }
+// and 256 rows take 118 and 139 us at 5 pairs per expert, 154 and 181 at 10, 210 and 242 at 20, 325 and
+// 336 at 40; on 64 experts of 9 MB 98 and 98 us at 7.5, 116 and 119 at 19, 137 and 137 at 38, 174 and 165
+// at 75, 255 and 211 at 150.
+int chunk_rows(long long pairs, int E) { return pairs <= 40ll * E ? 64 : 256; }
 // Pairs that go to the dp4a kernels: two launches instead of six, but they read an expert's matrices
 // for every pair. The two ways meet at about 120 MB of such reads: 30 pairs on 3 MB experts take 26 us so
 // and 32 us grouped (40: 30 and 31, 50: 39 and 34), 8 pairs on 9 MB experts 21.5 and 27 us (16: 36 and 28).
