@@ -112,8 +112,9 @@ def int8_experts(x: torch.Tensor, ids: torch.Tensor, weights: torch.Tensor, gate
 
     x (T, H); ids (T, k) int32 and weights (T, k) fp32 as ``routing.route_scored``
     returns them: an id of -1 has no expert (any other id outside [0, E) is left out and
-    reported by ``check_error``, or in ``err``, (1) int32, an error word of the caller's own). gate, up: (E, I, H); down: (E, H, I). The activations
-    are quantised per (row, expert), the sum is fp32 and rounded once to the type of x.
+    reported by ``check_error``, or in ``err``, (1) int32, an error word of the caller's own).
+    gate, up: (E, I, H); down: (E, H, I). The activations are quantised per (row, expert),
+    the sum is fp32 and rounded once to the type of x.
     ``out``: (T, H) to write, rows of adjacent elements; it may be the residual."""
     dtype, dev = check_floats(x, "x"), x.get_device()
     if elsewhere(dev, stream):
