@@ -23,3 +23,38 @@ def test_rows_without_a_workspace():
         assert ws(rows, k) == 0, (rows, k)
     for rows, k in ((1, 98305), (2, 4096), (3, 2049), (4, 1), (3, 4096)):
         assert ws(rows, k) >= rows * k, (rows, k)
+
+
+def test_pointers_that_are_not_aligned_to_their_elements():
+    # a kernel would fault on them
+    import ctypes as C
+
+    from tests.test_ops_refusals import P, mat, rule
+    lib, odd, half = _lib.lib(), C.c_void_p(257), C.c_void_p(258)
+    r = rule()
+
+    def route(logits=P, dtype=0, bias=None, ids=P, w=P):
+        return lib.yn_route_scored(C.byref(r), logits, dtype, 64, 2, bias, None, ids, w, None)
+
+    for kw in (dict(logits=half), dict(logits=odd, dtype=1), dict(logits=odd, dtype=2), dict(bias=half), dict(ids=half), dict(w=odd)):
+        assert route(**kw) == INV, kw
+
+    def logprobs(at, p):
+        a = [P] * 6
+        a[at] = p
+        return lib.yn_token_logprobs(P, 1, 100, 3, 100, a[0], 4, a[1], a[2], a[3], a[4], a[5], None)
+
+    for at in range(6):
+        assert logprobs(at, half) == INV, at
+    assert lib.yn_i8_quant_rows(odd, 1, 64, 2, 64, P, 64, P, None) == INV
+    assert lib.yn_i8_quant_rows(P, 1, 64, 2, 64, P, 64, half, None) == INV
+    m = mat(scales=258)
+    assert lib.yn_i8_linear(C.byref(m), P, 0, 64, 2, P, 0, 32, None, 0, None) == INV
+    g, d = mat(4, 32, 64, 64, 2048, 32), mat(4, 64, 32, 32, 2048, 64)
+
+    def experts_err(x=P, ids=P, w=P, res=None, out=P, err=None):
+        return lib.yn_i8_experts_err(C.byref(g), C.byref(g), C.byref(d), x, 1, 64, 2, ids, w, 2, res, 64, out, 64, P, 1 << 30,
+                                     err, None)
+
+    for kw in (dict(x=odd), dict(ids=half), dict(w=half), dict(res=odd), dict(out=odd), dict(err=half)):
+        assert experts_err(**kw) == INV, kw

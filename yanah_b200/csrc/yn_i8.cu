@@ -715,6 +715,7 @@ int check_mat(const yn_i8_mat& w, const char* what) {
   if (w.cols > I8_MAX_K) return host_fail(YN_E_UNSUPPORTED, n + ": at most 131072 columns (32-bit sums)");
   if (reinterpret_cast<uintptr_t>(w.codes) % 16 || w.row_stride % 16 || (w.n_mats > 1 && w.mat_stride % 16))
     return host_fail(YN_E_INVALID, n + ": rows of codes must start at multiples of 16 bytes");
+  if (!host_aligned(4, w.scales)) return host_fail(YN_E_INVALID, n + ": scales must be aligned to their element");
   if (w.row_stride < w.cols || (w.n_mats > 1 && (w.mat_stride < 1 || w.scale_stride < w.rows)))
     return host_fail(YN_E_INVALID, n + ": rows or matrices overlap");
   if (w.row_stride >= (1ll << 40) || w.mat_stride >= (1ll << 40)) return host_fail(YN_E_UNSUPPORTED, n + ": stride above 2^40");
@@ -798,7 +799,8 @@ extern "C" int yn_i8_quant_rows(const void* x, int32_t dtype, int64_t row_stride
     return host_fail(YN_E_INVALID, "rows must be in [0, 2^31), strides at least cols, cols at least 1");
   if (rows == 0) return YN_OK;
   if (!x || !codes || !scales) return host_fail(YN_E_INVALID, "null argument");
-  if (reinterpret_cast<uintptr_t>(x) % dtype_size(dtype)) return host_fail(YN_E_INVALID, "x must be aligned to its element");
+  if (!host_aligned(dtype_size(dtype), x) || !host_aligned(4, scales))
+    return host_fail(YN_E_INVALID, "x and scales must be aligned to their elements");
   return launch_quant(dtype, x, row_stride, rows, cols, nullptr, nullptr, 1, reinterpret_cast<int8_t*>(codes), code_stride, scales, true,
                       reinterpret_cast<cudaStream_t>(stream));
 }
@@ -819,7 +821,7 @@ extern "C" int yn_i8_linear(const yn_i8_mat* w, const void* x, int32_t dtype, in
     return host_fail(YN_E_INVALID, "rows must be in [0, 2^31 - 256), strides at least the row lengths");
   if (rows == 0) return YN_OK;
   if (!x || !y) return host_fail(YN_E_INVALID, "null argument");
-  if (reinterpret_cast<uintptr_t>(x) % dtype_size(dtype) || reinterpret_cast<uintptr_t>(y) % dtype_size(y_dtype))
+  if (!host_aligned(dtype_size(dtype), x) || !host_aligned(dtype_size(y_dtype), y))
     return host_fail(YN_E_INVALID, "x and y must be aligned to their elements");
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
   if (linear_few(rows, w->cols, w->rows)) {
@@ -900,10 +902,8 @@ extern "C" int yn_i8_experts_err(const yn_i8_mat* gate, const yn_i8_mat* up, con
     return host_fail(YN_E_INVALID, "rows * top_k must be in [0, 2^22], strides at least hidden");
   if (rows == 0) return YN_OK;
   if (!x || !ids || !weights || !out || !ws) return host_fail(YN_E_INVALID, "null argument");
-  const int size = dtype_size(dtype);
-  if (reinterpret_cast<uintptr_t>(x) % size || reinterpret_cast<uintptr_t>(out) % size ||
-      (residual && reinterpret_cast<uintptr_t>(residual) % size))
-    return host_fail(YN_E_INVALID, "rows must be aligned to their element");
+  if (!host_aligned(dtype_size(dtype), x, out, residual) || !host_aligned(4, ids, weights, err))
+    return host_fail(YN_E_INVALID, "rows, ids, weights and the error word must be aligned to their elements");
   const ExpertsWs L = experts_ws(rows, top_k, E, H, I);
   if (ws_bytes < L.total || reinterpret_cast<uintptr_t>(ws) % 256)
     return host_fail(YN_E_INVALID, "workspace too small or not 256-byte aligned");

@@ -19,6 +19,12 @@ int host_check_qmat(const yn_qmat& m, int rows, int cols, int bits, const char* 
 // Raise a kernel's dynamic shared-memory limit (once per device).
 int host_set_smem(const void* kernel, size_t bytes);
 
+// Whether every pointer starts at a multiple of `size` bytes (null does).
+template <typename... P>
+bool host_aligned(size_t size, const P*... p) {
+  return (... && (reinterpret_cast<uintptr_t>(p) % size == 0));
+}
+
 // The driver's cuTensorMapEncodeTiled.
 using TmapEncode = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*,
                                 const cuuint64_t*, const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave,

@@ -669,7 +669,8 @@ extern "C" int yn_token_logprobs(const void* logits, int32_t dtype, int64_t row_
   if (rows == 0) return YN_OK;
   if (!logits || (tokens && (!logprob || !rank)) || (n_top && (!top_ids || !top_logprobs)))
     return host_fail(YN_E_INVALID, "null argument");
-  if (reinterpret_cast<uintptr_t>(logits) % size) return host_fail(YN_E_INVALID, "logits must be aligned to their element");
+  if (!host_aligned(size, logits) || !host_aligned(4, tokens, logprob, entropy, rank, top_ids, top_logprobs))
+    return host_fail(YN_E_INVALID, "logits, tokens and outputs must be aligned to their elements");
   LpArgs a{};
   a.z = reinterpret_cast<const uint8_t*>(logits);
   a.ld = row_stride;

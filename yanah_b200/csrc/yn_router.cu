@@ -499,6 +499,8 @@ extern "C" int yn_route_scored(const yn_route_rule* rule, const void* logits, in
     return host_fail(YN_E_INVALID, "rows must be in [0, 2^31), row_stride at least n_experts");
   if (rows == 0) return YN_OK;
   if (!logits || !ids || !weights) return host_fail(YN_E_INVALID, "null argument");
+  if (!host_aligned(dtype == YN_F32 ? 4 : 2, logits) || !host_aligned(4, bias, ids, weights))
+    return host_fail(YN_E_INVALID, "logits, bias, ids and weights must be aligned to their elements");
   RouterArgs a{};
   a.z = logits;
   a.ld = row_stride;
