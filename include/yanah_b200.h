@@ -460,8 +460,10 @@ int yn_rows_route_logits(const yn_dims* dims, int32_t T, void* ws, float** logit
 
 /* `n_mats` matrices of (rows, cols) signed 8-bit codes with one fp32 scale per
  * row (output channel): value = code * scale. Rows `row_stride` and matrices
- * `mat_stride` bytes apart, both and the base multiples of 16; scales of a
- * matrix contiguous, those of matrices `scale_stride` elements apart. */
+ * `mat_stride` bytes apart, both and the base multiples of 16; matrices one
+ * after another (mat_stride a multiple of row_stride) or interleaved row by row
+ * (row_stride a multiple of mat_stride); scales of a matrix contiguous, those of
+ * matrices `scale_stride` elements apart. */
 typedef struct yn_i8_mat {
   const void* codes;
   const float* scales;

@@ -101,3 +101,61 @@ def test_chunks_of_either_size(k, rows, dtype):
     whole = check_experts(x, ids, w, mats, res)
     for n in rows:
         assert torch.equal(int8_experts(x[:n], ids[:n], w[:n], *mats, residual=res[:n]), whole[:n])
+
+
+def at_the_end(t):
+    """A copy of a matrix's codes that ends where its memory does (a block of its own of whole 2 MiB pages)."""
+    E, N, K = t.shape
+    pitch = (K + 15) // 16 * 16
+    size = E * N * pitch
+    block = torch.zeros((size + (20 << 20) + (2 << 20) - 1) >> 21 << 21, dtype=torch.int8, device="cuda")
+    out = block[block.numel() - size:].view(E, N, pitch)
+    out[..., :K] = t
+    return out[..., :K]
+
+
+@pytest.mark.parametrize("E,I,H,T,k", [(9, 32, 2, 149, 7), (3, 16, 100, 60, 2), (2, 64, 128, 40, 2), (5, 80, 255, 30, 4),
+                                       (4, 131, 300, 90, 1), (1, 208, 374, 10, 8)])
+def test_matrices_at_the_end_of_their_memory(E, I, H, T, k):
+    # tiles that lie partly or wholly past the last rows: nothing there is touched
+    x, ids, w, mats, res = setup(max(E, k), I, H, T, k, seed=70 + E)
+    mats = [Int8Matrix(m.codes[:E], m.scales[:E]) for m in mats]
+    ids = ids % E
+    want = check_experts(x, ids, w, mats, res)
+    for which in ((0,), (1,), (2,), (0, 1, 2), (1, 0, 2)):
+        moved = list(mats)
+        for i in which:
+            moved[i] = Int8Matrix(at_the_end(mats[i].codes), mats[i].scales)
+        assert torch.equal(int8_experts(x, ids, w, *moved, residual=res), want), which
+    for i in range(3):      # a product's matrix
+        one = Int8Matrix(at_the_end(mats[i].codes[:1])[0], mats[i].scales[0])
+        rows = normal(40, one.codes.shape[1], seed=i)
+        assert torch.equal(int8_linear(rows, one), int8_linear(rows, Int8Matrix(mats[i].codes[0], mats[i].scales[0])))
+
+
+@pytest.mark.parametrize("T", [3, 90])
+def test_matrices_interleaved_row_by_row(T):
+    E, I, H, k = 6, 100, 200, 4
+    x, ids, w, mats, res = setup(E, I, H, T, k, seed=80)
+    want = check_experts(x, ids, w, mats, res)
+
+    def interleaved(m, extra=0):
+        n, _, c = m.codes.shape
+        buf = torch.zeros(m.codes.shape[1], n + extra, (c + 15) // 16 * 16, dtype=torch.int8, device="cuda")
+        v = buf[:, :n, :c].transpose(0, 1)
+        v.copy_(m.codes)
+        return Int8Matrix(v, m.scales)
+
+    for extra in (0, 2):
+        inter = [interleaved(m, extra) for m in mats]
+        for pick in ((1, 1, 1), (1, 0, 0), (0, 1, 0), (0, 0, 1)):
+            got = int8_experts(x, ids, w, *[inter[i] if p else mats[i] for i, p in enumerate(pick)], residual=res)
+            assert torch.equal(got, want), (extra, pick)
+
+
+def test_one_row_matrices_of_any_distance():
+    x, ids, w, (gate, up, down), res = setup(5, 1, 40, 90, 2, seed=81)
+    want = check_experts(x, ids, w, (gate, up, down), res)
+    wide = torch.zeros(5, 3, 80, dtype=torch.int8, device="cuda")
+    wide[:, 1, :40] = gate.codes[:, 0]
+    assert torch.equal(int8_experts(x, ids, w, Int8Matrix(wide[:, 1:2, :40], gate.scales), up, down, residual=res), want)

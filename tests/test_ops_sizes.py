@@ -58,3 +58,18 @@ def test_pointers_that_are_not_aligned_to_their_elements():
 
     for kw in (dict(x=odd), dict(ids=half), dict(w=half), dict(res=odd), dict(out=odd), dict(err=half)):
         assert experts_err(**kw) == INV, kw
+
+
+def test_strides_of_matrices_that_are_not_in_order():
+    # a tensor map whose strides are not multiples of one another reads past the matrices
+    from tests.test_ops_refusals import mat
+    UNS = _lib.YN_E_UNSUPPORTED
+    ok = mat(4, 32, 64, 64, 2048, 32)
+    d = mat(4, 64, 32, 32, 2048, 64)
+    for ms, rs in ((2048 + 16, 64), (2048 - 64, 64), (2000, 80), (64, 64 * 3), (80, 320 + 80 + 16), (96, 64 * 4)):
+        bad = mat(4, 32, 64, rs, ms, 32)
+        assert experts(g=bad, u=ok, d=d) == UNS and experts(g=ok, u=bad, d=d) == UNS, (ms, rs)
+        assert experts(g=ok, u=ok, d=mat(4, 64, 32, rs, ms, 64)) == (UNS if (ms, rs) != (2048 - 64, 64) else UNS)
+    # matrices that overlap
+    for m in (mat(4, 32, 64, 64, 48, 32), mat(4, 32, 64, 64, 2048, 31)):
+        assert experts(g=m, u=ok, d=d) == INV

@@ -630,32 +630,28 @@ int tmap_rows(I8Maps* maps, const void* base, long long cols, long long rows, lo
   }
   return YN_OK;
 }
-int tmap_mats(CUtensorMap* m, const yn_i8_mat& w, int box_rows) {
-  const cuuint64_t dims[3] = {(cuuint64_t)w.cols, (cuuint64_t)w.rows, (cuuint64_t)w.n_mats};
-  const cuuint64_t strides[2] = {(cuuint64_t)w.row_stride,
-                                 (cuuint64_t)(w.n_mats > 1 ? w.mat_stride : w.row_stride * (int64_t)w.rows)};
-  const cuuint32_t box[3] = {128u, (cuuint32_t)box_rows, 1u};
-  return tmap(m, w.codes, 3, dims, strides, box);
+// The matrices' rows: (K, rows, matrices), or (K, matrices, rows) where the matrices are interleaved row by
+// row. cuTensorMapEncodeTiled asks that each stride be a multiple of the one before; a map whose strides
+// are not so is accepted, but its boxes may touch memory past the last row.
+bool mats_first(const yn_i8_mat& w) { return w.n_mats > 1 && w.rows > 1 && w.mat_stride < w.row_stride; }
+bool strides_in_order(const yn_i8_mat& w) {
+  if (w.n_mats == 1 || w.rows == 1) return true;
+  if (mats_first(w)) return w.row_stride % w.mat_stride == 0 && w.row_stride / w.mat_stride >= w.n_mats;
+  return w.mat_stride % w.row_stride == 0 && w.mat_stride / w.row_stride >= w.rows;
 }
-// Gate and up in one map, (K, 16 rows, 2 matrices, rows / 16, E), where the two are laid out
-// alike and their rows are whole groups of 16: one copy per stage instead of eight (11 -> 16
-// TB/s from L2). Sets `both`; else two maps of 16-row boxes.
-int tmap_gate_up(I8Gemm* g, I8Maps* maps, const yn_i8_mat& gate, const yn_i8_mat& up) {
-  const int64_t delta = reinterpret_cast<int64_t>(up.codes) - reinterpret_cast<int64_t>(gate.codes);
-  const int64_t apart = delta < 0 ? -delta : delta;
-  g->both = gate.rows % 16 == 0 && gate.row_stride == up.row_stride && (gate.n_mats == 1 || gate.mat_stride == up.mat_stride) &&
-            apart > 0 && apart < (1ll << 40);
-  g->swapped = g->both && delta < 0;
-  if (!g->both) {
-    const int rc = tmap_mats(&maps->a, gate, 16);
-    return rc ? rc : tmap_mats(&maps->a_up, up, 16);
-  }
-  const yn_i8_mat& first = g->swapped ? up : gate;
-  const cuuint64_t dims[5] = {(cuuint64_t)gate.cols, 16u, 2u, (cuuint64_t)gate.rows / 16, (cuuint64_t)gate.n_mats};
-  const cuuint64_t strides[4] = {(cuuint64_t)gate.row_stride, (cuuint64_t)apart, (cuuint64_t)gate.row_stride * 16,
-                                 (cuuint64_t)(gate.n_mats > 1 ? gate.mat_stride : gate.row_stride * (int64_t)gate.rows)};
-  const cuuint32_t box[5] = {128u, 16u, 2u, 4u, 1u};
-  return tmap(&maps->a, first.codes, 5, dims, strides, box);
+int tmap_mats(CUtensorMap* m, const yn_i8_mat& w, int box_rows) {
+  const int r = mats_first(w) ? 2 : 1, e = 3 - r;   // places of the rows and of the matrices
+  cuuint64_t dims[3], strides[2];
+  cuuint32_t box[3];
+  dims[0] = (cuuint64_t)w.cols;
+  dims[r] = (cuuint64_t)w.rows;
+  dims[e] = (cuuint64_t)w.n_mats;
+  strides[r - 1] = (cuuint64_t)(w.n_mats > 1 && w.rows == 1 ? w.mat_stride : w.row_stride);
+  strides[e - 1] = (cuuint64_t)(w.n_mats > 1 ? w.mat_stride : w.row_stride * (int64_t)w.rows);
+  box[0] = 128u;
+  box[r] = (cuuint32_t)box_rows;
+  box[e] = 1u;
+  return tmap(m, w.codes, 3, dims, strides, box);
 }
 
 int sm_count(int* out) {
@@ -716,8 +712,10 @@ int check_mat(const yn_i8_mat& w, const char* what) {
   if (reinterpret_cast<uintptr_t>(w.codes) % 16 || w.row_stride % 16 || (w.n_mats > 1 && w.mat_stride % 16))
     return host_fail(YN_E_INVALID, n + ": rows of codes must start at multiples of 16 bytes");
   if (!host_aligned(4, w.scales)) return host_fail(YN_E_INVALID, n + ": scales must be aligned to their element");
-  if (w.row_stride < w.cols || (w.n_mats > 1 && (w.mat_stride < 1 || w.scale_stride < w.rows)))
+  if (w.row_stride < w.cols || (w.n_mats > 1 && (w.mat_stride < w.cols || w.scale_stride < w.rows)))
     return host_fail(YN_E_INVALID, n + ": rows or matrices overlap");
+  if (!strides_in_order(w))
+    return host_fail(YN_E_UNSUPPORTED, n + ": matrices must lie one after another, whole rows apart, or be interleaved row by row");
   if (w.row_stride >= (1ll << 40) || w.mat_stride >= (1ll << 40)) return host_fail(YN_E_UNSUPPORTED, n + ": stride above 2^40");
   return YN_OK;
 }
@@ -939,7 +937,11 @@ extern "C" int yn_i8_experts_err(const yn_i8_mat* gate, const yn_i8_mat* up, con
   const long long max_chunks = E + P / L.nb + 1;
   I8Maps maps{};
   I8Gemm g{};
-  if ((rc = tmap_gate_up(&g, &maps, *gate, *up)) || (rc = tmap_rows(&maps, codes, H, P, L.ldc))) return rc;
+  if ((rc = tmap_mats(&maps.a, *gate, 16)) || (rc = tmap_mats(&maps.a_up, *up, 16)) ||
+      (rc = tmap_rows(&maps, codes, H, P, L.ldc)))
+    return rc;
+  g.mats_first = mats_first(*gate);
+  g.up_mats_first = mats_first(*up);
   g.chunks = chunks;
   g.err = err;
   g.n_chunks = n_out;
@@ -967,6 +969,7 @@ extern "C" int yn_i8_experts_err(const yn_i8_mat* gate, const yn_i8_mat* up, con
   d.channels = H;
   d.K = I;
   d.half = 128;
+  d.mats_first = mats_first(*down);
   d.sx = sa;
   d.sw = down->scales;
   d.sw_stride = down->scale_stride;

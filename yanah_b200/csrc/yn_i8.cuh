@@ -176,11 +176,12 @@ struct I8Gemm {
   void* y;                 // (rows, y_stride): output, or UP: fp32 activations
   long long y_stride;
   int* err;                // error word, null: the device's
-  bool both, swapped;      // UP: map a holds both matrices; up before gate in it
+  bool mats_first, up_mats_first;   // map a (a_up) is (K, matrices, rows) instead of (K, rows, matrices)
   bool pairs;              // 16-bit outputs may be written two channels at a time (4-byte aligned rows)
 };
-// Tensor maps. a: the matrices' rows, boxes of 128 (UP: of 16; or, `both`, of 4 x 2 x 16: four times
-// 16 rows of gate and the same of up in one copy). b[i]: the rows' codes, boxes of 16 << i.
+// Tensor maps. a: the matrices' rows, boxes of 128 (UP: gate and up by a map each, boxes of 16; one map
+// over both, whose strides are not in order, read past the end of the matrices). b[i]: the rows' codes,
+// boxes of 16 << i.
 constexpr int I8_BMAPS = 4;
 struct I8Maps {
   CUtensorMap a, a_up, b[I8_BMAPS];
@@ -278,12 +279,6 @@ YN_DEV void i8_tma_3d(void* dst, const CUtensorMap* map, int x, int y, int z, ui
   asm volatile(
       "cp.async.bulk.tensor.3d.cta_group::2.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];" ::
           "r"(smem_u32(dst)), "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(z), "r"(cluster_bar)
-      : "memory");
-}
-YN_DEV void i8_tma_5d(void* dst, const CUtensorMap* map, int x, int hi, int z, uint32_t cluster_bar) {
-  asm volatile(
-      "cp.async.bulk.tensor.5d.cta_group::2.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %3, %4, %5}], [%6];" ::
-          "r"(smem_u32(dst)), "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(0), "r"(hi), "r"(z), "r"(cluster_bar)
       : "memory");
 }
 YN_DEV void i8_tma_2d(void* dst, const CUtensorMap* map, int x, int y, uint32_t cluster_bar) {
@@ -449,14 +444,13 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(I8_THREADS, 1)
         if (UP) {
           // lanes below 16 take the even rows, the others the odd ones
           const bool up = lane & 16;
-          const float s_lo = a.swapped ? su : sw, s_hi = a.swapped ? sw : su;
           float* out = reinterpret_cast<float*>(a.y) + (row + up) * a.y_stride + r;
 #pragma unroll
           for (int k = 0; k < 16; k += 2) {
             const int got = __shfl_xor_sync(0xffffffffu, up ? v[k] : v[k + 1], 16);
             const float s = __shfl_sync(0xffffffffu, sx, k + up);
-            const float lo = (float)(up ? got : v[k]) * s * s_lo, hi = (float)(up ? v[k + 1] : got) * s * s_hi;
-            if (k + up < left && in) out[(size_t)k * a.y_stride] = a.swapped ? i8_swiglu(hi, lo) : i8_swiglu(lo, hi);
+            const float g = (float)(up ? got : v[k]) * s * sw, u = (float)(up ? v[k + 1] : got) * s * su;
+            if (k + up < left && in) out[(size_t)k * a.y_stride] = i8_swiglu(g, u);
           }
         } else if (sizeof(O) == 2 && a.pairs) {
           // two lanes exchange so that each writes two adjacent channels of every second row
@@ -542,16 +536,17 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(I8_THREADS, 1)
           uint8_t* st = smem + s * F::STAGE;
           const uint32_t bar = i8_leader(&full[s]);
           if (rank == 0) mbar_arrive_expect_tx(&full[s], bytes);
-          if (UP && a.both) {
-            i8_tma_5d(st, &maps.a, 128 * kc, u0 >> 4, c.e, bar);
-          } else if (UP) {
+          auto weights = [&](void* dst, const CUtensorMap* map, bool first, int r) {
+            i8_tma_3d(dst, map, 128 * kc, first ? c.e : r, first ? r : c.e, bar);
+          };
+          if (UP) {
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-              i8_tma_3d(st + 4096 * i, &maps.a, 128 * kc, u0 + 16 * i, c.e, bar);
-              i8_tma_3d(st + 4096 * i + 2048, &maps.a_up, 128 * kc, u0 + 16 * i, c.e, bar);
+              weights(st + 4096 * i, &maps.a, a.mats_first, u0 + 16 * i);
+              weights(st + 4096 * i + 2048, &maps.a_up, a.up_mats_first, u0 + 16 * i);
             }
           } else {
-            i8_tma_3d(st, &maps.a, 128 * kc, u0, c.e, bar);
+            weights(st, &maps.a, a.mats_first, u0);
           }
           i8_tma_2d(st + I8_A_BYTES, &maps.b[bi], 128 * kc, row, bar);
           if (++s == F::S) {

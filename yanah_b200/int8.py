@@ -27,7 +27,8 @@ from .launch import DTYPES, check_constant, check_floats, check_like, elsewhere,
 class Int8Matrix(NamedTuple):
     """``codes`` (N, K) int8, or (E, N, K) for a matrix per expert, and ``scales`` (N) or
     (E, N) fp32 of the output channels. Rows of codes start at multiples of 16 bytes, as
-    ``quantize_rows`` lays them out."""
+    ``quantize_rows`` lays them out; matrices lie whole rows apart, or are interleaved row by
+    row."""
     codes: torch.Tensor
     scales: torch.Tensor
 
